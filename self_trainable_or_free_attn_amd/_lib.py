@@ -1,5 +1,5 @@
-"""Bindings of the C ABI in include/echosparse_hip.h and include/vsa_hip.h (libechosparse_hip.so, built in-tree by
-build_lib).
+"""Bindings of the C ABI in include/echosparse_hip.h, include/vsa_hip.h and include/packed_hip.h (libechosparse_hip.so,
+built in-tree by build_lib).
 
 Kernel calls (`call`) go through the torch operators torch.ops.echosparse_gfx950.<entry point> (torch_ops.py,
 lib/libechosparse_torch.so): arguments are tensors (None = NULL) and Python scalars in the header's order, and each
@@ -75,17 +75,24 @@ SIGNATURES = {
     "vsa_rep_unpool": [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I],
     "vsa_row_dot": [P, P, P, P, I, I, I],
     "vsa_tier_b_lists": [P, P, P, P, P, P, I, I],
+    # include/packed_hip.h
+    "es_packed_fwd": [P, P, P, P, P, P, P, I, I, P, P, P, Z, I, I, I, I, I, I, I, F],
+    "es_packed_bwd": [P, P, P, P, P, P, P, P, P, P, I, I, P, P, P, P, P, Z, I, I, I, I, I, I, I, F],
+    "es_shared_prefix_fwd": [P, P, P, P, P, P, P, P, P, Z, I, I, I, I, I, I, I, F],
 }
-# include/vsa_hip.h: the fp16 twins (suffix _f16) of the entry points that take token tensors, same arguments
+# the fp16 twins (suffix _f16) of the VSA and packed-sequence entry points that take token tensors, same arguments
 F16_TWINS = ("vsa_pool", "vsa_fuse_fwd", "vsa_fuse_bwd", "vsa_finalize", "vsa_attn_fwd", "vsa_attn_fwd_tasks",
              "vsa_attn_bwd_kv", "vsa_attn_bwd_kv_tasks", "vsa_attn_bwd_q", "vsa_attn_bwd_q_tasks", "vsa_block_scores",
              "vsa_route_rows", "vsa_row_topk", "vsa_router_lse", "vsa_router_scores", "vsa_split_merge_fwd",
              "vsa_split_merge_sum", "vsa_rep_build", "vsa_rep_build_kmeans", "vsa_rep_attn_fwd", "vsa_rep_attn_bwd_q", "vsa_rep_bwd_tables",
-             "vsa_rep_bwd_both_tables", "vsa_rep_unpool", "vsa_row_dot")
+             "vsa_rep_bwd_both_tables", "vsa_rep_unpool", "vsa_row_dot", "es_packed_fwd", "es_packed_bwd",
+             "es_shared_prefix_fwd")
 SIGNATURES.update({n + "_f16": SIGNATURES[n] for n in F16_TWINS})
 NO_STREAM = {"es_representatives_workspace": ([I, I, I], Z), "es_dense_attention_workspace": ([I, I, I], Z),
              "es_representatives_noalloc_limit": ([], Z), "es_last_error_string": ([], ctypes.c_char_p),
-             "es_abi_version": ([], I), "vsa_topk_workspace": ([I, I], Z)}
+             "es_abi_version": ([], I), "vsa_topk_workspace": ([I, I], Z),
+             "es_packed_fwd_workspace": ([I] * 6, Z), "es_packed_bwd_workspace": ([I] * 8, Z),
+             "es_shared_prefix_workspace": ([I] * 7, Z)}
 
 _lib = None
 _ops = None

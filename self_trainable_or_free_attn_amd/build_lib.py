@@ -2,7 +2,8 @@
 the torch operator library over it (torch_ops.py, lib/libechosparse_torch.so).
 
 Every HIP source under csrc/ is compiled to an object in parallel and linked into lib/libechosparse_hip.so; the
-VSA sources (vsa_*.hip) are compiled a second time with -DES_ELEM_F16 for their fp16 entry points (suffix _f16).
+VSA and packed-sequence sources (vsa_*.hip, packed_*.hip) are compiled a second time with -DES_ELEM_F16 for their fp16
+entry points (suffix _f16).
 Flags: -O3, gfx950 only, and packed FP32 instructions disabled (-Xclang -target-feature -Xclang -packed-fp32-ops).
 """
 import os
@@ -25,11 +26,12 @@ def sources():
 
 
 def units():
-    """(source, extra flags, object suffix) for every compilation: each source once, the VSA ones also for fp16."""
+    """(source, extra flags, object suffix) for every compilation: each source once, the VSA and packed ones also for
+    fp16."""
     out = []
     for src in sources():
         out.append((src, [], ""))
-        if os.path.basename(src).startswith("vsa_"):
+        if os.path.basename(src).startswith(("vsa_", "packed_")):
             out.append((src, ["-DES_ELEM_F16"], ".f16"))
     return out
 

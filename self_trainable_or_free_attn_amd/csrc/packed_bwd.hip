@@ -1,0 +1,566 @@
+// Backward of attention over packed sequences (gfx950, MFMA 32x32x16, bf16 / fp16).
+//
+// With P = exp(S - lse) and dS = P (dP - delta), dP = dO V^T, delta = rowsum(dO O) (rows that see no key: P = 0):
+//   row_stats   one pass over dO and O: lse in log2 units (+inf for rows without keys) and delta, laid out by kv head and
+//               row of the list (token, head in group), so that a row tile's values are contiguous
+//   bwd_kv      one workgroup per (64 keys, kv head): dV = P^T dO and dK = scale dS^T Q over all rows of the list that see
+//               the keys, which sums over the heads of a group without atomics. Four waves = 2 key halves x 2 row halves
+//               of each staged 64-row tile; S and dP come out with keys on lanes, so that P and dS are B operands.
+//   bwd_q       one workgroup per (64 rows, kv head): dQ = scale dS K over the keys, 2 row groups x 2 key halves, S^T and
+//               dP^T with rows on lanes; with a bias it also sums dS by clamped distance
+//   bias_sums   those sums over the row tiles and into buckets
+// Every sum has a fixed order, so the same inputs give the same bits. The scores are computed twice (7 products for 5): a
+// single pass would need dQ in float32 atomics or a dQ partial a key tile.
+// dS is rounded to the token type without the softmax scale (applied to the finished sums), which keeps it about ten times
+// further from the subnormal range of fp16.
+#include "packed.h"
+
+namespace es {
+
+namespace {
+
+// fp16: the probabilities of dV = P^T dO are taken 2^14 higher, out of the type's subnormal range for all down to 2^-28; dS
+// and the finished sum take the factor back exactly
+#ifdef ES_ELEM_F16
+constexpr float P_SHIFT = 14.0f, P_BACK = 1.0f / 16384.0f;
+#else
+constexpr float P_SHIFT = 0.0f, P_BACK = 1.0f;
+#endif
+
+struct BwdArgs {
+  const e16_t *q, *k, *v, *dout, *out;
+  const float *lse, *bias;
+  const int *cu_q, *cu_k, *buckets;
+  e16_t *dq, *dk, *dv;
+  float *dbias;
+  float *lse2, *delta;  // [Hk][Tq * G]
+  float* dist;          // [row tile numbers][Hk][G * (2 R + 1)]: dS by clamped distance
+  FastDiv div_g;
+  int B, Tq, Tk, H, Hk, G, R, num_buckets, causal;
+  int q_tiles, k_tiles;  // tile numbers of a head
+  float scale_log2, scale;
+};
+
+// D / 8 lanes a row of dO and O
+template <int D>
+__global__ __launch_bounds__(256) void row_stats_kernel(BwdArgs a) {
+  constexpr int LPR = D / 8;
+  const size_t row = (size_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (row >= (size_t)a.Tq * a.H) return;
+  const size_t at = row * D + 8 * (threadIdx.x % LPR);
+  const ev8 x = *reinterpret_cast<const ev8*>(a.dout + at), y = *reinterpret_cast<const ev8*>(a.out + at);
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum = fmaf((float)x[i], (float)y[i], sum);
+#pragma unroll
+  for (int m = 1; m < LPR; m <<= 1) sum += __shfl_xor(sum, m, 64);
+  if (threadIdx.x % LPR) return;
+  const int tok = (int)(row / a.H), h = (int)(row - (size_t)tok * a.H), hk = divide(a.div_g, h);
+  const size_t to = ((size_t)hk * a.Tq + tok) * a.G + (h - hk * a.G);
+  const float l = a.lse[row];
+  a.lse2[to] = l == -INFINITY ? INFINITY : l * LOG2E;
+  a.delta[to] = sum;
+}
+
+template <int D, bool BIAS>
+__global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
+  constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
+  __shared__ __attribute__((aligned(16))) char qd_s[2][2][TILE_BYTES];  // [buffer][Q | dO]
+  __shared__ __attribute__((aligned(16))) float st_s[2][2][BK];         // [buffer][lse2 | delta]
+  __shared__ __attribute__((aligned(16))) int pos_s[2][BK];             // [buffer] position of the row
+  __shared__ __attribute__((aligned(16))) int gb_s[BIAS ? 2 : 1][BIAS ? BK : 1];  // the row's part of the bias table
+  __shared__ float lse_s[BK];                                           // the next tile's lse2 as stored
+  __shared__ float tab[BIAS ? BIAS_ROWS : 1];
+  const int hk = blockIdx.x / a.k_tiles, w = blockIdx.x - hk * a.k_tiles;
+  const int b = seq_of_tile<BK>(a.cu_k, a.B, a.Tk, 1, w);
+  Seq s;
+  s.k0 = __builtin_amdgcn_readfirstlane(seq_start(a.cu_k, b, a.B, a.Tk));
+  const int kend = b >= a.B ? a.Tk : __builtin_amdgcn_readfirstlane(seq_start(a.cu_k, b + 1, a.B, a.Tk));
+  s.nk = max(kend - s.k0, 0);
+  const int kb = w - (s.k0 / BK + b);
+  if (kb < 0 || kb * BK >= s.nk) return;
+  s.q0 = 0;
+  s.nq = 0;  // (key rows behind the last sequence: zero gradients)
+  if (b < a.B) {
+    s.q0 = __builtin_amdgcn_readfirstlane(seq_start(a.cu_q, b, a.B, a.Tq));
+    s.nq = max(__builtin_amdgcn_readfirstlane(seq_start(a.cu_q, b + 1, a.B, a.Tq)) - s.q0, 0);
+  }
+  const int rows = s.nq * a.G, shift = s.nk - s.nq;
+  const int end = (rows + BK - 1) / BK;
+  // causal: the first row that sees this tile's first key
+  const int beg = a.causal ? min(max(kb * BK - shift, 0) * a.G / BK, end) : 0;
+  const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qh = wv >> 1, kh = wv & 1;
+  const int key = kb * BK + 32 * kh + lq;
+  const bool kvalid = key < s.nk;
+  const size_t krow = ((size_t)(s.k0 + (kvalid ? key : 0)) * a.Hk + hk) * D;
+  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
+
+  ev8 kreg[NKS], vreg[NKS];  // this lane's key row
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    const ev8 z = {};
+    kreg[ks] = kvalid ? *reinterpret_cast<const ev8*>(a.k + krow + 8 * hi + 16 * ks) : z;
+    vreg[ks] = kvalid ? *reinterpret_cast<const ev8*>(a.v + krow + 8 * hi + 16 * ks) : z;
+  }
+  // Row tile i: Q and dO rows (16 of each a wave) through a resource based at the tile's first token, and, wave 0, its lse2
+  // and delta. Rows of a list are `row / G` tokens of H * D values and `row % G` heads apart.
+  const size_t list = (size_t)hk * a.Tq * a.G + (size_t)s.q0 * a.G;
+  auto issue = [&](int i, int sb) {
+    const int t0 = divide(a.div_g, i * BK), toks = min(s.nq - t0, BK + 1);
+    const size_t base = ((size_t)(s.q0 + t0) * a.H + hk * a.G) * D;
+    const unsigned bytes = (unsigned)((toks - 1) * a.H + a.G) * ROW;
+    const srd_t rq = make_srd(a.q + base, bytes), rd = make_srd(a.dout + base, bytes);
+#pragma unroll
+    for (int r = 0; r < NI; ++r) {
+      const int R = wv * 16 + r * (64 / LPR) + l / LPR, row = i * BK + R, tok = divide(a.div_g, row);
+      const unsigned at = (unsigned)((tok - t0) * a.H + row - tok * a.G) * ROW + (unsigned)(((l % LPR) ^ swizzle<D>(R)) * 16);
+      dma16(rq, qd_s[sb][0] + (wv * NI + r) * 1024, at, 0u);
+      dma16(rd, qd_s[sb][1] + (wv * NI + r) * 1024, at, 0u);
+    }
+    if (wv == 0) {
+      const unsigned left = (unsigned)min(rows - i * BK, BK) * 4u;
+      dma4(make_srd(a.lse2 + list + (size_t)i * BK, left), lse_s, 4u * l, 0u);
+      dma4(make_srd(a.delta + list + (size_t)i * BK, left), st_s[sb][1], 4u * l, 0u);
+    }
+  };
+  auto stats = [&](int i, int sb) {  // wave 0, after dma_wait()
+    const int row = i * BK + l, tok = divide(a.div_g, row);
+    st_s[sb][0][l] = row < rows ? lse_s[l] - P_SHIFT : INFINITY;
+    if (P_BACK != 1.0f) st_s[sb][1][l] *= P_BACK;
+    pos_s[sb][l] = tok + shift;
+    if (BIAS) gb_s[sb][l] = (row - tok * a.G) * (2 * a.R + 1) + a.R;
+  };
+  // LDS offsets of this wave's row half (packed_fwd.hip: Offsets)
+  int aoff = qh * (TILE_BYTES / 2) + tile_at<D>(lq, hi);
+  int toff0, toff1;
+  {
+    const int g1 = (l >> 4) & 1, sub = (l & 1) * 8, rowA = 4 * hi + ((l & 15) >> 2);
+    toff0 = qh * (TILE_BYTES / 2) + tile_at<D>(rowA, 2 * g1 + ((l & 3) >> 1)) + sub;
+    toff1 = qh * (TILE_BYTES / 2) + tile_at<D>(rowA + 8, 2 * g1 + ((l & 3) >> 1)) + sub;
+  }
+  f32x16 acc_v[NDB], acc_k[NDB];  // this lane's key: dV and dK over this row half
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) acc_v[db] = acc_k[db] = f32x16{};
+
+  if (beg < end) {
+    issue(beg, 0);
+    dma_wait();
+    if (wv == 0) stats(beg, 0);
+  }
+  dma_wait();
+  __syncthreads();
+  // masked key columns: every row's lse2 becomes +inf for this lane, so P = 2^(s - inf) = 0 without a branch
+  const float kmask = kvalid ? 0.0f : INFINITY;
+  for (int i = beg; i < end; ++i) {
+    const int sb = (i - beg) & 1;
+    if (i + 1 < end) issue(i + 1, sb ^ 1);
+    asm volatile("" : "+v"(aoff), "+v"(toff0), "+v"(toff1));  // (keeps the offsets from being hoisted)
+    const char* qt = qd_s[sb][0];
+    const char* dt = qd_s[sb][1];
+    auto product = [&](const char* xt, const ev8& xa, const ev8& xb, f32x16 (&acc)[NDB]) {  // acc += xt^T [xa | xb]
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const int t0 = toff0 ^ (64 * db), t1 = toff1 ^ (64 * db);
+        acc[db] = emfma(ecat_tr(lds_read_tr(xt, t0), lds_read_tr(xt, t1)), xa, acc[db]);
+        acc[db] = emfma(ecat_tr(lds_read_tr(xt + TILE_BYTES / 4, t0), lds_read_tr(xt + TILE_BYTES / 4, t1)), xb, acc[db]);
+      }
+    };
+    f32x16 p = {}, dp = {};
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) p = emfma(elds16(qt, aoff ^ (32 * ks)), kreg[ks], p);
+    // the wave's rows 32 qh .. + 31 of the tile, whose positions ascend; a key is seen from its own position on
+    const bool diagonal = a.causal && pos_s[sb][32 * qh] < kb * BK + 32 * kh + 31;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int r0 = 32 * qh + 8 * g + 4 * hi;
+      f32x4 l4 = *reinterpret_cast<const f32x4*>(&st_s[sb][0][r0]);  // (lse2 - P_SHIFT)
+      if (BIAS || diagonal) {
+        const int4 p4 = *reinterpret_cast<const int4*>(&pos_s[sb][r0]);
+        const int ps[4] = {p4.x, p4.y, p4.z, p4.w};
+        if (BIAS) {
+          const int4 b4 = *reinterpret_cast<const int4*>(&gb_s[sb][r0]);
+          const int gs[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) l4[e] -= tab[gs[e] + min(max(key - ps[e], -a.R), a.R)];
+        }
+        if (diagonal) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key > ps[e]) l4[e] = INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[4 * g + e] = exp2f_fast(fmaf(p[4 * g + e], a.scale_log2, -(l4[e] + kmask)));
+    }
+    {
+      float x[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = p[r];
+      product(dt, epack8(&x[0]), epack8(&x[8]), acc_v);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (dP after dV: raised above it, its operands do not fit the registers)
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(dt, aoff ^ (32 * ks)), vreg[ks], dp);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 d4 = *reinterpret_cast<const f32x4*>(&st_s[sb][1][32 * qh + 8 * g + 4 * hi]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[4 * g + e] = p[4 * g + e] * fmaf(dp[4 * g + e], P_BACK, -d4[e]);
+    }
+    {
+      float x[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = p[r];
+      product(qt, epack8(&x[0]), epack8(&x[8]), acc_k);
+    }
+    dma_wait();
+    if (i + 1 < end && wv == 0) stats(i + 1, sb ^ 1);
+    __syncthreads();
+  }
+
+  // the second row half hands its sums over through the staging buffers: [key half][dV | dK][register][lane]
+  float* xch = reinterpret_cast<float*>(&qd_s[0][0][0]) + kh * (2 * NDB * 16 * 64);
+  if (qh == 1) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        xch[(db * 16 + r) * 64 + l] = acc_v[db][r];
+        xch[((NDB + db) * 16 + r) * 64 + l] = acc_k[db][r];
+      }
+  }
+  __syncthreads();
+  if (qh == 1 || !kvalid) return;
+  auto store = [&](f32x16 (&acc)[NDB], int base, float f, e16_t* out) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (acc[db][4 * i + e] + xch[((base + db) * 16 + 4 * i + e) * 64 + l]) * f;
+        ushort4 o4;
+        o4.x = f2e(x[0]); o4.y = f2e(x[1]); o4.z = f2e(x[2]); o4.w = f2e(x[3]);
+        *reinterpret_cast<ushort4*>(out + krow + 32 * db + 8 * i + 4 * hi) = o4;
+      }
+  };
+  store(acc_v, 0, P_BACK, a.dv);
+  store(acc_k, NDB, a.scale, a.dk);
+}
+
+template <int D, bool BIAS>
+__global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
+  constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
+  __shared__ __attribute__((aligned(16))) char kv_s[2][2][TILE_BYTES];
+  __shared__ float tab[BIAS ? BIAS_ROWS : 1];
+  __shared__ float hist[BIAS ? 4 : 1][BIAS ? BIAS_ROWS : 1];  // per wave: dS by (head in group, clamped distance)
+  const int hk = blockIdx.x / a.q_tiles, w = a.q_tiles - 1 - (blockIdx.x - hk * a.q_tiles);
+  const int b = seq_of_tile<BK>(a.cu_q, a.B, a.Tq, a.G, w);
+  const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, b);
+  const int t = w - (s.q0 * a.G / BK + b), rows = s.nq * a.G, shift = s.nk - s.nq, width = 2 * a.R + 1;
+  const bool none = t < 0 || t * BK >= rows;
+  float* dist = BIAS ? a.dist + ((size_t)w * a.Hk + hk) * (a.G * width) : nullptr;
+  if (none) {
+    if (BIAS)  // (a tile number without a tile: its sums are read all the same)
+      for (int i = threadIdx.x; i < a.G * width; i += 256) dist[i] = 0.0f;
+    return;
+  }
+  const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rg = wv & 1, kh = wv >> 1;
+  const int r0 = t * BK + 32 * rg, row = r0 + lq;
+  const bool valid = row < rows;
+  const int tok = divide(a.div_g, row), g = valid ? row - tok * a.G : 0, pos = tok + shift, gb = g * width + a.R;
+  const size_t at = (((size_t)(s.q0 + (valid ? tok : 0)) * a.Hk + hk) * a.G + g) * D;
+  const size_t list = ((size_t)hk * a.Tq + s.q0) * a.G + (valid ? row : 0);
+  const int seen = !valid ? 0 : a.causal ? min(max(pos + 1, 0), s.nk) : s.nk;
+  // the wave's rows: the first one sees the fewest keys, the last one the most
+  const int first = min(r0, rows - 1), last = min(r0 + 31, rows - 1);
+  const int low = divide(a.div_g, first) + shift, high = divide(a.div_g, last) + shift;
+  const int seen_min = a.causal ? min(max(low + 1, 0), s.nk) : s.nk;
+  const int seen_max = r0 >= rows ? 0 : a.causal ? min(max(high + 1, 0), s.nk) : s.nk;
+  const int tile_high = divide(a.div_g, min(t * BK + BK, rows) - 1) + shift;
+  const int end = ((a.causal ? min(max(tile_high + 1, 0), s.nk) : s.nk) + BK - 1) / BK;
+
+  ev8 qreg[NKS], dreg[NKS];
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    const ev8 z = {};
+    qreg[ks] = valid ? *reinterpret_cast<const ev8*>(a.q + at + 16 * ks + 8 * hi) : z;
+    dreg[ks] = valid ? *reinterpret_cast<const ev8*>(a.dout + at + 16 * ks + 8 * hi) : z;
+  }
+  const float ls = valid ? a.lse2[list] : INFINITY;
+  const float dl = valid ? a.delta[list] : 0.0f;
+  if (BIAS) {
+    for (int i = tid; i < 4 * BIAS_ROWS; i += 256) (&hist[0][0])[i] = 0.0f;
+    fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
+  }
+
+  const unsigned stride = (unsigned)a.Hk * ROW;
+  unsigned src[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int R = (wv * NI + i) * (64 / LPR) + l / LPR;
+    src[i] = (unsigned)R * stride + (unsigned)(((l % LPR) ^ swizzle<D>(R)) * 16);
+  }
+  auto issue = [&](int c, int sb) {
+    const size_t base = ((size_t)(s.k0 + c * BK) * a.Hk + hk) * D;
+    const unsigned bytes = (unsigned)(min(BK, s.nk - c * BK) - 1) * stride + ROW;
+    const srd_t rk = make_srd(a.k + base, bytes), rv = make_srd(a.v + base, bytes);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      dma16(rk, kv_s[sb][0] + (wv * NI + i) * 1024, src[i], 0u);
+      dma16(rv, kv_s[sb][1] + (wv * NI + i) * 1024, src[i], 0u);
+    }
+  };
+  const int koff = kh * (TILE_BYTES / 2) + tile_at<D>(lq, hi);
+  int toff0, toff1;
+  {
+    const int g1 = (l >> 4) & 1, sub = (l & 1) * 8, rowA = 4 * hi + ((l & 15) >> 2);
+    toff0 = kh * (TILE_BYTES / 2) + tile_at<D>(rowA, 2 * g1 + ((l & 3) >> 1)) + sub;
+    toff1 = kh * (TILE_BYTES / 2) + tile_at<D>(rowA + 8, 2 * g1 + ((l & 3) >> 1)) + sub;
+  }
+  f32x16 dq[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) dq[db] = f32x16{};
+  float far_lo = 0.0f, far_hi = 0.0f;  // dS at distances of -R and below, of R and beyond
+
+  if (end > 0) issue(0, 0);
+  dma_wait();
+  __syncthreads();
+  for (int c = 0; c < end; ++c) {
+    const int sb = c & 1;
+    if (c + 1 < end) issue(c + 1, sb ^ 1);
+    const char* kt = kv_s[sb][0];
+    const char* vt = kv_s[sb][1];
+    const int key0 = c * BK + 32 * kh;
+    if (key0 < seen_max) {
+      f32x16 x = {}, dp = {};
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) x = emfma(elds16(kt, koff ^ (32 * ks)), qreg[ks], x);
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(vt, koff ^ (32 * ks)), dreg[ks], dp);
+      float ds[16];
+      const int d0 = key0 + 4 * hi - pos;
+      bool near = false;
+      float cb = 0.0f;
+      if (BIAS) {
+        if (key0 - high >= a.R) cb = tab[gb + a.R];
+        else if (key0 + 31 - low <= -a.R) cb = tab[gb - a.R];
+        else near = true;
+      }
+      float sc = a.scale_log2;
+      if (near) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], sc, tab[gb + min(max(d0 + 8 * (r / 4) + r % 4, -a.R), a.R)]);
+        sc = 1.0f;
+      }
+      if (key0 + 32 > seen_min) {
+        const int left = seen - key0 - 4 * hi;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (8 * (r / 4) + r % 4 >= left) x[r] = -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] = exp2f_fast(fmaf(x[r], sc, cb - ls)) * (dp[r] - dl);
+      if (BIAS) {
+        if (!near) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum += ds[r];
+          if (key0 - high >= a.R) far_hi += sum;
+          else far_lo += sum;
+        } else {
+          // One key of the run a step: the 32 rows of a half wave stand at different distances or in different heads, so
+          // no two lanes of a half add to one entry; the halves go one after the other, which fixes the order.
+          float* h = hist[wv];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int d = d0 + 8 * (r / 4) + r % 4;
+            if (d <= -a.R) far_lo += ds[r];
+            else if (d >= a.R) far_hi += ds[r];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (hi == half && valid && d > -a.R && d < a.R) h[gb + d] += ds[r];
+              __builtin_amdgcn_wave_barrier();
+            }
+          }
+        }
+      }
+      const ev8 sa = epack8(&ds[0]), sb8 = epack8(&ds[8]);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const int t0 = toff0 ^ (64 * db), t1 = toff1 ^ (64 * db);
+        dq[db] = emfma(ecat_tr(lds_read_tr(kt, t0), lds_read_tr(kt, t1)), sa, dq[db]);
+        dq[db] = emfma(ecat_tr(lds_read_tr(kt + TILE_BYTES / 4, t0), lds_read_tr(kt + TILE_BYTES / 4, t1)), sb8, dq[db]);
+      }
+    }
+    dma_wait();
+    __syncthreads();
+  }
+
+  // the second key half hands its sums over through the staging buffers; with a bias the far sums follow
+  float* xq = reinterpret_cast<float*>(&kv_s[0][0][0]) + rg * (NDB * 16 * 64);
+  float* far = reinterpret_cast<float*>(&kv_s[1][0][0]);  // [wave][low | high][lane]
+  if (kh == 1) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) xq[(db * 16 + r) * 64 + l] = dq[db][r];
+  }
+  if (BIAS) {
+    far[wv * 128 + l] = valid ? far_lo : 0.0f;
+    far[wv * 128 + 64 + l] = valid ? far_hi : 0.0f;
+  }
+  __syncthreads();
+  if (BIAS) {
+    for (int i = tid; i < a.G * width; i += 256) {
+      const int gi = i / width, d = i - gi * width - a.R;
+      float sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum += hist[x][i];
+      if (d == -a.R || d == a.R) {
+        // (R = 0: one entry, which takes both)
+        for (int x = 0; x < 4; ++x) {
+          for (int n = 0; n < 64; ++n) {
+            const int rr = t * BK + 32 * (x & 1) + (n & 31);
+            if (rr - divide(a.div_g, rr) * a.G != gi) continue;
+            if (d == -a.R) sum += far[x * 128 + n];
+            if (d == a.R) sum += far[x * 128 + 64 + n];
+          }
+        }
+      }
+      dist[i] = sum;
+    }
+  }
+  if (kh == 1 || !valid) return;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = (dq[db][4 * i + e] + xq[(db * 16 + 4 * i + e) * 64 + l]) * a.scale;
+      ushort4 q4;
+      q4.x = f2e(x[0]); q4.y = f2e(x[1]); q4.z = f2e(x[2]); q4.w = f2e(x[3]);
+      *reinterpret_cast<ushort4*>(a.dq + at + 32 * db + 8 * i + 4 * hi) = q4;
+    }
+}
+
+// dbias[n][h] = sum over the row tiles and over the distances of bucket n: one workgroup a head, a distance a thread, then a
+// bucket a thread
+__global__ __launch_bounds__(256) void bias_sums_kernel(BwdArgs a) {
+  __shared__ float sums[BIAS_ROWS];
+  const int h = blockIdx.x, hk = divide(a.div_g, h), g = h - hk * a.G, width = 2 * a.R + 1;
+  const size_t step = (size_t)a.Hk * a.G * width;
+  for (int d = threadIdx.x; d < width; d += 256) {
+    const float* p = a.dist + ((size_t)hk * a.G + g) * width + d;
+    float sum = 0.0f;
+    for (int w = 0; w < a.q_tiles; ++w) sum += p[w * step];
+    sums[d] = sum;
+  }
+  __syncthreads();
+  for (int n = threadIdx.x; n < a.num_buckets; n += 256) {
+    float sum = 0.0f;
+    for (int d = 0; d < width; ++d)
+      if (min(max(a.buckets[d], 0), a.num_buckets - 1) == n) sum += sums[d];
+    a.dbias[(size_t)n * a.H + h] = sum;
+  }
+}
+
+}  // namespace
+
+}  // namespace es
+
+using namespace es;
+
+#ifndef ES_ELEM_F16
+// lse2 and delta, then the distance sums of every (row tile, kv head)
+extern "C" size_t es_packed_bwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D, int R, int with_bias) {
+  if (B <= 0 || Tq < 0 || Tk < 0 || H <= 0 || Hk <= 0 || H % Hk || R < 0) return 0;
+  (void)D;
+  size_t floats = 2 * (size_t)Tq * H;
+  if (with_bias) floats += (size_t)tile_numbers<BK>(B, Tq, H / Hk) * H * (2 * R + 1);
+  return floats * sizeof(float);
+}
+#endif
+
+extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const void* v, const void* dout, const void* out,
+                                         const float* lse, const int* cu_q, const int* cu_k, const float* bias,
+                                         const int* buckets, int num_buckets, int R, void* dq, void* dk, void* dv,
+                                         float* dbias, void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H,
+                                         int Hk, int D, int causal, float scale, hipStream_t stream) {
+  if (int st = packed_check(q, k, v, cu_q, cu_k, bias, buckets, num_buckets, R, B, Tq, Tk, H, Hk, D, scale)) return st;
+  ES_REQUIRE((Tq == 0 || (dout && out && lse && dq && workspace)) && (Tk == 0 || (dk && dv)), ES_ERR_INVALID,
+             "packed: null tensor pointer");
+  ES_REQUIRE((bias != nullptr) == (dbias != nullptr), ES_ERR_INVALID, "packed: dbias goes with bias");
+  ES_REQUIRE(workspace_bytes >= es_packed_bwd_workspace(B, Tq, Tk, H, Hk, D, bias ? R : 0, bias != nullptr),
+             ES_ERR_INVALID, "packed: workspace too small");
+  BwdArgs a = {};
+  a.q = (const e16_t*)q;
+  a.k = (const e16_t*)k;
+  a.v = (const e16_t*)v;
+  a.dout = (const e16_t*)dout;
+  a.out = (const e16_t*)out;
+  a.lse = lse;
+  a.bias = bias;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.buckets = buckets;
+  a.dq = (e16_t*)dq;
+  a.dk = (e16_t*)dk;
+  a.dv = (e16_t*)dv;
+  a.dbias = dbias;
+  a.lse2 = (float*)workspace;
+  a.delta = a.lse2 + (size_t)Tq * H;
+  a.dist = a.delta + (size_t)Tq * H;
+  a.B = B;
+  a.Tq = Tq;
+  a.Tk = Tk;
+  a.H = H;
+  a.Hk = Hk;
+  a.G = H / Hk;
+  a.div_g = fast_div(a.G);
+  a.R = bias ? R : 0;
+  a.num_buckets = num_buckets;
+  a.causal = causal != 0;
+  a.scale = scale;
+  a.scale_log2 = scale * LOG2E;
+  a.q_tiles = (int)tile_numbers<BK>(B, Tq, a.G);
+  a.k_tiles = (int)tile_numbers<BK>(B, Tk, 1);
+  ES_REQUIRE((long long)a.q_tiles * Hk < (1LL << 31) && (long long)a.k_tiles * Hk < (1LL << 31), ES_ERR_UNSUPPORTED,
+             "packed: grid too large");
+  if (Tq > 0) {
+    const long long per = D == 64 ? 32 : 16;
+    const dim3 grid((unsigned)(((long long)Tq * H + per - 1) / per));
+    if (D == 64) hipLaunchKernelGGL((row_stats_kernel<64>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((row_stats_kernel<128>), grid, dim3(256), 0, stream, a);
+  }
+  if (Tk > 0) {
+    const dim3 grid((unsigned)(a.k_tiles * Hk));
+    if (D == 64) {
+      if (bias) hipLaunchKernelGGL((packed_bwd_kv_kernel<64, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((packed_bwd_kv_kernel<64, false>), grid, dim3(256), 0, stream, a);
+    } else {
+      if (bias) hipLaunchKernelGGL((packed_bwd_kv_kernel<128, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((packed_bwd_kv_kernel<128, false>), grid, dim3(256), 0, stream, a);
+    }
+  }
+  if (Tq > 0) {
+    const dim3 grid((unsigned)(a.q_tiles * Hk));
+    if (D == 64) {
+      if (bias) hipLaunchKernelGGL((packed_bwd_q_kernel<64, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((packed_bwd_q_kernel<64, false>), grid, dim3(256), 0, stream, a);
+    } else {
+      if (bias) hipLaunchKernelGGL((packed_bwd_q_kernel<128, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((packed_bwd_q_kernel<128, false>), grid, dim3(256), 0, stream, a);
+    }
+  }
+  if (bias) {
+    if (Tq == 0) a.q_tiles = 0;
+    hipLaunchKernelGGL(bias_sums_kernel, dim3((unsigned)H), dim3(256), 0, stream, a);
+  }
+  return check_launch("es_packed_bwd");
+}

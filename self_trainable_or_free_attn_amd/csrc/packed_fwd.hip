@@ -1,0 +1,742 @@
+// Forward of attention over packed sequences and over a shared prefix (gfx950, MFMA 32x32x16, bf16 / fp16).
+//
+// One workgroup of four waves owns a tile of up to 128 rows of (token, head in group) (packed.h) and streams the keys its
+// rows see in 64-key chunks, online softmax: S^T = K Q^T, so that exp(S^T) is the B operand of O^T += V^T P^T.
+//   wide tiles (more than 32 rows): each wave has 32 rows; a chunk is staged once in LDS for all four, the next one's
+//     transfers in flight under its products.
+//   narrow tiles (up to 32 rows: single tokens with their head group): every wave has the same 32 rows and takes every
+//     fourth run of 32 keys, staged in its own quarter of LDS without a barrier; the four softmax states are merged at the
+//     end. The next K run is requested when this one's products have read it, the next V run likewise, so one of them is
+//     always in flight.
+// Key ranges: with few tiles the chunks of a tile are cut into ranges, one workgroup each, that leave unnormalised partials
+// (O, running maximum, sum) in the workspace; merge_kernel adds them in order.
+#include "packed.h"
+
+#include <algorithm>
+
+namespace es {
+
+namespace {
+
+constexpr float SLACK = 8.0f;  // log2 growth of a row's maximum that triggers a rescale of O and the sum
+// fp16 probabilities are taken 2^7 higher (up to 2^15 with the slack), which keeps those down to 2^-21 of the maximum out of
+// the type's subnormal range; the shift cancels in O / sum and is taken off the LSE
+#ifdef ES_ELEM_F16
+constexpr float P_SHIFT = 7.0f;
+#else
+constexpr float P_SHIFT = 0.0f;
+#endif
+
+struct FwdArgs {
+  const e16_t *q, *k, *v;
+  const int *cu_q, *cu_k, *buckets;
+  const float* bias;
+  e16_t* out;
+  float *lse, *part;
+  FastDiv div_g;
+  int B, Tq, Tk, H, Hk, G, R, num_buckets, causal;
+  int tiles;      // tile numbers of a head
+  int target;     // ranged launches: workgroups that the GPU holds at once
+  float scale;    // log2(e) * softmax scale
+  // shared prefix: rows 0 .. P - 1 of k_prefix / v_prefix are seen by every row
+  const e16_t *kp, *vp;
+  const int* lens;
+  int n, P, S;
+};
+
+// What one workgroup computes: rows of tile t of the list of nq * G rows that starts at token q0, against key rows
+// 0 .. nk - 1 behind k / v (this kv head's first row), chunks c0 .. c1 - 1 of them.
+struct Job {
+  const e16_t *k, *v;
+  int q0, nq, nk, hk, t, c0, c1, causal;
+  float* part;  // nullptr: finished rows go to out / lse
+};
+
+// floats of one partial: O [128][D], m [128], l [128]
+__host__ __device__ constexpr int part_floats(int D) { return TILE * D + 2 * TILE; }
+
+// keys that row r of the job's list sees
+__device__ __forceinline__ int keys_seen(const FwdArgs& a, const Job& j, int r) {
+  return j.causal ? min(max(divide(a.div_g, r) + 1 + j.nk - j.nq, 0), j.nk) : j.nk;
+}
+// chunks that any row of the job's tile sees
+__device__ __forceinline__ int tile_chunks(const FwdArgs& a, const Job& j) {
+  const int last = min(j.nq * a.G, (j.t + 1) * TILE) - 1;
+  return (keys_seen(a, j, last) + BK - 1) / BK;
+}
+
+// A lane's row, its softmax state and the exponentials of a 32-key run of S^T.
+template <int D, bool BIAS>
+struct Rows {
+  ev8 q[D / 16];
+  f32x16 o[D / 32];
+  float lsum, mrun;
+  int seen, pos, gb;  // keys seen, position, the row's part of the bias table
+  size_t at;          // row of out / lse
+  bool valid;
+
+  __device__ __forceinline__ void load(const FwdArgs& a, const Job& j, int r, int hi) {
+    valid = r < j.nq * a.G;
+    const int tok = divide(a.div_g, r), g = r - tok * a.G;
+    at = ((size_t)(j.q0 + (valid ? tok : 0)) * a.Hk + j.hk) * a.G + (valid ? g : 0);
+    seen = valid ? keys_seen(a, j, r) : 0;
+    pos = tok + j.nk - j.nq;
+    gb = (valid ? g : 0) * (2 * a.R + 1) + a.R;
+    const e16_t* p = a.q + at * D + 8 * hi;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const ev8 z = {};
+      q[ks] = valid ? *reinterpret_cast<const ev8*>(p + 16 * ks) : z;
+    }
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
+    lsum = 0.0f;
+    mrun = -INFINITY;
+  }
+
+  // p = exp(s - maximum) of keys key0 .. key0 + 31 as two B operands; masked: some row does not see all of them;
+  // low / high: the positions of the wave's rows (bias only)
+  __device__ __forceinline__ void exponentials(const FwdArgs& a, const float* tab, f32x16 s, int key0, int hi, bool masked,
+                                               int low, int high, ev8& pa, ev8& pb) {
+    float sc = a.scale, c = 0.0f;
+    if (BIAS) {
+      if (key0 - high >= a.R) {
+        c = tab[gb + a.R];
+      } else if (key0 + 31 - low <= -a.R) {
+        c = tab[gb - a.R];
+      } else {
+        const int d0 = key0 + 4 * hi - pos;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = fmaf(s[r], sc, tab[gb + min(max(d0 + 8 * (r / 4) + r % 4, -a.R), a.R)]);
+        sc = 1.0f;
+      }
+    }
+    if (masked) {
+      const int left = seen - key0 - 4 * hi;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r / 4) + r % 4 >= left) s[r] = -INFINITY;
+    }
+    // (the maximum of the products is that of the scores: the scale is positive and the rounding monotone)
+    float mx = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = fmaf(max_xor32(mx), sc, c);
+    if (mx > mrun + SLACK) {
+      const float alpha = exp2f_fast(mrun - mx);
+      lsum *= alpha;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+      mrun = mx;
+    }
+    c -= (mrun == -INFINITY ? 0.0f : mrun) - P_SHIFT;
+    float p[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) p[r] = exp2f_fast(fmaf(s[r], sc, c));
+    pa = epack8(&p[0]);
+    pb = epack8(&p[8]);
+    // (the sum takes the probabilities before their rounding: the LSE is a float32 result of its own)
+    float sum[4] = {p[0], p[1], p[2], p[3]};
+#pragma unroll
+    for (int r = 4; r < 16; ++r) sum[r & 3] += p[r];
+    lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  }
+
+  // O^T += V^T P^T of sixteen keys at `v`
+  __device__ __forceinline__ void values(const char* v, int t0, int t1, const ev8& p) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+      o[db] = emfma(ecat_tr(lds_read_tr(v, t0 ^ (64 * db)), lds_read_tr(v, t1 ^ (64 * db))), p, o[db]);
+  }
+};
+
+// LDS offsets of a lane: K rows (A operand of S^T) at k-step ks: k0 ^ 32 ks; V columns (transposed reads) of channel block
+// db: t0 / t1 ^ 64 db (exact: the swizzle is an XOR of the 16-byte chunk)
+template <int D>
+struct Offsets {
+  int k0, t0, t1;
+  __device__ __forceinline__ Offsets(int l) {
+    const int hi = l >> 5, g1 = (l >> 4) & 1, sub = (l & 1) * 8, row = 4 * hi + ((l & 15) >> 2);
+    k0 = tile_at<D>(l & 31, hi);
+    t0 = tile_at<D>(row, 2 * g1 + ((l & 3) >> 1)) + sub;
+    t1 = tile_at<D>(row + 8, 2 * g1 + ((l & 3) >> 1)) + sub;
+  }
+};
+
+template <int D>
+__device__ __forceinline__ void store_row(const FwdArgs& a, size_t at, int col, f32x4 x) {
+  ushort4 v4;
+  v4.x = f2e(x[0]); v4.y = f2e(x[1]); v4.z = f2e(x[2]); v4.w = f2e(x[3]);
+  *reinterpret_cast<ushort4*>(a.out + at * D + col) = v4;
+}
+
+template <int D, bool BIAS>
+__device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* lds, const float* tab) {
+  constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
+  const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r0 = j.t * TILE + wv * 32, rows = j.nq * a.G;
+  Rows<D, BIAS> x;
+  x.load(a, j, r0 + lq, hi);
+  const Offsets<D> off(l);
+  // this wave's rows: the first one sees the fewest keys, the last one the most
+  const int first = min(r0, rows - 1), last = min(r0 + 31, rows - 1);
+  const int seen_min = keys_seen(a, j, first), seen_max = r0 < rows ? keys_seen(a, j, last) : 0;
+  const int low = divide(a.div_g, first) + j.nk - j.nq, high = divide(a.div_g, last) + j.nk - j.nq;
+
+  // a lane's transfers: NI 1 KB runs of 64 / LPR rows each a wave
+  const unsigned stride = (unsigned)a.Hk * D * 2;
+  unsigned src[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int R = (wv * NI + i) * (64 / LPR) + l / LPR;
+    src[i] = (unsigned)R * stride + (unsigned)(((l % LPR) ^ swizzle<D>(R)) * 16);
+  }
+  const unsigned lds0 = uni(lds_addr(lds) + (unsigned)wv * (NI * 1024u));
+  auto issue = [&](int c, int sb) {
+    const size_t row = (size_t)c * BK * a.Hk * D;
+    const unsigned bytes = (unsigned)(min(BK, j.nk - c * BK) - 1) * stride + ROW;
+    const srd_t rk = make_srd(j.k + row, bytes), rv = make_srd(j.v + row, bytes);
+    const unsigned dst = lds0 + (unsigned)sb * (2u * TILE_BYTES);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma16_at(rk, dst + i * 1024, src[i], 0u);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma16_at(rv, dst + TILE_BYTES + i * 1024, src[i], 0u);
+  };
+  if (j.c0 < j.c1) issue(j.c0, 0);
+  dma_wait();
+  __syncthreads();
+  for (int c = j.c0; c < j.c1; ++c) {
+    const int sb = (c - j.c0) & 1;
+    const char* kb = lds + sb * 2 * TILE_BYTES;
+    const char* vb = kb + TILE_BYTES;
+    // K of the first 32 keys is read before the next chunk's transfers are issued: the first products then find their
+    // operands ready
+    ev8 kf[NKS];
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) kf[ks] = elds16(kb, off.k0 ^ (32 * ks));
+    if (c + 1 < j.c1) issue(c + 1, sb ^ 1);
+    if (c * BK < seen_max) {
+      const bool masked = (c + 1) * BK > seen_min;
+      f32x16 s0 = {}, s1 = {};
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) s0 = emfma(kf[ks], x.q[ks], s0);
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) s1 = emfma(elds16(kb + TILE_BYTES / 2, off.k0 ^ (32 * ks)), x.q[ks], s1);
+      ev8 pa, pb;
+      x.exponentials(a, tab, s0, c * BK, hi, masked, low, high, pa, pb);
+      x.values(vb, off.t0, off.t1, pa);
+      x.values(vb + TILE_BYTES / 4, off.t0, off.t1, pb);
+      x.exponentials(a, tab, s1, c * BK + 32, hi, masked, low, high, pa, pb);
+      x.values(vb + TILE_BYTES / 2, off.t0, off.t1, pa);
+      x.values(vb + 3 * (TILE_BYTES / 4), off.t0, off.t1, pb);
+    }
+    dma_wait();
+    __syncthreads();
+  }
+
+  const float tot = sum_xor32(x.lsum);
+  if (j.part != nullptr) {
+    const int r = wv * 32 + lq;
+    if (r0 >= rows) return;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(j.part + r * D + 32 * db + 8 * i + 4 * hi) =
+            f32x4{x.o[db][4 * i], x.o[db][4 * i + 1], x.o[db][4 * i + 2], x.o[db][4 * i + 3]};
+    if (hi == 0) {
+      j.part[TILE * D + r] = x.mrun;
+      j.part[TILE * D + TILE + r] = tot;
+    }
+    return;
+  }
+  if (!x.valid) return;
+  const float inv = tot == 0.0f ? 0.0f : 1.0f / tot;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      store_row<D>(a, x.at, 32 * db + 8 * i + 4 * hi,
+                   f32x4{x.o[db][4 * i], x.o[db][4 * i + 1], x.o[db][4 * i + 2], x.o[db][4 * i + 3]} * inv);
+  if (hi == 0) a.lse[x.at] = tot == 0.0f ? -INFINITY : (x.mrun - P_SHIFT + log2f(tot)) * PK_LN2;
+}
+
+// up to 32 rows; `lds`: 64 KB of staging, `stats`: [4 waves][m | l][64 lanes]
+template <int D, bool BIAS>
+__device__ __forceinline__ void narrow_tile(const FwdArgs& a, const Job& j, char* lds, float* stats, const float* tab) {
+  constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, RUN = 32 * ROW, NI = D / 16, LPR = D / 8;
+  const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r0 = j.t * TILE, rows = j.nq * a.G;
+  Rows<D, BIAS> x;
+  x.load(a, j, r0 + lq, hi);
+  const Offsets<D> off(l);
+  const int last = min(r0 + 31, rows - 1);
+  const int seen_min = keys_seen(a, j, r0), seen_max = keys_seen(a, j, last);
+  const int low = divide(a.div_g, r0) + j.nk - j.nq, high = divide(a.div_g, last) + j.nk - j.nq;
+
+  const unsigned stride = (unsigned)a.Hk * D * 2;
+  unsigned src[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int R = i * (64 / LPR) + l / LPR;
+    src[i] = (unsigned)R * stride + (unsigned)(((l % LPR) ^ swizzle<D>(R)) * 16);
+  }
+  char* kb = lds + wv * 2 * RUN;
+  char* vb = kb + RUN;
+  const unsigned kd = uni(lds_addr(kb)), vd = uni(lds_addr(vb));
+  auto issue = [&](const e16_t* base, int u, unsigned dst) {
+    const srd_t rs = make_srd(base + (size_t)u * 32 * a.Hk * D, (unsigned)(min(32, j.nk - u * 32) - 1) * stride + ROW);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma16_at(rs, dst + i * 1024, src[i], 0u);
+  };
+  const int end = min(2 * j.c1, (seen_max + 31) / 32);
+  int u = 2 * j.c0 + wv;
+  if (u < end) {
+    issue(j.k, u, kd);
+    issue(j.v, u, vd);
+  }
+  for (; u < end; u += 4) {
+    const bool more = u + 4 < end;
+    wait_transfers<NI>();  // K: all but the V run's transfers
+    f32x16 s = {};
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) s = emfma(elds16(kb, off.k0 ^ (32 * ks)), x.q[ks], s);
+    wait_lds();
+    if (more) issue(j.k, u + 4, kd);
+    ev8 pa, pb;
+    x.exponentials(a, tab, s, 32 * u, hi, 32 * (u + 1) > seen_min, low, high, pa, pb);
+    if (more) wait_transfers<NI>();
+    else wait_transfers<0>();
+    x.values(vb, off.t0, off.t1, pa);
+    x.values(vb + RUN / 2, off.t0, off.t1, pb);
+    wait_lds();
+    if (more) issue(j.v, u + 4, vd);
+  }
+
+  // merge of the four waves' states: each wave finishes a quarter of the channels
+  wait_transfers<0>();
+  float* mine = reinterpret_cast<float*>(lds + wv * 2 * RUN);  // [NDB * 16 registers][64 lanes]
+  static_assert(NDB * 16 * 64 * 4 <= 2 * RUN, "a wave's O fits its staging");
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mine[(db * 16 + r) * 64 + l] = x.o[db][r];
+  stats[wv * 128 + l] = x.mrun;
+  stats[wv * 128 + 64 + l] = sum_xor32(x.lsum);
+  __syncthreads();
+  float m[4], w[4], M = -INFINITY, tot = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = stats[i * 128 + l];
+    M = fmaxf(M, m[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = m[i] == -INFINITY ? 0.0f : exp2f_fast(m[i] - M);
+    tot += w[i] * stats[i * 128 + 64 + l];
+  }
+  const float inv = j.part != nullptr ? 1.0f : tot == 0.0f ? 0.0f : 1.0f / tot;
+#pragma unroll
+  for (int e = 0; e < NDB; ++e) {
+    const int q4 = wv * NDB + e;  // group of four registers: channels 32 (q4 / 4) + 8 (q4 % 4) + 4 hi ..
+    f32x4 acc = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* other = reinterpret_cast<const float*>(lds + i * 2 * RUN);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[c] = fmaf(w[i], other[(q4 * 4 + c) * 64 + l], acc[c]);
+    }
+    const int col = 32 * (q4 >> 2) + 8 * (q4 & 3) + 4 * hi;
+    if (j.part != nullptr) *reinterpret_cast<f32x4*>(j.part + lq * D + col) = acc;
+    else if (x.valid) store_row<D>(a, x.at, col, acc * inv);
+  }
+  if (wv == 0 && hi == 0) {
+    if (j.part != nullptr) {
+      j.part[TILE * D + lq] = M;
+      j.part[TILE * D + TILE + lq] = tot;
+    } else if (x.valid) {
+      a.lse[x.at] = tot == 0.0f ? -INFINITY : (M - P_SHIFT + log2f(tot)) * PK_LN2;
+    }
+  }
+}
+
+template <int D, bool BIAS>
+__device__ __forceinline__ void run_tile(const FwdArgs& a, const Job& j, char* lds, float* stats, const float* tab) {
+  if (j.nq * a.G - j.t * TILE <= 32) narrow_tile<D, BIAS>(a, j, lds, stats, tab);
+  else wide_tile<D, BIAS>(a, j, lds, tab);
+}
+
+// whole tiles: grid tiles * Hk, a head's tiles on neighbouring workgroups (so on all XCDs), the last ones, which under a
+// causal mask see the most keys, first
+template <int D, bool BIAS>
+__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
+  __shared__ float stats[4 * 128];
+  __shared__ float tab[BIAS ? BIAS_ROWS : 1];
+  const int hk = blockIdx.x / a.tiles, w = a.tiles - 1 - (blockIdx.x - hk * a.tiles);
+  const int b = seq_of_tile<TILE>(a.cu_q, a.B, a.Tq, a.G, w);
+  const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, b);
+  Job j;
+  j.t = w - (s.q0 * a.G / TILE + b);
+  if (j.t < 0 || j.t * TILE >= s.nq * a.G) return;
+  j.k = a.k + ((size_t)s.k0 * a.Hk + hk) * D;
+  j.v = a.v + ((size_t)s.k0 * a.Hk + hk) * D;
+  j.q0 = s.q0;
+  j.nq = s.nq;
+  j.nk = s.nk;
+  j.hk = hk;
+  j.causal = a.causal;
+  j.part = nullptr;
+  j.c0 = 0;
+  j.c1 = tile_chunks(a, j);
+  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
+  run_tile<D, BIAS>(a, j, lds, stats, tab);
+}
+
+// ------------------------------------------------------------------------------------------------ key ranges
+// A ranged launch cuts each tile's chunks into ranges of about the same number of chunks, as many as fill the GPU once.
+// Every wave derives the plan from the lengths by itself (a load and some shuffles a 64 sequences), so the lengths stay on
+// the device and no launch is spent on it. `lists` lists of rows, list i with tiles(i) tiles of chunks(i) chunks each:
+//   sum = Hk * total of tiles * chunks; a range has at least ceil(sum / target) chunks (and at least four where a tile has
+//   up to 32 rows, eight where it has more and its partial costs more), list i has ceil(chunks / that) ranges a tile.
+// Items are numbered list by list, tile by tile, range by range.
+struct ListShape {
+  int tiles, chunks, rows;
+};
+struct Ranges {
+  int list, ranges, item0;  // the list, its ranges a tile, its first item
+};
+
+__device__ __forceinline__ int ranges_of(const ListShape& x, int per) {
+  const int least = max(per, x.rows <= 32 ? 4 : 8);
+  return max((x.chunks + least - 1) / least, 1);
+}
+
+// chunks of a range before the two lower limits
+template <class F>
+__device__ __forceinline__ int range_chunks(const FwdArgs& a, int lists, const F& shape) {
+  unsigned long long sum = 0;
+  for (int i0 = 0; i0 < lists; i0 += 64) {
+    const int i = i0 + lane_id();
+    if (i < lists) {
+      const ListShape x = shape(i);
+      sum += (unsigned long long)x.tiles * x.chunks;
+    }
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+  return (int)min((sum * a.Hk + a.target - 1) / a.target, 1ull << 30);
+}
+
+// the list that holds item w (BY_LIST: the list w); ranges = 0: none
+template <bool BY_LIST, class F>
+__device__ __forceinline__ Ranges find_ranges(int lists, int per, int w, const F& shape) {
+  int base = 0;
+  for (int i0 = 0; i0 < lists; i0 += 64) {
+    const int i = i0 + lane_id();
+    int items = 0, ranges = 0;
+    if (i < lists) {
+      const ListShape x = shape(i);
+      ranges = ranges_of(x, per);
+      items = x.tiles * ranges;
+    }
+    int upto = items;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int y = __shfl_up(upto, m, 64);
+      if (lane_id() >= m) upto += y;
+    }
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(BY_LIST ? i == w : base + upto > w);
+    if (hit) {
+      const int from = __builtin_ctzll(hit);
+      Ranges r;
+      r.list = i0 + from;
+      r.ranges = __builtin_amdgcn_readlane(ranges, from);
+      r.item0 = base + __builtin_amdgcn_readlane(upto - items, from);
+      return r;
+    }
+    base += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return Ranges{0, 0, 0};
+}
+
+// packed sequences: list b, the rows behind the last sequence being list B
+struct PackedLists {
+  const FwdArgs& a;
+  __device__ __forceinline__ ListShape operator()(int b) const {
+    const int q0 = seq_start(a.cu_q, b, a.B, a.Tq);
+    if (b >= a.B) return ListShape{((a.Tq - q0) * a.G + TILE - 1) / TILE, 0, (a.Tq - q0) * a.G};
+    const int rows = max(seq_start(a.cu_q, b + 1, a.B, a.Tq) - q0, 0) * a.G;
+    const int nk = max(seq_start(a.cu_k, b + 1, a.B, a.Tk) - seq_start(a.cu_k, b, a.B, a.Tk), 0);
+    return ListShape{(rows + TILE - 1) / TILE, (nk + BK - 1) / BK, rows};
+  }
+};
+// shared prefix: list 0 holds all rows of the batch against the prefix, list 1 + b sequence b's rows against its own cache
+struct SharedLists {
+  const FwdArgs& a;
+  __device__ __forceinline__ ListShape operator()(int i) const {
+    const int rows = (i == 0 ? a.B * a.n : a.n) * a.G;
+    const int nk = i == 0 ? a.P : min(max(a.lens[i - 1], 0), a.S);
+    return ListShape{(rows + TILE - 1) / TILE, (nk + BK - 1) / BK, rows};
+  }
+};
+
+// item w of a list: its job's tile and chunks, its partial
+__device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Ranges& r, int w, int D, bool always) {
+  const int i = w - r.item0, range = i % r.ranges;
+  j.t = i / r.ranges;
+  const int chunks = tile_chunks(a, j);
+  j.c0 = (int)((long long)chunks * range / r.ranges);
+  j.c1 = (int)((long long)chunks * (range + 1) / r.ranges);
+  j.part = r.ranges == 1 && !always ? nullptr : a.part + ((size_t)w * a.Hk + j.hk) * part_floats(D);
+}
+
+// grid: items * Hk, a token's heads on neighbouring workgroups
+template <int D, bool BIAS>
+__global__ __launch_bounds__(256, 2) void packed_ranges_kernel(FwdArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
+  __shared__ float stats[4 * 128];
+  __shared__ float tab[BIAS ? BIAS_ROWS : 1];
+  const int w = blockIdx.x / a.Hk;
+  const PackedLists lists{a};
+  const Ranges r = find_ranges<false>(a.B + 1, range_chunks(a, a.B + 1, lists), w, lists);
+  if (r.ranges == 0) return;
+  const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, r.list);
+  Job j;
+  j.hk = blockIdx.x - w * a.Hk;
+  j.k = a.k + ((size_t)s.k0 * a.Hk + j.hk) * D;
+  j.v = a.v + ((size_t)s.k0 * a.Hk + j.hk) * D;
+  j.q0 = s.q0;
+  j.nq = s.nq;
+  j.nk = s.nk;
+  j.causal = a.causal;
+  take_range(a, j, r, w, D, false);
+  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, j.hk);
+  run_tile<D, BIAS>(a, j, lds, stats, tab);
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void shared_prefix_kernel(FwdArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
+  __shared__ float stats[4 * 128];
+  const int w = blockIdx.x / a.Hk;
+  const SharedLists lists{a};
+  const Ranges r = find_ranges<false>(a.B + 1, range_chunks(a, a.B + 1, lists), w, lists);
+  if (r.ranges == 0) return;
+  Job j;
+  j.hk = blockIdx.x - w * a.Hk;
+  if (r.list == 0) {
+    j.k = a.kp + (size_t)j.hk * D;
+    j.v = a.vp + (size_t)j.hk * D;
+    j.q0 = 0;
+    j.nq = a.B * a.n;
+    j.nk = a.P;
+    j.causal = 0;
+  } else {
+    const int b = r.list - 1;
+    j.k = a.k + ((size_t)b * a.S * a.Hk + j.hk) * D;
+    j.v = a.v + ((size_t)b * a.S * a.Hk + j.hk) * D;
+    j.q0 = b * a.n;
+    j.nq = a.n;
+    j.nk = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
+    j.causal = 1;
+  }
+  take_range(a, j, r, w, D, true);
+  run_tile<D, false>(a, j, lds, stats, nullptr);
+}
+
+// O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's partials in order: D / 4 lanes a row. SHARED: a row's prefix
+// partials, then those of its own cache. Grid: (tile numbers * Hk, 4), rows in turn over the second index.
+template <int D, bool SHARED>
+__global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
+  constexpr int LPR = D / 4, RPB = 256 / LPR;
+  const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
+  int list, t, q0, nq, per;
+  Ranges own, pre = {0, 0, 0};
+  if (SHARED) {
+    const SharedLists lists{a};
+    const int tiles = (a.n * a.G + TILE - 1) / TILE;
+    list = 1 + w / tiles;
+    t = w % tiles;
+    q0 = (list - 1) * a.n;
+    nq = a.n;
+    per = range_chunks(a, a.B + 1, lists);
+    own = find_ranges<true>(a.B + 1, per, list, lists);
+    pre = find_ranges<true>(a.B + 1, per, 0, lists);
+  } else {
+    const PackedLists lists{a};
+    list = seq_of_tile<TILE>(a.cu_q, a.B, a.Tq, a.G, w);
+    const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, list);
+    q0 = s.q0;
+    nq = s.nq;
+    t = w - (q0 * a.G / TILE + list);
+    if (t < 0 || t * TILE >= nq * a.G) return;
+    per = range_chunks(a, a.B + 1, lists);
+    own = find_ranges<true>(a.B + 1, per, list, lists);
+    if (own.ranges == 1) return;  // (finished by its only range)
+  }
+  const int rows = min(nq * a.G - t * TILE, TILE), c = (threadIdx.x % LPR) * 4;
+  const size_t step = (size_t)a.Hk * part_floats(D);
+  const float* own0 = a.part + (size_t)(own.item0 + t * own.ranges) * step + (size_t)hk * part_floats(D);
+  for (int r = blockIdx.y * RPB + threadIdx.x / LPR; r < rows; r += gridDim.y * RPB) {
+    const float* pre0 = nullptr;
+    int rp = 0;
+    if (SHARED) {
+      const int all = q0 * a.G + t * TILE + r;  // the row among all rows of the batch
+      rp = all % TILE;
+      pre0 = a.part + (size_t)(all / TILE * pre.ranges) * step + (size_t)hk * part_floats(D);
+    }
+    float M = -INFINITY;
+    for (int i = 0; i < pre.ranges; ++i) M = fmaxf(M, pre0[i * step + TILE * D + rp]);
+    for (int i = 0; i < own.ranges; ++i) M = fmaxf(M, own0[i * step + TILE * D + r]);
+    f32x4 acc = {};
+    float sum = 0.0f;
+    auto add = [&](const float* p, int row) {
+      const float m = p[TILE * D + row];
+      const float f = m == -INFINITY ? 0.0f : exp2f_fast(m - M);
+      sum = fmaf(f, p[TILE * D + TILE + row], sum);
+      acc += f * *reinterpret_cast<const f32x4*>(p + row * D + c);
+    };
+    for (int i = 0; i < pre.ranges; ++i) add(pre0 + i * step, rp);
+    for (int i = 0; i < own.ranges; ++i) add(own0 + i * step, r);
+    const int row = t * TILE + r, tok = divide(a.div_g, row);
+    const size_t at = ((size_t)(q0 + tok) * a.Hk + hk) * a.G + (row - tok * a.G);
+    store_row<D>(a, at, c, acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
+    if (c == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (M - P_SHIFT + log2f(sum)) * PK_LN2;
+  }
+}
+
+}  // namespace
+
+}  // namespace es
+
+using namespace es;
+
+// Workgroups that the GPU holds at once: 256 CUs, two workgroups each at D = 128 (64 KB of staging), four at D = 64.
+static int resident(int D) { return D == 64 ? 1024 : 512; }
+// Items a head of a ranged launch: at most one a tile more than the ranges' chunks fill.
+static long long range_items(long long tiles, int Hk, int D) { return tiles + resident(D) / Hk + 1; }
+// Key ranges are worth a second launch where the tiles do not fill the GPU and the keys are more than a few chunks.
+static bool ranged(long long tiles, int Tk, int Hk, int D) { return tiles * Hk < 2 * resident(D) && Tk >= 16 * BK; }
+
+#ifndef ES_ELEM_F16
+extern "C" size_t es_packed_fwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D) {
+  if (B <= 0 || Tq <= 0 || Tk < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
+  const long long tiles = tile_numbers<TILE>(B, Tq, H / Hk);
+  return ranged(tiles, Tk, Hk, D) ? (size_t)range_items(tiles, Hk, D) * Hk * part_floats(D) * sizeof(float) : 0;
+}
+extern "C" size_t es_shared_prefix_workspace(int B, int n, int P, int S, int H, int Hk, int D) {
+  if (B <= 0 || n <= 0 || P < 0 || S < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
+  const long long G = H / Hk, rows = n * G, tiles = (B * rows + TILE - 1) / TILE + B * ((rows + TILE - 1) / TILE);
+  return (size_t)range_items(tiles, Hk, D) * Hk * part_floats(D) * sizeof(float);
+}
+#endif
+
+
+extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k,
+                                         const float* bias, const int* buckets, int num_buckets, int R, void* out,
+                                         float* lse, void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H,
+                                         int Hk, int D, int causal, float scale, hipStream_t stream) {
+  if (int st = packed_check(q, k, v, cu_q, cu_k, bias, buckets, num_buckets, R, B, Tq, Tk, H, Hk, D, scale)) return st;
+  if (Tq == 0) return ES_OK;
+  ES_REQUIRE(out && lse, ES_ERR_INVALID, "packed: null out / lse");
+  FwdArgs a = {};
+  a.q = (const e16_t*)q;
+  a.k = (const e16_t*)k;
+  a.v = (const e16_t*)v;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.bias = bias;
+  a.buckets = buckets;
+  a.num_buckets = num_buckets;
+  a.R = bias ? R : 0;
+  a.out = (e16_t*)out;
+  a.lse = lse;
+  a.B = B;
+  a.Tq = Tq;
+  a.Tk = Tk;
+  a.H = H;
+  a.Hk = Hk;
+  a.G = H / Hk;
+  a.div_g = fast_div(a.G);
+  a.causal = causal != 0;
+  a.scale = scale * LOG2E;
+  a.tiles = (int)tile_numbers<TILE>(B, Tq, a.G);
+  ES_REQUIRE((long long)a.tiles * Hk < (1LL << 31), ES_ERR_UNSUPPORTED, "packed: grid too large");
+  if (ranged(a.tiles, Tk, Hk, D)) {
+    ES_REQUIRE(workspace && workspace_bytes >= es_packed_fwd_workspace(B, Tq, Tk, H, Hk, D), ES_ERR_INVALID,
+               "packed: workspace too small");
+    a.part = (float*)workspace;
+    a.target = resident(D);
+    const dim3 grid((unsigned)(range_items(a.tiles, Hk, D) * Hk)), merge((unsigned)(a.tiles * Hk), 4);
+    if (D == 64) {
+      if (bias) hipLaunchKernelGGL((packed_ranges_kernel<64, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((packed_ranges_kernel<64, false>), grid, dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((merge_kernel<64, false>), merge, dim3(256), 0, stream, a);
+    } else {
+      if (bias) hipLaunchKernelGGL((packed_ranges_kernel<128, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((packed_ranges_kernel<128, false>), grid, dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((merge_kernel<128, false>), merge, dim3(256), 0, stream, a);
+    }
+    return check_launch("es_packed_fwd");
+  }
+  const dim3 grid((unsigned)(a.tiles * Hk));
+  if (D == 64) {
+    if (bias) hipLaunchKernelGGL((packed_fwd_kernel<64, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((packed_fwd_kernel<64, false>), grid, dim3(256), 0, stream, a);
+  } else {
+    if (bias) hipLaunchKernelGGL((packed_fwd_kernel<128, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((packed_fwd_kernel<128, false>), grid, dim3(256), 0, stream, a);
+  }
+  return check_launch("es_packed_fwd");
+}
+
+extern "C" int ES_VSA_API(es_shared_prefix_fwd)(const void* q, const void* k_prefix, const void* v_prefix, const void* k,
+                                                const void* v, const int* lens, void* out, float* lse, void* workspace,
+                                                size_t workspace_bytes, int B, int n, int P, int S, int H, int Hk, int D,
+                                                float scale, hipStream_t stream) {
+  ES_REQUIRE(B > 0 && n > 0 && P >= 0 && S >= 0, ES_ERR_INVALID, "shared prefix: B and n must be positive, P and S not negative");
+  ES_REQUIRE((long long)B * n < (1LL << 30) && S < (1 << 30), ES_ERR_UNSUPPORTED, "shared prefix: too many rows");
+  ES_REQUIRE(lens && out && lse && workspace && (S == 0 || (k && v)), ES_ERR_INVALID, "shared prefix: null tensor pointer");
+  if (int st = packed_check(q, k_prefix, v_prefix, nullptr, lens, nullptr, nullptr, 0, 0, B, B * n, P, H, Hk, D, scale))
+    return st;
+  ES_REQUIRE(workspace_bytes >= es_shared_prefix_workspace(B, n, P, S, H, Hk, D), ES_ERR_INVALID,
+             "shared prefix: workspace too small");
+  FwdArgs a = {};
+  a.q = (const e16_t*)q;
+  a.kp = (const e16_t*)k_prefix;
+  a.vp = (const e16_t*)v_prefix;
+  a.k = (const e16_t*)k;
+  a.v = (const e16_t*)v;
+  a.lens = lens;
+  a.out = (e16_t*)out;
+  a.lse = lse;
+  a.part = (float*)workspace;
+  a.B = B;
+  a.n = n;
+  a.P = P;
+  a.S = S;
+  a.H = H;
+  a.Hk = Hk;
+  a.G = H / Hk;
+  a.div_g = fast_div(a.G);
+  a.scale = scale * LOG2E;
+  a.target = resident(D);
+  const long long own = (long long)B * (((long long)n * a.G + TILE - 1) / TILE);
+  const long long tiles = ((long long)B * n * a.G + TILE - 1) / TILE + own;
+  ES_REQUIRE(range_items(tiles, Hk, D) * Hk < (1LL << 31), ES_ERR_UNSUPPORTED, "shared prefix: grid too large");
+  const dim3 grid((unsigned)(range_items(tiles, Hk, D) * Hk)), merge((unsigned)(own * Hk), 4);
+  if (D == 64) {
+    hipLaunchKernelGGL((shared_prefix_kernel<64>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((merge_kernel<64, true>), merge, dim3(256), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((shared_prefix_kernel<128>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((merge_kernel<128, true>), merge, dim3(256), 0, stream, a);
+  }
+  return check_launch("es_shared_prefix_fwd");
+}

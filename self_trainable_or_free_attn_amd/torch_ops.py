@@ -1,5 +1,5 @@
-"""Torch operator registration of the C ABI: every stream-taking entry point of include/echosparse_hip.h and
-include/vsa_hip.h becomes the operator torch.ops.echosparse_gfx950.<entry point>, with the header's argument names
+"""Torch operator registration of the C ABI: every stream-taking entry point of include/echosparse_hip.h,
+include/vsa_hip.h and include/packed_hip.h becomes the operator torch.ops.echosparse_gfx950.<entry point>, with the header's argument names
 and order (the stream is torch's current HIP stream of the tensors' device).
 
 The C++ registration (csrc/torch/ops.cpp) is generated from the headers, so the operator set can not drift from
@@ -29,7 +29,7 @@ import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-HEADERS = [os.path.join(ROOT, "include", h) for h in ("echosparse_hip.h", "vsa_hip.h")]
+HEADERS = [os.path.join(ROOT, "include", h) for h in ("echosparse_hip.h", "vsa_hip.h", "packed_hip.h")]
 SOURCE = os.path.join(HERE, "csrc", "torch", "ops.cpp")
 LIB = os.path.join(HERE, "lib", "libechosparse_torch.so")
 NAMESPACE = "echosparse_gfx950"
@@ -117,9 +117,10 @@ def source():
     """The generated C++ registration."""
     eps = entry_points()
     lines = [
-        "// Generated by self_trainable_or_free_attn_amd/torch_ops.py from include/echosparse_hip.h and",
-        "// include/vsa_hip.h: one torch operator per stream-taking C entry point. Do not edit by hand.",
+        "// Generated by self_trainable_or_free_attn_amd/torch_ops.py from include/echosparse_hip.h, include/vsa_hip.h and",
+        "// include/packed_hip.h: one torch operator per stream-taking C entry point. Do not edit by hand.",
         '#include "../../../include/vsa_hip.h"',
+        '#include "../../../include/packed_hip.h"',
         "",
         "#include <ATen/core/Tensor.h>",
         "#include <c10/core/DeviceGuard.h>",
