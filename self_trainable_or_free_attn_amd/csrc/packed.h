@@ -61,6 +61,32 @@ __host__ __device__ __forceinline__ long long tile_numbers(int B, int T, int G) 
   return (long long)T * G / M + B + 1;
 }
 
+// Tile number w of a launch without ranges: the sequences in descending order of weight(b), so that the tiles with the most
+// work start first and those that start last are short (workgroups are dispatched in order), each with its tiles(b) tiles.
+// Up to 64 sequences (the rows behind the last one included): each lane takes one and adds up the tiles of those before it.
+// More: their own order, by seq_of_tile. false: no tile has this number.
+template <int M, class TILES, class WEIGHT>
+__device__ __forceinline__ bool tile_of(const int* cu, int B, int T, int G, int w, const TILES& tiles, const WEIGHT& weight,
+                                        int& b, int& t) {
+  if (B < 64) {
+    const int l = lane_id();
+    const int mine = l <= B ? tiles(l) : 0, heavy = l <= B ? weight(l) : -1;
+    int base = 0;
+    for (int j = 0; j <= B; ++j) {
+      const int tj = __builtin_amdgcn_readlane(mine, j), hj = __builtin_amdgcn_readlane(heavy, j);
+      base += hj > heavy || (hj == heavy && j < l) ? tj : 0;
+    }
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(l <= B && base <= w && w < base + mine);
+    if (hit == 0) return false;
+    b = __builtin_ctzll(hit);
+    t = w - __builtin_amdgcn_readlane(base, b);
+    return true;
+  }
+  b = seq_of_tile<M>(cu, B, T, G, w);
+  t = w - (__builtin_amdgcn_readfirstlane(seq_start(cu, b, B, T)) * G / M + b);
+  return t >= 0 && t < __builtin_amdgcn_readfirstlane(tiles(b));
+}
+
 struct Seq {
   int q0, nq, k0, nk;
 };
@@ -76,6 +102,15 @@ __device__ __forceinline__ Seq sequence(const int* cu_q, const int* cu_k, int B,
   s.nq = max(__builtin_amdgcn_readfirstlane(seq_start(cu_q, b + 1, B, Tq)) - s.q0, 0);
   s.nk = max(__builtin_amdgcn_readfirstlane(seq_start(cu_k, b + 1, B, Tk)) - s.k0, 0);
   return s;
+}
+
+// rows of the list of sequence b (b == B: the rows behind the last sequence), and its keys
+__device__ __forceinline__ int list_rows(const int* cu_q, int B, int Tq, int G, int b) {
+  const int q0 = seq_start(cu_q, b, B, Tq);
+  return b >= B ? (Tq - q0) * G : max(seq_start(cu_q, b + 1, B, Tq) - q0, 0) * G;
+}
+__device__ __forceinline__ int list_keys(const int* cu_k, int B, int Tk, int b) {
+  return b >= B ? 0 : max(seq_start(cu_k, b + 1, B, Tk) - seq_start(cu_k, b, B, Tk), 0);
 }
 
 // Tiles of D-column rows in LDS, 16-byte chunks XOR-swizzled so that sixteen consecutive rows read at one chunk, and four

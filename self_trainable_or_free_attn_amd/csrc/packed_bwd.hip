@@ -3,14 +3,20 @@
 // With P = exp(S - lse) and dS = P (dP - delta), dP = dO V^T, delta = rowsum(dO O) (rows that see no key: P = 0):
 //   row_stats   one pass over dO and O: lse in log2 units (+inf for rows without keys) and delta, laid out by kv head and
 //               row of the list (token, head in group), so that a row tile's values are contiguous
+//   bwd_q       one workgroup per (64 rows, kv head): dQ = scale dS K over the keys, 2 row groups x 2 key halves, S^T and
+//               dP^T with rows on lanes; with a bias it also sums dS by clamped distance
 //   bwd_kv      one workgroup per (64 keys, kv head): dV = P^T dO and dK = scale dS^T Q over all rows of the list that see
 //               the keys, which sums over the heads of a group without atomics. Four waves = 2 key halves x 2 row halves
 //               of each staged 64-row tile; S and dP come out with keys on lanes, so that P and dS are B operands.
-//   bwd_q       one workgroup per (64 rows, kv head): dQ = scale dS K over the keys, 2 row groups x 2 key halves, S^T and
-//               dP^T with rows on lanes; with a bias it also sums dS by clamped distance
 //   bias_sums   those sums over the row tiles and into buckets
 // Every sum has a fixed order, so the same inputs give the same bits. The scores are computed twice (7 products for 5): a
 // single pass would need dQ in float32 atomics or a dQ partial a key tile.
+// delta: O carries the roundings of its probabilities and its own, so rowsum(dO O) is off by up to 2^-8 (bf16) of |dO| |O|,
+// the same for all keys of a row. Over n keys of about equal weight that shifts a row's dQ by 1 / sqrt(n) of what the
+// rounding of dS does, but with few keys it adds to it, and sums of unrounded dS (the bias gradient) have no other error.
+// So bwd_q takes delta = sum P dP / sum P over the keys in a pass of its own before the main one where a tile sees up to
+// EXACT_CHUNKS * 64 keys, and always with a bias, and stores it for bwd_kv, which runs after it. (Relative errors of dQ
+// against 64 bits, causal prompts of 1 to 6553 tokens in bf16: 2.6e-3 -> 2.4e-3; of the bias gradient 1e-3 -> 1e-6.)
 // dS is rounded to the token type without the softmax scale (applied to the finished sums), which keeps it about ten times
 // further from the subnormal range of fp16.
 #include "packed.h"
@@ -26,6 +32,7 @@ constexpr float P_SHIFT = 14.0f, P_BACK = 1.0f / 16384.0f;
 #else
 constexpr float P_SHIFT = 0.0f, P_BACK = 1.0f;
 #endif
+constexpr int EXACT_CHUNKS = 8;
 
 struct BwdArgs {
   const e16_t *q, *k, *v, *dout, *out;
@@ -40,6 +47,11 @@ struct BwdArgs {
   int q_tiles, k_tiles;  // tile numbers of a head
   float scale_log2, scale;
 };
+
+// *p += x without waiting for it (ds_add_f32); lanes of one instruction must not share an address where order matters
+__device__ __forceinline__ void lds_add(float* p, float x) {
+  __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float*)p, x, 0, 0, false);
+}
 
 // D / 8 lanes a row of dO and O
 template <int D>
@@ -71,14 +83,15 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
   __shared__ __attribute__((aligned(16))) int gb_s[BIAS ? 2 : 1][BIAS ? BK : 1];  // the row's part of the bias table
   __shared__ float lse_s[BK];                                           // the next tile's lse2 as stored
   __shared__ float tab[BIAS ? BIAS_ROWS : 1];
-  const int hk = blockIdx.x / a.k_tiles, w = blockIdx.x - hk * a.k_tiles;
-  const int b = seq_of_tile<BK>(a.cu_k, a.B, a.Tk, 1, w);
+  const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
+  int b, kb;
+  if (!tile_of<BK>(a.cu_k, a.B, a.Tk, 1, w, [&](int i) { return (list_rows(a.cu_k, a.B, a.Tk, 1, i) + BK - 1) / BK; },
+                   [&](int i) { return i >= a.B ? 0 : list_rows(a.cu_q, a.B, a.Tq, a.G, i); }, b, kb))
+    return;
   Seq s;
   s.k0 = __builtin_amdgcn_readfirstlane(seq_start(a.cu_k, b, a.B, a.Tk));
   const int kend = b >= a.B ? a.Tk : __builtin_amdgcn_readfirstlane(seq_start(a.cu_k, b + 1, a.B, a.Tk));
   s.nk = max(kend - s.k0, 0);
-  const int kb = w - (s.k0 / BK + b);
-  if (kb < 0 || kb * BK >= s.nk) return;
   s.q0 = 0;
   s.nq = 0;  // (key rows behind the last sequence: zero gradients)
   if (b < a.B) {
@@ -255,18 +268,20 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
   __shared__ __attribute__((aligned(16))) char kv_s[2][2][TILE_BYTES];
   __shared__ float tab[BIAS ? BIAS_ROWS : 1];
-  __shared__ float hist[BIAS ? 4 : 1][BIAS ? BIAS_ROWS : 1];  // per wave: dS by (head in group, clamped distance)
-  const int hk = blockIdx.x / a.q_tiles, w = a.q_tiles - 1 - (blockIdx.x - hk * a.q_tiles);
-  const int b = seq_of_tile<BK>(a.cu_q, a.B, a.Tq, a.G, w);
-  const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, b);
-  const int t = w - (s.q0 * a.G / BK + b), rows = s.nq * a.G, shift = s.nk - s.nq, width = 2 * a.R + 1;
-  const bool none = t < 0 || t * BK >= rows;
+  // per wave: dS by (head in group, clamped distance); before the main pass (sum P dP, sum P) of its 32 rows
+  __shared__ __attribute__((aligned(8))) float hist[4][BIAS ? BIAS_ROWS : 64];
+  const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk, width = 2 * a.R + 1;
   float* dist = BIAS ? a.dist + ((size_t)w * a.Hk + hk) * (a.G * width) : nullptr;
-  if (none) {
+  int b, t;
+  if (!tile_of<BK>(a.cu_q, a.B, a.Tq, a.G, w, [&](int i) { return (list_rows(a.cu_q, a.B, a.Tq, a.G, i) + BK - 1) / BK; },
+                   [&](int i) { return list_keys(a.cu_k, a.B, a.Tk, i); }, b, t)) {
     if (BIAS)  // (a tile number without a tile: its sums are read all the same)
       for (int i = threadIdx.x; i < a.G * width; i += 256) dist[i] = 0.0f;
     return;
   }
+  const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, b);
+  const int rows = s.nq * a.G, shift = s.nk - s.nq;
+  t = (rows + BK - 1) / BK - 1 - t;  // (under a causal mask the last tiles see the most keys)
   const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rg = wv & 1, kh = wv >> 1;
@@ -292,11 +307,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     dreg[ks] = valid ? *reinterpret_cast<const ev8*>(a.dout + at + 16 * ks + 8 * hi) : z;
   }
   const float ls = valid ? a.lse2[list] : INFINITY;
-  const float dl = valid ? a.delta[list] : 0.0f;
-  if (BIAS) {
-    for (int i = tid; i < 4 * BIAS_ROWS; i += 256) (&hist[0][0])[i] = 0.0f;
-    fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
-  }
+  float dl = valid ? a.delta[list] : 0.0f;
+  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
 
   const unsigned stride = (unsigned)a.Hk * ROW;
   unsigned src[NI];
@@ -327,44 +339,82 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
   for (int db = 0; db < NDB; ++db) dq[db] = f32x16{};
   float far_lo = 0.0f, far_hi = 0.0f;  // dS at distances of -R and below, of R and beyond
 
+  // P and dP of keys key0 .. key0 + 31 (near: by distance, neither all at -R and below nor all at R and beyond)
+  auto scores = [&](const char* kt, const char* vt, int key0, f32x16& x, f32x16& dp, bool& near) {
+    x = f32x16{};
+    dp = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) x = emfma(elds16(kt, koff ^ (32 * ks)), qreg[ks], x);
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(vt, koff ^ (32 * ks)), dreg[ks], dp);
+    const int d0 = key0 + 4 * hi - pos;
+    float sc = a.scale_log2, cb = 0.0f;
+    near = false;
+    if (BIAS) {
+      if (key0 - high >= a.R) cb = tab[gb + a.R];
+      else if (key0 + 31 - low <= -a.R) cb = tab[gb - a.R];
+      else near = true;
+    }
+    if (near) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], sc, tab[gb + min(max(d0 + 8 * (r / 4) + r % 4, -a.R), a.R)]);
+      sc = 1.0f;
+    }
+    if (key0 + 32 > seen_min) {
+      const int left = seen - key0 - 4 * hi;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r / 4) + r % 4 >= left) x[r] = -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = exp2f_fast(fmaf(x[r], sc, cb - ls));
+  };
   if (end > 0) issue(0, 0);
   dma_wait();
   __syncthreads();
+  int sb = 0;
+  if (end > 0 && (BIAS || end <= EXACT_CHUNKS)) {
+    float num = 0.0f, den = 0.0f;
+    for (int c = 0; c < end; ++c) {
+      issue(c + 1 < end ? c + 1 : 0, sb ^ 1);  // (after the last chunk the first one again, for the main pass)
+      if (c * BK + 32 * kh < seen_max) {
+        f32x16 p, dp;
+        bool near;
+        scores(kv_s[sb][0], kv_s[sb][1], c * BK + 32 * kh, p, dp, near);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          num = fmaf(p[r], dp[r], num);
+          den += p[r];
+        }
+      }
+      sb ^= 1;
+      dma_wait();
+      __syncthreads();
+    }
+    reinterpret_cast<float2*>(hist[wv])[lq] = make_float2(sum_xor32(num), sum_xor32(den));
+    __syncthreads();
+    const float2 s0 = reinterpret_cast<const float2*>(hist[rg])[lq], s1 = reinterpret_cast<const float2*>(hist[rg + 2])[lq];
+    if (s0.y + s1.y > 0.0f) dl = (s0.x + s1.x) / (s0.y + s1.y);
+    if (valid && kh == 0 && hi == 0) a.delta[list] = dl;
+  }
+  if (BIAS) {
+    __syncthreads();
+    for (int i = tid; i < 4 * BIAS_ROWS; i += 256) (&hist[0][0])[i] = 0.0f;
+    __syncthreads();
+  }
   for (int c = 0; c < end; ++c) {
-    const int sb = c & 1;
     if (c + 1 < end) issue(c + 1, sb ^ 1);
     const char* kt = kv_s[sb][0];
     const char* vt = kv_s[sb][1];
     const int key0 = c * BK + 32 * kh;
     if (key0 < seen_max) {
-      f32x16 x = {}, dp = {};
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) x = emfma(elds16(kt, koff ^ (32 * ks)), qreg[ks], x);
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(vt, koff ^ (32 * ks)), dreg[ks], dp);
-      float ds[16];
+      f32x16 x, dp;
+      bool near;
+      scores(kt, vt, key0, x, dp, near);
       const int d0 = key0 + 4 * hi - pos;
-      bool near = false;
-      float cb = 0.0f;
-      if (BIAS) {
-        if (key0 - high >= a.R) cb = tab[gb + a.R];
-        else if (key0 + 31 - low <= -a.R) cb = tab[gb - a.R];
-        else near = true;
-      }
-      float sc = a.scale_log2;
-      if (near) {
+      float ds[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], sc, tab[gb + min(max(d0 + 8 * (r / 4) + r % 4, -a.R), a.R)]);
-        sc = 1.0f;
-      }
-      if (key0 + 32 > seen_min) {
-        const int left = seen - key0 - 4 * hi;
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (8 * (r / 4) + r % 4 >= left) x[r] = -INFINITY;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] = exp2f_fast(fmaf(x[r], sc, cb - ls)) * (dp[r] - dl);
+      for (int r = 0; r < 16; ++r) ds[r] = x[r] * (dp[r] - dl);
       if (BIAS) {
         if (!near) {
           float sum = 0.0f;
@@ -374,18 +424,19 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
           else far_lo += sum;
         } else {
           // One key of the run a step: the 32 rows of a half wave stand at different distances or in different heads, so
-          // no two lanes of a half add to one entry; the halves go one after the other, which fixes the order.
-          float* h = hist[wv];
+          // no two lanes of a half add to one entry; the halves go one after the other, and a wave's LDS operations are
+          // done in order: the sums have a fixed order without waiting for each.
+          float* h = hist[wv] + gb + d0;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int d = d0 + 8 * (r / 4) + r % 4;
-            if (d <= -a.R) far_lo += ds[r];
-            else if (d >= a.R) far_hi += ds[r];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              if (hi == half && valid && d > -a.R && d < a.R) h[gb + d] += ds[r];
-              __builtin_amdgcn_wave_barrier();
-            }
+            const int e = 8 * (r / 4) + r % 4, d = d0 + e;
+            far_lo += d <= -a.R ? ds[r] : 0.0f;
+            far_hi += d >= a.R && d > -a.R ? ds[r] : 0.0f;
+            const bool in = valid && d > -a.R && d < a.R;
+            if (in && hi == 0) lds_add(h + e, ds[r]);
+            __builtin_amdgcn_wave_barrier();  // (keeps the compiler from making one instruction of the two)
+            if (in && hi == 1) lds_add(h + e, ds[r]);
+            __builtin_amdgcn_wave_barrier();
           }
         }
       }
@@ -397,44 +448,31 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
         dq[db] = emfma(ecat_tr(lds_read_tr(kt + TILE_BYTES / 4, t0), lds_read_tr(kt + TILE_BYTES / 4, t1)), sb8, dq[db]);
       }
     }
+    sb ^= 1;
     dma_wait();
     __syncthreads();
   }
 
-  // the second key half hands its sums over through the staging buffers; with a bias the far sums follow
+  if (BIAS) {  // the far sums of the wave's rows, head by head
+    for (int i = 0; i < a.G; ++i) {
+      const float lo = wave_sum_dpp(valid && g == i ? far_lo : 0.0f), up = wave_sum_dpp(valid && g == i ? far_hi : 0.0f);
+      if (l == 0) {
+        hist[wv][i * width] += lo;
+        hist[wv][i * width + 2 * a.R] += up;
+      }
+    }
+  }
+  // the second key half hands its sums over through the staging buffers
   float* xq = reinterpret_cast<float*>(&kv_s[0][0][0]) + rg * (NDB * 16 * 64);
-  float* far = reinterpret_cast<float*>(&kv_s[1][0][0]);  // [wave][low | high][lane]
   if (kh == 1) {
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) xq[(db * 16 + r) * 64 + l] = dq[db][r];
   }
-  if (BIAS) {
-    far[wv * 128 + l] = valid ? far_lo : 0.0f;
-    far[wv * 128 + 64 + l] = valid ? far_hi : 0.0f;
-  }
   __syncthreads();
-  if (BIAS) {
-    for (int i = tid; i < a.G * width; i += 256) {
-      const int gi = i / width, d = i - gi * width - a.R;
-      float sum = 0.0f;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) sum += hist[x][i];
-      if (d == -a.R || d == a.R) {
-        // (R = 0: one entry, which takes both)
-        for (int x = 0; x < 4; ++x) {
-          for (int n = 0; n < 64; ++n) {
-            const int rr = t * BK + 32 * (x & 1) + (n & 31);
-            if (rr - divide(a.div_g, rr) * a.G != gi) continue;
-            if (d == -a.R) sum += far[x * 128 + n];
-            if (d == a.R) sum += far[x * 128 + 64 + n];
-          }
-        }
-      }
-      dist[i] = sum;
-    }
-  }
+  if (BIAS)
+    for (int i = tid; i < a.G * width; i += 256) dist[i] = (hist[0][i] + hist[1][i]) + (hist[2][i] + hist[3][i]);
   if (kh == 1 || !valid) return;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
@@ -449,24 +487,30 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     }
 }
 
-// dbias[n][h] = sum over the row tiles and over the distances of bucket n: one workgroup a head, a distance a thread, then a
-// bucket a thread
-__global__ __launch_bounds__(256) void bias_sums_kernel(BwdArgs a) {
-  __shared__ float sums[BIAS_ROWS];
+// dbias[n][h] = sum over the row tiles and over the distances of bucket n: one workgroup a head. First each of four slices of
+// 256 lanes adds every fourth tile, a distance a lane, eight tiles in flight; then a wave adds up a bucket's distances.
+__global__ __launch_bounds__(1024) void bias_sums_kernel(BwdArgs a) {
+  __shared__ float sums[4][BIAS_ROWS];
+  __shared__ int which[BIAS_ROWS];
   const int h = blockIdx.x, hk = divide(a.div_g, h), g = h - hk * a.G, width = 2 * a.R + 1;
+  const int slice = threadIdx.x >> 8, x = threadIdx.x & 255;
   const size_t step = (size_t)a.Hk * a.G * width;
-  for (int d = threadIdx.x; d < width; d += 256) {
+  for (int d = x; d < width; d += 256) {
     const float* p = a.dist + ((size_t)hk * a.G + g) * width + d;
-    float sum = 0.0f;
-    for (int w = 0; w < a.q_tiles; ++w) sum += p[w * step];
-    sums[d] = sum;
+    float sum[8] = {};
+    for (int w = slice; w < a.q_tiles; w += 32)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += w + 4 * e < a.q_tiles ? p[(w + 4 * e) * step] : 0.0f;
+    sums[slice][d] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+    if (slice == 0) which[d] = min(max(a.buckets[d], 0), a.num_buckets - 1);
   }
   __syncthreads();
-  for (int n = threadIdx.x; n < a.num_buckets; n += 256) {
+  for (int n = threadIdx.x >> 6; n < a.num_buckets; n += 16) {
     float sum = 0.0f;
-    for (int d = 0; d < width; ++d)
-      if (min(max(a.buckets[d], 0), a.num_buckets - 1) == n) sum += sums[d];
-    a.dbias[(size_t)n * a.H + h] = sum;
+    for (int d = threadIdx.x & 63; d < width; d += 64)
+      if (which[d] == n) sum += (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
+    sum = wave_sum_dpp(sum);
+    if ((threadIdx.x & 63) == 0) a.dbias[(size_t)n * a.H + h] = sum;
   }
 }
 
@@ -538,16 +582,6 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
     if (D == 64) hipLaunchKernelGGL((row_stats_kernel<64>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((row_stats_kernel<128>), grid, dim3(256), 0, stream, a);
   }
-  if (Tk > 0) {
-    const dim3 grid((unsigned)(a.k_tiles * Hk));
-    if (D == 64) {
-      if (bias) hipLaunchKernelGGL((packed_bwd_kv_kernel<64, true>), grid, dim3(256), 0, stream, a);
-      else hipLaunchKernelGGL((packed_bwd_kv_kernel<64, false>), grid, dim3(256), 0, stream, a);
-    } else {
-      if (bias) hipLaunchKernelGGL((packed_bwd_kv_kernel<128, true>), grid, dim3(256), 0, stream, a);
-      else hipLaunchKernelGGL((packed_bwd_kv_kernel<128, false>), grid, dim3(256), 0, stream, a);
-    }
-  }
   if (Tq > 0) {
     const dim3 grid((unsigned)(a.q_tiles * Hk));
     if (D == 64) {
@@ -558,9 +592,19 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
       else hipLaunchKernelGGL((packed_bwd_q_kernel<128, false>), grid, dim3(256), 0, stream, a);
     }
   }
+  if (Tk > 0) {
+    const dim3 grid((unsigned)(a.k_tiles * Hk));
+    if (D == 64) {
+      if (bias) hipLaunchKernelGGL((packed_bwd_kv_kernel<64, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((packed_bwd_kv_kernel<64, false>), grid, dim3(256), 0, stream, a);
+    } else {
+      if (bias) hipLaunchKernelGGL((packed_bwd_kv_kernel<128, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((packed_bwd_kv_kernel<128, false>), grid, dim3(256), 0, stream, a);
+    }
+  }
   if (bias) {
     if (Tq == 0) a.q_tiles = 0;
-    hipLaunchKernelGGL(bias_sums_kernel, dim3((unsigned)H), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(bias_sums_kernel, dim3((unsigned)H), dim3(1024), 0, stream, a);
   }
   return check_launch("es_packed_bwd");
 }

@@ -371,19 +371,22 @@ __device__ __forceinline__ void run_tile(const FwdArgs& a, const Job& j, char* l
   else wide_tile<D, BIAS>(a, j, lds, tab);
 }
 
-// whole tiles: grid tiles * Hk, a head's tiles on neighbouring workgroups (so on all XCDs), the last ones, which under a
-// causal mask see the most keys, first
+// whole tiles: grid tiles * Hk, a tile's heads on neighbouring workgroups (workgroup i runs on XCD i % 8: with eight kv heads
+// each XCD's L2 then holds one head's keys); under a causal mask a sequence's last tiles, which see the most keys, first
 template <int D, bool BIAS>
-__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_fwd_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
   __shared__ float stats[4 * 128];
   __shared__ float tab[BIAS ? BIAS_ROWS : 1];
-  const int hk = blockIdx.x / a.tiles, w = a.tiles - 1 - (blockIdx.x - hk * a.tiles);
-  const int b = seq_of_tile<TILE>(a.cu_q, a.B, a.Tq, a.G, w);
-  const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, b);
+  const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
+  int b;
   Job j;
-  j.t = w - (s.q0 * a.G / TILE + b);
-  if (j.t < 0 || j.t * TILE >= s.nq * a.G) return;
+  if (!tile_of<TILE>(a.cu_q, a.B, a.Tq, a.G, w,
+                     [&](int i) { return (list_rows(a.cu_q, a.B, a.Tq, a.G, i) + TILE - 1) / TILE; },
+                     [&](int i) { return list_keys(a.cu_k, a.B, a.Tk, i); }, b, j.t))
+    return;
+  const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, b);
+  j.t = (s.nq * a.G + TILE - 1) / TILE - 1 - j.t;
   j.k = a.k + ((size_t)s.k0 * a.Hk + hk) * D;
   j.v = a.v + ((size_t)s.k0 * a.Hk + hk) * D;
   j.q0 = s.q0;
@@ -417,62 +420,65 @@ __device__ __forceinline__ int ranges_of(const ListShape& x, int per) {
   return max((x.chunks + least - 1) / least, 1);
 }
 
-// chunks of a range before the two lower limits
+// The shapes of the lists, a lane each; up to 64 are read once.
 template <class F>
-__device__ __forceinline__ int range_chunks(const FwdArgs& a, int lists, const F& shape) {
-  unsigned long long sum = 0;
-  for (int i0 = 0; i0 < lists; i0 += 64) {
-    const int i = i0 + lane_id();
-    if (i < lists) {
-      const ListShape x = shape(i);
+struct Lists {
+  const F& shape;
+  int lists;
+  ListShape mine;
+  __device__ __forceinline__ Lists(const F& f, int n) : shape(f), lists(n), mine{0, 0, 0} {
+    if (lane_id() < n) mine = f(lane_id());
+  }
+  __device__ __forceinline__ ListShape at(int i0) const {
+    if (i0 == 0) return mine;
+    return i0 + lane_id() < lists ? shape(i0 + lane_id()) : ListShape{0, 0, 0};
+  }
+
+  // chunks of a range before the two lower limits
+  __device__ __forceinline__ int range_chunks(const FwdArgs& a) const {
+    unsigned long long sum = 0;
+    for (int i0 = 0; i0 < lists; i0 += 64) {
+      const ListShape x = at(i0);
       sum += (unsigned long long)x.tiles * x.chunks;
     }
-  }
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
-  return (int)min((sum * a.Hk + a.target - 1) / a.target, 1ull << 30);
-}
+    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+    return (int)min((sum * a.Hk + a.target - 1) / a.target, 1ull << 30);
+  }
 
-// the list that holds item w (BY_LIST: the list w); ranges = 0: none
-template <bool BY_LIST, class F>
-__device__ __forceinline__ Ranges find_ranges(int lists, int per, int w, const F& shape) {
-  int base = 0;
-  for (int i0 = 0; i0 < lists; i0 += 64) {
-    const int i = i0 + lane_id();
-    int items = 0, ranges = 0;
-    if (i < lists) {
-      const ListShape x = shape(i);
-      ranges = ranges_of(x, per);
-      items = x.tiles * ranges;
-    }
-    int upto = items;
+  // the list that holds item w (BY_LIST: the list w); ranges = 0: none
+  template <bool BY_LIST>
+  __device__ __forceinline__ Ranges find(int per, int w) const {
+    int base = 0;
+    for (int i0 = 0; i0 < lists; i0 += 64) {
+      const ListShape x = at(i0);
+      const int i = i0 + lane_id(), ranges = i < lists ? ranges_of(x, per) : 0, items = x.tiles * ranges;
+      int upto = items;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int y = __shfl_up(upto, m, 64);
-      if (lane_id() >= m) upto += y;
+      for (int m = 1; m < 64; m <<= 1) {
+        const int y = __shfl_up(upto, m, 64);
+        if (lane_id() >= m) upto += y;
+      }
+      const unsigned long long hit = __builtin_amdgcn_ballot_w64(BY_LIST ? i == w : base + upto > w);
+      if (hit) {
+        const int from = __builtin_ctzll(hit);
+        Ranges r;
+        r.list = i0 + from;
+        r.ranges = __builtin_amdgcn_readlane(ranges, from);
+        r.item0 = base + __builtin_amdgcn_readlane(upto - items, from);
+        return r;
+      }
+      base += __builtin_amdgcn_readlane(upto, 63);
     }
-    const unsigned long long hit = __builtin_amdgcn_ballot_w64(BY_LIST ? i == w : base + upto > w);
-    if (hit) {
-      const int from = __builtin_ctzll(hit);
-      Ranges r;
-      r.list = i0 + from;
-      r.ranges = __builtin_amdgcn_readlane(ranges, from);
-      r.item0 = base + __builtin_amdgcn_readlane(upto - items, from);
-      return r;
-    }
-    base += __builtin_amdgcn_readlane(upto, 63);
+    return Ranges{0, 0, 0};
   }
-  return Ranges{0, 0, 0};
-}
+};
 
 // packed sequences: list b, the rows behind the last sequence being list B
 struct PackedLists {
   const FwdArgs& a;
   __device__ __forceinline__ ListShape operator()(int b) const {
-    const int q0 = seq_start(a.cu_q, b, a.B, a.Tq);
-    if (b >= a.B) return ListShape{((a.Tq - q0) * a.G + TILE - 1) / TILE, 0, (a.Tq - q0) * a.G};
-    const int rows = max(seq_start(a.cu_q, b + 1, a.B, a.Tq) - q0, 0) * a.G;
-    const int nk = max(seq_start(a.cu_k, b + 1, a.B, a.Tk) - seq_start(a.cu_k, b, a.B, a.Tk), 0);
+    const int rows = list_rows(a.cu_q, a.B, a.Tq, a.G, b), nk = list_keys(a.cu_k, a.B, a.Tk, b);
     return ListShape{(rows + TILE - 1) / TILE, (nk + BK - 1) / BK, rows};
   }
 };
@@ -498,13 +504,14 @@ __device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Range
 
 // grid: items * Hk, a token's heads on neighbouring workgroups
 template <int D, bool BIAS>
-__global__ __launch_bounds__(256, 2) void packed_ranges_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_ranges_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
   __shared__ float stats[4 * 128];
   __shared__ float tab[BIAS ? BIAS_ROWS : 1];
   const int w = blockIdx.x / a.Hk;
-  const PackedLists lists{a};
-  const Ranges r = find_ranges<false>(a.B + 1, range_chunks(a, a.B + 1, lists), w, lists);
+  const PackedLists shape{a};
+  const Lists<PackedLists> lists(shape, a.B + 1);
+  const Ranges r = lists.find<false>(lists.range_chunks(a), w);
   if (r.ranges == 0) return;
   const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, r.list);
   Job j;
@@ -521,12 +528,13 @@ __global__ __launch_bounds__(256, 2) void packed_ranges_kernel(FwdArgs a) {
 }
 
 template <int D>
-__global__ __launch_bounds__(256, 2) void shared_prefix_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void shared_prefix_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
   __shared__ float stats[4 * 128];
   const int w = blockIdx.x / a.Hk;
-  const SharedLists lists{a};
-  const Ranges r = find_ranges<false>(a.B + 1, range_chunks(a, a.B + 1, lists), w, lists);
+  const SharedLists shape{a};
+  const Lists<SharedLists> lists(shape, a.B + 1);
+  const Ranges r = lists.find<false>(lists.range_chunks(a), w);
   if (r.ranges == 0) return;
   Job j;
   j.hk = blockIdx.x - w * a.Hk;
@@ -550,60 +558,77 @@ __global__ __launch_bounds__(256, 2) void shared_prefix_kernel(FwdArgs a) {
   run_tile<D, false>(a, j, lds, stats, nullptr);
 }
 
-// O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's partials in order: D / 4 lanes a row. SHARED: a row's prefix
-// partials, then those of its own cache. Grid: (tile numbers * Hk, 4), rows in turn over the second index.
+// O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's partials in order: D / 4 lanes a row, which first take one
+// partial's m and l each and then, eight partials in flight, four channels each. SHARED: a row's prefix partials, then those
+// of its own cache. Grid: (tile numbers * Hk, 4), rows in turn over the second index.
 template <int D, bool SHARED>
 __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
   constexpr int LPR = D / 4, RPB = 256 / LPR;
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
-  int list, t, q0, nq, per;
+  int list, t, q0, nq;
   Ranges own, pre = {0, 0, 0};
   if (SHARED) {
-    const SharedLists lists{a};
     const int tiles = (a.n * a.G + TILE - 1) / TILE;
     list = 1 + w / tiles;
     t = w % tiles;
     q0 = (list - 1) * a.n;
     nq = a.n;
-    per = range_chunks(a, a.B + 1, lists);
-    own = find_ranges<true>(a.B + 1, per, list, lists);
-    pre = find_ranges<true>(a.B + 1, per, 0, lists);
+    if (t * TILE + (int)blockIdx.y * RPB >= nq * a.G) return;
+    const SharedLists shape{a};
+    const Lists<SharedLists> lists(shape, a.B + 1);
+    const int per = lists.range_chunks(a);
+    own = lists.find<true>(per, list);
+    pre = lists.find<true>(per, 0);
   } else {
-    const PackedLists lists{a};
     list = seq_of_tile<TILE>(a.cu_q, a.B, a.Tq, a.G, w);
     const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, list);
     q0 = s.q0;
     nq = s.nq;
     t = w - (q0 * a.G / TILE + list);
-    if (t < 0 || t * TILE >= nq * a.G) return;
-    per = range_chunks(a, a.B + 1, lists);
-    own = find_ranges<true>(a.B + 1, per, list, lists);
+    if (t < 0 || t * TILE + (int)blockIdx.y * RPB >= nq * a.G) return;
+    const PackedLists shape{a};
+    const Lists<PackedLists> lists(shape, a.B + 1);
+    own = lists.find<true>(lists.range_chunks(a), list);
     if (own.ranges == 1) return;  // (finished by its only range)
   }
-  const int rows = min(nq * a.G - t * TILE, TILE), c = (threadIdx.x % LPR) * 4;
+  const int rows = min(nq * a.G - t * TILE, TILE), lane = threadIdx.x % LPR, c = lane * 4, n = pre.ranges + own.ranges;
   const size_t step = (size_t)a.Hk * part_floats(D);
   const float* own0 = a.part + (size_t)(own.item0 + t * own.ranges) * step + (size_t)hk * part_floats(D);
   for (int r = blockIdx.y * RPB + threadIdx.x / LPR; r < rows; r += gridDim.y * RPB) {
-    const float* pre0 = nullptr;
-    int rp = 0;
-    if (SHARED) {
-      const int all = q0 * a.G + t * TILE + r;  // the row among all rows of the batch
-      rp = all % TILE;
-      pre0 = a.part + (size_t)(all / TILE * pre.ranges) * step + (size_t)hk * part_floats(D);
-    }
+    const int all = q0 * a.G + t * TILE + r, rp = SHARED ? all % TILE : 0;  // the row among all rows of the batch
+    const float* pre0 = SHARED ? a.part + (size_t)(all / TILE * pre.ranges) * step + (size_t)hk * part_floats(D) : nullptr;
+    auto part = [&](int i) { return i < pre.ranges ? pre0 + i * step : own0 + (i - pre.ranges) * step; };
+    auto row_of = [&](int i) { return i < pre.ranges ? rp : r; };
     float M = -INFINITY;
-    for (int i = 0; i < pre.ranges; ++i) M = fmaxf(M, pre0[i * step + TILE * D + rp]);
-    for (int i = 0; i < own.ranges; ++i) M = fmaxf(M, own0[i * step + TILE * D + r]);
+    for (int i = lane; i < n; i += LPR) M = fmaxf(M, part(i)[TILE * D + row_of(i)]);
+#pragma unroll
+    for (int m = LPR / 2; m >= 1; m >>= 1) M = fmaxf(M, __shfl_xor(M, m, 64));
+    const float msub = M == -INFINITY ? 0.0f : M;
     f32x4 acc = {};
     float sum = 0.0f;
-    auto add = [&](const float* p, int row) {
-      const float m = p[TILE * D + row];
-      const float f = m == -INFINITY ? 0.0f : exp2f_fast(m - M);
-      sum = fmaf(f, p[TILE * D + TILE + row], sum);
-      acc += f * *reinterpret_cast<const f32x4*>(p + row * D + c);
-    };
-    for (int i = 0; i < pre.ranges; ++i) add(pre0 + i * step, rp);
-    for (int i = 0; i < own.ranges; ++i) add(own0 + i * step, r);
+    for (int i0 = 0; i0 < n; i0 += LPR) {
+      const int count = min(n - i0, LPR);
+      float f = 0.0f, l = 0.0f;
+      if (lane < count) {
+        const float* p = part(i0 + lane) + TILE * D + row_of(i0 + lane);
+        f = exp2f_fast(p[0] - msub);
+        l = p[TILE];
+      }
+      for (int i = 0; i < count; i += 8) {
+        f32x4 x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int at = min(i + e, count - 1) + i0;
+          x[e] = *reinterpret_cast<const f32x4*>(part(at) + row_of(at) * D + c);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float fe = i + e < count ? __shfl(f, i + e, LPR) : 0.0f, le = __shfl(l, min(i + e, count - 1), LPR);
+          acc += fe * x[e];
+          sum = fmaf(fe, le, sum);
+        }
+      }
+    }
     const int row = t * TILE + r, tok = divide(a.div_g, row);
     const size_t at = ((size_t)(q0 + tok) * a.Hk + hk) * a.G + (row - tok * a.G);
     store_row<D>(a, at, c, acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
@@ -621,14 +646,17 @@ using namespace es;
 static int resident(int D) { return D == 64 ? 1024 : 512; }
 // Items a head of a ranged launch: at most one a tile more than the ranges' chunks fill.
 static long long range_items(long long tiles, int Hk, int D) { return tiles + resident(D) / Hk + 1; }
-// Key ranges are worth a second launch where the tiles do not fill the GPU and the keys are more than a few chunks.
-static bool ranged(long long tiles, int Tk, int Hk, int D) { return tiles * Hk < 2 * resident(D) && Tk >= 16 * BK; }
+// Key ranges are worth a second launch where the tiles do not fill the GPU and the keys are more than a few chunks: 1024 for
+// single tokens and the like (up to 32 rows a sequence on average), 4096 for longer lists, whose partials are large.
+static bool ranged(long long tiles, int B, int Tq, int Tk, int H, int Hk, int D) {
+  return tiles * Hk < 2 * resident(D) && Tk >= ((long long)Tq * (H / Hk) <= 32LL * B ? 16 : 64) * BK;
+}
 
 #ifndef ES_ELEM_F16
 extern "C" size_t es_packed_fwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D) {
   if (B <= 0 || Tq <= 0 || Tk < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
   const long long tiles = tile_numbers<TILE>(B, Tq, H / Hk);
-  return ranged(tiles, Tk, Hk, D) ? (size_t)range_items(tiles, Hk, D) * Hk * part_floats(D) * sizeof(float) : 0;
+  return ranged(tiles, B, Tq, Tk, H, Hk, D) ? (size_t)range_items(tiles, Hk, D) * Hk * part_floats(D) * sizeof(float) : 0;
 }
 extern "C" size_t es_shared_prefix_workspace(int B, int n, int P, int S, int H, int Hk, int D) {
   if (B <= 0 || n <= 0 || P < 0 || S < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
@@ -668,7 +696,7 @@ extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const voi
   a.scale = scale * LOG2E;
   a.tiles = (int)tile_numbers<TILE>(B, Tq, a.G);
   ES_REQUIRE((long long)a.tiles * Hk < (1LL << 31), ES_ERR_UNSUPPORTED, "packed: grid too large");
-  if (ranged(a.tiles, Tk, Hk, D)) {
+  if (ranged(a.tiles, B, Tq, Tk, H, Hk, D)) {
     ES_REQUIRE(workspace && workspace_bytes >= es_packed_fwd_workspace(B, Tq, Tk, H, Hk, D), ES_ERR_INVALID,
                "packed: workspace too small");
     a.part = (float*)workspace;

@@ -38,7 +38,7 @@ def forward_workspace_bytes(B, Tq, Tk, H, Hk, D):
     if Tq <= 0:
         return 0
     tiles = _tile_numbers(128, B, Tq, H // Hk)
-    if tiles * Hk >= (2048 if D == 64 else 1024) or Tk < 1024:
+    if tiles * Hk >= (2048 if D == 64 else 1024) or Tk < (1024 if Tq * (H // Hk) <= 32 * B else 4096):
         return 0
     return _range_bytes(tiles, Hk, D)
 

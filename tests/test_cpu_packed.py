@@ -107,6 +107,26 @@ def test_every_tile_has_one_number():
         assert found == {(b, t) for b in range(B + 1) for t in range(-(-(start[b + 1] - start[b]) * G // M))}
 
 
+def test_tiles_in_order_of_their_work():
+    """tile_of: up to 64 lists in descending order of weight, equal ones in their own order; every tile once, numbers below the
+    sum of the tiles."""
+    rng = random.Random(8)
+    for _ in range(200):
+        n = rng.choice([1, 2, 5, 64])
+        tiles = [rng.choice([0, 1, rng.randint(0, 30)]) for _ in range(n)]
+        weight = [rng.choice([0, 7, rng.randint(0, 1000)]) for _ in range(n)]
+        base = [sum(tiles[j] for j in range(n) if weight[j] > weight[i] or (weight[j] == weight[i] and j < i))
+                for i in range(n)]
+        found = []
+        for w in range(sum(tiles) + 3):
+            hit = [i for i in range(n) if base[i] <= w < base[i] + tiles[i]]
+            assert len(hit) == (w < sum(tiles))
+            found += [(i, w - base[i]) for i in hit]
+        assert sorted(found) == [(i, t) for i in range(n) for t in range(tiles[i])]
+        heavy = [weight[i] for i, _ in found]
+        assert heavy == sorted(heavy, reverse=True)
+
+
 def test_range_items_fit_the_grid():
     """The items of a ranged launch (csrc/packed_fwd.hip, key ranges) never outnumber the workgroups that the host starts, and
     each has at most the chunks that fill the GPU once."""

@@ -79,10 +79,10 @@ def test_forward(dev, D, dtype, H, Hk, causal, lens, keys):
 
 @pytest.mark.parametrize("D, dtype", TYPES)
 @pytest.mark.parametrize("lens, keys, H, Hk", [
-    ([1500, 700], [1500, 700], 3, 1),                           # ranges of wide tiles
+    ([1500, 700], [2500, 1700], 3, 1),                           # ranges of wide tiles
     ([1, 1, 1], [5000, 64, 1029], 10, 2),                       # ranges of single tokens
     ([33, 2, 300], [4100, 2500, 70], 5, 5),                     # narrow and wide tiles in one launch
-    ([2, 1, 1, 600], [0, 1100, 1, 600], 4, 2),
+    ([2, 1, 1, 600], [0, 3500, 1, 600], 4, 2),
     ([1], [40000], 16, 2),
 ])
 @pytest.mark.parametrize("causal", [False, True])
