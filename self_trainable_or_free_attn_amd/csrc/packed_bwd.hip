@@ -43,6 +43,7 @@ struct BwdArgs {
   float *lse2, *delta;  // [Hk][Tq * G]
   float* dist;          // [row tile numbers][Hk][G * (2 R + 1)]: dS by clamped distance
   FastDiv div_g;
+  float inv_g;  // 1 / G
   int B, Tq, Tk, H, Hk, G, R, num_buckets, causal;
   int q_tiles, k_tiles;  // tile numbers of a head
   float scale_log2, scale;
@@ -120,17 +121,28 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
   // Row tile i: Q and dO rows (16 of each a wave) through a resource based at the tile's first token, and, wave 0, its lse2
   // and delta. Rows of a list are `row / G` tokens of H * D values and `row % G` heads apart.
   const size_t list = (size_t)hk * a.Tq * a.G + (size_t)s.q0 * a.G;
+  const unsigned lds_q = uni(lds_addr(&qd_s[0][0][0]) + (unsigned)wv * (NI * 1024u));
+  // A lane's transfer r moves 16 bytes of tile row R + RPT r, R = 16 wv + l / LPR, whose chunk the swizzle moves by one XOR a
+  // step: of its address in a list without gaps one register holds step 0 (`lane_at`). A token's rows are (H - G) rows further
+  // apart than that, and the row's token within the tile is (rows since the first token's + 1/2) / G in float32 (exact: rows
+  // up to G + 63, G up to 4096, the nearest border 1 / (2 G) away). Few registers matter here: with more the compiler spills
+  // some, and a reload in this loop waits for every transfer before it (a tile's transfers took 2970 cycles instead of 920).
+  constexpr int RPT = 64 / LPR, XOR = D == 128 ? 16 : 32;
+  int lane_at = (wv * 16 + l / LPR) * ROW + (((l % LPR) ^ swizzle<D>(l / LPR)) << 4);
   auto issue = [&](int i, int sb) {
-    const int t0 = divide(a.div_g, i * BK), toks = min(s.nq - t0, BK + 1);
+    const int t0 = divide(a.div_g, i * BK), toks = min(s.nq - t0, BK + 1), rel = i * BK - t0 * a.G;
     const size_t base = ((size_t)(s.q0 + t0) * a.H + hk * a.G) * D;
     const unsigned bytes = (unsigned)((toks - 1) * a.H + a.G) * ROW;
     const srd_t rq = make_srd(a.q + base, bytes), rd = make_srd(a.dout + base, bytes);
+    const unsigned gap = (unsigned)(a.H - a.G) * ROW;
+    const float first = (float)rel + 0.5f;
+    const unsigned qd = lds_q + (unsigned)sb * (2u * TILE_BYTES);
 #pragma unroll
     for (int r = 0; r < NI; ++r) {
-      const int R = wv * 16 + r * (64 / LPR) + l / LPR, row = i * BK + R, tok = divide(a.div_g, row);
-      const unsigned at = (unsigned)((tok - t0) * a.H + row - tok * a.G) * ROW + (unsigned)(((l % LPR) ^ swizzle<D>(R)) * 16);
-      dma16(rq, qd_s[sb][0] + (wv * NI + r) * 1024, at, 0u);
-      dma16(rd, qd_s[sb][1] + (wv * NI + r) * 1024, at, 0u);
+      const unsigned tok = (unsigned)(((float)(lane_at / ROW) + (first + (float)(RPT * r))) * a.inv_g);
+      const unsigned at = __umul24(tok, gap) + (unsigned)((lane_at ^ (XOR * r)) + (RPT * r + rel) * ROW);
+      dma16_at(rq, qd + r * 1024, at, 0u);
+      dma16_at(rd, qd + TILE_BYTES + r * 1024, at, 0u);
     }
     if (wv == 0) {
       const unsigned left = (unsigned)min(rows - i * BK, BK) * 4u;
@@ -139,11 +151,12 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
     }
   };
   auto stats = [&](int i, int sb) {  // wave 0, after dma_wait()
-    const int row = i * BK + l, tok = divide(a.div_g, row);
-    st_s[sb][0][l] = row < rows ? lse_s[l] - P_SHIFT : INFINITY;
+    const int t0 = divide(a.div_g, i * BK), rel = i * BK - t0 * a.G + l;
+    const int tok = (int)(((float)rel + 0.5f) * a.inv_g);
+    st_s[sb][0][l] = i * BK + l < rows ? lse_s[l] - P_SHIFT : INFINITY;
     if (P_BACK != 1.0f) st_s[sb][1][l] *= P_BACK;
-    pos_s[sb][l] = tok + shift;
-    if (BIAS) gb_s[sb][l] = (row - tok * a.G) * (2 * a.R + 1) + a.R;
+    pos_s[sb][l] = t0 + tok + shift;
+    if (BIAS) gb_s[sb][l] = (rel - tok * a.G) * (2 * a.R + 1) + a.R;
   };
   // LDS offsets of this wave's row half (packed_fwd.hip: Offsets)
   int aoff = qh * (TILE_BYTES / 2) + tile_at<D>(lq, hi);
@@ -169,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
   for (int i = beg; i < end; ++i) {
     const int sb = (i - beg) & 1;
     if (i + 1 < end) issue(i + 1, sb ^ 1);
-    asm volatile("" : "+v"(aoff), "+v"(toff0), "+v"(toff1));  // (keeps the offsets from being hoisted)
+    asm volatile("" : "+v"(aoff), "+v"(toff0), "+v"(toff1), "+v"(lane_at));  // (keeps the offsets from being hoisted)
     const char* qt = qd_s[sb][0];
     const char* dt = qd_s[sb][1];
     auto product = [&](const char* xt, const ev8& xa, const ev8& xb, f32x16 (&acc)[NDB]) {  // acc += xt^T [xa | xb]
@@ -567,6 +580,7 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
   a.Hk = Hk;
   a.G = H / Hk;
   a.div_g = fast_div(a.G);
+  a.inv_g = 1.0f / (float)a.G;
   a.R = bias ? R : 0;
   a.num_buckets = num_buckets;
   a.causal = causal != 0;
