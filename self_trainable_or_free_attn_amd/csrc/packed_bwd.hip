@@ -2,7 +2,8 @@
 //
 // With P = exp(S - lse) and dS = P (dP - delta), dP = dO V^T, delta = rowsum(dO O) (rows that see no key: P = 0):
 //   row_stats   one pass over dO and O: lse in log2 units (+inf for rows without keys) and delta, laid out by kv head and
-//               row of the list (token, head in group), so that a row tile's values are contiguous
+//               row of the list (token, head in group), so that a row tile's values are contiguous (with the fp16 factor of
+//               P and its inverse in them)
 //   bwd_q       one workgroup per (64 rows, kv head): dQ = scale dS K over the keys, 2 row groups x 2 key halves, S^T and
 //               dP^T with rows on lanes; with a bias it also sums dS by clamped distance
 //   bwd_kv      one workgroup per (64 keys, kv head): dV = P^T dO and dK = scale dS^T Q over all rows of the list that see
@@ -71,8 +72,8 @@ __global__ __launch_bounds__(256) void row_stats_kernel(BwdArgs a) {
   const int tok = (int)(row / a.H), h = (int)(row - (size_t)tok * a.H), hk = divide(a.div_g, h);
   const size_t to = ((size_t)hk * a.Tq + tok) * a.G + (h - hk * a.G);
   const float l = a.lse[row];
-  a.lse2[to] = l == -INFINITY ? INFINITY : l * LOG2E;
-  a.delta[to] = sum;
+  a.lse2[to] = l == -INFINITY ? INFINITY : l * LOG2E - P_SHIFT;
+  a.delta[to] = sum * P_BACK;
 }
 
 template <int D, bool BIAS>
@@ -80,9 +81,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
   __shared__ __attribute__((aligned(16))) char qd_s[2][2][TILE_BYTES];  // [buffer][Q | dO]
   __shared__ __attribute__((aligned(16))) float st_s[2][2][BK];         // [buffer][lse2 | delta]
-  __shared__ __attribute__((aligned(16))) int pos_s[2][BK];             // [buffer] position of the row
-  __shared__ __attribute__((aligned(16))) int gb_s[BIAS ? 2 : 1][BIAS ? BK : 1];  // the row's part of the bias table
-  __shared__ float lse_s[BK];                                           // the next tile's lse2 as stored
+  // [buffer][position of the row | its part of the bias table]
+  __shared__ __attribute__((aligned(16))) int pos_s[BIAS ? 2 : 1][2][BIAS ? BK : 1];
   __shared__ float tab[BIAS ? BIAS_ROWS : 1];
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
   int b, kb;
@@ -128,6 +128,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
   // up to G + 63, G up to 4096, the nearest border 1 / (2 G) away). Few registers matter here: with more the compiler spills
   // some, and a reload in this loop waits for every transfer before it (a tile's transfers took 2970 cycles instead of 920).
   constexpr int RPT = 64 / LPR, XOR = D == 128 ? 16 : 32;
+  auto token_in_tile = [&](int row) { return (int)(((float)row + 0.5f) * a.inv_g); };  // of rows since the first token's
   int lane_at = (wv * 16 + l / LPR) * ROW + (((l % LPR) ^ swizzle<D>(l / LPR)) << 4);
   auto issue = [&](int i, int sb) {
     const int t0 = divide(a.div_g, i * BK), toks = min(s.nq - t0, BK + 1), rel = i * BK - t0 * a.G;
@@ -144,19 +145,16 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
       dma16_at(rq, qd + r * 1024, at, 0u);
       dma16_at(rd, qd + TILE_BYTES + r * 1024, at, 0u);
     }
-    if (wv == 0) {
-      const unsigned left = (unsigned)min(rows - i * BK, BK) * 4u;
-      dma4(make_srd(a.lse2 + list + (size_t)i * BK, left), lse_s, 4u * l, 0u);
-      dma4(make_srd(a.delta + list + (size_t)i * BK, left), st_s[sb][1], 4u * l, 0u);
+    // (rows past the list's end read as zeros: their P is finite and meets zeros of dO, dP and delta, and `masked` covers
+    // the case of a bias that makes it infinite)
+    if (wv < 2)
+      dma4(make_srd((wv == 0 ? a.lse2 : a.delta) + list + (size_t)i * BK, (unsigned)min(rows - i * BK, BK) * 4u),
+           st_s[sb][wv], 4u * l, 0u);
+    if (BIAS && wv == 2) {
+      const int tok = token_in_tile(rel + l);
+      pos_s[sb][0][l] = t0 + tok + shift;
+      pos_s[sb][1][l] = (rel + l - tok * a.G) * (2 * a.R + 1) + a.R;
     }
-  };
-  auto stats = [&](int i, int sb) {  // wave 0, after dma_wait()
-    const int t0 = divide(a.div_g, i * BK), rel = i * BK - t0 * a.G + l;
-    const int tok = (int)(((float)rel + 0.5f) * a.inv_g);
-    st_s[sb][0][l] = i * BK + l < rows ? lse_s[l] - P_SHIFT : INFINITY;
-    if (P_BACK != 1.0f) st_s[sb][1][l] *= P_BACK;
-    pos_s[sb][l] = t0 + tok + shift;
-    if (BIAS) gb_s[sb][l] = (rel - tok * a.G) * (2 * a.R + 1) + a.R;
   };
   // LDS offsets of this wave's row half (packed_fwd.hip: Offsets)
   int aoff = qh * (TILE_BYTES / 2) + tile_at<D>(lq, hi);
@@ -172,8 +170,6 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
 
   if (beg < end) {
     issue(beg, 0);
-    dma_wait();
-    if (wv == 0) stats(beg, 0);
   }
   dma_wait();
   __syncthreads();
@@ -181,6 +177,10 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
   const float kmask = kvalid ? 0.0f : INFINITY;
   for (int i = beg; i < end; ++i) {
     const int sb = (i - beg) & 1;
+    // the rows of Q are read before the next tile's transfers are issued: S then finds its operands ready
+    ev8 qf[NKS];
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) qf[ks] = elds16(qd_s[sb][0], aoff ^ (32 * ks));
     if (i + 1 < end) issue(i + 1, sb ^ 1);
     asm volatile("" : "+v"(aoff), "+v"(toff0), "+v"(toff1), "+v"(lane_at));  // (keeps the offsets from being hoisted)
     const char* qt = qd_s[sb][0];
@@ -195,26 +195,26 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
     };
     f32x16 p = {}, dp = {};
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) p = emfma(elds16(qt, aoff ^ (32 * ks)), kreg[ks], p);
-    // the wave's rows 32 qh .. + 31 of the tile, whose positions ascend; a key is seen from its own position on
-    const bool diagonal = a.causal && pos_s[sb][32 * qh] < kb * BK + 32 * kh + 31;
+    for (int ks = 0; ks < NKS; ++ks) p = emfma(qf[ks], kreg[ks], p);
+    // the wave's rows, whose positions ascend: a key is seen from its own position on
+    const int t0 = divide(a.div_g, i * BK), rel = i * BK - t0 * a.G;
+    const bool masked = (a.causal && t0 + token_in_tile(rel + 32 * qh) + shift < kb * BK + 32 * kh + 31) ||
+                        (BIAS && (i + 1) * BK > rows);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int r0 = 32 * qh + 8 * g + 4 * hi;
-      f32x4 l4 = *reinterpret_cast<const f32x4*>(&st_s[sb][0][r0]);  // (lse2 - P_SHIFT)
-      if (BIAS || diagonal) {
-        const int4 p4 = *reinterpret_cast<const int4*>(&pos_s[sb][r0]);
-        const int ps[4] = {p4.x, p4.y, p4.z, p4.w};
-        if (BIAS) {
-          const int4 b4 = *reinterpret_cast<const int4*>(&gb_s[sb][r0]);
-          const int gs[4] = {b4.x, b4.y, b4.z, b4.w};
+      f32x4 l4 = *reinterpret_cast<const f32x4*>(&st_s[sb][0][r0]);
+      if (BIAS) {
+        const int4 p4 = *reinterpret_cast<const int4*>(&pos_s[sb][0][r0]), b4 = *reinterpret_cast<const int4*>(&pos_s[sb][1][r0]);
+        const int ps[4] = {p4.x, p4.y, p4.z, p4.w}, gs[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) l4[e] -= tab[gs[e] + min(max(key - ps[e], -a.R), a.R)];
-        }
-        if (diagonal) {
+        for (int e = 0; e < 4; ++e) l4[e] -= tab[min(max(gs[e] + min(max(key - ps[e], -a.R), a.R), 0), BIAS_ROWS - 1)];
+      }
+      if (masked) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (key > ps[e]) l4[e] = INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          const int row = i * BK + r0 + e, pos = t0 + token_in_tile(rel + r0 + e) + shift;
+          if (row >= rows || (a.causal && key > pos)) l4[e] = INFINITY;
         }
       }
 #pragma unroll
@@ -242,7 +242,6 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
       product(qt, epack8(&x[0]), epack8(&x[8]), acc_k);
     }
     dma_wait();
-    if (i + 1 < end && wv == 0) stats(i + 1, sb ^ 1);
     __syncthreads();
   }
 
@@ -319,8 +318,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     qreg[ks] = valid ? *reinterpret_cast<const ev8*>(a.q + at + 16 * ks + 8 * hi) : z;
     dreg[ks] = valid ? *reinterpret_cast<const ev8*>(a.dout + at + 16 * ks + 8 * hi) : z;
   }
-  const float ls = valid ? a.lse2[list] : INFINITY;
-  float dl = valid ? a.delta[list] : 0.0f;
+  const float ls = valid ? a.lse2[list] + P_SHIFT : INFINITY;
+  float dl = valid ? a.delta[list] * (1.0f / P_BACK) : 0.0f;
   if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
 
   const unsigned stride = (unsigned)a.Hk * ROW;
@@ -330,14 +329,15 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     const int R = (wv * NI + i) * (64 / LPR) + l / LPR;
     src[i] = (unsigned)R * stride + (unsigned)(((l % LPR) ^ swizzle<D>(R)) * 16);
   }
+  const unsigned lds_k = uni(lds_addr(&kv_s[0][0][0]) + (unsigned)wv * (NI * 1024u));
   auto issue = [&](int c, int sb) {
     const size_t base = ((size_t)(s.k0 + c * BK) * a.Hk + hk) * D;
     const unsigned bytes = (unsigned)(min(BK, s.nk - c * BK) - 1) * stride + ROW;
     const srd_t rk = make_srd(a.k + base, bytes), rv = make_srd(a.v + base, bytes);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      dma16(rk, kv_s[sb][0] + (wv * NI + i) * 1024, src[i], 0u);
-      dma16(rv, kv_s[sb][1] + (wv * NI + i) * 1024, src[i], 0u);
+      dma16_at(rk, lds_k + (unsigned)sb * (2u * TILE_BYTES) + i * 1024, src[i], 0u);
+      dma16_at(rv, lds_k + (unsigned)sb * (2u * TILE_BYTES) + TILE_BYTES + i * 1024, src[i], 0u);
     }
   };
   const int koff = kh * (TILE_BYTES / 2) + tile_at<D>(lq, hi);
@@ -353,11 +353,11 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
   float far_lo = 0.0f, far_hi = 0.0f;  // dS at distances of -R and below, of R and beyond
 
   // P and dP of keys key0 .. key0 + 31 (near: by distance, neither all at -R and below nor all at R and beyond)
-  auto scores = [&](const char* kt, const char* vt, int key0, f32x16& x, f32x16& dp, bool& near) {
+  auto scores = [&](const ev8 (&kf)[NKS], const char* vt, int key0, f32x16& x, f32x16& dp, bool& near) {
     x = f32x16{};
     dp = f32x16{};
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) x = emfma(elds16(kt, koff ^ (32 * ks)), qreg[ks], x);
+    for (int ks = 0; ks < NKS; ++ks) x = emfma(kf[ks], qreg[ks], x);
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(vt, koff ^ (32 * ks)), dreg[ks], dp);
     const int d0 = key0 + 4 * hi - pos;
@@ -382,6 +382,11 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = exp2f_fast(fmaf(x[r], sc, cb - ls));
   };
+  // the chunk's rows of K, read before the next chunk's transfers are issued: S then finds its operands ready
+  auto read_k = [&](const char* kt, ev8 (&kf)[NKS]) {
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) kf[ks] = elds16(kt, koff ^ (32 * ks));
+  };
   if (end > 0) issue(0, 0);
   dma_wait();
   __syncthreads();
@@ -389,11 +394,13 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
   if (end > 0 && (BIAS || end <= EXACT_CHUNKS)) {
     float num = 0.0f, den = 0.0f;
     for (int c = 0; c < end; ++c) {
+      ev8 kf[NKS];
+      read_k(kv_s[sb][0], kf);
       issue(c + 1 < end ? c + 1 : 0, sb ^ 1);  // (after the last chunk the first one again, for the main pass)
       if (c * BK + 32 * kh < seen_max) {
         f32x16 p, dp;
         bool near;
-        scores(kv_s[sb][0], kv_s[sb][1], c * BK + 32 * kh, p, dp, near);
+        scores(kf, kv_s[sb][1], c * BK + 32 * kh, p, dp, near);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           num = fmaf(p[r], dp[r], num);
@@ -408,7 +415,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     __syncthreads();
     const float2 s0 = reinterpret_cast<const float2*>(hist[rg])[lq], s1 = reinterpret_cast<const float2*>(hist[rg + 2])[lq];
     if (s0.y + s1.y > 0.0f) dl = (s0.x + s1.x) / (s0.y + s1.y);
-    if (valid && kh == 0 && hi == 0) a.delta[list] = dl;
+    if (valid && kh == 0 && hi == 0) a.delta[list] = dl * P_BACK;
   }
   if (BIAS) {
     __syncthreads();
@@ -416,6 +423,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     __syncthreads();
   }
   for (int c = 0; c < end; ++c) {
+    ev8 kf[NKS];
+    read_k(kv_s[sb][0], kf);
     if (c + 1 < end) issue(c + 1, sb ^ 1);
     const char* kt = kv_s[sb][0];
     const char* vt = kv_s[sb][1];
@@ -423,7 +432,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     if (key0 < seen_max) {
       f32x16 x, dp;
       bool near;
-      scores(kt, vt, key0, x, dp, near);
+      scores(kf, vt, key0, x, dp, near);
       const int d0 = key0 + 4 * hi - pos;
       float ds[16];
 #pragma unroll
