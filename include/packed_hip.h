@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define ES_PACKED_BIAS_ROWS 816
+#define ES_PACKED_BIAS_ROWS 784
 
 /* Forward. workspace: es_packed_fwd_workspace bytes (0: none needed; NULL / 0 is then accepted), for batches of few query
  * rows against many keys, whose keys are cut into ranges that run side by side and are merged in a fixed order. */

@@ -19,7 +19,10 @@ namespace {
 
 constexpr float PK_LN2 = 0.6931471805599453f;
 constexpr int TILE = 128;                       // query rows of a forward tile
-constexpr int BIAS_ROWS = ES_PACKED_BIAS_ROWS;  // entries of the LDS bias table: G * (2 R + 1)
+constexpr int BIAS_ROWS = ES_PACKED_BIAS_ROWS;  // G * (2 R + 1) at most
+// With one head a group the table repeats its ends for BIAS_PAD distances more on either side: the 32 keys of a run that is
+// not all at -R and below or all at R and beyond stand within 31 + 31 of that range, and need no clamp.
+constexpr int BIAS_PAD = 64, BIAS_TABLE = BIAS_ROWS + 2 * BIAS_PAD;
 
 // x / d for 0 <= x < 2^31 by one multiplication: mul = ceil(2^(32 + sh) / d) with 2^sh < d <= 2^(sh + 1), whose error
 // mul * d - 2^(32 + sh) < d <= 2^(sh + 1) keeps x * error under 2^(32 + sh). d = 1: mul = 0.
@@ -61,32 +64,6 @@ __host__ __device__ __forceinline__ long long tile_numbers(int B, int T, int G) 
   return (long long)T * G / M + B + 1;
 }
 
-// Tile number w of a launch without ranges: the sequences in descending order of weight(b), so that the tiles with the most
-// work start first and those that start last are short (workgroups are dispatched in order), each with its tiles(b) tiles.
-// Up to 64 sequences (the rows behind the last one included): each lane takes one and adds up the tiles of those before it.
-// More: their own order, by seq_of_tile. false: no tile has this number.
-template <int M, class TILES, class WEIGHT>
-__device__ __forceinline__ bool tile_of(const int* cu, int B, int T, int G, int w, const TILES& tiles, const WEIGHT& weight,
-                                        int& b, int& t) {
-  if (B < 64) {
-    const int l = lane_id();
-    const int mine = l <= B ? tiles(l) : 0, heavy = l <= B ? weight(l) : -1;
-    int base = 0;
-    for (int j = 0; j <= B; ++j) {
-      const int tj = __builtin_amdgcn_readlane(mine, j), hj = __builtin_amdgcn_readlane(heavy, j);
-      base += hj > heavy || (hj == heavy && j < l) ? tj : 0;
-    }
-    const unsigned long long hit = __builtin_amdgcn_ballot_w64(l <= B && base <= w && w < base + mine);
-    if (hit == 0) return false;
-    b = __builtin_ctzll(hit);
-    t = w - __builtin_amdgcn_readlane(base, b);
-    return true;
-  }
-  b = seq_of_tile<M>(cu, B, T, G, w);
-  t = w - (__builtin_amdgcn_readfirstlane(seq_start(cu, b, B, T)) * G / M + b);
-  return t >= 0 && t < __builtin_amdgcn_readfirstlane(tiles(b));
-}
-
 struct Seq {
   int q0, nq, k0, nk;
 };
@@ -102,6 +79,47 @@ __device__ __forceinline__ Seq sequence(const int* cu_q, const int* cu_k, int B,
   s.nq = max(__builtin_amdgcn_readfirstlane(seq_start(cu_q, b + 1, B, Tq)) - s.q0, 0);
   s.nk = max(__builtin_amdgcn_readfirstlane(seq_start(cu_k, b + 1, B, Tk)) - s.k0, 0);
   return s;
+}
+
+// Tile number w of a launch without ranges: the sequences in descending order of their other length (keys where tiles are of
+// rows, rows where KEYS), so that the tiles with the most work start first and those that start last are short (workgroups are
+// dispatched in order), each with its tiles. Up to 64 sequences (the rows behind the last one included): each lane takes one
+// and adds up the tiles of those before it. More: their own order, by seq_of_tile. false: no tile has this number.
+template <int M, bool KEYS>
+__device__ __forceinline__ bool tile_of(const int* cu_q, const int* cu_k, int B, int Tq, int Tk, int G, int w, Seq& s, int& b,
+                                        int& t) {
+  if (B < 64) {
+    const int l = min(lane_id(), B), last = KEYS ? Tk : Tq;
+    Seq x;
+    x.q0 = seq_start(cu_q, l, B, Tq);
+    x.k0 = seq_start(cu_k, l, B, Tk);
+    x.nq = l < B ? max(seq_start(cu_q, l + 1, B, Tq) - x.q0, 0) : 0;
+    x.nk = l < B ? max(seq_start(cu_k, l + 1, B, Tk) - x.k0, 0) : 0;
+    if (l == B) (KEYS ? x.nk : x.nq) = last - (KEYS ? x.k0 : x.q0);
+    const int tiles = ((KEYS ? x.nk : x.nq * G) + M - 1) / M, weight = KEYS ? x.nq : x.nk;
+    int base = 0;
+    for (int j = 0; j <= B; ++j) {
+      const int tj = __builtin_amdgcn_readlane(tiles, j), wj = __builtin_amdgcn_readlane(weight, j);
+      base += wj > weight || (wj == weight && j < l) ? tj : 0;
+    }
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(base <= w && w < base + tiles);
+    if (hit == 0) return false;
+    b = __builtin_ctzll(hit);  // (lanes past B repeat lane B's)
+    t = w - __builtin_amdgcn_readlane(base, b);
+    s.q0 = __builtin_amdgcn_readlane(x.q0, b);
+    s.nq = __builtin_amdgcn_readlane(x.nq, b);
+    s.k0 = __builtin_amdgcn_readlane(x.k0, b);
+    s.nk = __builtin_amdgcn_readlane(x.nk, b);
+    return true;
+  }
+  b = KEYS ? seq_of_tile<M>(cu_k, B, Tk, 1, w) : seq_of_tile<M>(cu_q, B, Tq, G, w);
+  s = sequence(cu_q, cu_k, B, Tq, Tk, b);
+  if (KEYS && b >= B) {
+    s.nk = Tk - s.k0;
+    s.nq = 0;
+  }
+  t = w - ((KEYS ? s.k0 : s.q0 * G) / M + b);
+  return t >= 0 && t * M < (KEYS ? s.nk : s.nq * G);
 }
 
 // rows of the list of sequence b (b == B: the rows behind the last sequence), and its keys
@@ -137,15 +155,28 @@ __device__ __forceinline__ void wait_lds() {
   asm volatile("" ::: "memory");
 }
 
-// The bias of a head group by clamped distance in log2 units: tab[g * (2 R + 1) + d + R], filled by the whole workgroup.
+// The bias of a head group by distance in log2 units, filled by the whole workgroup (which waits at a barrier before it reads
+// it): bias_at(g, d) with d clamped to -R .. R, or for G = 1 within BIAS_PAD of that.
+__device__ __forceinline__ int bias_width(int G, int R) { return 2 * R + 1 + (G == 1 ? 2 * BIAS_PAD : 0); }
+__device__ __forceinline__ int bias_row(int G, int R, int g) { return g * bias_width(G, R) + R + (G == 1 ? BIAS_PAD : 0); }
 __device__ __forceinline__ void fill_bias(float* tab, const float* bias, const int* buckets, int num_buckets, int R, int G,
                                           int H, int hk) {
-  const int n = 2 * R + 1;
+  const int n = bias_width(G, R);
   for (int i = threadIdx.x; i < G * n; i += blockDim.x) {
-    const int g = i / n, bk = min(max(buckets[i - g * n], 0), num_buckets - 1);
+    const int g = i / n, d = min(max(i - bias_row(G, R, g), -R), R), bk = min(max(buckets[d + R], 0), num_buckets - 1);
     tab[i] = bias[(size_t)bk * H + hk * G + g] * LOG2E;
   }
-  __syncthreads();
+}
+// x[r] = x[r] * sc + bias of the key at distance d0 + 8 (r / 4) + r % 4; row: the table at distance 0
+__device__ __forceinline__ void add_bias(f32x16& x, float sc, const float* row, int d0, int G, int R) {
+  if (G == 1) {
+    row += d0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], sc, row[8 * (r / 4) + r % 4]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], sc, row[min(max(d0 + 8 * (r / 4) + r % 4, -R), R)]);
+  }
 }
 
 }  // namespace
@@ -167,7 +198,7 @@ static inline int packed_check(const void* q, const void* k, const void* v, cons
   if (bias) {
     ES_REQUIRE(buckets && num_buckets > 0 && R >= 0, ES_ERR_INVALID, "packed: a bias needs buckets");
     ES_REQUIRE(R <= BIAS_ROWS && (long long)(H / Hk) * (2 * R + 1) <= BIAS_ROWS, ES_ERR_UNSUPPORTED,
-               "packed: (H / Hk) * (2 R + 1) must be at most 816");
+               "packed: (H / Hk) * (2 R + 1) must be at most 784");
   }
   return ES_OK;
 }

@@ -83,22 +83,11 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
   __shared__ __attribute__((aligned(16))) float st_s[2][2][BK];         // [buffer][lse2 | delta]
   // [buffer][position of the row | its part of the bias table]
   __shared__ __attribute__((aligned(16))) int pos_s[BIAS ? 2 : 1][2][BIAS ? BK : 1];
-  __shared__ float tab[BIAS ? BIAS_ROWS : 1];
+  __shared__ float tab[BIAS ? BIAS_TABLE : 1];
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
   int b, kb;
-  if (!tile_of<BK>(a.cu_k, a.B, a.Tk, 1, w, [&](int i) { return (list_rows(a.cu_k, a.B, a.Tk, 1, i) + BK - 1) / BK; },
-                   [&](int i) { return i >= a.B ? 0 : list_rows(a.cu_q, a.B, a.Tq, a.G, i); }, b, kb))
-    return;
-  Seq s;
-  s.k0 = __builtin_amdgcn_readfirstlane(seq_start(a.cu_k, b, a.B, a.Tk));
-  const int kend = b >= a.B ? a.Tk : __builtin_amdgcn_readfirstlane(seq_start(a.cu_k, b + 1, a.B, a.Tk));
-  s.nk = max(kend - s.k0, 0);
-  s.q0 = 0;
-  s.nq = 0;  // (key rows behind the last sequence: zero gradients)
-  if (b < a.B) {
-    s.q0 = __builtin_amdgcn_readfirstlane(seq_start(a.cu_q, b, a.B, a.Tq));
-    s.nq = max(__builtin_amdgcn_readfirstlane(seq_start(a.cu_q, b + 1, a.B, a.Tq)) - s.q0, 0);
-  }
+  Seq s;  // (key rows behind the last sequence: no rows, so zero gradients)
+  if (!tile_of<BK, true>(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, a.G, w, s, b, kb)) return;
   const int rows = s.nq * a.G, shift = s.nk - s.nq;
   const int end = (rows + BK - 1) / BK;
   // causal: the first row that sees this tile's first key
@@ -109,8 +98,6 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
   const int key = kb * BK + 32 * kh + lq;
   const bool kvalid = key < s.nk;
   const size_t krow = ((size_t)(s.k0 + (kvalid ? key : 0)) * a.Hk + hk) * D;
-  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
-
   ev8 kreg[NKS], vreg[NKS];  // this lane's key row
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) {
@@ -153,7 +140,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
     if (BIAS && wv == 2) {
       const int tok = token_in_tile(rel + l);
       pos_s[sb][0][l] = t0 + tok + shift;
-      pos_s[sb][1][l] = (rel + l - tok * a.G) * (2 * a.R + 1) + a.R;
+      pos_s[sb][1][l] = bias_row(a.G, a.R, rel + l - tok * a.G);
     }
   };
   // LDS offsets of this wave's row half (packed_fwd.hip: Offsets)
@@ -168,9 +155,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
 #pragma unroll
   for (int db = 0; db < NDB; ++db) acc_v[db] = acc_k[db] = f32x16{};
 
-  if (beg < end) {
-    issue(beg, 0);
-  }
+  if (beg < end) issue(beg, 0);
+  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
   dma_wait();
   __syncthreads();
   // masked key columns: every row's lse2 becomes +inf for this lane, so P = 2^(s - inf) = 0 without a branch
@@ -208,7 +194,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
         const int4 p4 = *reinterpret_cast<const int4*>(&pos_s[sb][0][r0]), b4 = *reinterpret_cast<const int4*>(&pos_s[sb][1][r0]);
         const int ps[4] = {p4.x, p4.y, p4.z, p4.w}, gs[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) l4[e] -= tab[min(max(gs[e] + min(max(key - ps[e], -a.R), a.R), 0), BIAS_ROWS - 1)];
+        for (int e = 0; e < 4; ++e) l4[e] -= tab[gs[e] + min(max(key - ps[e], -a.R), a.R)];
       }
       if (masked) {
 #pragma unroll
@@ -279,19 +265,18 @@ template <int D, bool BIAS>
 __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
   __shared__ __attribute__((aligned(16))) char kv_s[2][2][TILE_BYTES];
-  __shared__ float tab[BIAS ? BIAS_ROWS : 1];
+  __shared__ float tab[BIAS ? BIAS_TABLE : 1];
   // per wave: dS by (head in group, clamped distance); before the main pass (sum P dP, sum P) of its 32 rows
   __shared__ __attribute__((aligned(8))) float hist[4][BIAS ? BIAS_ROWS : 64];
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk, width = 2 * a.R + 1;
   float* dist = BIAS ? a.dist + ((size_t)w * a.Hk + hk) * (a.G * width) : nullptr;
   int b, t;
-  if (!tile_of<BK>(a.cu_q, a.B, a.Tq, a.G, w, [&](int i) { return (list_rows(a.cu_q, a.B, a.Tq, a.G, i) + BK - 1) / BK; },
-                   [&](int i) { return list_keys(a.cu_k, a.B, a.Tk, i); }, b, t)) {
+  Seq s;
+  if (!tile_of<BK, false>(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, a.G, w, s, b, t)) {
     if (BIAS)  // (a tile number without a tile: its sums are read all the same)
       for (int i = threadIdx.x; i < a.G * width; i += 256) dist[i] = 0.0f;
     return;
   }
-  const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, b);
   const int rows = s.nq * a.G, shift = s.nk - s.nq;
   t = (rows + BK - 1) / BK - 1 - t;  // (under a causal mask the last tiles see the most keys)
   const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
@@ -299,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
   const int rg = wv & 1, kh = wv >> 1;
   const int r0 = t * BK + 32 * rg, row = r0 + lq;
   const bool valid = row < rows;
-  const int tok = divide(a.div_g, row), g = valid ? row - tok * a.G : 0, pos = tok + shift, gb = g * width + a.R;
+  const int tok = divide(a.div_g, row), g = valid ? row - tok * a.G : 0, pos = tok + shift, gb = bias_row(a.G, a.R, g);
   const size_t at = (((size_t)(s.q0 + (valid ? tok : 0)) * a.Hk + hk) * a.G + g) * D;
   const size_t list = ((size_t)hk * a.Tq + s.q0) * a.G + (valid ? row : 0);
   const int seen = !valid ? 0 : a.causal ? min(max(pos + 1, 0), s.nk) : s.nk;
@@ -320,8 +305,6 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
   }
   const float ls = valid ? a.lse2[list] + P_SHIFT : INFINITY;
   float dl = valid ? a.delta[list] * (1.0f / P_BACK) : 0.0f;
-  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
-
   const unsigned stride = (unsigned)a.Hk * ROW;
   unsigned src[NI];
 #pragma unroll
@@ -360,7 +343,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     for (int ks = 0; ks < NKS; ++ks) x = emfma(kf[ks], qreg[ks], x);
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(vt, koff ^ (32 * ks)), dreg[ks], dp);
-    const int d0 = key0 + 4 * hi - pos;
+    const int d0 = key0 + 4 * hi - (valid ? pos : low);  // (a position of the wave's)
     float sc = a.scale_log2, cb = 0.0f;
     near = false;
     if (BIAS) {
@@ -369,8 +352,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
       else near = true;
     }
     if (near) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], sc, tab[gb + min(max(d0 + 8 * (r / 4) + r % 4, -a.R), a.R)]);
+      add_bias(x, sc, tab + gb, d0, a.G, a.R);
       sc = 1.0f;
     }
     if (key0 + 32 > seen_min) {
@@ -388,6 +370,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     for (int ks = 0; ks < NKS; ++ks) kf[ks] = elds16(kt, koff ^ (32 * ks));
   };
   if (end > 0) issue(0, 0);
+  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
   dma_wait();
   __syncthreads();
   int sb = 0;
@@ -445,20 +428,46 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
           if (key0 - high >= a.R) far_hi += sum;
           else far_lo += sum;
         } else {
-          // One key of the run a step: the 32 rows of a half wave stand at different distances or in different heads, so
-          // no two lanes of a half add to one entry; the halves go one after the other, and a wave's LDS operations are
-          // done in order: the sums have a fixed order without waiting for each.
-          float* h = hist[wv] + gb + d0;
+          float* h = hist[wv] + g * width + a.R;
+          if (a.G == 1) {
+            // The run's diagonals, in a 64-lane shift register: row q's dS for key e enters at lane q and moves up a lane
+            // a key, so that all of one distance meet; after key 31 lane i holds distance key0 + 31 - (first row) - i. Keys
+            // 8 n .. 8 n + 3 are in the low half wave, the next four in the high one, which the swap brings down. (One LDS
+            // add for 32 x 32 values; adding each by itself, below, took a training pass of 2303 tokens, 24 heads from 171
+            // to 126 us.)
+            float v = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int e = 8 * (r / 4) + r % 4, d = d0 + e;
-            far_lo += d <= -a.R ? ds[r] : 0.0f;
-            far_hi += d >= a.R && d > -a.R ? ds[r] : 0.0f;
-            const bool in = valid && d > -a.R && d < a.R;
-            if (in && hi == 0) lds_add(h + e, ds[r]);
-            __builtin_amdgcn_wave_barrier();  // (keeps the compiler from making one instruction of the two)
-            if (in && hi == 1) lds_add(h + e, ds[r]);
-            __builtin_amdgcn_wave_barrier();
+            for (int n = 0; n < 4; ++n) {
+              unsigned up[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(ds[4 * n + e]), 0u, false, false);
+                v = dpp_f<0x138>(v) + __uint_as_float(two[0]);
+                up[e] = two[1];
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v = dpp_f<0x138>(v) + __uint_as_float(up[e]);
+            }
+            const int d = key0 + 31 - low - l;
+            if (d <= -a.R) far_lo += v;
+            else if (d >= a.R) far_hi += v;
+            else lds_add(h + d, v);
+          } else {
+            // One key of the run a step: the 32 rows of a half wave stand at different distances or in different heads, so
+            // no two lanes of a half add to one entry; the halves go one after the other, and a wave's LDS operations are
+            // done in order: the sums have a fixed order without waiting for each.
+            h += d0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int e = 8 * (r / 4) + r % 4, d = d0 + e;
+              far_lo += d <= -a.R ? ds[r] : 0.0f;
+              far_hi += d >= a.R && d > -a.R ? ds[r] : 0.0f;
+              const bool in = valid && d > -a.R && d < a.R;
+              if (in && hi == 0) lds_add(h + e, ds[r]);
+              __builtin_amdgcn_wave_barrier();  // (keeps the compiler from making one instruction of the two)
+              if (in && hi == 1) lds_add(h + e, ds[r]);
+              __builtin_amdgcn_wave_barrier();
+            }
           }
         }
       }
@@ -477,7 +486,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
 
   if (BIAS) {  // the far sums of the wave's rows, head by head
     for (int i = 0; i < a.G; ++i) {
-      const float lo = wave_sum_dpp(valid && g == i ? far_lo : 0.0f), up = wave_sum_dpp(valid && g == i ? far_hi : 0.0f);
+      // (a lane of an invalid row holds zeros, or with one head a group sums of other rows)
+      const float lo = wave_sum_dpp(g == i ? far_lo : 0.0f), up = wave_sum_dpp(g == i ? far_hi : 0.0f);
       if (l == 0) {
         hist[wv][i * width] += lo;
         hist[wv][i * width + 2 * a.R] += up;

@@ -81,7 +81,7 @@ struct Rows {
     at = ((size_t)(j.q0 + (valid ? tok : 0)) * a.Hk + j.hk) * a.G + (valid ? g : 0);
     seen = valid ? keys_seen(a, j, r) : 0;
     pos = tok + j.nk - j.nq;
-    gb = (valid ? g : 0) * (2 * a.R + 1) + a.R;
+    gb = bias_row(a.G, a.R, valid ? g : 0);
     const e16_t* p = a.q + at * D + 8 * hi;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
@@ -105,10 +105,7 @@ struct Rows {
       } else if (key0 + 31 - low <= -a.R) {
         c = tab[gb - a.R];
       } else {
-        const int d0 = key0 + 4 * hi - pos;
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = fmaf(s[r], sc, tab[gb + min(max(d0 + 8 * (r / 4) + r % 4, -a.R), a.R)]);
+        add_bias(s, sc, tab + gb, key0 + 4 * hi - (valid ? pos : low), a.G, a.R);  // (a position of the wave's)
         sc = 1.0f;
       }
     }
@@ -174,7 +171,7 @@ __device__ __forceinline__ void store_row(const FwdArgs& a, size_t at, int col, 
 }
 
 template <int D, bool BIAS>
-__device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* lds, const float* tab) {
+__device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* lds, float* tab) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
   const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -207,6 +204,7 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
     for (int i = 0; i < NI; ++i) dma16_at(rv, dst + TILE_BYTES + i * 1024, src[i], 0u);
   };
   if (j.c0 < j.c1) issue(j.c0, 0);
+  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, j.hk);
   dma_wait();
   __syncthreads();
   for (int c = j.c0; c < j.c1; ++c) {
@@ -267,7 +265,7 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
 
 // up to 32 rows; `lds`: 64 KB of staging, `stats`: [4 waves][m | l][64 lanes]
 template <int D, bool BIAS>
-__device__ __forceinline__ void narrow_tile(const FwdArgs& a, const Job& j, char* lds, float* stats, const float* tab) {
+__device__ __forceinline__ void narrow_tile(const FwdArgs& a, const Job& j, char* lds, float* stats, float* tab) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, RUN = 32 * ROW, NI = D / 16, LPR = D / 8;
   const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -299,6 +297,10 @@ __device__ __forceinline__ void narrow_tile(const FwdArgs& a, const Job& j, char
   if (u < end) {
     issue(j.k, u, kd);
     issue(j.v, u, vd);
+  }
+  if (BIAS) {
+    fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, j.hk);
+    __syncthreads();
   }
   for (; u < end; u += 4) {
     const bool more = u + 4 < end;
@@ -366,7 +368,7 @@ __device__ __forceinline__ void narrow_tile(const FwdArgs& a, const Job& j, char
 }
 
 template <int D, bool BIAS>
-__device__ __forceinline__ void run_tile(const FwdArgs& a, const Job& j, char* lds, float* stats, const float* tab) {
+__device__ __forceinline__ void run_tile(const FwdArgs& a, const Job& j, char* lds, float* stats, float* tab) {
   if (j.nq * a.G - j.t * TILE <= 32) narrow_tile<D, BIAS>(a, j, lds, stats, tab);
   else wide_tile<D, BIAS>(a, j, lds, tab);
 }
@@ -377,15 +379,12 @@ template <int D, bool BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_fwd_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
   __shared__ float stats[4 * 128];
-  __shared__ float tab[BIAS ? BIAS_ROWS : 1];
+  __shared__ float tab[BIAS ? BIAS_TABLE : 1];
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
   int b;
+  Seq s;
   Job j;
-  if (!tile_of<TILE>(a.cu_q, a.B, a.Tq, a.G, w,
-                     [&](int i) { return (list_rows(a.cu_q, a.B, a.Tq, a.G, i) + TILE - 1) / TILE; },
-                     [&](int i) { return list_keys(a.cu_k, a.B, a.Tk, i); }, b, j.t))
-    return;
-  const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, b);
+  if (!tile_of<TILE, false>(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, a.G, w, s, b, j.t)) return;
   j.t = (s.nq * a.G + TILE - 1) / TILE - 1 - j.t;
   j.k = a.k + ((size_t)s.k0 * a.Hk + hk) * D;
   j.v = a.v + ((size_t)s.k0 * a.Hk + hk) * D;
@@ -397,7 +396,6 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_fwd_kernel(FwdArg
   j.part = nullptr;
   j.c0 = 0;
   j.c1 = tile_chunks(a, j);
-  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
   run_tile<D, BIAS>(a, j, lds, stats, tab);
 }
 
@@ -507,7 +505,7 @@ template <int D, bool BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_ranges_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
   __shared__ float stats[4 * 128];
-  __shared__ float tab[BIAS ? BIAS_ROWS : 1];
+  __shared__ float tab[BIAS ? BIAS_TABLE : 1];
   const int w = blockIdx.x / a.Hk;
   const PackedLists shape{a};
   const Lists<PackedLists> lists(shape, a.B + 1);
@@ -523,7 +521,6 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_ranges_kernel(Fwd
   j.nk = s.nk;
   j.causal = a.causal;
   take_range(a, j, r, w, D, false);
-  if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, j.hk);
   run_tile<D, BIAS>(a, j, lds, stats, tab);
 }
 

@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 DTYPES = {torch.bfloat16: "", torch.float16: "_f16"}     # token dtype -> suffix of the entry points
-MAX_BIAS_ROWS = 816                                      # ES_PACKED_BIAS_ROWS of include/packed_hip.h
+MAX_BIAS_ROWS = 784                                      # ES_PACKED_BIAS_ROWS of include/packed_hip.h
 
 
 # ------------------------------------------------------------------ workspace sizes
@@ -193,7 +193,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: Op
     With nq queries and nk keys query i stands at position i + nk - nq (the last query at the last key): with causal it sees
     the keys up to that position. A row that sees no key gives zeros and an LSE of -inf, and no gradient. scale: 1 / sqrt(D)
     if None. bias [num_buckets, H] with buckets (`relative_buckets`, int32 [2 R + 1]) adds bias[buckets[d + R], h] to the
-    score of a key at distance d from the query, d clamped to -R .. R; (H // Hk) * (2 R + 1) is at most 816.
+    score of a key at distance d from the query, d clamped to -R .. R; (H // Hk) * (2 R + 1) is at most 784.
 
     Returns out like q, with return_lse also the natural-log LSE [Tq, H] ([B, Lq, H]) in float32 (no gradient). Gradients
     are deterministic, and those of a bias are summed in float32; the backward itself is not differentiable."""

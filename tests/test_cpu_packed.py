@@ -144,6 +144,19 @@ def test_range_items_fit_the_grid():
         assert items <= sum(tiles) + resident // Hk + 1
 
 
+def test_tokens_of_a_row_tile():
+    """The KV owner's token of a row within a tile (csrc/packed_bwd.hip, token_in_tile): (row + 1/2) / G in float32, rows up to
+    G + 63 from the tile's first token on."""
+    import numpy as np
+    half, rows = np.float32(0.5), np.arange(64)
+    for G in range(1, 4097):
+        inv = np.float32(1) / np.float32(G)
+        for first in {0, 1, G // 2, G - 1}:
+            want = (first + rows) // G
+            assert (((rows.astype(np.float32) + (np.float32(first) + half)) * inv).astype(np.int64) == want).all()
+            assert ((((first + rows).astype(np.float32) + half) * inv).astype(np.int64) == want).all()
+
+
 def test_division_by_multiplication():
     """fast_div of csrc/packed.h: mul = ceil(2^(32 + sh) / d), 2^sh < d <= 2^(sh + 1)."""
     rng = random.Random(7)
@@ -225,10 +238,10 @@ def test_packed_bias_refusals():
         packed_attention(q, k, k, cu, bias=w, buckets=t[:-1].contiguous())
     with pytest.raises(TypeError, match="int32"):
         packed_attention(q, k, k, cu, bias=w, buckets=t.long())
-    with pytest.raises(ValueError, match="at most 816"):
-        packed_attention(q, k, k, cu, bias=w, buckets=torch.zeros(409, dtype=torch.int32))
-    with pytest.raises(ValueError, match="on the GPU"):     # 2 heads a group, 407 distances: 814
-        packed_attention(q, k, k, cu, bias=w, buckets=torch.zeros(407, dtype=torch.int32))
+    with pytest.raises(ValueError, match="at most 784"):
+        packed_attention(q, k, k, cu, bias=w, buckets=torch.zeros(393, dtype=torch.int32))
+    with pytest.raises(ValueError, match="on the GPU"):     # 2 heads a group, 391 distances: 782
+        packed_attention(q, k, k, cu, bias=w, buckets=torch.zeros(391, dtype=torch.int32))
 
 
 def test_shared_prefix_refusals():
@@ -287,8 +300,8 @@ def test_c_entry_points_refuse_before_any_launch():
             (lambda: fwd(Tq=1 << 29), 2, "too many rows"), (lambda: fwd(Tk=1 << 30), 2, "too many rows"),
             (lambda: fwd(wsb=100), 1, "workspace too small"), (lambda: fwd(ws=None), 1, "workspace too small"),
             (lambda: fwd(bias=p, nb=4, R=3), 1, "needs buckets"), (lambda: fwd(bias=p, buckets=p, R=3), 1, "needs buckets"),
-            (lambda: fwd(bias=p, buckets=p, nb=4, R=204), 2, "at most 816"),
-            (lambda: fwd(bias=p, buckets=p, nb=4, R=1 << 30), 2, "at most 816"),
+            (lambda: fwd(bias=p, buckets=p, nb=4, R=196), 2, "at most 784"),
+            (lambda: fwd(bias=p, buckets=p, nb=4, R=1 << 30), 2, "at most 784"),
             (lambda: fwd(D=96, suffix="_f16"), 2, "64 or 128"),
             (lambda: bwd(dout=None), 1, "null tensor"), (lambda: bwd(dq=None), 1, "null tensor"),
             (lambda: bwd(dk=None), 1, "null tensor"), (lambda: bwd(ws=None), 1, "null tensor"),
