@@ -19,6 +19,8 @@ the ABI:
 The reference registers its native op set as a pybind11 module (csrc/vsa/vsa2_api.cpp:904-941); here the same role
 is played by torch.library (TORCH_LIBRARY), loaded with torch.ops.load_library.
 
+csrc/torch/packed.cpp adds written operators in the same namespace: the packed-sequence calls with their outputs and gradient.
+
 The library is built by build_lib.build() (g++, host code only) into lib/libechosparse_torch.so. It does not link
 libechosparse_hip.so: its C symbols resolve against the copy the ctypes binding loaded with RTLD_GLOBAL, so an
 alternative build of the ABI (ECHOSPARSE_HIP_LIB) serves both bindings.
@@ -26,11 +28,13 @@ alternative build of the ABI (ECHOSPARSE_HIP_LIB) serves both bindings.
 import os
 import re
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 HEADERS = [os.path.join(ROOT, "include", h) for h in ("echosparse_hip.h", "vsa_hip.h", "packed_hip.h")]
 SOURCE = os.path.join(HERE, "csrc", "torch", "ops.cpp")
+WRITTEN = [os.path.join(HERE, "csrc", "torch", "packed.cpp")]     # operators with outputs and a gradient of their own
 LIB = os.path.join(HERE, "lib", "libechosparse_torch.so")
 NAMESPACE = "echosparse_gfx950"
 
@@ -240,17 +244,26 @@ def generate():
 
 
 def build(verbose=False):
-    """Generate and compile lib/libechosparse_torch.so (host C++ against the installed torch)."""
+    """Generate and compile lib/libechosparse_torch.so (host C++ against the installed torch): the generated operators and
+    the written ones, side by side."""
     import torch.utils.cpp_extension as ce
-    src = generate()
+    sources = [generate(), *WRITTEN]
     tlib = os.path.join(os.path.dirname(ce.__file__), "..", "lib")
     incs = [f"-I{p}" for p in ce.include_paths(device_type="cuda")]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", *incs, src,
-           "-o", LIB + ".tmp", f"-L{os.path.abspath(tlib)}", "-lc10", "-lc10_hip", "-ltorch_cpu"]
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"torch operator library failed to build:\n{r.stderr[-4000:]}")
+    obj_dir = os.path.join(HERE, "_build", os.path.basename(LIB))
+    os.makedirs(obj_dir, exist_ok=True)
+    objs = [os.path.join(obj_dir, os.path.basename(src) + ".o") for src in sources]
+    cmds = [["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", *incs, "-c", src, "-o", obj]
+            for src, obj in zip(sources, objs)]
+    link = ["g++", "-shared", *objs, "-o", LIB + ".tmp", f"-L{os.path.abspath(tlib)}", "-lc10", "-lc10_hip", "-ltorch_cpu"]
+    with ThreadPoolExecutor(max_workers=len(cmds)) as ex:
+        results = list(ex.map(lambda c: subprocess.run(c, capture_output=True, text=True), cmds))
+    if all(r.returncode == 0 for r in results):
+        results.append(subprocess.run(link, capture_output=True, text=True))
+    failed = [r for r in results if r.returncode != 0]
+    if failed:
+        raise RuntimeError(f"torch operator library failed to build:\n{failed[0].stderr[-4000:]}")
     os.replace(LIB + ".tmp", LIB)
     if verbose:
         print(f"built {LIB} ({len(entry_points())} operators)")

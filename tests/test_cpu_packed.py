@@ -57,27 +57,6 @@ def test_relative_buckets_refuse_what_has_no_steps(args):
         relative_buckets(*args)
 
 
-# ------------------------------------------------------------------ workspace sizes
-def test_workspace_sizes_match_the_library():
-    so, rng = _lib.lib(), random.Random(3)
-    ranged = 0
-    for _ in range(4000):
-        Hk = rng.choice([1, 2, 3, 8, 40])
-        H = Hk * rng.choice([1, 2, 3, 5, 8, 16])
-        B, Tq, Tk = rng.randint(1, 70), rng.choice([0, 1, rng.randint(2, 300), rng.randint(300, 60000)]), rng.randint(0, 200000)
-        D, R = rng.choice([64, 128]), rng.choice([1, 91, 128])
-        got = packed.forward_workspace_bytes(B, Tq, Tk, H, Hk, D)
-        ranged += got > 0
-        assert got == so.es_packed_fwd_workspace(B, Tq, Tk, H, Hk, D)
-        for with_bias in (0, 1):
-            assert (packed.backward_workspace_bytes(B, Tq, Tk, H, Hk, D, R, with_bias)
-                    == so.es_packed_bwd_workspace(B, Tq, Tk, H, Hk, D, R, with_bias))
-        n = rng.randint(1, 40)
-        assert (packed.shared_workspace_bytes(B, n, Tk, 100, H, Hk, D)
-                == so.es_shared_prefix_workspace(B, n, Tk, 100, H, Hk, D))
-    assert 500 < ranged < 3500
-
-
 # ------------------------------------------------------------------ what the kernels derive from the lengths
 def _starts(lens):
     out = [0]
@@ -321,6 +300,22 @@ def test_empty_calls_launch_nothing():
 
 
 # ------------------------------------------------------------------ the ABI and the sources
+def test_operators_trace_with_meta_tensors():
+    """Shapes and dtypes of the written operators and of their gradient, without a GPU."""
+    q = torch.empty(10, 4, 64, dtype=torch.float16, device="meta", requires_grad=True)
+    k = torch.empty(12, 2, 64, dtype=torch.float16, device="meta", requires_grad=True)
+    cu = torch.empty(3, dtype=torch.int32, device="meta")
+    out, lse = packed_attention(q, k, k, cu, cu, return_lse=True)
+    assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (10, 4) and lse.dtype == torch.float32
+    assert out.requires_grad and not lse.requires_grad
+    dq, dk = torch.autograd.grad(out, [q, k], torch.empty_like(out))
+    assert dq.shape == q.shape and dk.shape == k.shape
+    c = torch.empty(3, 7, 2, 64, dtype=torch.float16, device="meta")
+    t = torch.empty(3, 5, 4, 64, dtype=torch.float16, device="meta")
+    out, lse = shared_prefix_attention(t, k.detach(), k.detach(), c, c, cu, return_lse=True)
+    assert out.shape == t.shape and lse.shape == (3, 5, 4)
+
+
 def test_header_and_bindings_agree():
     text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "packed_hip.h")).read(), flags=re.S)
     found = re.findall(r"\b(es_[a-z0-9_]+)\s*\(([^)]*)\)\s*;", text)

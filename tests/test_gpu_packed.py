@@ -17,6 +17,11 @@ def _api():
     return api
 
 
+def _workspace(B, Tq, Tk, H, Hk, D):
+    from self_trainable_or_free_attn_amd import _lib
+    return _lib.lib().es_packed_fwd_workspace(B, Tq, Tk, H, Hk, D)
+
+
 def _cu(lens, dev):
     return torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=dev)
 
@@ -87,15 +92,13 @@ def test_forward(dev, D, dtype, H, Hk, causal, lens, keys):
 ])
 @pytest.mark.parametrize("causal", [False, True])
 def test_key_ranges(dev, D, dtype, lens, keys, H, Hk, causal):
-    from self_trainable_or_free_attn_amd import packed
-    assert packed.forward_workspace_bytes(len(lens), sum(lens), sum(keys), H, Hk, D) > 0
+    assert _workspace(len(lens), sum(lens), sum(keys), H, Hk, D) > 0
     _case(lens, keys, H, Hk, D, dtype, causal, dev, seed=2)
 
 
 @pytest.mark.parametrize("D, dtype, T, H, Hk", [(128, BF, 2200, 64, 16), (64, FP, 4300, 64, 32)])
 def test_whole_tiles(dev, D, dtype, T, H, Hk):
-    from self_trainable_or_free_attn_amd import packed
-    assert packed.forward_workspace_bytes(2, T, T, H, Hk, D) == 0
+    assert _workspace(2, T, T, H, Hk, D) == 0
     _case([T - 130, 130], [T - 130, 130], H, Hk, D, dtype, True, dev, seed=3)
 
 
@@ -479,8 +482,21 @@ def test_refusals_on_the_gpu(dev):
         api.packed_attention(q, q, q, cu)
     out = api.packed_attention(q, q, q)
     gr, = torch.autograd.grad(out, [q], torch.ones_like(out), create_graph=True)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(RuntimeError, match="not differentiable"):
         gr.sum().backward()
+    # the operators below refuse what would hand a kernel other memory than it expects
+    from self_trainable_or_free_attn_amd import _lib
+    op, x = _lib.ops().packed_attention, q.detach()
+    cu = cu.to(dev)
+    for bad in ((x.transpose(0, 1), x, x, None, None, None, None, 1), (x, x, x[:3], None, None, None, None, 1),
+                (x, x, x.half(), None, None, None, None, 1), (x, x, x, None, cu, cu, None, 2),
+                (x, x, x, None, cu.long(), None, None, 1), (x, x, x.cpu(), None, None, None, None, 1),
+                (x, x, x, torch.zeros(4, 3, device=dev), None, None, cu[:1], 1),
+                (x, x, x, torch.zeros(4, 2, device=dev), None, None, cu, 1),
+                (x, x, x, torch.zeros(4, 2, device=dev), None, None, None, 1), (x, x, x, None, None, None, None, 0),
+                (x, x, x, None, None, None, None, 3), (x.float(), x.float(), x.float(), None, None, None, None, 1)):
+        with pytest.raises(RuntimeError):
+            op(*bad, False, 1.0)
 
 
 def test_compiled(dev):
