@@ -1,11 +1,10 @@
 // Backward of attention over packed sequences (gfx950, MFMA 32x32x16, bf16 / fp16).
 //
 // With P = exp(S - lse) and dS = P (dP - delta), dP = dO V^T, delta = rowsum(dO O) (rows that see no key: P = 0):
-//   row_stats   one pass over dO and O: lse in log2 units (+inf for rows without keys) and delta, laid out by kv head and
-//               row of the list (token, head in group), so that a row tile's values are contiguous (with the fp16 factor of
-//               P and its inverse in them)
 //   bwd_q       one workgroup per (64 rows, kv head): dQ = scale dS K over the keys, 2 row groups x 2 key halves, S^T and
-//               dP^T with rows on lanes; with a bias it also sums dS by clamped distance
+//               dP^T with rows on lanes; with a bias it also sums dS by clamped distance. It leaves lse in log2 units (+inf
+//               for rows without keys) and delta for bwd_kv, laid out by kv head and row of the list (token, head in group),
+//               so that a row tile's values are contiguous, the fp16 factor of P and its inverse in them.
 //   bwd_kv      one workgroup per (64 keys, kv head): dV = P^T dO and dK = scale dS^T Q over all rows of the list that see
 //               the keys, which sums over the heads of a group without atomics. Four waves = 2 key halves x 2 row halves
 //               of each staged 64-row tile; S and dP come out with keys on lanes, so that P and dS are B operands.
@@ -53,27 +52,6 @@ struct BwdArgs {
 // *p += x without waiting for it (ds_add_f32); lanes of one instruction must not share an address where order matters
 __device__ __forceinline__ void lds_add(float* p, float x) {
   __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float*)p, x, 0, 0, false);
-}
-
-// D / 8 lanes a row of dO and O
-template <int D>
-__global__ __launch_bounds__(256) void row_stats_kernel(BwdArgs a) {
-  constexpr int LPR = D / 8;
-  const size_t row = (size_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  if (row >= (size_t)a.Tq * a.H) return;
-  const size_t at = row * D + 8 * (threadIdx.x % LPR);
-  const ev8 x = *reinterpret_cast<const ev8*>(a.dout + at), y = *reinterpret_cast<const ev8*>(a.out + at);
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sum = fmaf((float)x[i], (float)y[i], sum);
-#pragma unroll
-  for (int m = 1; m < LPR; m <<= 1) sum += __shfl_xor(sum, m, 64);
-  if (threadIdx.x % LPR) return;
-  const int tok = (int)(row / a.H), h = (int)(row - (size_t)tok * a.H), hk = divide(a.div_g, h);
-  const size_t to = ((size_t)hk * a.Tq + tok) * a.G + (h - hk * a.G);
-  const float l = a.lse[row];
-  a.lse2[to] = l == -INFINITY ? INFINITY : l * LOG2E - P_SHIFT;
-  a.delta[to] = sum * P_BACK;
 }
 
 template <int D, bool BIAS>
@@ -137,7 +115,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
     if (wv < 2)
       dma4(make_srd((wv == 0 ? a.lse2 : a.delta) + list + (size_t)i * BK, (unsigned)min(rows - i * BK, BK) * 4u),
            st_s[sb][wv], 4u * l, 0u);
-    if (BIAS && wv == 2) {
+    if (BIAS && a.G > 1 && wv == 2) {
       const int tok = token_in_tile(rel + l);
       pos_s[sb][0][l] = t0 + tok + shift;
       pos_s[sb][1][l] = bias_row(a.G, a.R, rel + l - tok * a.G);
@@ -186,11 +164,28 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
     const int t0 = divide(a.div_g, i * BK), rel = i * BK - t0 * a.G;
     const bool masked = (a.causal && t0 + token_in_tile(rel + 32 * qh) + shift < kb * BK + 32 * kh + 31) ||
                         (BIAS && (i + 1) * BK > rows);
+    // one head a group: rows stand at consecutive positions, so a lane's 16 entries of the bias table are a fixed pattern
+    const int key0 = kb * BK + 32 * kh, pos0 = i * BK + 32 * qh + shift;
+    const float* one = nullptr;
+    float far = 0.0f;
+    if (BIAS && a.G == 1) {
+      if (key0 - pos0 - 31 >= a.R) far = tab[bias_row(1, a.R, 0) + a.R];
+      else if (key0 + 31 - pos0 <= -a.R) far = tab[bias_row(1, a.R, 0) - a.R];
+      else one = tab + bias_row(1, a.R, 0) + key - pos0 - 4 * hi;
+    }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int r0 = 32 * qh + 8 * g + 4 * hi;
       f32x4 l4 = *reinterpret_cast<const f32x4*>(&st_s[sb][0][r0]);
-      if (BIAS) {
+      if (BIAS && a.G == 1) {
+        if (one != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) l4[e] -= one[-(8 * g + e)];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) l4[e] -= far;
+        }
+      } else if (BIAS) {
         const int4 p4 = *reinterpret_cast<const int4*>(&pos_s[sb][0][r0]), b4 = *reinterpret_cast<const int4*>(&pos_s[sb][1][r0]);
         const int ps[4] = {p4.x, p4.y, p4.z, p4.w}, gs[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
@@ -285,7 +280,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
   const int r0 = t * BK + 32 * rg, row = r0 + lq;
   const bool valid = row < rows;
   const int tok = divide(a.div_g, row), g = valid ? row - tok * a.G : 0, pos = tok + shift, gb = bias_row(a.G, a.R, g);
-  const size_t at = (((size_t)(s.q0 + (valid ? tok : 0)) * a.Hk + hk) * a.G + g) * D;
+  const size_t qrow = ((size_t)(s.q0 + (valid ? tok : 0)) * a.Hk + hk) * a.G + g, at = qrow * D;
   const size_t list = ((size_t)hk * a.Tq + s.q0) * a.G + (valid ? row : 0);
   const int seen = !valid ? 0 : a.causal ? min(max(pos + 1, 0), s.nk) : s.nk;
   // the wave's rows: the first one sees the fewest keys, the last one the most
@@ -303,8 +298,19 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     qreg[ks] = valid ? *reinterpret_cast<const ev8*>(a.q + at + 16 * ks + 8 * hi) : z;
     dreg[ks] = valid ? *reinterpret_cast<const ev8*>(a.dout + at + 16 * ks + 8 * hi) : z;
   }
-  const float ls = valid ? a.lse2[list] + P_SHIFT : INFINITY;
-  float dl = valid ? a.delta[list] * (1.0f / P_BACK) : 0.0f;
+  const float lse = valid ? a.lse[qrow] : -INFINITY, ls = lse == -INFINITY ? INFINITY : lse * LOG2E;
+  const bool exact = end > 0 && (BIAS || end <= EXACT_CHUNKS);
+  float dl = 0.0f;
+  if (!exact) {
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const ev8 z = {};
+      const ev8 x = valid ? *reinterpret_cast<const ev8*>(a.out + at + 16 * ks + 8 * hi) : z;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dl = fmaf((float)x[e], (float)dreg[ks][e], dl);
+    }
+    dl = sum_xor32(dl);
+  }
   const unsigned stride = (unsigned)a.Hk * ROW;
   unsigned src[NI];
 #pragma unroll
@@ -374,7 +380,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
   dma_wait();
   __syncthreads();
   int sb = 0;
-  if (end > 0 && (BIAS || end <= EXACT_CHUNKS)) {
+  if (exact) {
     float num = 0.0f, den = 0.0f;
     for (int c = 0; c < end; ++c) {
       ev8 kf[NKS];
@@ -398,7 +404,10 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
     __syncthreads();
     const float2 s0 = reinterpret_cast<const float2*>(hist[rg])[lq], s1 = reinterpret_cast<const float2*>(hist[rg + 2])[lq];
     if (s0.y + s1.y > 0.0f) dl = (s0.x + s1.x) / (s0.y + s1.y);
-    if (valid && kh == 0 && hi == 0) a.delta[list] = dl * P_BACK;
+  }
+  if (valid && kh == 0 && hi == 0) {
+    a.lse2[list] = ls - P_SHIFT;
+    a.delta[list] = dl * P_BACK;
   }
   if (BIAS) {
     __syncthreads();
@@ -609,12 +618,6 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
   a.k_tiles = (int)tile_numbers<BK>(B, Tk, 1);
   ES_REQUIRE((long long)a.q_tiles * Hk < (1LL << 31) && (long long)a.k_tiles * Hk < (1LL << 31), ES_ERR_UNSUPPORTED,
              "packed: grid too large");
-  if (Tq > 0) {
-    const long long per = D == 64 ? 32 : 16;
-    const dim3 grid((unsigned)(((long long)Tq * H + per - 1) / per));
-    if (D == 64) hipLaunchKernelGGL((row_stats_kernel<64>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((row_stats_kernel<128>), grid, dim3(256), 0, stream, a);
-  }
   if (Tq > 0) {
     const dim3 grid((unsigned)(a.q_tiles * Hk));
     if (D == 64) {

@@ -36,7 +36,8 @@ struct FwdArgs {
   FastDiv div_g;
   int B, Tq, Tk, H, Hk, G, R, num_buckets, causal;
   int tiles;      // tile numbers of a head
-  int target;     // ranged launches: workgroups that the GPU holds at once
+  int2* plan;       // ranged launches: (ranges a tile, first item) of each list
+  float inv_slots;  // ranged launches: Hk / the workgroups that the GPU holds at once
   float scale;    // log2(e) * softmax scale
   // shared prefix: rows 0 .. P - 1 of k_prefix / v_prefix are seen by every row
   const e16_t *kp, *vp;
@@ -401,11 +402,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_fwd_kernel(FwdArg
 
 // ------------------------------------------------------------------------------------------------ key ranges
 // A ranged launch cuts each tile's chunks into ranges of about the same number of chunks, as many as fill the GPU once.
-// Every wave derives the plan from the lengths by itself (a load and some shuffles a 64 sequences), so the lengths stay on
+// Every wave derives the plan from the lengths by itself (a load and some DPP sums a 64 sequences), so the lengths stay on
 // the device and no launch is spent on it. `lists` lists of rows, list i with tiles(i) tiles of chunks(i) chunks each:
-//   sum = Hk * total of tiles * chunks; a range has at least ceil(sum / target) chunks (and at least four where a tile has
-//   up to 32 rows, eight where it has more and its partial costs more), list i has ceil(chunks / that) ranges a tile.
-// Items are numbered list by list, tile by tile, range by range.
+//   list i has ceil(chunks / per) ranges a tile, `per` at least its fair share, all tiles' chunks * Hk / target (and at least
+//   four where a tile has up to 32 rows, eight where it has more and its partial costs more). Among the fair share and the
+//   chunk counts that cut the longest list into whole numbers of ranges near it the one with the shortest schedule is taken:
+//   the longest item times the rounds that the items over half its size need, or all work evenly spread. At the fair share
+//   alone the items may be a few more than the GPU holds, and the last ones take as long again (1280 rows against 32760 keys,
+//   8 heads, caches of 16 to 4096: 270 us, with the search 250).
+// Items are numbered list by list, tile by tile, range by range; up to 64 lists: those with items over half the longest one's
+// size first, since workgroups are dispatched in order. The first workgroup leaves the plan for the merge.
 struct ListShape {
   int tiles, chunks, rows;
 };
@@ -413,10 +419,33 @@ struct Ranges {
   int list, ranges, item0;  // the list, its ranges a tile, its first item
 };
 
-__device__ __forceinline__ int ranges_of(const ListShape& x, int per) {
-  const int least = max(per, x.rows <= 32 ? 4 : 8);
-  return max((x.chunks + least - 1) / least, 1);
+// sums of the lanes up to this one (DPP row shifts and broadcasts, as wave_sum_dpp)
+template <int CTRL, int ROWMASK = 0xF>
+__device__ __forceinline__ int dpp_i(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWMASK, 0xF, true);
 }
+__device__ __forceinline__ int wave_scan(int x) {
+  x += dpp_i<0x111>(x);
+  x += dpp_i<0x112>(x);
+  x += dpp_i<0x114>(x);
+  x += dpp_i<0x118>(x);
+  x += dpp_i<0x142, 0xA>(x);
+  x += dpp_i<0x143, 0xC>(x);
+  return x;
+}
+
+// ceil(x / y) of positive values by a reciprocal: up to one in 2^22 off on either side, which moves a range's border but
+// leaves the plan the same on every wave
+__device__ __forceinline__ float parts(float x, float y) { return ceilf(x * __builtin_amdgcn_rcpf(y) - 1e-5f); }
+
+// A list's ranges a tile and chunks a range.
+struct Cut {
+  float ranges, size;
+  __device__ __forceinline__ Cut(const ListShape& x, float per) {
+    ranges = fmaxf(parts((float)x.chunks, fmaxf(per, x.rows <= 32 ? 4.0f : 8.0f)), 1.0f);
+    size = x.tiles > 0 ? parts((float)x.chunks, ranges) : 0.0f;
+  }
+};
 
 // The shapes of the lists, a lane each; up to 64 are read once.
 template <class F>
@@ -432,45 +461,70 @@ struct Lists {
     return i0 + lane_id() < lists ? shape(i0 + lane_id()) : ListShape{0, 0, 0};
   }
 
-  // chunks of a range before the two lower limits
-  __device__ __forceinline__ int range_chunks(const FwdArgs& a) const {
-    unsigned long long sum = 0;
+  // `per`, and the longest item's chunks. (Sums in float32: every wave computes the same ones.)
+  __device__ __forceinline__ float range_chunks(const FwdArgs& a, float& longest_item) const {
+    float sum = 0.0f, most = 0.0f;
     for (int i0 = 0; i0 < lists; i0 += 64) {
       const ListShape x = at(i0);
-      sum += (unsigned long long)x.tiles * x.chunks;
+      sum += wave_sum_dpp((float)x.tiles * (float)x.chunks);
+      most = fmaxf(most, wave_max_dpp(x.tiles > 0 ? (float)x.chunks : 0.0f));
     }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
-    return (int)min((sum * a.Hk + a.target - 1) / a.target, 1ull << 30);
+    const float fair = fmaxf(ceilf(sum * a.inv_slots), 1.0f);
+    const int near = (int)parts(most, fair);
+    float best = fair, least = INFINITY;
+    longest_item = most;
+    for (int n = max(near - 2, 1); n <= near; ++n) {
+      const float per = fmaxf(parts(most, (float)n), fair);
+      float size = 0.0f, big = 0.0f, work = 0.0f;
+      for (int i0 = 0; i0 < lists; i0 += 64) size = fmaxf(size, wave_max_dpp(Cut(at(i0), per).size));
+      for (int i0 = 0; i0 < lists; i0 += 64) {
+        const ListShape x = at(i0);
+        const Cut c(x, per);
+        const float items = (float)x.tiles * c.ranges;
+        big += wave_sum_dpp(2.0f * c.size > size ? items : 0.0f);
+        work += wave_sum_dpp(items * c.size);
+      }
+      const float time = fmaxf(ceilf(big * a.inv_slots) * size, work * a.inv_slots);
+      if (time < 0.98f * least) {  // (more ranges for a shorter schedule only)
+        least = time;
+        best = per;
+        longest_item = size;
+      }
+    }
+    return best;
   }
 
-  // the list that holds item w (BY_LIST: the list w); ranges = 0: none
-  template <bool BY_LIST>
-  __device__ __forceinline__ Ranges find(int per, int w) const {
-    int base = 0;
+  // the list that holds item w, ranges = 0: none; `plan`: where the first workgroup leaves (ranges, first item) of each list
+  __device__ __forceinline__ Ranges find(const FwdArgs& a, int w) const {
+    float longest;
+    const float per = range_chunks(a, longest);
+    const bool leave = blockIdx.x == 0 && threadIdx.x < 64;
+    int first = 0;
+    Ranges found = {0, 0, 0};
     for (int i0 = 0; i0 < lists; i0 += 64) {
       const ListShape x = at(i0);
-      const int i = i0 + lane_id(), ranges = i < lists ? ranges_of(x, per) : 0, items = x.tiles * ranges;
-      int upto = items;
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) {
-        const int y = __shfl_up(upto, m, 64);
-        if (lane_id() >= m) upto += y;
-      }
-      const unsigned long long hit = __builtin_amdgcn_ballot_w64(BY_LIST ? i == w : base + upto > w);
+      const Cut c(x, per);
+      const int i = i0 + lane_id(), ranges = (int)c.ranges, items = i < lists ? x.tiles * ranges : 0;
+      const bool late = lists <= 64 && 2.0f * c.size <= longest;
+      const int early_upto = wave_scan(late ? 0 : items), early = __builtin_amdgcn_readlane(early_upto, 63);
+      const int late_upto = wave_scan(late ? items : 0);
+      const int item0 = first + (late ? early + late_upto : early_upto) - items;
+      if (leave && i < lists) a.plan[i] = make_int2(ranges, item0);
+      const unsigned long long hit = __builtin_amdgcn_ballot_w64(item0 <= w && w < item0 + items);
       if (hit) {
         const int from = __builtin_ctzll(hit);
-        Ranges r;
-        r.list = i0 + from;
-        r.ranges = __builtin_amdgcn_readlane(ranges, from);
-        r.item0 = base + __builtin_amdgcn_readlane(upto - items, from);
-        return r;
+        found = Ranges{i0 + from, __builtin_amdgcn_readlane(ranges, from), __builtin_amdgcn_readlane(item0, from)};
+        if (!leave) break;
       }
-      base += __builtin_amdgcn_readlane(upto, 63);
+      first += early + __builtin_amdgcn_readlane(late_upto, 63);
     }
-    return Ranges{0, 0, 0};
+    return found;
   }
 };
+__device__ __forceinline__ Ranges planned(const FwdArgs& a, int list) {
+  const int2 p = a.plan[list];
+  return Ranges{list, __builtin_amdgcn_readfirstlane(p.x), __builtin_amdgcn_readfirstlane(p.y)};
+}
 
 // packed sequences: list b, the rows behind the last sequence being list B
 struct PackedLists {
@@ -509,7 +563,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_ranges_kernel(Fwd
   const int w = blockIdx.x / a.Hk;
   const PackedLists shape{a};
   const Lists<PackedLists> lists(shape, a.B + 1);
-  const Ranges r = lists.find<false>(lists.range_chunks(a), w);
+  const Ranges r = lists.find(a, w);
   if (r.ranges == 0) return;
   const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, r.list);
   Job j;
@@ -531,7 +585,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void shared_prefix_kernel(Fwd
   const int w = blockIdx.x / a.Hk;
   const SharedLists shape{a};
   const Lists<SharedLists> lists(shape, a.B + 1);
-  const Ranges r = lists.find<false>(lists.range_chunks(a), w);
+  const Ranges r = lists.find(a, w);
   if (r.ranges == 0) return;
   Job j;
   j.hk = blockIdx.x - w * a.Hk;
@@ -571,11 +625,8 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
     q0 = (list - 1) * a.n;
     nq = a.n;
     if (t * TILE + (int)blockIdx.y * RPB >= nq * a.G) return;
-    const SharedLists shape{a};
-    const Lists<SharedLists> lists(shape, a.B + 1);
-    const int per = lists.range_chunks(a);
-    own = lists.find<true>(per, list);
-    pre = lists.find<true>(per, 0);
+    own = planned(a, list);
+    pre = planned(a, 0);
   } else {
     list = seq_of_tile<TILE>(a.cu_q, a.B, a.Tq, a.G, w);
     const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, list);
@@ -583,9 +634,7 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
     nq = s.nq;
     t = w - (q0 * a.G / TILE + list);
     if (t < 0 || t * TILE + (int)blockIdx.y * RPB >= nq * a.G) return;
-    const PackedLists shape{a};
-    const Lists<PackedLists> lists(shape, a.B + 1);
-    own = lists.find<true>(lists.range_chunks(a), list);
+    own = planned(a, list);
     if (own.ranges == 1) return;  // (finished by its only range)
   }
   const int rows = min(nq * a.G - t * TILE, TILE), lane = threadIdx.x % LPR, c = lane * 4, n = pre.ranges + own.ranges;
@@ -593,7 +642,8 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
   const float* own0 = a.part + (size_t)(own.item0 + t * own.ranges) * step + (size_t)hk * part_floats(D);
   for (int r = blockIdx.y * RPB + threadIdx.x / LPR; r < rows; r += gridDim.y * RPB) {
     const int all = q0 * a.G + t * TILE + r, rp = SHARED ? all % TILE : 0;  // the row among all rows of the batch
-    const float* pre0 = SHARED ? a.part + (size_t)(all / TILE * pre.ranges) * step + (size_t)hk * part_floats(D) : nullptr;
+    const float* pre0 =
+        SHARED ? a.part + (size_t)(pre.item0 + all / TILE * pre.ranges) * step + (size_t)hk * part_floats(D) : nullptr;
     auto part = [&](int i) { return i < pre.ranges ? pre0 + i * step : own0 + (i - pre.ranges) * step; };
     auto row_of = [&](int i) { return i < pre.ranges ? rp : r; };
     float M = -INFINITY;
@@ -641,6 +691,9 @@ using namespace es;
 
 // Workgroups that the GPU holds at once: 256 CUs, two workgroups each at D = 128 (64 KB of staging), four at D = 64.
 static int resident(int D) { return D == 64 ? 1024 : 512; }
+// Bytes of a ranged launch's workspace: the partials, then the plan.
+static size_t plan_offset(long long items, int D) { return (size_t)items * part_floats(D) * sizeof(float); }
+static size_t range_bytes(long long items, int lists, int D) { return plan_offset(items, D) + (size_t)lists * sizeof(int2); }
 // Items a head of a ranged launch: at most one a tile more than the ranges' chunks fill.
 static long long range_items(long long tiles, int Hk, int D) { return tiles + resident(D) / Hk + 1; }
 // Key ranges are worth a second launch where the tiles do not fill the GPU and the keys are more than a few chunks: 1024 for
@@ -653,12 +706,12 @@ static bool ranged(long long tiles, int B, int Tq, int Tk, int H, int Hk, int D)
 extern "C" size_t es_packed_fwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D) {
   if (B <= 0 || Tq <= 0 || Tk < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
   const long long tiles = tile_numbers<TILE>(B, Tq, H / Hk);
-  return ranged(tiles, B, Tq, Tk, H, Hk, D) ? (size_t)range_items(tiles, Hk, D) * Hk * part_floats(D) * sizeof(float) : 0;
+  return ranged(tiles, B, Tq, Tk, H, Hk, D) ? range_bytes(range_items(tiles, Hk, D) * Hk, B + 1, D) : 0;
 }
 extern "C" size_t es_shared_prefix_workspace(int B, int n, int P, int S, int H, int Hk, int D) {
   if (B <= 0 || n <= 0 || P < 0 || S < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
   const long long G = H / Hk, rows = n * G, tiles = (B * rows + TILE - 1) / TILE + B * ((rows + TILE - 1) / TILE);
-  return (size_t)range_items(tiles, Hk, D) * Hk * part_floats(D) * sizeof(float);
+  return range_bytes(range_items(tiles, Hk, D) * Hk, B + 1, D);
 }
 #endif
 
@@ -697,7 +750,8 @@ extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const voi
     ES_REQUIRE(workspace && workspace_bytes >= es_packed_fwd_workspace(B, Tq, Tk, H, Hk, D), ES_ERR_INVALID,
                "packed: workspace too small");
     a.part = (float*)workspace;
-    a.target = resident(D);
+    a.plan = (int2*)((char*)workspace + plan_offset(range_items(a.tiles, Hk, D) * Hk, D));
+    a.inv_slots = (float)Hk / (float)resident(D);
     const dim3 grid((unsigned)(range_items(a.tiles, Hk, D) * Hk)), merge((unsigned)(a.tiles * Hk), 4);
     if (D == 64) {
       if (bias) hipLaunchKernelGGL((packed_ranges_kernel<64, true>), grid, dim3(256), 0, stream, a);
@@ -751,10 +805,11 @@ extern "C" int ES_VSA_API(es_shared_prefix_fwd)(const void* q, const void* k_pre
   a.G = H / Hk;
   a.div_g = fast_div(a.G);
   a.scale = scale * LOG2E;
-  a.target = resident(D);
   const long long own = (long long)B * (((long long)n * a.G + TILE - 1) / TILE);
   const long long tiles = ((long long)B * n * a.G + TILE - 1) / TILE + own;
   ES_REQUIRE(range_items(tiles, Hk, D) * Hk < (1LL << 31), ES_ERR_UNSUPPORTED, "shared prefix: grid too large");
+  a.plan = (int2*)((char*)workspace + plan_offset(range_items(tiles, Hk, D) * Hk, D));
+  a.inv_slots = (float)Hk / (float)resident(D);
   const dim3 grid((unsigned)(range_items(tiles, Hk, D) * Hk)), merge((unsigned)(own * Hk), 4);
   if (D == 64) {
     hipLaunchKernelGGL((shared_prefix_kernel<64>), grid, dim3(256), 0, stream, a);

@@ -7,6 +7,7 @@ import random
 import re
 from concurrent.futures import ThreadPoolExecutor
 
+import numpy as np
 import pytest
 import torch
 
@@ -107,10 +108,15 @@ def test_tiles_in_order_of_their_work():
 
 
 def test_range_items_fit_the_grid():
-    """The items of a ranged launch (csrc/packed_fwd.hip, key ranges) never outnumber the workgroups that the host starts, and
-    each has at most the chunks that fill the GPU once."""
+    """The items of a ranged launch (csrc/packed_fwd.hip, range_chunks and Cut, in float32 with a reciprocal that is off by up
+    to 2^-23 either way) never outnumber the workgroups that the host starts, whichever chunk count is taken."""
+    f = np.float32
+
+    def parts(x, y, off):
+        return np.ceil(f(x) * (f(1) / f(y) * f(1 + off)) - f(1e-5))
+
     rng = random.Random(6)
-    for _ in range(2000):
+    for _ in range(1500):
         B, Hk, D = rng.choice([1, 2, 9, 64, 100]), rng.choice([1, 2, 3, 8, 40]), rng.choice([64, 128])
         G = rng.choice([1, 3, 8])
         lists = [(rng.choice([1, 1, rng.randint(0, 500)]), rng.choice([0, 1, rng.randint(0, 70), rng.randint(0, 90000)]))
@@ -118,15 +124,24 @@ def test_range_items_fit_the_grid():
         rows = [n * G for n, _ in lists]
         tiles, chunks = [-(-r // 128) for r in rows], [-(-m // 64) for _, m in lists]
         resident = 1024 if D == 64 else 512
-        per = -(-sum(t * c for t, c in zip(tiles, chunks)) * Hk // resident)
-        items = sum(t * max(1, -(-c // max(per, 4 if r <= 32 else 8))) for t, c, r in zip(tiles, chunks, rows))
-        assert items <= sum(tiles) + resident // Hk + 1
+        inv_slots = f(Hk) / f(resident)
+        total = f(sum(f(t) * f(c) for t, c in zip(tiles, chunks)))
+        most = max([f(c) for t, c in zip(tiles, chunks) if t > 0], default=f(0))
+        fair = max(np.ceil(total * inv_slots), f(1))
+        for off in (-2.0 ** -23, 0.0, 2.0 ** -23):
+            near = int(parts(most, fair, off))
+            for n in range(max(near - 2, 1), near + 1):
+                per = max(parts(most, n, off), fair)
+                ranges = [max(parts(c, max(per, 4 if r <= 32 else 8), off), 1) for c, r in zip(chunks, rows)]
+                items = int(sum(t * r for t, r in zip(tiles, ranges)))
+                assert items <= sum(tiles) + resident // Hk + 1
+                # every chunk lies in one of its tile's ranges [c i / r, c (i + 1) / r)
+                assert all(int(r) >= 1 for r in ranges)
 
 
 def test_tokens_of_a_row_tile():
     """The KV owner's token of a row within a tile (csrc/packed_bwd.hip, token_in_tile): (row + 1/2) / G in float32, rows up to
     G + 63 from the tile's first token on."""
-    import numpy as np
     half, rows = np.float32(0.5), np.arange(64)
     for G in range(1, 4097):
         inv = np.float32(1) / np.float32(G)
