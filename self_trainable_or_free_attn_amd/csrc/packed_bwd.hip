@@ -55,7 +55,7 @@ __device__ __forceinline__ void lds_add(float* p, float x) {
 }
 
 template <int D, bool BIAS>
-__global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(BwdArgs a) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
   __shared__ __attribute__((aligned(16))) char qd_s[2][2][TILE_BYTES];  // [buffer][Q | dO]
   __shared__ __attribute__((aligned(16))) float st_s[2][2][BK];         // [buffer][lse2 | delta]
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_kv_kernel(BwdArgs a) {
 }
 
 template <int D, bool BIAS>
-__global__ __launch_bounds__(256, 2) void packed_bwd_q_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdArgs a) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
   __shared__ __attribute__((aligned(16))) char kv_s[2][2][TILE_BYTES];
   __shared__ float tab[BIAS ? BIAS_TABLE : 1];

@@ -556,7 +556,7 @@ __device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Range
 
 // grid: items * Hk, a token's heads on neighbouring workgroups
 template <int D, bool BIAS>
-__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_ranges_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_ranges_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
   __shared__ float stats[4 * 128];
   __shared__ float tab[BIAS ? BIAS_TABLE : 1];
@@ -579,7 +579,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_ranges_kernel(Fwd
 }
 
 template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void shared_prefix_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
   __shared__ float stats[4 * 128];
   const int w = blockIdx.x / a.Hk;
@@ -689,8 +689,9 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
 
 using namespace es;
 
-// Workgroups that the GPU holds at once: 256 CUs, two workgroups each at D = 128 (64 KB of staging), four at D = 64.
-static int resident(int D) { return D == 64 ? 1024 : 512; }
+// Workgroups of a ranged launch that the GPU holds at once: 256 CUs, two workgroups each at D = 128 (64 KB of staging), three
+// at D = 64 (134 registers: at 128, for four, the wide loop reloads spilled ones).
+static int resident(int D) { return D == 64 ? 768 : 512; }
 // Bytes of a ranged launch's workspace: the partials, then the plan.
 static size_t plan_offset(long long items, int D) { return (size_t)items * part_floats(D) * sizeof(float); }
 static size_t range_bytes(long long items, int lists, int D) { return plan_offset(items, D) + (size_t)lists * sizeof(int2); }

@@ -123,7 +123,7 @@ def test_range_items_fit_the_grid():
                  for _ in range(B)]
         rows = [n * G for n, _ in lists]
         tiles, chunks = [-(-r // 128) for r in rows], [-(-m // 64) for _, m in lists]
-        resident = 1024 if D == 64 else 512
+        resident = 768 if D == 64 else 512
         inv_slots = f(Hk) / f(resident)
         total = f(sum(f(t) * f(c) for t, c in zip(tiles, chunks)))
         most = max([f(c) for t, c in zip(tiles, chunks) if t > 0], default=f(0))
