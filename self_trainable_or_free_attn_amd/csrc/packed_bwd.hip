@@ -347,8 +347,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
     dp = f32x16{};
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) x = emfma(kf[ks], qreg[ks], x);
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(vt, koff ^ (32 * ks)), dreg[ks], dp);
     const int d0 = key0 + 4 * hi - (valid ? pos : low);  // (a position of the wave's)
     float sc = a.scale_log2, cb = 0.0f;
     near = false;
@@ -367,6 +365,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
       for (int r = 0; r < 16; ++r)
         if (8 * (r / 4) + r % 4 >= left) x[r] = -INFINITY;
     }
+    // (dP's products run under the exponentials)
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(vt, koff ^ (32 * ks)), dreg[ks], dp);
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = exp2f_fast(fmaf(x[r], sc, cb - ls));
   };
