@@ -5,7 +5,7 @@
  * Entry points that take token tensors (const void* / void*) read and write bf16; each has a twin with the suffix _f16
  * and the same arguments for fp16. The reference has no counterpart of these operators.
  *
- * Layouts (row-major):
+ * Layouts (row-major; token tensors and the workspace aligned to 16 bytes):
  *   q, out, dout, dq   (Tq, H, D)      D = 64 or 128, H a multiple of Hk: query head h reads kv head h / (H / Hk)
  *   k, v, dk, dv       (Tk, Hk, D)
  *   lse                (Tq, H) float32, natural logarithm, -inf for rows that see no key

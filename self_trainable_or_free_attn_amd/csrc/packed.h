@@ -13,6 +13,8 @@
 #include "../../include/packed_hip.h"
 #include "elem.h"
 
+#include <initializer_list>
+
 namespace es {
 
 namespace {
@@ -182,6 +184,12 @@ __device__ __forceinline__ void add_bias(f32x16& x, float sc, const float* row, 
 }  // namespace
 
 // ------------------------------------------------------------------------------------------------ host checks
+static inline bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p & 15) return false;
+  return true;
+}
+
 static inline int packed_check(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k,
                                const float* bias, const int* buckets, int num_buckets, int R, int B, int Tq, int Tk,
                                int H, int Hk, int D, float scale) {

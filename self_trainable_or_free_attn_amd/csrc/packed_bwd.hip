@@ -581,6 +581,8 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
   if (int st = packed_check(q, k, v, cu_q, cu_k, bias, buckets, num_buckets, R, B, Tq, Tk, H, Hk, D, scale)) return st;
   ES_REQUIRE((Tq == 0 || (dout && out && lse && dq && workspace)) && (Tk == 0 || (dk && dv)), ES_ERR_INVALID,
              "packed: null tensor pointer");
+  ES_REQUIRE(aligned16({q, k, v, dout, out, dq, dk, dv, workspace}), ES_ERR_INVALID,
+             "packed: tensors must be aligned to 16 bytes");
   ES_REQUIRE((bias != nullptr) == (dbias != nullptr), ES_ERR_INVALID, "packed: dbias goes with bias");
   ES_REQUIRE(workspace_bytes >= es_packed_bwd_workspace(B, Tq, Tk, H, Hk, D, bias ? R : 0, bias != nullptr),
              ES_ERR_INVALID, "packed: workspace too small");

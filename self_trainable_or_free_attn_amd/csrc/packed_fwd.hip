@@ -32,7 +32,7 @@ struct FwdArgs {
   const int *cu_q, *cu_k, *buckets;
   const float* bias;
   e16_t* out;
-  float *lse, *part;
+  float *lse, *part, *part_prefix;
   FastDiv div_g;
   int B, Tq, Tk, H, Hk, G, R, num_buckets, causal;
   int tiles;      // tile numbers of a head
@@ -43,6 +43,7 @@ struct FwdArgs {
   const e16_t *kp, *vp;
   const int* lens;
   int n, P, S;
+  int part_rows;  // rows of a sequence's partial
 };
 
 // What one workgroup computes: rows of tile t of the list of nq * G rows that starts at token q0, against key rows
@@ -50,11 +51,12 @@ struct FwdArgs {
 struct Job {
   const e16_t *k, *v;
   int q0, nq, nk, hk, t, c0, c1, causal;
-  float* part;  // nullptr: finished rows go to out / lse
+  float* part;  // a partial of `part_rows` rows; nullptr: finished rows go to out / lse
+  int part_rows;
 };
 
-// floats of one partial: O [128][D], m [128], l [128]
-__host__ __device__ constexpr int part_floats(int D) { return TILE * D + 2 * TILE; }
+// floats of a partial of `rows` rows: m, l, O [D] of each
+__host__ __device__ constexpr int part_floats(int rows, int D) { return rows * (D + 2); }
 
 // keys that row r of the job's list sees
 __device__ __forceinline__ int keys_seen(const FwdArgs& a, const Job& j, int r) {
@@ -273,15 +275,16 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
   if (j.part != nullptr) {
     const int r = wv * 32 + lq;
     if (r0 >= rows) return;
+    float* o = j.part + 2 * j.part_rows;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(j.part + r * D + 32 * db + 8 * i + 4 * hi) =
+        *reinterpret_cast<f32x4*>(o + r * D + 32 * db + 8 * i + 4 * hi) =
             f32x4{x.o[db][4 * i], x.o[db][4 * i + 1], x.o[db][4 * i + 2], x.o[db][4 * i + 3]};
     if (hi == 0) {
-      j.part[TILE * D + r] = x.mrun;
-      j.part[TILE * D + TILE + r] = tot;
+      j.part[r] = x.mrun;
+      j.part[j.part_rows + r] = tot;
     }
     return;
   }
@@ -389,13 +392,13 @@ __device__ __forceinline__ void narrow_tile(const FwdArgs& a, const Job& j, char
       for (int c = 0; c < 4; ++c) acc[c] = fmaf(w[i], other[(q4 * 4 + c) * 64 + l], acc[c]);
     }
     const int col = 32 * (q4 >> 2) + 8 * (q4 & 3) + 4 * hi;
-    if (j.part != nullptr) *reinterpret_cast<f32x4*>(j.part + lq * D + col) = acc;
+    if (j.part != nullptr) *reinterpret_cast<f32x4*>(j.part + 2 * j.part_rows + lq * D + col) = acc;
     else if (x.valid) store_row<D>(a, x.at, col, acc * inv);
   }
   if (wv == 0 && hi == 0) {
     if (j.part != nullptr) {
-      j.part[TILE * D + lq] = M;
-      j.part[TILE * D + TILE + lq] = tot;
+      j.part[lq] = M;
+      j.part[j.part_rows + lq] = tot;
     } else if (x.valid) {
       a.lse[x.at] = tot == 0.0f ? -INFINITY : (M - P_SHIFT + log2f(tot)) * PK_LN2;
     }
@@ -578,14 +581,20 @@ struct SharedLists {
   }
 };
 
-// item w of a list: its job's tile and chunks, its partial
-__device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Ranges& r, int w, int D, bool always) {
+// item w of a list: its job's tile and chunks
+__device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Ranges& r, int w) {
   const int i = w - r.item0, range = i % r.ranges;
   j.t = i / r.ranges;
   const int chunks = tile_chunks(a, j);
   j.c0 = (int)((long long)chunks * range / r.ranges);
   j.c1 = (int)((long long)chunks * (range + 1) / r.ranges);
-  j.part = r.ranges == 1 && !always ? nullptr : a.part + ((size_t)w * a.Hk + j.hk) * part_floats(D);
+}
+
+// Partial `item` of a launch, all kv heads of an item side by side. Shared prefix: the prefix's items have a part of their own,
+// with whole tiles; those of the sequences are as long as their lists.
+template <int D>
+__device__ __forceinline__ float* partial(float* base, int rows, const FwdArgs& a, int item, int hk) {
+  return base + ((size_t)item * a.Hk + hk) * part_floats(rows, D);
 }
 
 // grid: items * Hk, a token's heads on neighbouring workgroups
@@ -608,7 +617,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_ranges_kernel(Fwd
   j.nq = s.nq;
   j.nk = s.nk;
   j.causal = a.causal;
-  take_range(a, j, r, w, D, false);
+  take_range(a, j, r, w);
+  j.part_rows = TILE;
+  j.part = r.ranges == 1 ? nullptr : partial<D>(a.part, TILE, a, w, j.hk);
   run_tile<D, BIAS>(a, j, lds, stats, tab);
 }
 
@@ -639,7 +650,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(Fwd
     j.nk = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
     j.causal = 1;
   }
-  take_range(a, j, r, w, D, true);
+  take_range(a, j, r, w);
+  j.part_rows = r.list == 0 ? TILE : a.part_rows;
+  j.part = r.list == 0 ? partial<D>(a.part_prefix, TILE, a, w - r.item0, j.hk) : partial<D>(a.part, a.part_rows, a, w, j.hk);
   run_tile<D, false>(a, j, lds, stats, nullptr);
 }
 
@@ -672,16 +685,23 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
     if (own.ranges == 1) return;  // (finished by its only range)
   }
   const int rows = min(nq * a.G - t * TILE, TILE), lane = threadIdx.x % LPR, c = lane * 4, n = pre.ranges + own.ranges;
-  const size_t step = (size_t)a.Hk * part_floats(D);
-  const float* own0 = a.part + (size_t)(own.item0 + t * own.ranges) * step + (size_t)hk * part_floats(D);
+  const int own_rows = SHARED ? a.part_rows : TILE;
   for (int r = blockIdx.y * RPB + threadIdx.x / LPR; r < rows; r += gridDim.y * RPB) {
     const int all = q0 * a.G + t * TILE + r, rp = SHARED ? all % TILE : 0;  // the row among all rows of the batch
-    const float* pre0 =
-        SHARED ? a.part + (size_t)(pre.item0 + all / TILE * pre.ranges) * step + (size_t)hk * part_floats(D) : nullptr;
-    auto part = [&](int i) { return i < pre.ranges ? pre0 + i * step : own0 + (i - pre.ranges) * step; };
-    auto row_of = [&](int i) { return i < pre.ranges ? rp : r; };
+    // a row's partial i: m at [row], l at [rows + row], O behind them
+    auto part = [&](int i, int& stored, int& row) -> const float* {
+      const bool p = SHARED && i < pre.ranges;
+      stored = p ? TILE : own_rows;
+      row = p ? rp : r;
+      return p ? partial<D>(a.part_prefix, TILE, a, all / TILE * pre.ranges + i, hk)
+               : partial<D>(a.part, own_rows, a, own.item0 + t * own.ranges + i - pre.ranges, hk);
+    };
+    int stored, row;
     float M = -INFINITY;
-    for (int i = lane; i < n; i += LPR) M = fmaxf(M, part(i)[TILE * D + row_of(i)]);
+    for (int i = lane; i < n; i += LPR) {
+      const float* p = part(i, stored, row);
+      M = fmaxf(M, p[row]);
+    }
 #pragma unroll
     for (int m = LPR / 2; m >= 1; m >>= 1) M = fmaxf(M, __shfl_xor(M, m, 64));
     const float msub = M == -INFINITY ? 0.0f : M;
@@ -691,16 +711,16 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
       const int count = min(n - i0, LPR);
       float f = 0.0f, l = 0.0f;
       if (lane < count) {
-        const float* p = part(i0 + lane) + TILE * D + row_of(i0 + lane);
-        f = exp2f_fast(p[0] - msub);
-        l = p[TILE];
+        const float* p = part(i0 + lane, stored, row);
+        f = exp2f_fast(p[row] - msub);
+        l = p[stored + row];
       }
       for (int i = 0; i < count; i += 8) {
         f32x4 x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int at = min(i + e, count - 1) + i0;
-          x[e] = *reinterpret_cast<const f32x4*>(part(at) + row_of(at) * D + c);
+          const float* p = part(min(i + e, count - 1) + i0, stored, row);
+          x[e] = *reinterpret_cast<const f32x4*>(p + 2 * stored + row * D + c);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -710,8 +730,8 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
         }
       }
     }
-    const int row = t * TILE + r, tok = divide(a.div_g, row);
-    const size_t at = ((size_t)(q0 + tok) * a.Hk + hk) * a.G + (row - tok * a.G);
+    const int lrow = t * TILE + r, tok = divide(a.div_g, lrow);
+    const size_t at = ((size_t)(q0 + tok) * a.Hk + hk) * a.G + (lrow - tok * a.G);
     store_row<D>(a, at, c, acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
     if (c == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (M - P_SHIFT + log2f(sum)) * PK_LN2;
   }
@@ -726,9 +746,6 @@ using namespace es;
 // Workgroups of a ranged launch that the GPU holds at once: 256 CUs, two workgroups each at D = 128 (64 KB of staging), three
 // at D = 64 (134 registers: at 128, for four, the wide loop reloads spilled ones).
 static int resident(int D) { return D == 64 ? 768 : 512; }
-// Bytes of a ranged launch's workspace: the partials, then the plan.
-static size_t plan_offset(long long items, int D) { return (size_t)items * part_floats(D) * sizeof(float); }
-static size_t range_bytes(long long items, int lists, int D) { return plan_offset(items, D) + (size_t)lists * sizeof(int2); }
 // Items a head of a ranged launch: at most one a tile more than the ranges' chunks fill.
 static long long range_items(long long tiles, int Hk, int D) { return tiles + resident(D) / Hk + 1; }
 // Key ranges are worth a second launch where the tiles do not fill the GPU and the keys are more than a few chunks: 1024 for
@@ -737,19 +754,38 @@ static bool ranged(long long tiles, int B, int Tq, int Tk, int H, int Hk, int D)
   return tiles * Hk < 2 * resident(D) && Tk >= ((long long)Tq * (H / Hk) <= 32LL * B ? 16 : 64) * BK;
 }
 
+// Workspace of a shared-prefix call: partials of the sequences, partials of the prefix, plan; of a packed one: partials, plan.
+struct Layout {
+  long long items;               // a head
+  size_t prefix, plan, bytes;    // offsets
+  int rows;                      // of a sequence's partial
+};
+static Layout packed_layout(long long tiles, int B, int Hk, int D) {
+  Layout l = {range_items(tiles, Hk, D), 0, 0, 0, TILE};
+  l.plan = (size_t)l.items * Hk * part_floats(TILE, D) * sizeof(float);
+  l.bytes = l.plan + (size_t)(B + 1) * sizeof(int2);
+  return l;
+}
+static Layout shared_layout(int B, int n, int H, int Hk, int D) {
+  const long long list = (long long)n * (H / Hk), tiles = (B * list + TILE - 1) / TILE, own = B * ((list + TILE - 1) / TILE);
+  Layout l = {range_items(tiles + own, Hk, D), 0, 0, 0, (int)std::min<long long>((list + 31) / 32 * 32, TILE)};
+  l.prefix = (size_t)l.items * Hk * part_floats(l.rows, D) * sizeof(float);
+  l.plan = l.prefix + (size_t)range_items(tiles, Hk, D) * Hk * part_floats(TILE, D) * sizeof(float);
+  l.bytes = l.plan + (size_t)(B + 1) * sizeof(int2);
+  return l;
+}
+
 #ifndef ES_ELEM_F16
 extern "C" size_t es_packed_fwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D) {
   if (B <= 0 || Tq <= 0 || Tk < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
   const long long tiles = tile_numbers<TILE>(B, Tq, H / Hk);
-  return ranged(tiles, B, Tq, Tk, H, Hk, D) ? range_bytes(range_items(tiles, Hk, D) * Hk, B + 1, D) : 0;
+  return ranged(tiles, B, Tq, Tk, H, Hk, D) ? packed_layout(tiles, B, Hk, D).bytes : 0;
 }
 extern "C" size_t es_shared_prefix_workspace(int B, int n, int P, int S, int H, int Hk, int D) {
   if (B <= 0 || n <= 0 || P < 0 || S < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
-  const long long G = H / Hk, rows = n * G, tiles = (B * rows + TILE - 1) / TILE + B * ((rows + TILE - 1) / TILE);
-  return range_bytes(range_items(tiles, Hk, D) * Hk, B + 1, D);
+  return shared_layout(B, n, H, Hk, D).bytes;
 }
 #endif
-
 
 extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k,
                                          const float* bias, const int* buckets, int num_buckets, int R, void* out,
@@ -758,6 +794,7 @@ extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const voi
   if (int st = packed_check(q, k, v, cu_q, cu_k, bias, buckets, num_buckets, R, B, Tq, Tk, H, Hk, D, scale)) return st;
   if (Tq == 0) return ES_OK;
   ES_REQUIRE(out && lse, ES_ERR_INVALID, "packed: null out / lse");
+  ES_REQUIRE(aligned16({q, k, v, out, workspace}), ES_ERR_INVALID, "packed: tensors must be aligned to 16 bytes");
   FwdArgs a = {};
   a.q = (const e16_t*)q;
   a.k = (const e16_t*)k;
@@ -785,9 +822,10 @@ extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const voi
     ES_REQUIRE(workspace && workspace_bytes >= es_packed_fwd_workspace(B, Tq, Tk, H, Hk, D), ES_ERR_INVALID,
                "packed: workspace too small");
     a.part = (float*)workspace;
-    a.plan = (int2*)((char*)workspace + plan_offset(range_items(a.tiles, Hk, D) * Hk, D));
+    const Layout l = packed_layout(a.tiles, B, Hk, D);
+    a.plan = (int2*)((char*)workspace + l.plan);
     a.inv_slots = (float)Hk / (float)resident(D);
-    const dim3 grid((unsigned)(range_items(a.tiles, Hk, D) * Hk)), merge((unsigned)(a.tiles * Hk), 4);
+    const dim3 grid((unsigned)(l.items * Hk)), merge((unsigned)(a.tiles * Hk), 4);
     if (D == 64) {
       if (bias) hipLaunchKernelGGL((packed_ranges_kernel<64, true>), grid, dim3(256), 0, stream, a);
       else hipLaunchKernelGGL((packed_ranges_kernel<64, false>), grid, dim3(256), 0, stream, a);
@@ -819,6 +857,8 @@ extern "C" int ES_VSA_API(es_shared_prefix_fwd)(const void* q, const void* k_pre
   ES_REQUIRE(lens && out && lse && workspace && (S == 0 || (k && v)), ES_ERR_INVALID, "shared prefix: null tensor pointer");
   if (int st = packed_check(q, k_prefix, v_prefix, nullptr, lens, nullptr, nullptr, 0, 0, B, B * n, P, H, Hk, D, scale))
     return st;
+  ES_REQUIRE(aligned16({q, k_prefix, v_prefix, k, v, out, workspace}), ES_ERR_INVALID,
+             "shared prefix: tensors must be aligned to 16 bytes");
   ES_REQUIRE(workspace_bytes >= es_shared_prefix_workspace(B, n, P, S, H, Hk, D), ES_ERR_INVALID,
              "shared prefix: workspace too small");
   FwdArgs a = {};
@@ -840,12 +880,14 @@ extern "C" int ES_VSA_API(es_shared_prefix_fwd)(const void* q, const void* k_pre
   a.G = H / Hk;
   a.div_g = fast_div(a.G);
   a.scale = scale * LOG2E;
+  const Layout l = shared_layout(B, n, H, Hk, D);
   const long long own = (long long)B * (((long long)n * a.G + TILE - 1) / TILE);
-  const long long tiles = ((long long)B * n * a.G + TILE - 1) / TILE + own;
-  ES_REQUIRE(range_items(tiles, Hk, D) * Hk < (1LL << 31), ES_ERR_UNSUPPORTED, "shared prefix: grid too large");
-  a.plan = (int2*)((char*)workspace + plan_offset(range_items(tiles, Hk, D) * Hk, D));
+  ES_REQUIRE(l.items * Hk < (1LL << 31), ES_ERR_UNSUPPORTED, "shared prefix: grid too large");
+  a.part_prefix = (float*)((char*)workspace + l.prefix);
+  a.plan = (int2*)((char*)workspace + l.plan);
+  a.part_rows = l.rows;
   a.inv_slots = (float)Hk / (float)resident(D);
-  const dim3 grid((unsigned)(range_items(tiles, Hk, D) * Hk)), merge((unsigned)(own * Hk), 4);
+  const dim3 grid((unsigned)(l.items * Hk)), merge((unsigned)(own * Hk), 4);
   if (D == 64) {
     hipLaunchKernelGGL((shared_prefix_kernel<64>), grid, dim3(256), 0, stream, a);
     hipLaunchKernelGGL((merge_kernel<64, true>), merge, dim3(256), 0, stream, a);

@@ -51,6 +51,9 @@ Tensor workspace(size_t bytes, const Tensor& q) {
   return bytes ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : Tensor();
 }
 
+// a tensor that starts inside another's storage at an address the kernels' 16-byte loads do not take is copied
+Tensor aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) & 15 ? t.clone() : t; }
+
 // the checked arguments of one packed call
 struct Packed {
   Tensor bias, cu_q, cu_k, buckets;
@@ -85,11 +88,12 @@ struct Packed {
   const int* ints(const Tensor& t) const { return static_cast<const int*>(data(t)); }
 };
 
-std::tuple<Tensor, Tensor> packed_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
+std::tuple<Tensor, Tensor> packed_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& bias,
                                           const OptTensor& cu_q, const OptTensor& cu_k, const OptTensor& buckets, int64_t B,
                                           bool causal, double scale) {
-  const c10::OptionalDeviceGuard guard(q.device());
-  const Packed a(q, k, v, bias, cu_q, cu_k, buckets, B);
+  const c10::OptionalDeviceGuard guard(q_.device());
+  const Packed a(q_, k_, v_, bias, cu_q, cu_k, buckets, B);
+  const Tensor q = aligned(q_), k = aligned(k_), v = aligned(v_);
   Tensor out = at::empty_like(q), lse = at::empty({a.Tq, a.H}, q.options().dtype(at::kFloat));
   const size_t bytes = es_packed_fwd_workspace(a.B, a.Tq, a.Tk, a.H, a.Hk, a.D);
   const Tensor ws = workspace(bytes, q);
@@ -100,14 +104,14 @@ std::tuple<Tensor, Tensor> packed_forward(const Tensor& q, const Tensor& k, cons
   return {out, lse};
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> packed_backward(const Tensor& dout_, const Tensor& q, const Tensor& k,
-                                                           const Tensor& v, const Tensor& out, const Tensor& lse,
+std::tuple<Tensor, Tensor, Tensor, Tensor> packed_backward(const Tensor& dout_, const Tensor& q_, const Tensor& k_,
+                                                           const Tensor& v_, const Tensor& out, const Tensor& lse,
                                                            const OptTensor& bias, const OptTensor& cu_q,
                                                            const OptTensor& cu_k, const OptTensor& buckets, int64_t B,
                                                            bool causal, double scale) {
-  const c10::OptionalDeviceGuard guard(q.device());
-  const Packed a(q, k, v, bias, cu_q, cu_k, buckets, B);
-  const Tensor dout = dout_.contiguous();
+  const c10::OptionalDeviceGuard guard(q_.device());
+  const Packed a(q_, k_, v_, bias, cu_q, cu_k, buckets, B);
+  const Tensor q = aligned(q_), k = aligned(k_), v = aligned(v_), dout = aligned(dout_.contiguous());
   check_tokens("dout", dout, q, 3);
   check_tokens("out", out, q, 3);
   TORCH_CHECK(dout.sizes() == q.sizes() && out.sizes() == q.sizes(), "out and its gradient must be like q");

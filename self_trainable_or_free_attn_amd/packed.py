@@ -193,7 +193,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: Op
         if B == 0:
             return (q.clone(), q.new_empty(shape[:-1], dtype=torch.float32)) if return_lse else q.clone()
         q, k, v = (x.flatten(0, 1) for x in (q, k, v))
-    out, lse = _ops().packed_attention(q, k, v, bias, cu_q, cu_k, buckets, B, causal, scale)
+    out, lse = _ops().packed_attention(q, k, v, bias, cu_q, cu_k, buckets, B, bool(causal), scale)
     if dims == 4:
         out, lse = out.view(shape), lse.view(shape[:-1])
     return (out, lse) if return_lse else out
@@ -209,8 +209,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     q [B, n, H, D]; k_prefix, v_prefix [P, Hk, D], seen whole by every token; k, v [B, S, Hk, D], the caches as they were
     allocated, and lens int32 [B] how many rows of each are in use (clamped to 0 .. S), the n tokens' own keys, which the
     caller has written, the last of them. Token i of sequence b sees its cache rows 0 to lens[b] - n + i. Cache rows from
-    lens[b] on are never used. bf16 or fp16, D 64 or 128, H a multiple of Hk, every tensor contiguous. scale: 1 / sqrt(D) if
-    None.
+    lens[b] on are never used. bf16 or fp16, D 64 or 128, H a multiple of Hk, every tensor contiguous and
+    aligned to 16 bytes. scale: 1 / sqrt(D) if None.
 
     Returns out like q, with return_lse also the natural-log LSE [B, n, H] in float32; a token without keys gives zeros and
     -inf. There is no backward: tensors that require a gradient are refused unless gradients are off."""

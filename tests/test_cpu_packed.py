@@ -297,6 +297,8 @@ def test_c_entry_points_refuse_before_any_launch():
             (lambda: fwd(bias=p, buckets=p, nb=4, R=196), 2, "at most 784"),
             (lambda: fwd(bias=p, buckets=p, nb=4, R=1 << 30), 2, "at most 784"),
             (lambda: fwd(D=96, suffix="_f16"), 2, "64 or 128"),
+            (lambda: fwd(q=ctypes.c_void_p(264)), 1, "aligned"), (lambda: fwd(ws=ctypes.c_void_p(260)), 1, "aligned"),
+            (lambda: bwd(dq=ctypes.c_void_p(258)), 1, "aligned"), (lambda: shared(k=ctypes.c_void_p(8)), 1, "aligned"),
             (lambda: bwd(dout=None), 1, "null tensor"), (lambda: bwd(dq=None), 1, "null tensor"),
             (lambda: bwd(dk=None), 1, "null tensor"), (lambda: bwd(ws=None), 1, "null tensor"),
             (lambda: bwd(bias=p), 1, "dbias goes with bias"), (lambda: bwd(dbias=p), 1, "dbias goes with bias"),

@@ -188,6 +188,26 @@ def test_batch_form_equals_packed_form(dev):
     assert not gq.any() and not gk.any()
 
 
+def test_inputs_that_start_anywhere(dev):
+    """Views one value into a storage: contiguous, but not at the 16 bytes that the kernels load."""
+    api = _api()
+    t = _inputs([60], [60], 2, 2, 64, BF, dev, 40)
+
+    def shifted(x):
+        y = torch.empty(x.numel() + 1, device=dev, dtype=x.dtype)[1:].view(x.shape)
+        return y.copy_(x)
+
+    a = [t[n].clone().requires_grad_() for n in "qkv"]
+    b = [shifted(t[n]).requires_grad_() for n in "qkv"]
+    oa, ob = api.packed_attention(*a, causal=True), api.packed_attention(*b, causal=True)
+    assert b[0].data_ptr() % 16 and torch.equal(oa, ob)
+    ga, gb = torch.autograd.grad(oa, a, t["dout"]), torch.autograd.grad(ob, b, shifted(t["dout"]))
+    assert all(torch.equal(x, y) for x, y in zip(ga, gb))
+    s = _shared(2, 1, 10, 8, [1, 2], 2, 2, 64, BF, dev, 41)
+    with pytest.raises(RuntimeError, match="aligned"):
+        api.shared_prefix_attention(s["q"], s["kp"], s["vp"], shifted(s["k"]), s["v"], s["lens"])
+
+
 def test_strided_inputs_and_gradients(dev):
     """Views of one projection, a gradient that is an expanded view, a bias in the token type."""
     api = _api()
@@ -403,6 +423,8 @@ def _shared_check(t, out, lse, scale=None):
     (1, 5000, 300, [299, 300, 1, 17, 64, 65, 128, 8], 16, 2), (40, 700, 512, [512, 40, 41], 5, 5),
     (1, 2000, 100, [50] * 70, 4, 1), (2, 64, 3000, [3000, 2, 1999], 8, 1),
     (1, 300, 20, [25, -3], 4, 4),                    # lengths out of range are cut off
+    (40, 300, 600, [600, 40, 77], 8, 2), (1, 0, 0, [0], 2, 2), (33, 65, 40, [40, 33], 4, 4),
+    (1, 4000, 16, [16] * 130, 8, 2),
 ])
 def test_shared_prefix(dev, D, dtype, n, P, S, lens, H, Hk):
     t = _shared(len(lens), n, P, S, lens, H, Hk, D, dtype, dev, 30)
