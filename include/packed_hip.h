@@ -41,7 +41,7 @@ int es_packed_fwd_f16(const void* q, const void* k, const void* v, const int* cu
 
 /* Backward of the same call from its out and lse; dbias (num_buckets, H) float32 with bias, NULL without. No atomics on
  * global memory: the same inputs give the same bits. workspace: es_packed_bwd_workspace bytes. */
-size_t es_packed_bwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D, int R, int with_bias);
+size_t es_packed_bwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D, int R, int with_bias, int causal);
 int es_packed_bwd(const void* q, const void* k, const void* v, const void* dout, const void* out, const float* lse,
                   const int* cu_q, const int* cu_k, const float* bias, const int* buckets, int num_buckets, int R, void* dq,
                   void* dk, void* dv, float* dbias, void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H,

@@ -91,7 +91,7 @@ SIGNATURES.update({n + "_f16": SIGNATURES[n] for n in F16_TWINS})
 NO_STREAM = {"es_representatives_workspace": ([I, I, I], Z), "es_dense_attention_workspace": ([I, I, I], Z),
              "es_representatives_noalloc_limit": ([], Z), "es_last_error_string": ([], ctypes.c_char_p),
              "es_abi_version": ([], I), "vsa_topk_workspace": ([I, I], Z),
-             "es_packed_fwd_workspace": ([I] * 6, Z), "es_packed_bwd_workspace": ([I] * 8, Z),
+             "es_packed_fwd_workspace": ([I] * 6, Z), "es_packed_bwd_workspace": ([I] * 9, Z),
              "es_shared_prefix_workspace": ([I] * 7, Z)}
 
 _lib = None

@@ -8,6 +8,8 @@
 //   bwd_kv      one workgroup per (64 keys, kv head): dV = P^T dO and dK = scale dS^T Q over all rows of the list that see
 //               the keys, which sums over the heads of a group without atomics. Four waves = 2 key halves x 2 row halves
 //               of each staged 64-row tile; S and dP come out with keys on lanes, so that P and dS are B operands.
+//               With few (key tile, kv head) pairs the rows of each are cut into ranges, one workgroup each, whose float32
+//               sums kv_sums adds in order.
 //   bias_sums   those sums over the row tiles and into buckets
 // Every sum has a fixed order, so the same inputs give the same bits. The scores are computed twice (7 products for 5): a
 // single pass would need dQ in float32 atomics or a dQ partial a key tile.
@@ -20,6 +22,9 @@
 // dS is rounded to the token type without the softmax scale (applied to the finished sums), which keeps it about ten times
 // further from the subnormal range of fp16.
 #include "packed.h"
+
+#include <algorithm>
+#include <cmath>
 
 namespace es {
 
@@ -46,6 +51,8 @@ struct BwdArgs {
   float inv_g;  // 1 / G
   int B, Tq, Tk, H, Hk, G, R, num_buckets, causal;
   int q_tiles, k_tiles;  // tile numbers of a head
+  int ranges;            // row ranges of bwd_kv
+  float* part;           // their sums [range][Tk][Hk][dV | dK][D]
   float scale_log2, scale;
 };
 
@@ -62,14 +69,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
   // [buffer][position of the row | its part of the bias table]
   __shared__ __attribute__((aligned(16))) int pos_s[BIAS ? 2 : 1][2][BIAS ? BK : 1];
   __shared__ float tab[BIAS ? BIAS_TABLE : 1];
-  const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
+  const int item = blockIdx.x / a.ranges, range = blockIdx.x - item * a.ranges, w = item / a.Hk, hk = item - w * a.Hk;
   int b, kb;
   Seq s;  // (key rows behind the last sequence: no rows, so zero gradients)
   if (!tile_of<BK, true>(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, a.G, w, s, b, kb)) return;
   const int rows = s.nq * a.G, shift = s.nk - s.nq;
-  const int end = (rows + BK - 1) / BK;
+  const int row_tiles = (rows + BK - 1) / BK;
   // causal: the first row that sees this tile's first key
-  const int beg = a.causal ? min(max(kb * BK - shift, 0) * a.G / BK, end) : 0;
+  const int first_tile = a.causal ? min(max(kb * BK - shift, 0) * a.G / BK, row_tiles) : 0;
+  const int beg = first_tile + (int)((long long)(row_tiles - first_tile) * range / a.ranges);
+  const int end = first_tile + (int)((long long)(row_tiles - first_tile) * (range + 1) / a.ranges);
   const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qh = wv >> 1, kh = wv & 1;
@@ -247,6 +256,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = (acc[db][4 * i + e] + xch[((base + db) * 16 + 4 * i + e) * 64 + l]) * f;
+        if (a.ranges > 1) {
+          const size_t row = (size_t)range * a.Tk * a.Hk + krow / D;
+          *reinterpret_cast<f32x4*>(a.part + (2 * row + (base != 0)) * D + 32 * db + 8 * i + 4 * hi) =
+              f32x4{x[0], x[1], x[2], x[3]};
+          continue;
+        }
         ushort4 o4;
         o4.x = f2e(x[0]); o4.y = f2e(x[1]); o4.z = f2e(x[2]); o4.w = f2e(x[3]);
         *reinterpret_cast<ushort4*>(out + krow + 32 * db + 8 * i + 4 * hi) = o4;
@@ -529,6 +544,19 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
     }
 }
 
+// dV and dK from the row ranges' sums, in order: four channels a thread
+template <int D>
+__global__ __launch_bounds__(256) void kv_sums_kernel(BwdArgs a) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, rows = (size_t)a.Tk * a.Hk, row = i / (D / 2);
+  if (row >= rows) return;
+  const int c = (int)(i - row * (D / 2)) * 4;  // channels of [dV | dK]
+  f32x4 sum = {};
+  for (int r = 0; r < a.ranges; ++r) sum += *reinterpret_cast<const f32x4*>(a.part + (r * rows + row) * 2 * D + c);
+  ushort4 o4;
+  o4.x = f2e(sum[0]); o4.y = f2e(sum[1]); o4.z = f2e(sum[2]); o4.w = f2e(sum[3]);
+  *reinterpret_cast<ushort4*>((c < D ? a.dv + row * D + c : a.dk + row * D + c - D)) = o4;
+}
+
 // dbias[n][h] = sum over the row tiles and over the distances of bucket n: one workgroup a head. First each of four slices of
 // 256 lanes adds every fourth tile, a distance a lane, eight tiles in flight; then a wave adds up a bucket's distances.
 __global__ __launch_bounds__(1024) void bias_sums_kernel(BwdArgs a) {
@@ -562,14 +590,47 @@ __global__ __launch_bounds__(1024) void bias_sums_kernel(BwdArgs a) {
 
 using namespace es;
 
+// Row ranges of bwd_kv: one to sixteen, by the shortest schedule in steps of one row tile, for sequences of average length. An
+// item takes its row tiles and about four steps before and behind them, two more where its sums go through memory. Without a
+// mask all items are alike and run in rounds of what the GPU holds; under a causal one they halve on average, start with the
+// longest, and end with it or when all work is done. From two rounds of items on the ranges' memory is not worth it. (Whole
+// backward, causal, D = 128, us with one range and by this rule: 8192 tokens of 8 heads over one kv head 1793 -> 675, 2000
+// tokens 432 -> 91, 4000 tokens of 40 heads over 5 1086 -> 812, 1000 of 64 over 8 253 -> 125.)
+static int row_ranges(int B, int Tq, int Tk, int H, int Hk, int D, int causal) {
+  const double items = (double)tile_numbers<BK>(B, Tk, 1) * Hk, steps = (double)Tq * (H / Hk) / B / BK;
+  const double slots = D == 64 ? 768 : 512;
+  int best = 1;
+  double least = 0;
+  for (int r = 1; r <= 16 && (r == 1 || (steps >= 4.0 * r && items < 2 * slots)); ++r) {
+    const double more = r == 1 ? 4 : 6, each = steps / r;
+    const double time = causal ? std::max(each + more, items * r / slots * (each / 2 + more))
+                               : std::ceil(items * r / slots) * (each + more);
+    if (r == 1 || time < 0.97 * least) {
+      least = time;
+      best = r;
+    }
+  }
+  return best;
+}
+// lse2 and delta, the distance sums of every (row tile, kv head), the row ranges' sums
+struct Offsets {
+  size_t dist, part, floats;
+};
+static Offsets bwd_layout(int B, int Tq, int Tk, int H, int Hk, int D, int R, int with_bias, int causal) {
+  Offsets o;
+  o.dist = 2 * (size_t)Tq * H;
+  o.part = o.dist + (with_bias ? (size_t)tile_numbers<BK>(B, Tq, H / Hk) * H * (2 * R + 1) : 0);
+  o.part = (o.part + 3) / 4 * 4;
+  const int ranges = row_ranges(B, Tq, Tk, H, Hk, D, causal);
+  o.floats = o.part + (ranges > 1 ? (size_t)ranges * Tk * Hk * 2 * D : 0);
+  return o;
+}
+
 #ifndef ES_ELEM_F16
-// lse2 and delta, then the distance sums of every (row tile, kv head)
-extern "C" size_t es_packed_bwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D, int R, int with_bias) {
+extern "C" size_t es_packed_bwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D, int R, int with_bias,
+                                          int causal) {
   if (B <= 0 || Tq < 0 || Tk < 0 || H <= 0 || Hk <= 0 || H % Hk || R < 0) return 0;
-  (void)D;
-  size_t floats = 2 * (size_t)Tq * H;
-  if (with_bias) floats += (size_t)tile_numbers<BK>(B, Tq, H / Hk) * H * (2 * R + 1);
-  return floats * sizeof(float);
+  return bwd_layout(B, Tq, Tk, H, Hk, D, R, with_bias, causal != 0).floats * sizeof(float);
 }
 #endif
 
@@ -584,7 +645,7 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
   ES_REQUIRE(aligned16({q, k, v, dout, out, dq, dk, dv, workspace}), ES_ERR_INVALID,
              "packed: tensors must be aligned to 16 bytes");
   ES_REQUIRE((bias != nullptr) == (dbias != nullptr), ES_ERR_INVALID, "packed: dbias goes with bias");
-  ES_REQUIRE(workspace_bytes >= es_packed_bwd_workspace(B, Tq, Tk, H, Hk, D, bias ? R : 0, bias != nullptr),
+  ES_REQUIRE(workspace_bytes >= es_packed_bwd_workspace(B, Tq, Tk, H, Hk, D, bias ? R : 0, bias != nullptr, causal),
              ES_ERR_INVALID, "packed: workspace too small");
   BwdArgs a = {};
   a.q = (const e16_t*)q;
@@ -603,7 +664,10 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
   a.dbias = dbias;
   a.lse2 = (float*)workspace;
   a.delta = a.lse2 + (size_t)Tq * H;
-  a.dist = a.delta + (size_t)Tq * H;
+  const Offsets o = bwd_layout(B, Tq, Tk, H, Hk, D, bias ? R : 0, bias != nullptr, causal != 0);
+  a.dist = a.lse2 + o.dist;
+  a.part = a.lse2 + o.part;
+  a.ranges = row_ranges(B, Tq, Tk, H, Hk, D, causal != 0);
   a.B = B;
   a.Tq = Tq;
   a.Tk = Tk;
@@ -619,7 +683,7 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
   a.scale_log2 = scale * LOG2E;
   a.q_tiles = (int)tile_numbers<BK>(B, Tq, a.G);
   a.k_tiles = (int)tile_numbers<BK>(B, Tk, 1);
-  ES_REQUIRE((long long)a.q_tiles * Hk < (1LL << 31) && (long long)a.k_tiles * Hk < (1LL << 31), ES_ERR_UNSUPPORTED,
+  ES_REQUIRE((long long)a.q_tiles * Hk < (1LL << 31) && (long long)a.k_tiles * Hk * a.ranges < (1LL << 31), ES_ERR_UNSUPPORTED,
              "packed: grid too large");
   if (Tq > 0) {
     const dim3 grid((unsigned)(a.q_tiles * Hk));
@@ -632,13 +696,18 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
     }
   }
   if (Tk > 0) {
-    const dim3 grid((unsigned)(a.k_tiles * Hk));
+    const dim3 grid((unsigned)(a.k_tiles * Hk * a.ranges));
     if (D == 64) {
       if (bias) hipLaunchKernelGGL((packed_bwd_kv_kernel<64, true>), grid, dim3(256), 0, stream, a);
       else hipLaunchKernelGGL((packed_bwd_kv_kernel<64, false>), grid, dim3(256), 0, stream, a);
     } else {
       if (bias) hipLaunchKernelGGL((packed_bwd_kv_kernel<128, true>), grid, dim3(256), 0, stream, a);
       else hipLaunchKernelGGL((packed_bwd_kv_kernel<128, false>), grid, dim3(256), 0, stream, a);
+    }
+    if (a.ranges > 1) {
+      const dim3 sums((unsigned)(((long long)Tk * Hk * (D / 2) + 255) / 256));
+      if (D == 64) hipLaunchKernelGGL((kv_sums_kernel<64>), sums, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((kv_sums_kernel<128>), sums, dim3(256), 0, stream, a);
     }
   }
   if (bias) {

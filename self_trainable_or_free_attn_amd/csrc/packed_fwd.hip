@@ -748,10 +748,16 @@ using namespace es;
 static int resident(int D) { return D == 64 ? 768 : 512; }
 // Items a head of a ranged launch: at most one a tile more than the ranges' chunks fill.
 static long long range_items(long long tiles, int Hk, int D) { return tiles + resident(D) / Hk + 1; }
-// Key ranges are worth a second launch where the tiles do not fill the GPU and the keys are more than a few chunks: 1024 for
-// single tokens and the like (up to 32 rows a sequence on average), 4096 for longer lists, whose partials are large.
+// Key ranges are worth a second launch where the tiles do not fill the GPU and a tile may have many chunks: from 1024 keys on
+// for single tokens and the like (up to 32 rows a sequence on average, whose partials are small), from 1792 where the tiles
+// take a quarter of the GPU's places or fewer, otherwise from 4096. (us whole and in ranges: 200 tokens of 32 heads over 8
+// against 2000 keys 44 and 29, 2000 causal tokens of 8 heads over one 45 and 39; 1500 of 10 over 2 26 and 26, 3000 of 8 over
+// one 68 and 74, 1024 of 8 over 8 25 and 28.)
 static bool ranged(long long tiles, int B, int Tq, int Tk, int H, int Hk, int D) {
-  return tiles * Hk < 2 * resident(D) && Tk >= ((long long)Tq * (H / Hk) <= 32LL * B ? 16 : 64) * BK;
+  const long long items = tiles * Hk;
+  if (items >= 2 * resident(D)) return false;
+  const int chunks = (long long)Tq * (H / Hk) <= 32LL * B ? 16 : 4 * items <= resident(D) ? 28 : 64;
+  return Tk >= chunks * BK;
 }
 
 // Workspace of a shared-prefix call: partials of the sequences, partials of the prefix, plan; of a packed one: partials, plan.

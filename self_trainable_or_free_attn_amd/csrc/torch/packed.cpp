@@ -120,7 +120,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> packed_backward(const Tensor& dout_, 
               "lse must be the forward's");
   Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
   Tensor dbias = a.bias.defined() ? at::empty_like(a.bias) : at::empty({0}, q.options().dtype(at::kFloat));
-  const size_t bytes = es_packed_bwd_workspace(a.B, a.Tq, a.Tk, a.H, a.Hk, a.D, a.R, a.bias.defined());
+  const size_t bytes = es_packed_bwd_workspace(a.B, a.Tq, a.Tk, a.H, a.Hk, a.D, a.R, a.bias.defined(), causal);
   const Tensor ws = workspace(bytes, q);
   check_status("es_packed_bwd", (a.f16 ? es_packed_bwd_f16 : es_packed_bwd)(
       data(q), data(k), data(v), data(dout), data(out), static_cast<const float*>(data(lse)), a.ints(a.cu_q), a.ints(a.cu_k),

@@ -125,6 +125,23 @@ def test_backward(dev, D, dtype, H, Hk, causal, lens, keys):
 
 
 @pytest.mark.parametrize("D, dtype", TYPES)
+@pytest.mark.parametrize("lens, keys, H, Hk, pad", [([1500], [1500], 8, 1, 0), ([700, 5, 600], [650, 0, 1100], 6, 1, 3),
+                                                    ([1030], [70], 3, 3, 1), ([900, 901], [900, 901], 5, 1, 0)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_row_ranges(dev, D, dtype, lens, keys, H, Hk, pad, causal):
+    """Few key tiles against many rows: the KV owner's rows in ranges."""
+    from self_trainable_or_free_attn_amd import _lib
+    Tq, Tk = sum(lens) + pad, sum(keys) + pad
+    assert _lib.lib().es_packed_bwd_workspace(len(lens), Tq, Tk, H, Hk, D, 0, 0, causal) > 8 * Tq * H + 16
+    _case(lens, keys, H, Hk, D, dtype, causal, dev, train=True, pad=pad, seed=22)
+
+
+def test_row_ranges_with_a_bias(dev):
+    table = _api().relative_buckets(16, 60, device=dev)
+    _case([1200, 300], [1200, 300], 2, 1, 64, BF, False, dev, train=True, table=table, seed=23)
+
+
+@pytest.mark.parametrize("D, dtype", TYPES)
 @pytest.mark.parametrize("H, Hk", [(2, 2), (6, 3), (4, 1)])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("lens, keys", [([1], [1]), ([0, 70, 200, 3], [0, 70, 200, 3]), ([40, 5], [300, 0]), ([600], [450])])
