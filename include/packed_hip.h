@@ -16,7 +16,8 @@
  * to its position; its score against key j is scale * q.k + bias[buckets[clamp(j - position, -R, R) + R]][h].
  * Rows that see no key get out = 0 and lse = -inf and give no gradient. Rows behind the last sequence are such rows;
  * key rows behind it get zero gradients, and their values are never used.
- * (H / Hk) * (2 * R + 1) is at most ES_PACKED_BIAS_ROWS.
+ * Scores are float32 and must stay below 2^22 in magnitude. (H / Hk) * (2 * R + 1) is at most ES_PACKED_BIAS_ROWS. Bias values are finite or -inf (which masks); finite ones beyond
+ * +-ES_PACKED_BIAS_MAX count as that. Calls of about 2^24 / Hk sequences and more are refused.
  */
 #pragma once
 #include "echosparse_hip.h"
@@ -26,6 +27,7 @@ extern "C" {
 #endif
 
 #define ES_PACKED_BIAS_ROWS 784
+#define ES_PACKED_BIAS_MAX 131072.0f
 
 /* Forward. workspace: es_packed_fwd_workspace bytes (0: none needed; NULL / 0 is then accepted), for batches of few query
  * rows against many keys, whose keys are cut into ranges that run side by side and are merged in a fixed order. */

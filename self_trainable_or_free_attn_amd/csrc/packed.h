@@ -25,6 +25,9 @@ constexpr int BIAS_ROWS = ES_PACKED_BIAS_ROWS;  // G * (2 R + 1) at most
 // With one head a group the table repeats its ends for BIAS_PAD distances more on either side: the 32 keys of a run that is
 // not all at -R and below or all at R and beyond stand within 31 + 31 of that range, and need no clamp.
 constexpr int BIAS_PAD = 64, BIAS_TABLE = BIAS_ROWS + 2 * BIAS_PAD;
+// Finite bias values are held to this magnitude (see fill_bias).
+constexpr float BIAS_MAX = ES_PACKED_BIAS_MAX;
+constexpr long long MAX_GRID = 1LL << 24;  // workgroups of a launch: its threads are counted in 32 bits
 
 // x / d for 0 <= x < 2^31 by one multiplication: mul = ceil(2^(32 + sh) / d) with 2^sh < d <= 2^(sh + 1), whose error
 // mul * d - 2^(32 + sh) < d <= 2^(sh + 1) keeps x * error under 2^(32 + sh). d = 1: mul = 0.
@@ -158,7 +161,10 @@ __device__ __forceinline__ void wait_lds() {
 }
 
 // The bias of a head group by distance in log2 units, filled by the whole workgroup (which waits at a barrier before it reads
-// it): bias_at(g, d) with d clamped to -R .. R, or for G = 1 within BIAS_PAD of that.
+// it): bias_at(g, d) with d clamped to -R .. R, or for G = 1 within BIAS_PAD of that. Values like -1e9 or the lowest float, as
+// masks have them, leave a float32 score no bits of its product; where all keys of a row have one, the probabilities are taken
+// against a maximum rounded by more than the exponent's range and overflow. At 2^17 a score still has steps of 2^-6, and keys
+// with any other value beside them vanish all the same. -inf stays.
 __device__ __forceinline__ int bias_width(int G, int R) { return 2 * R + 1 + (G == 1 ? 2 * BIAS_PAD : 0); }
 __device__ __forceinline__ int bias_row(int G, int R, int g) { return g * bias_width(G, R) + R + (G == 1 ? BIAS_PAD : 0); }
 __device__ __forceinline__ void fill_bias(float* tab, const float* bias, const int* buckets, int num_buckets, int R, int G,
@@ -166,7 +172,8 @@ __device__ __forceinline__ void fill_bias(float* tab, const float* bias, const i
   const int n = bias_width(G, R);
   for (int i = threadIdx.x; i < G * n; i += blockDim.x) {
     const int g = i / n, d = min(max(i - bias_row(G, R, g), -R), R), bk = min(max(buckets[d + R], 0), num_buckets - 1);
-    tab[i] = bias[(size_t)bk * H + hk * G + g] * LOG2E;
+    const float x = bias[(size_t)bk * H + hk * G + g];
+    tab[i] = (fabsf(x) < INFINITY ? fminf(fmaxf(x, -BIAS_MAX), BIAS_MAX) : x) * LOG2E;
   }
 }
 // x[r] = x[r] * sc + bias of the key at distance d0 + 8 (r / 4) + r % 4; row: the table at distance 0

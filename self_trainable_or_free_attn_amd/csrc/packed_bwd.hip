@@ -17,8 +17,14 @@
 // the same for all keys of a row. Over n keys of about equal weight that shifts a row's dQ by 1 / sqrt(n) of what the
 // rounding of dS does, but with few keys it adds to it, and sums of unrounded dS (the bias gradient) have no other error.
 // So bwd_q takes delta = sum P dP / sum P over the keys in a pass of its own before the main one where a tile sees up to
-// EXACT_CHUNKS * 64 keys, and always with a bias, and stores it for bwd_kv, which runs after it. (Relative errors of dQ
-// against 64 bits, causal prompts of 1 to 6553 tokens in bf16: 2.6e-3 -> 2.4e-3; of the bias gradient 1e-3 -> 1e-6.)
+// EXACT_CHUNKS * 64 keys, and always with a bias, and stores it for bwd_kv, which runs after it. (Relative errors against 64
+// bits, causal sequences of 1 to 1200 tokens, bf16: dQ 2.55e-3 -> 2.36e-3, dK 2.52e-3 -> 2.34e-3, which is that of the
+// rounding of dS and the result, the bias gradient 1.3e-3 -> 2e-7; fp16: 3.3e-4 -> 2.9e-4, 3.4e-4 -> 8e-7.)
+// Bounds: the matrix units on long sequences. Clips of 13770, 11880 and 4096 tokens without a mask, 12 heads, D = 128: bwd_q
+// 2.89 ms, 1110 TFLOP/s of its three products (57 % of the cycles issue a matrix instruction, LDS 29 %), bwd_kv 4.54 ms, 940
+// TFLOP/s of its four (46 %; it waits the most, for its transfers and at the tile's barrier, with two workgroups a CU at 255
+// registers); causal prompts of 1 to 6553 tokens, 24 heads over 8: 0.61 and 0.88 ms. What bounds short ones is the chain of a tile's few chunks:
+// transfers, two products, exponentials, two products.
 // dS is rounded to the token type without the softmax scale (applied to the finished sums), which keeps it about ten times
 // further from the subnormal range of fp16.
 #include "packed.h"
@@ -61,6 +67,10 @@ __device__ __forceinline__ void lds_add(float* p, float x) {
   __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float*)p, x, 0, 0, false);
 }
 
+// Tiles of 64 keys x 64 rows: a wave's 32 x 32 of S and dP, its key's K and V rows and two sums of D x 32 just fit the
+// registers of two waves a SIMD (three at D = 64; four would spill: 8192 tokens of 16 heads, whole backward 1081 -> 1367 us).
+// (dP's products under the exponentials, as bwd_q has them, spill: 4428 -> 4500 us at 13770 tokens, 12 heads. Staging dO later
+// than Q computes the row addresses twice: whole backward 4.31 -> 4.43 ms.)
 template <int D, bool BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(BwdArgs a) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
@@ -271,6 +281,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
   store(acc_k, NDB, a.scale, a.dk);
 }
 
+// Tiles of 64 rows x 64 keys; Q and dO stay in registers, K and V are staged. Row statistics are per lane, so P needs no
+// reduction. With a bias the LDS (staging, table, four histograms) still leaves two workgroups a CU.
 template <int D, bool BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdArgs a) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
@@ -458,8 +470,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
             // The run's diagonals, in a 64-lane shift register: row q's dS for key e enters at lane q and moves up a lane
             // a key, so that all of one distance meet; after key 31 lane i holds distance key0 + 31 - (first row) - i. Keys
             // 8 n .. 8 n + 3 are in the low half wave, the next four in the high one, which the swap brings down. (One LDS
-            // add for 32 x 32 values; adding each by itself, below, took a training pass of 2303 tokens, 24 heads from 171
-            // to 126 us.)
+            // add for 32 x 32 values: 2303 tokens of 24 heads, D = 64, this kernel 93 us with each added by itself, as
+            // below, and 42 so.)
             float v = 0.0f;
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
@@ -544,7 +556,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
     }
 }
 
-// dV and dK from the row ranges' sums, in order: four channels a thread
+// dV and dK from the row ranges' sums, in order: four channels a thread. Memory bound: the sums once (ranges * Tk * Hk * 8 D
+// bytes), which the rule below weighs as two steps a range.
 template <int D>
 __global__ __launch_bounds__(256) void kv_sums_kernel(BwdArgs a) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, rows = (size_t)a.Tk * a.Hk, row = i / (D / 2);
@@ -558,7 +571,8 @@ __global__ __launch_bounds__(256) void kv_sums_kernel(BwdArgs a) {
 }
 
 // dbias[n][h] = sum over the row tiles and over the distances of bucket n: one workgroup a head. First each of four slices of
-// 256 lanes adds every fourth tile, a distance a lane, eight tiles in flight; then a wave adds up a bucket's distances.
+// 256 lanes adds every fourth tile, a distance a lane, eight tiles in flight; then a wave adds up a bucket's distances. Latency
+// bound: 2303 tokens of 24 heads 4.1 us.
 __global__ __launch_bounds__(1024) void bias_sums_kernel(BwdArgs a) {
   __shared__ float sums[4][BIAS_ROWS];
   __shared__ int which[BIAS_ROWS];
@@ -683,8 +697,8 @@ extern "C" int ES_VSA_API(es_packed_bwd)(const void* q, const void* k, const voi
   a.scale_log2 = scale * LOG2E;
   a.q_tiles = (int)tile_numbers<BK>(B, Tq, a.G);
   a.k_tiles = (int)tile_numbers<BK>(B, Tk, 1);
-  ES_REQUIRE((long long)a.q_tiles * Hk < (1LL << 31) && (long long)a.k_tiles * Hk * a.ranges < (1LL << 31), ES_ERR_UNSUPPORTED,
-             "packed: grid too large");
+  ES_REQUIRE((long long)a.q_tiles * Hk < MAX_GRID && (long long)a.k_tiles * Hk * a.ranges < MAX_GRID, ES_ERR_UNSUPPORTED,
+             "packed: too many sequences");
   if (Tq > 0) {
     const dim3 grid((unsigned)(a.q_tiles * Hk));
     if (D == 64) {

@@ -8,6 +8,13 @@
 //     fourth run of 32 keys, staged in its own quarter of LDS without a barrier; the four softmax states are merged at the
 //     end. The next K run is requested when this one's products have read it, the next V run likewise, so one of them is
 //     always in flight.
+// What bounds them: wide tiles the matrix units and what runs beside them on long sequences (32760 causal tokens of 24 heads over
+// 8, D = 128: 6.06 ms, 1090 TFLOP/s; 53 % of the cycles issue a matrix instruction, 51 % vector work, LDS 27 %, no bank
+// conflicts), the transfers where many tiles stream different keys from HBM, and on sequences of a few hundred rows the chain
+// of a tile's few chunks. Narrow tiles: HBM (8 tokens, 40 heads over 8, caches of 513 to 75600 keys: 654 MB in 137 us, 4.8
+// TB/s, what a large copy reaches).
+// 128 rows a wide tile and not 256 on eight waves: those read K and V half as often, but stop at their barriers together (32760
+// causal tokens 6.57 -> 6.95 ms; 13770 of 12 heads without a mask 1433 -> 1360 us).
 // Key ranges: with few tiles the chunks of a tile are cut into ranges, one workgroup each, that leave unnormalised partials
 // (O, running maximum, sum) in the workspace; merge_kernel adds them in order.
 #include "packed.h"
@@ -35,10 +42,11 @@ struct FwdArgs {
   float *lse, *part, *part_prefix;
   FastDiv div_g;
   int B, Tq, Tk, H, Hk, G, R, num_buckets, causal;
-  int tiles;      // tile numbers of a head
+  int tiles;        // tile numbers of a head
+  int items;        // ranged launches: items of a head
   int2* plan;       // ranged launches: (ranges a tile, first item) of each list
   float inv_slots;  // ranged launches: Hk / the workgroups that the GPU holds at once
-  float scale;    // log2(e) * softmax scale
+  float scale;      // log2(e) * softmax scale
   // shared prefix: rows 0 .. P - 1 of k_prefix / v_prefix are seen by every row
   const e16_t *kp, *vp;
   const int* lens;
@@ -591,9 +599,11 @@ __device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Range
 }
 
 // Partial `item` of a launch, all kv heads of an item side by side. Shared prefix: the prefix's items have a part of their own,
-// with whole tiles; those of the sequences are as long as their lists.
+// with whole tiles; those of the sequences are as long as their lists. (Running lengths that decrease, which the header rules
+// out, may name more items than the launch has: the merge then reads the last one.)
 template <int D>
 __device__ __forceinline__ float* partial(float* base, int rows, const FwdArgs& a, int item, int hk) {
+  item = min(max(item, 0), a.items - 1);
   return base + ((size_t)item * a.Hk + hk) * part_floats(rows, D);
 }
 
@@ -623,6 +633,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_ranges_kernel(Fwd
   run_tile<D, BIAS>(a, j, lds, stats, tab);
 }
 
+// A tile of the prefix's list holds rows of several sequences, so a prefix is read once for 128 rows of the batch and not once a
+// sequence. Single tokens are HBM bound (the prefix is read once, every cache once), more of them matrix bound.
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
@@ -658,7 +670,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(Fwd
 
 // O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's partials in order: D / 4 lanes a row, which first take one
 // partial's m and l each and then, eight partials in flight, four channels each. SHARED: a row's prefix partials, then those
-// of its own cache. Grid: (tile numbers * Hk, 4), rows in turn over the second index.
+// of its own cache. Grid: (tile numbers * Hk, 4), rows in turn over the second index. Latency bound: 4 to 12 us.
 template <int D, bool SHARED>
 __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
   constexpr int LPR = D / 4, RPB = 256 / LPR;
@@ -823,7 +835,7 @@ extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const voi
   a.causal = causal != 0;
   a.scale = scale * LOG2E;
   a.tiles = (int)tile_numbers<TILE>(B, Tq, a.G);
-  ES_REQUIRE((long long)a.tiles * Hk < (1LL << 31), ES_ERR_UNSUPPORTED, "packed: grid too large");
+  ES_REQUIRE((long long)a.tiles * Hk < MAX_GRID, ES_ERR_UNSUPPORTED, "packed: too many sequences");
   if (ranged(a.tiles, B, Tq, Tk, H, Hk, D)) {
     ES_REQUIRE(workspace && workspace_bytes >= es_packed_fwd_workspace(B, Tq, Tk, H, Hk, D), ES_ERR_INVALID,
                "packed: workspace too small");
@@ -831,6 +843,7 @@ extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const voi
     const Layout l = packed_layout(a.tiles, B, Hk, D);
     a.plan = (int2*)((char*)workspace + l.plan);
     a.inv_slots = (float)Hk / (float)resident(D);
+    a.items = (int)l.items;
     const dim3 grid((unsigned)(l.items * Hk)), merge((unsigned)(a.tiles * Hk), 4);
     if (D == 64) {
       if (bias) hipLaunchKernelGGL((packed_ranges_kernel<64, true>), grid, dim3(256), 0, stream, a);
@@ -888,11 +901,12 @@ extern "C" int ES_VSA_API(es_shared_prefix_fwd)(const void* q, const void* k_pre
   a.scale = scale * LOG2E;
   const Layout l = shared_layout(B, n, H, Hk, D);
   const long long own = (long long)B * (((long long)n * a.G + TILE - 1) / TILE);
-  ES_REQUIRE(l.items * Hk < (1LL << 31), ES_ERR_UNSUPPORTED, "shared prefix: grid too large");
+  ES_REQUIRE(l.items * Hk < MAX_GRID, ES_ERR_UNSUPPORTED, "shared prefix: too many sequences");
   a.part_prefix = (float*)((char*)workspace + l.prefix);
   a.plan = (int2*)((char*)workspace + l.plan);
   a.part_rows = l.rows;
   a.inv_slots = (float)Hk / (float)resident(D);
+  a.items = (int)l.items;
   const dim3 grid((unsigned)(l.items * Hk)), merge((unsigned)(own * Hk), 4);
   if (D == 64) {
     hipLaunchKernelGGL((shared_prefix_kernel<64>), grid, dim3(256), 0, stream, a);

@@ -1,7 +1,7 @@
 // Torch operators of the packed-sequence entry points with their outputs, workspaces and gradient (the generated ones in
 // ops.cpp write into given tensors): echosparse_gfx950::packed_attention and ::shared_prefix_attention, called by packed.py,
-// which checks the arguments against the documentation. A Python autograd function took 100 us more of host time a training
-// call than this one, about as long as the kernels of 2000 tokens run.
+// which checks the arguments against the documentation. (Host time of a training call with a Python autograd function 150 us,
+// with this one 99; the kernels of 2300 tokens of 24 heads run about as long.)
 //
 // Every kernel checks what the C entry points rely on (device, dtype, layout, sizes), so a direct call cannot reach them with
 // other pointers than it names.

@@ -130,12 +130,13 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: Op
     h // (H // Hk)). cu_q, cu_k: int32 [B + 1] GPU tensors of running lengths from 0; sequence b holds rows cu[b] to
     cu[b + 1] - 1 (cu_k None: the queries' own). Without both, q / k / v are one sequence, or a batch [B, Lq, H, D] /
     [B, Lk, Hk, D]. Lengths may be zero. Rows behind the last sequence give zeros, and key rows there are never used; within
-    a sequence values must be finite, also where the causal mask hides them.
+    a sequence values must be finite, also where the causal mask hides them, and scores below 2^22 in magnitude.
 
     With nq queries and nk keys query i stands at position i + nk - nq (the last query at the last key): with causal it sees
     the keys up to that position. A row that sees no key gives zeros and an LSE of -inf, and no gradient. scale: 1 / sqrt(D)
     if None. bias [num_buckets, H] with buckets (`relative_buckets`, int32 [2 R + 1]) adds bias[buckets[d + R], h] to the
-    score of a key at distance d from the query, d clamped to -R .. R; (H // Hk) * (2 R + 1) is at most 784.
+    score of a key at distance d from the query, d clamped to -R .. R; (H // Hk) * (2 R + 1) is at most 784. Its values are finite
+    or -inf, which masks; finite ones are held to +-131072.
 
     Returns out like q, with return_lse also the natural-log LSE [Tq, H] ([B, Lq, H]) in float32 (no gradient). Gradients
     are deterministic, and those of a bias are summed in float32; the backward itself is not differentiable."""

@@ -278,8 +278,8 @@ def test_c_entry_points_refuse_before_any_launch():
         return _c("es_packed_fwd" + suffix, q, k, k, cu_q, cu_k, bias, buckets, nb, R, out, out, ws, wsb, B, Tq, Tk, H, Hk, D,
                   0, scale)
 
-    def bwd(dout=p, dq=p, dk=p, bias=None, dbias=None, ws=p, wsb=big, Tq=8, R=0):
-        return _c("es_packed_bwd", p, p, p, dout, p, p, p, p, bias, bias, 4, R, dq, dk, dk, dbias, ws, wsb, 1, Tq, 9, 4, 2, 64,
+    def bwd(dout=p, dq=p, dk=p, bias=None, dbias=None, ws=p, wsb=big, Tq=8, R=0, B=1, Hk=2):
+        return _c("es_packed_bwd", p, p, p, dout, p, p, p, p, bias, bias, 4, R, dq, dk, dk, dbias, ws, wsb, B, Tq, 9, 4, Hk, 64,
                   0, 1.0)
 
     def shared(q=p, kp=p, k=p, lens=p, out=p, ws=p, wsb=big, B=2, n=1, P=9, S=5, H=4, Hk=2, D=128, scale=1.0):
@@ -297,6 +297,8 @@ def test_c_entry_points_refuse_before_any_launch():
             (lambda: fwd(bias=p, buckets=p, nb=4, R=196), 2, "at most 784"),
             (lambda: fwd(bias=p, buckets=p, nb=4, R=1 << 30), 2, "at most 784"),
             (lambda: fwd(D=96, suffix="_f16"), 2, "64 or 128"),
+            (lambda: fwd(B=1 << 22, Hk=4), 2, "too many sequences"), (lambda: bwd(B=1 << 22, Hk=4), 2, "too many sequences"),
+            (lambda: shared(B=1 << 22, Hk=4), 2, "too many sequences"),
             (lambda: fwd(q=ctypes.c_void_p(264)), 1, "aligned"), (lambda: fwd(ws=ctypes.c_void_p(260)), 1, "aligned"),
             (lambda: bwd(dq=ctypes.c_void_p(258)), 1, "aligned"), (lambda: shared(k=ctypes.c_void_p(8)), 1, "aligned"),
             (lambda: bwd(dout=None), 1, "null tensor"), (lambda: bwd(dq=None), 1, "null tensor"),

@@ -136,6 +136,13 @@ def test_row_ranges(dev, D, dtype, lens, keys, H, Hk, pad, causal):
     _case(lens, keys, H, Hk, D, dtype, causal, dev, train=True, pad=pad, seed=22)
 
 
+@pytest.mark.parametrize("H, Hk", [(100, 1), (65, 1), (256, 2)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_more_heads_than_a_tile_has_rows(dev, H, Hk, causal):
+    _case([5, 1, 30], [9, 1, 30], H, Hk, 64, BF, causal, dev, train=True, seed=42)
+    _case([1, 2], [2000, 70], H, Hk, 128, FP, causal, dev, seed=43)
+
+
 def test_row_ranges_with_a_bias(dev):
     table = _api().relative_buckets(16, 60, device=dev)
     _case([1200, 300], [1200, 300], 2, 1, 64, BF, False, dev, train=True, table=table, seed=23)
@@ -178,6 +185,54 @@ def test_scores_of_any_size(dev, dtype):
     # (scores of -60000 keep 2^-8 of their last bits in float32: the probabilities are off by up to that in the exponent)
     value, bound = want["out"]
     ref.check("out", out, value, bound + 2.0 ** -7 * value.abs().amax() * 4)
+
+
+@pytest.mark.parametrize("D, dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("H, Hk", [(2, 2), (4, 2)])
+def test_bias_that_masks(dev, D, dtype, causal, H, Hk):
+    """Buckets of -inf: keys without weight, and rows (all of one head's, some of another's) without any key."""
+    table = _api().relative_buckets(16, 60, device=dev)
+    lens = [150, 1, 70]
+    t = _inputs(lens, lens, H, Hk, D, dtype, dev, 40, buckets=16)
+    t["bias"][:, 1] = -math.inf
+    t["bias"][2:6, 0] = -math.inf
+    t["bias"][:3, 0] = -math.inf        # (the first rows of a causal sequence then see nothing)
+    t["bias"][8, 0] = -math.inf
+    want = ref.packed(t["q"], t["k"], t["v"], lens, lens, causal, 1 / math.sqrt(D), t["bias"], table, t["dout"])
+    names = ("q", "k", "v", "bias")
+    leaves = [t[n].requires_grad_() for n in names]
+    out, lse = _api().packed_attention(*leaves[:3], _cu(lens, dev), causal=causal, bias=leaves[3], buckets=table,
+                                       return_lse=True)
+    ref.check("out", out, *want["out"])
+    ref.check("lse", lse, *want["lse"])
+    for n, x in zip(names, torch.autograd.grad(out, leaves, t["dout"])):
+        ref.check("d" + n, x, *want["d" + n])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("low", [-1e6, -1e9, -3.4028234663852886e38, 1e12])
+@pytest.mark.parametrize("R", [0, 4])
+def test_bias_of_any_size(dev, dtype, low, R):
+    """One value for all keys cancels, whatever it is. Held to 2^17 (189097 in log2 units, where float32 has steps of 2^-6), it
+    rounds a score by up to 2^-7, which puts a probability off by up to 2^-7 ln 2 and the row's sum by as much: 2^-6 of
+    sum p |v| <= max |v| together. The stored LSE adds its own half step 2^-8 (natural) and twice that of 2^-7 (log2), so the
+    backward's probabilities are off by less than 2^-5."""
+    L, D = 90, 64
+    t = _inputs([L], [L], 2, 2, D, dtype, dev, 41)
+    bias, table = torch.full((1, 2), low, device=dev), torch.zeros(2 * R + 1, dtype=torch.int32, device=dev)
+    want = ref.packed(t["q"], t["k"], t["v"], [L], [L], True, 0.125, None, None, t["dout"])
+    leaves = [t[n].requires_grad_() for n in "qkv"]
+    out = _api().packed_attention(*leaves, causal=True, bias=bias, buckets=table)
+    value, bound = want["out"]
+    ref.check("out", out, value, bound + 2.0 ** -6 * t["v"].detach().abs().max().double())
+    dq, dk, dv = torch.autograd.grad(out, leaves, t["dout"])
+    value, bound = want["dv"]
+    s = 0.125 * torch.einsum("ihd,jhd->hij", t["q"].detach().double(), t["k"].detach().double())
+    p = torch.softmax(s.masked_fill(torch.ones(L, L, device=dev, dtype=torch.bool).triu(1), -math.inf), -1)
+    moved = (p.transpose(1, 2) @ t["dout"].abs().double().transpose(0, 1).contiguous()).transpose(0, 1)
+    ref.check("dv", dv, value, bound + 2.0 ** -5 * moved)
+    assert dq.isfinite().all() and dk.isfinite().all()
 
 
 def test_batch_form_equals_packed_form(dev):
@@ -372,6 +427,67 @@ def test_streams_and_graphs(dev):
                 torch.cuda.synchronize()
                 assert torch.equal(o, want)
                 assert torch.equal(eager(), want)
+
+
+def test_two_streams_at_once(dev):
+    """Calls with key and row ranges, whose workspaces hold partial sums, side by side on two streams."""
+    api = _api()
+    ts = [_inputs([600], [5000], 8, 1, 128, BF, dev, 44 + i) for i in range(2)]
+    step = lambda t: (lambda out, leaves: [out.detach(), *torch.autograd.grad(out, leaves, t["dout"])])(
+        *(lambda x: (api.packed_attention(*x, causal=True), x))([t[n].detach().requires_grad_() for n in "qkv"]))
+    want = [step(t) for t in ts]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ts]
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(ts[i]))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        for r in runs:
+            assert all(torch.equal(x, y) for x, y in zip(r, w))
+
+
+def test_ranges_in_a_graph(dev):
+    """A captured step with key ranges and row ranges, replayed with other lengths between eager ones."""
+    api = _api()
+    t = _inputs([1500], [5000], 8, 1, 128, BF, dev, 46)
+    cu_q, cu_k = _cu([1500, 0], dev), _cu([5000, 0], dev)
+
+    def step():
+        leaves = [t[n].detach().requires_grad_() for n in "qkv"]
+        out = api.packed_attention(*leaves, cu_q, cu_k, causal=True)
+        return [out.detach(), *torch.autograd.grad(out, leaves, t["dout"])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for lens, keys in (([1500, 0], [5000, 0]), ([700, 800], [4200, 800]), ([1, 1400], [4000, 900])):
+        cu_q.copy_(_cu(lens, dev))
+        cu_k.copy_(_cu(keys, dev))
+        want = step()
+        for _ in range(2):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), lens
+
+
+def test_no_queries(dev):
+    """Keys without a query: zero gradients for them, and for the bias."""
+    api = _api()
+    t = _inputs([0], [70], 4, 2, 64, BF, dev, 47, buckets=8)
+    table = api.relative_buckets(8, 30, device=dev)
+    leaves = [t[n].requires_grad_() for n in ("q", "k", "v", "bias")]
+    out = api.packed_attention(*leaves[:3], _cu([0], dev), _cu([70], dev), bias=leaves[3], buckets=table)
+    for x, y in zip(torch.autograd.grad(out, leaves, t["dout"]), leaves):
+        assert x.shape == y.shape and not x.any()
 
 
 def test_training_step_in_a_graph(dev):
