@@ -160,6 +160,10 @@ __device__ __forceinline__ void wait_lds() {
   asm volatile("" ::: "memory");
 }
 
+// Two or three workgroups share a SIMD, a wave each: s_setprio(1) around a wave's runs of products lets it issue them before the
+// other waves' exponentials, whose instructions then fill the gaps; at one priority the two take turns and the matrix unit waits.
+// (Measured where it is used.)
+
 // The bias of a head group by distance in log2 units, filled by the whole workgroup (which waits at a barrier before it reads
 // it): bias_at(g, d) with d clamped to -R .. R, or for G = 1 within BIAS_PAD of that. Values like -1e9 or the lowest float, as
 // masks have them, leave a float32 score no bits of its product; where all keys of a row have one, the probabilities are taken

@@ -70,7 +70,9 @@ __device__ __forceinline__ void lds_add(float* p, float x) {
 // Tiles of 64 keys x 64 rows: a wave's 32 x 32 of S and dP, its key's K and V rows and two sums of D x 32 just fit the
 // registers of two waves a SIMD (three at D = 64; four would spill: 8192 tokens of 16 heads, whole backward 1081 -> 1367 us).
 // (dP's products under the exponentials, as bwd_q has them, spill: 4428 -> 4500 us at 13770 tokens, 12 heads. Staging dO later
-// than Q computes the row addresses twice: whole backward 4.31 -> 4.43 ms.)
+// than Q computes the row addresses twice: whole backward 4.31 -> 4.43 ms.) With the products of both kernels at a raised
+// priority (packed.h) the whole backward of 13770 tokens of 12 heads takes 4.26 ms, not 4.40, of 8192 causal tokens of 24 heads
+// over 8 1611 us, not 1661, at D = 64 1063, not 1076.
 template <int D, bool BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(BwdArgs a) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
@@ -177,8 +179,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
       }
     };
     f32x16 p = {}, dp = {};
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) p = emfma(qf[ks], kreg[ks], p);
+    __builtin_amdgcn_s_setprio(0);
     // the wave's rows, whose positions ascend: a key is seen from its own position on
     const int t0 = divide(a.div_g, i * BK), rel = i * BK - t0 * a.G;
     const bool masked = (a.causal && t0 + token_in_tile(rel + 32 * qh) + shift < kb * BK + 32 * kh + 31) ||
@@ -224,11 +228,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
       float x[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = p[r];
+      __builtin_amdgcn_s_setprio(1);
       product(dt, epack8(&x[0]), epack8(&x[8]), acc_v);
     }
     __builtin_amdgcn_sched_barrier(0);  // (dP after dV: raised above it, its operands do not fit the registers)
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(dt, aoff ^ (32 * ks)), vreg[ks], dp);
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const f32x4 d4 = *reinterpret_cast<const f32x4*>(&st_s[sb][1][32 * qh + 8 * g + 4 * hi]);
@@ -239,7 +245,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
       float x[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = p[r];
+      __builtin_amdgcn_s_setprio(1);
       product(qt, epack8(&x[0]), epack8(&x[8]), acc_k);
+      __builtin_amdgcn_s_setprio(0);
     }
     dma_wait();
     __syncthreads();
@@ -393,10 +401,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
         if (8 * (r / 4) + r % 4 >= left) x[r] = -INFINITY;
     }
     // (dP's products run under the exponentials)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(vt, koff ^ (32 * ks)), dreg[ks], dp);
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = exp2f_fast(fmaf(x[r], sc, cb - ls));
+    __builtin_amdgcn_s_setprio(0);
   };
   // the chunk's rows of K, read before the next chunk's transfers are issued: S then finds its operands ready
   auto read_k = [&](const char* kt, ev8 (&kf)[NKS]) {
@@ -509,12 +519,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
         }
       }
       const ev8 sa = epack8(&ds[0]), sb8 = epack8(&ds[8]);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
         const int t0 = toff0 ^ (64 * db), t1 = toff1 ^ (64 * db);
         dq[db] = emfma(ecat_tr(lds_read_tr(kt, t0), lds_read_tr(kt, t1)), sa, dq[db]);
         dq[db] = emfma(ecat_tr(lds_read_tr(kt + TILE_BYTES / 4, t0), lds_read_tr(kt + TILE_BYTES / 4, t1)), sb8, dq[db]);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
     sb ^= 1;
     dma_wait();

@@ -244,7 +244,8 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
       // second under the exponentials of the first, O += V^T P^T of the first under those of the second. (The first run's
       // probabilities are held back over the second's test of the maximum, and scaled with O where that one moves. Against
       // both S first and each run's exponentials before its own products: 32760 causal tokens, 24 heads 6.39 -> 6.08 ms, 8192
-      // at D = 64, 32 heads 345 -> 318 us.)
+      // at D = 64, 32 heads 345 -> 318 us.) Products run at a raised priority (packed.h): 32760 causal tokens 6.08 -> 5.94
+      // ms, 13770 of 12 heads without a mask 1332 -> 1225 us, 8192 causal of 32 heads 541 -> 522 (at D = 64 324 -> 326).
       const bool masked = (c + 1) * BK > seen_min;
       float sc, c0, c1, alpha;
       ev8 pa, pb, qa, qb;
@@ -254,6 +255,7 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) kf[ks] = elds16(kb + TILE_BYTES / 2, off.k0 ^ (32 * ks));
       x.raise(x.scores(a, tab, s0, c * BK, hi, masked, low, high, sc, c0), alpha);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) s1 = emfma(kf[ks], x.q[ks], s1);
       x.exponentials(s0, sc, c0, pa, pb);
@@ -262,6 +264,7 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
         __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
         __builtin_amdgcn_sched_group_barrier(0x402, 14, 0);
       }
+      __builtin_amdgcn_s_setprio(0);
       if (x.raise(x.scores(a, tab, s1, c * BK + 32, hi, masked, low, high, sc, c1), alpha)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -269,11 +272,13 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
           pb[e] = (elem_t)((float)pb[e] * alpha);
         }
       }
+      __builtin_amdgcn_s_setprio(1);
       x.values(vb, off.t0, off.t1, pa);
       x.values(vb + TILE_BYTES / 4, off.t0, off.t1, pb);
       x.exponentials(s1, sc, c1, qa, qb);
       x.values(vb + TILE_BYTES / 2, off.t0, off.t1, qa);
       x.values(vb + 3 * (TILE_BYTES / 4), off.t0, off.t1, qb);
+      __builtin_amdgcn_s_setprio(0);
     }
     dma_wait();
     __syncthreads();

@@ -185,16 +185,20 @@ using ForwardSignature = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&
 
 OptTensor maybe(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
+const c10::TypedOperatorHandle<BackwardSignature>& backward_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("echosparse_gfx950::packed_attention_backward", "")
+                             .typed<BackwardSignature>();
+  return op;
+}
+
 // the backward is an operator of its own, whose gradient is refused rather than left out
 struct PackedBackward : torch::autograd::Function<PackedBackward> {
   static variable_list forward(AutogradContext* ctx, const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
                                const Tensor& out, const Tensor& lse, const OptTensor& bias, const OptTensor& cu_q,
                                const OptTensor& cu_k, const OptTensor& buckets, int64_t B, bool causal, double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static const auto op = c10::Dispatcher::singleton()
-                               .findSchemaOrThrow("echosparse_gfx950::packed_attention_backward", "")
-                               .typed<BackwardSignature>();
-    auto [dq, dk, dv, dbias] = op.call(dout, q, k, v, out, lse, bias, cu_q, cu_k, buckets, B, causal, scale);
+    auto [dq, dk, dv, dbias] = backward_op().call(dout, q, k, v, out, lse, bias, cu_q, cu_k, buckets, B, causal, scale);
     return {dq, dk, dv, dbias};
   }
   static variable_list backward(AutogradContext*, const variable_list&) {
@@ -206,6 +210,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> packed_backward_autograd(const Tensor
                                                                     const OptTensor& bias, const OptTensor& cu_q,
                                                                     const OptTensor& cu_k, const OptTensor& buckets, int64_t B,
                                                                     bool causal, double scale) {
+  if (!at::GradMode::is_enabled()) {  // (a backward without create_graph: no node to make)
+    at::AutoDispatchBelowADInplaceOrView below;
+    return backward_op().call(dout, q, k, v, out, lse, bias, cu_q, cu_k, buckets, B, causal, scale);
+  }
   auto r = PackedBackward::apply(dout, q, k, v, out, lse, bias, cu_q, cu_k, buckets, B, causal, scale);
   return {r[0], r[1], r[2], r[3]};
 }
@@ -231,12 +239,9 @@ struct PackedForward : torch::autograd::Function<PackedForward> {
     variable_list res(10);
     if (!grads[0].defined()) return res;
     const auto s = ctx->get_saved_variables();
-    static const auto op = c10::Dispatcher::singleton()
-                               .findSchemaOrThrow("echosparse_gfx950::packed_attention_backward", "")
-                               .typed<BackwardSignature>();
-    auto [dq, dk, dv, dbias] = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], maybe(s[5]), maybe(s[6]), maybe(s[7]),
-                                       maybe(s[8]), ctx->saved_data["B"].toInt(), ctx->saved_data["causal"].toBool(),
-                                       ctx->saved_data["scale"].toDouble());
+    auto [dq, dk, dv, dbias] = backward_op().call(grads[0], s[0], s[1], s[2], s[3], s[4], maybe(s[5]), maybe(s[6]),
+                                                  maybe(s[7]), maybe(s[8]), ctx->saved_data["B"].toInt(),
+                                                  ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
     res[0] = dq;
     res[1] = dk;
     res[2] = dv;
