@@ -675,7 +675,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(Fwd
 
 // O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's partials in order: D / 4 lanes a row, which first take one
 // partial's m and l each and then, eight partials in flight, four channels each. SHARED: a row's prefix partials, then those
-// of its own cache. Grid: (tile numbers * Hk, 4), rows in turn over the second index. Latency bound: 4 to 12 us.
+// of its own cache. Grid: (tile numbers * Hk, merge_rows). Latency bound: 4 to 12 us.
 template <int D, bool SHARED>
 __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
   constexpr int LPR = D / 4, RPB = 256 / LPR;
@@ -777,6 +777,9 @@ static bool ranged(long long tiles, int B, int Tq, int Tk, int H, int Hk, int D)
   return Tk >= chunks * BK;
 }
 
+// Workgroups a tile of the merge: a row each thread group, as far as a sequence can have rows.
+static unsigned merge_rows(long long rows, int D) { return (unsigned)((std::min<long long>(rows, TILE) * D / 4 + 255) / 256); }
+
 // Workspace of a shared-prefix call: partials of the sequences, partials of the prefix, plan; of a packed one: partials, plan.
 struct Layout {
   long long items;               // a head
@@ -849,7 +852,7 @@ extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const voi
     a.plan = (int2*)((char*)workspace + l.plan);
     a.inv_slots = (float)Hk / (float)resident(D);
     a.items = (int)l.items;
-    const dim3 grid((unsigned)(l.items * Hk)), merge((unsigned)(a.tiles * Hk), 4);
+    const dim3 grid((unsigned)(l.items * Hk)), merge((unsigned)(a.tiles * Hk), merge_rows((long long)Tq * a.G, D));
     if (D == 64) {
       if (bias) hipLaunchKernelGGL((packed_ranges_kernel<64, true>), grid, dim3(256), 0, stream, a);
       else hipLaunchKernelGGL((packed_ranges_kernel<64, false>), grid, dim3(256), 0, stream, a);
@@ -912,7 +915,7 @@ extern "C" int ES_VSA_API(es_shared_prefix_fwd)(const void* q, const void* k_pre
   a.part_rows = l.rows;
   a.inv_slots = (float)Hk / (float)resident(D);
   a.items = (int)l.items;
-  const dim3 grid((unsigned)(l.items * Hk)), merge((unsigned)(own * Hk), 4);
+  const dim3 grid((unsigned)(l.items * Hk)), merge((unsigned)(own * Hk), merge_rows((long long)n * a.G, D));
   if (D == 64) {
     hipLaunchKernelGGL((shared_prefix_kernel<64>), grid, dim3(256), 0, stream, a);
     hipLaunchKernelGGL((merge_kernel<64, true>), merge, dim3(256), 0, stream, a);
