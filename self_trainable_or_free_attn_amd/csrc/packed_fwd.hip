@@ -1,15 +1,15 @@
 // Forward of attention over packed sequences and over a shared prefix (gfx950, MFMA 32x32x16, bf16 / fp16).
 //
-// One workgroup of four waves owns a tile of up to 128 rows of (token, head in group) (packed.h) and streams the keys its
+// One workgroup of four waves owns a tile of up to 128 (small grids: 64) rows of (token, head in group) (packed.h) and streams the keys its
 // rows see in 64-key chunks, online softmax: S^T = K Q^T, so that exp(S^T) is the B operand of O^T += V^T P^T.
 //   wide tiles (more than 32 rows): each wave has 32 rows; a chunk is staged once in LDS for all four, the next one's
-//     transfers in flight under its products.
+//     transfers in flight under its products. With 64 rows two waves share 32 rows and take half of each chunk's keys.
 //   narrow tiles (up to 32 rows: single tokens with their head group): every wave has the same 32 rows and takes every
 //     fourth run of 32 keys, staged in its own quarter of LDS without a barrier; the four softmax states are merged at the
 //     end. The next K run is requested when this one's products have read it, the next V run likewise, so one of them is
 //     always in flight.
 // What bounds them: wide tiles the matrix units and what runs beside them on long sequences (32760 causal tokens of 24 heads over
-// 8, D = 128: 6.06 ms, 1090 TFLOP/s; 53 % of the cycles issue a matrix instruction, 51 % vector work, LDS 27 %, no bank
+// 8, D = 128: 5.94 ms, 1110 TFLOP/s; 53 % of the cycles issue a matrix instruction, 51 % vector work, LDS 27 %, no bank
 // conflicts), the transfers where many tiles stream different keys from HBM, and on sequences of a few hundred rows the chain
 // of a tile's few chunks. Narrow tiles: HBM (8 tokens, 40 heads over 8, caches of 513 to 75600 keys: 654 MB in 137 us, 4.8
 // TB/s, what a large copy reaches).
@@ -20,6 +20,7 @@
 #include "packed.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace es {
 
@@ -54,11 +55,11 @@ struct FwdArgs {
   int part_rows;  // rows of a sequence's partial
 };
 
-// What one workgroup computes: rows of tile t of the list of nq * G rows that starts at token q0, against key rows
+// What one workgroup computes: the tile from row r0 on of the list of nq * G rows that starts at token q0, against key rows
 // 0 .. nk - 1 behind k / v (this kv head's first row), chunks c0 .. c1 - 1 of them.
 struct Job {
   const e16_t *k, *v;
-  int q0, nq, nk, hk, t, c0, c1, causal;
+  int q0, nq, nk, hk, r0, c0, c1, causal;
   float* part;  // a partial of `part_rows` rows; nullptr: finished rows go to out / lse
   int part_rows;
 };
@@ -70,9 +71,10 @@ __host__ __device__ constexpr int part_floats(int rows, int D) { return rows * (
 __device__ __forceinline__ int keys_seen(const FwdArgs& a, const Job& j, int r) {
   return j.causal ? min(max(divide(a.div_g, r) + 1 + j.nk - j.nq, 0), j.nk) : j.nk;
 }
-// chunks that any row of the job's tile sees
+// chunks that any of the M rows of the job's tile sees
+template <int M>
 __device__ __forceinline__ int tile_chunks(const FwdArgs& a, const Job& j) {
-  const int last = min(j.nq * a.G, (j.t + 1) * TILE) - 1;
+  const int last = min(j.nq * a.G, j.r0 + M) - 1;
   return (keys_seen(a, j, last) + BK - 1) / BK;
 }
 
@@ -192,12 +194,14 @@ __device__ __forceinline__ void store_row(const FwdArgs& a, size_t at, int col, 
   *reinterpret_cast<ushort4*>(a.out + at * D + col) = v4;
 }
 
-template <int D, bool BIAS>
-__device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* lds, float* tab) {
+// M = 128: 32 rows a wave; M = 64: two row groups x two key halves, whose softmax states are merged at the end
+template <int D, bool BIAS, int M>
+__device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* lds, float* stats, float* tab) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
   const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r0 = j.t * TILE + wv * 32, rows = j.nq * a.G;
+  const int rg = M == TILE ? wv : wv & 1, kh = M == TILE ? 0 : wv >> 1;
+  const int r0 = j.r0 + rg * 32, rows = j.nq * a.G;
   Rows<D, BIAS> x;
   x.load(a, j, r0 + lq, hi);
   const Offsets<D> off(l);
@@ -233,13 +237,31 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
     const int sb = (c - j.c0) & 1;
     const char* kb = lds + sb * 2 * TILE_BYTES;
     const char* vb = kb + TILE_BYTES;
-    // K of the first 32 keys is read before the next chunk's transfers are issued: the first products then find their
+    // K of the wave's first 32 keys is read before the next chunk's transfers are issued: the first products then find their
     // operands ready
     ev8 kf[NKS];
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) kf[ks] = elds16(kb, off.k0 ^ (32 * ks));
+    for (int ks = 0; ks < NKS; ++ks) kf[ks] = elds16(kb + kh * (TILE_BYTES / 2), off.k0 ^ (32 * ks));
     if (c + 1 < j.c1) issue(c + 1, sb ^ 1);
-    if (c * BK < seen_max) {
+    if (M != TILE) {
+      const int key0 = c * BK + 32 * kh;
+      if (key0 < seen_max) {
+        float sc, c0, alpha;
+        ev8 pa, pb;
+        f32x16 s0 = {};
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) s0 = emfma(kf[ks], x.q[ks], s0);
+        __builtin_amdgcn_s_setprio(0);
+        x.raise(x.scores(a, tab, s0, key0, hi, key0 + 32 > seen_min, low, high, sc, c0), alpha);
+        x.exponentials(s0, sc, c0, pa, pb);
+        const char* v = vb + kh * (TILE_BYTES / 2);
+        __builtin_amdgcn_s_setprio(1);
+        x.values(v, off.t0, off.t1, pa);
+        x.values(v + TILE_BYTES / 4, off.t0, off.t1, pb);
+        __builtin_amdgcn_s_setprio(0);
+      }
+    } else if (c * BK < seen_max) {
       // Two 32-key runs, one behind the other, so that one's products run while the other's exponentials are taken: S of the
       // second under the exponentials of the first, O += V^T P^T of the first under those of the second. (The first run's
       // probabilities are held back over the second's test of the maximum, and scaled with O where that one moves. Against
@@ -284,8 +306,29 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
     __syncthreads();
   }
 
-  const float tot = sum_xor32(x.lsum);
-  if (j.part != nullptr) {
+  float tot = sum_xor32(x.lsum);
+  if (M != TILE) {  // the second key half hands its state over: O through the staging buffers, [row group][register][lane]
+    float* xch = reinterpret_cast<float*>(lds) + rg * (NDB * 16 * 64);
+    if (kh == 1) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) xch[(db * 16 + r) * 64 + l] = x.o[db][r];
+      stats[rg * 128 + l] = x.mrun;
+      stats[rg * 128 + 64 + l] = tot;
+    }
+    __syncthreads();
+    if (kh == 1) return;
+    const float m1 = stats[rg * 128 + l], m = fmaxf(x.mrun, m1), msub = m == -INFINITY ? 0.0f : m;
+    const float w0 = exp2f_fast(x.mrun - msub), w1 = exp2f_fast(m1 - msub);
+    tot = w0 * tot + w1 * stats[rg * 128 + 64 + l];
+    x.mrun = m;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x.o[db][r] = w0 * x.o[db][r] + w1 * xch[(db * 16 + r) * 64 + l];
+  }
+  if (M == TILE && j.part != nullptr) {
     const int r = wv * 32 + lq;
     if (r0 >= rows) return;
     float* o = j.part + 2 * j.part_rows;
@@ -318,7 +361,7 @@ __device__ __forceinline__ void narrow_tile(const FwdArgs& a, const Job& j, char
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, RUN = 32 * ROW, NI = D / 16, LPR = D / 8;
   const int tid = threadIdx.x, l = tid & 63, hi = l >> 5, lq = l & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r0 = j.t * TILE, rows = j.nq * a.G;
+  const int r0 = j.r0, rows = j.nq * a.G;
   Rows<D, BIAS> x;
   x.load(a, j, r0 + lq, hi);
   const Offsets<D> off(l);
@@ -418,25 +461,25 @@ __device__ __forceinline__ void narrow_tile(const FwdArgs& a, const Job& j, char
   }
 }
 
-template <int D, bool BIAS>
+template <int D, bool BIAS, int M>
 __device__ __forceinline__ void run_tile(const FwdArgs& a, const Job& j, char* lds, float* stats, float* tab) {
-  if (j.nq * a.G - j.t * TILE <= 32) narrow_tile<D, BIAS>(a, j, lds, stats, tab);
-  else wide_tile<D, BIAS>(a, j, lds, tab);
+  if (j.nq * a.G - j.r0 <= 32) narrow_tile<D, BIAS>(a, j, lds, stats, tab);
+  else wide_tile<D, BIAS, M>(a, j, lds, stats, tab);
 }
 
 // whole tiles: grid tiles * Hk, a tile's heads on neighbouring workgroups (workgroup i runs on XCD i % 8: with eight kv heads
 // each XCD's L2 then holds one head's keys); under a causal mask a sequence's last tiles, which see the most keys, first
-template <int D, bool BIAS>
+template <int D, bool BIAS, int M>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_fwd_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
   __shared__ float stats[4 * 128];
   __shared__ float tab[BIAS ? BIAS_TABLE : 1];
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
-  int b;
+  int b, t;
   Seq s;
   Job j;
-  if (!tile_of<TILE, false>(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, a.G, w, s, b, j.t)) return;
-  j.t = (s.nq * a.G + TILE - 1) / TILE - 1 - j.t;
+  if (!tile_of<M, false>(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, a.G, w, s, b, t)) return;
+  j.r0 = ((s.nq * a.G + M - 1) / M - 1 - t) * M;
   j.k = a.k + ((size_t)s.k0 * a.Hk + hk) * D;
   j.v = a.v + ((size_t)s.k0 * a.Hk + hk) * D;
   j.q0 = s.q0;
@@ -446,8 +489,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_fwd_kernel(FwdArg
   j.causal = a.causal;
   j.part = nullptr;
   j.c0 = 0;
-  j.c1 = tile_chunks(a, j);
-  run_tile<D, BIAS>(a, j, lds, stats, tab);
+  j.c1 = tile_chunks<M>(a, j);
+  run_tile<D, BIAS, M>(a, j, lds, stats, tab);
 }
 
 // ------------------------------------------------------------------------------------------------ key ranges
@@ -597,8 +640,8 @@ struct SharedLists {
 // item w of a list: its job's tile and chunks
 __device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Ranges& r, int w) {
   const int i = w - r.item0, range = i % r.ranges;
-  j.t = i / r.ranges;
-  const int chunks = tile_chunks(a, j);
+  j.r0 = i / r.ranges * TILE;
+  const int chunks = tile_chunks<TILE>(a, j);
   j.c0 = (int)((long long)chunks * range / r.ranges);
   j.c1 = (int)((long long)chunks * (range + 1) / r.ranges);
 }
@@ -635,7 +678,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_ranges_kernel(Fwd
   take_range(a, j, r, w);
   j.part_rows = TILE;
   j.part = r.ranges == 1 ? nullptr : partial<D>(a.part, TILE, a, w, j.hk);
-  run_tile<D, BIAS>(a, j, lds, stats, tab);
+  run_tile<D, BIAS, TILE>(a, j, lds, stats, tab);
 }
 
 // A tile of the prefix's list holds rows of several sequences, so a prefix is read once for 128 rows of the batch and not once a
@@ -670,7 +713,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(Fwd
   take_range(a, j, r, w);
   j.part_rows = r.list == 0 ? TILE : a.part_rows;
   j.part = r.list == 0 ? partial<D>(a.part_prefix, TILE, a, w - r.item0, j.hk) : partial<D>(a.part, a.part_rows, a, w, j.hk);
-  run_tile<D, false>(a, j, lds, stats, nullptr);
+  run_tile<D, false, TILE>(a, j, lds, stats, nullptr);
 }
 
 // O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's partials in order: D / 4 lanes a row, which first take one
@@ -765,16 +808,30 @@ using namespace es;
 static int resident(int D) { return D == 64 ? 768 : 512; }
 // Items a head of a ranged launch: at most one a tile more than the ranges' chunks fill.
 static long long range_items(long long tiles, int Hk, int D) { return tiles + resident(D) / Hk + 1; }
-// Key ranges are worth a second launch where the tiles do not fill the GPU and a tile may have many chunks: from 1024 keys on
-// for single tokens and the like (up to 32 rows a sequence on average, whose partials are small), from 1792 where the tiles
-// take a quarter of the GPU's places or fewer, otherwise from 4096. (us whole and in ranges: 200 tokens of 32 heads over 8
-// against 2000 keys 44 and 29, 2000 causal tokens of 8 heads over one 45 and 39; 1500 of 10 over 2 26 and 26, 3000 of 8 over
-// one 68 and 74, 1024 of 8 over 8 25 and 28.)
+// Key ranges are worth a second launch where the tiles do not fill the GPU and a tile may have many chunks.
+// Single tokens and the like (up to 32 rows a sequence on average, whose partials are small): from 1024 keys on.
+// One sequence, or no more keys than rows (then the longest sequence has the most tiles): a launch of whole tiles takes about
+// 0.77 us a chunk of the longest one, ranges 0.0024 us a chunk and item and 15 us more for their plan, partials and merge. (us in
+// ranges and whole, D = 128, causal: 200 tokens of 32 heads over 8 against 1000 keys 24 and 19, 2000 keys 26 and 31, 4000 keys
+// 34 and 54; 2000 tokens of 2 heads over one 24 and 29, of 8 heads 36 and 31; 3000 of 8 58 and 45; 5000 of 4 heads 61 and 67,
+// of 8 heads over 8 117 and 77; 1500 of 10 over 2 35 and 25.)
+// Otherwise some sequences may have most of the keys and few of the tiles: from 4096 keys, from 1792 where the tiles take a
+// quarter of the GPU's places or fewer.
 static bool ranged(long long tiles, int B, int Tq, int Tk, int H, int Hk, int D) {
-  const long long items = tiles * Hk;
+  const long long items = tiles * Hk, chunks = Tk / BK;
   if (items >= 2 * resident(D)) return false;
-  const int chunks = (long long)Tq * (H / Hk) <= 32LL * B ? 16 : 4 * items <= resident(D) ? 28 : 64;
-  return Tk >= chunks * BK;
+  if ((long long)Tq * (H / Hk) <= 32LL * B) return chunks >= 16;
+  if (B == 1 || Tk <= Tq) return items < 246 && chunks * (246 - items) >= 4800;
+  return chunks >= (4 * items <= resident(D) ? 28 : 64);
+}
+
+// Tiles of 64 rows instead of 128, which take about two thirds of the time each and are twice as many, as long as the GPU holds
+// them all at once (512 at D = 128, 1024 at D = 64), under a causal mask half again as many. (us with 128 and 64 rows, D = 128:
+// 1462 causal tokens of 4 heads over one 32 and 23, 1700 of 16 heads 38 and 29, of 36 45 and 45, of 48 50 and 58; 1024 tokens
+// without a mask of 16 heads 25 and 19, of 32 27 and 26, of 36 37 and 40. D = 64: causal, 16 heads 28 and 21, 48 heads 35 and
+// 32, 60 heads 38 and 37; without a mask, 44 heads 25 and 22, 64 heads 27 and 28.)
+static bool small_tiles(long long tiles, int Hk, int D, bool causal) {
+  return tiles * Hk * (causal ? 2 : 3) <= (D == 64 ? 1536 : 768);
 }
 
 // Workgroups a tile of the merge: a row each thread group, as far as a sequence can have rows.
@@ -864,13 +921,22 @@ extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const voi
     }
     return check_launch("es_packed_fwd");
   }
+  const bool small = small_tiles(a.tiles, Hk, D, causal != 0);
+  if (small) a.tiles = (int)tile_numbers<TILE / 2>(B, Tq, a.G);
   const dim3 grid((unsigned)(a.tiles * Hk));
+  auto launch = [&](auto dim, auto with_bias) {
+    constexpr int d = decltype(dim)::value;
+    constexpr bool b = decltype(with_bias)::value;
+    if (small) hipLaunchKernelGGL((packed_fwd_kernel<d, b, TILE / 2>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((packed_fwd_kernel<d, b, TILE>), grid, dim3(256), 0, stream, a);
+  };
+  using std::integral_constant;
   if (D == 64) {
-    if (bias) hipLaunchKernelGGL((packed_fwd_kernel<64, true>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((packed_fwd_kernel<64, false>), grid, dim3(256), 0, stream, a);
+    if (bias) launch(integral_constant<int, 64>{}, std::true_type{});
+    else launch(integral_constant<int, 64>{}, std::false_type{});
   } else {
-    if (bias) hipLaunchKernelGGL((packed_fwd_kernel<128, true>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((packed_fwd_kernel<128, false>), grid, dim3(256), 0, stream, a);
+    if (bias) launch(integral_constant<int, 128>{}, std::true_type{});
+    else launch(integral_constant<int, 128>{}, std::false_type{});
   }
   return check_launch("es_packed_fwd");
 }

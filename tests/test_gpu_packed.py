@@ -102,6 +102,15 @@ def test_whole_tiles(dev, D, dtype, T, H, Hk):
     _case([T - 130, 130], [T - 130, 130], H, Hk, D, dtype, True, dev, seed=3)
 
 
+@pytest.mark.parametrize("D, dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("bias", [False, True])
+def test_many_heads(dev, D, dtype, causal, bias):
+    """Grids that fill the GPU take tiles of 128 rows, smaller ones (the other tests) of 64."""
+    table = _api().relative_buckets(16, 60, device=dev) if bias else None
+    _case([300, 1, 70, 0, 129], [300, 1, 200, 5, 129], 128, 128, D, dtype, causal, dev, table=table, pad=2, seed=48)
+
+
 @pytest.mark.parametrize("pad", [0, 3])
 @pytest.mark.parametrize("B", [63, 64, 65, 200])
 def test_many_sequences(dev, B, pad):
