@@ -9,7 +9,7 @@
 //     end. The next K run is requested when this one's products have read it, the next V run likewise, so one of them is
 //     always in flight.
 // What bounds them: wide tiles the matrix units and what runs beside them on long sequences (32760 causal tokens of 24 heads over
-// 8, D = 128: 5.94 ms, 1110 TFLOP/s; 53 % of the cycles issue a matrix instruction, 51 % vector work, LDS 27 %, no bank
+// 8, D = 128: 5.94 ms, 1110 TFLOP/s; 57 % of the cycles issue a matrix instruction, 55 % vector work, LDS 29 %, no bank
 // conflicts), the transfers where many tiles stream different keys from HBM, and on sequences of a few hundred rows the chain
 // of a tile's few chunks. Narrow tiles: HBM (8 tokens, 40 heads over 8, caches of 513 to 75600 keys: 654 MB in 137 us, 4.8
 // TB/s, what a large copy reaches).
