@@ -72,7 +72,8 @@ __device__ __forceinline__ void lds_add(float* p, float x) {
 // (dP's products under the exponentials, as bwd_q has them, spill: 4428 -> 4500 us at 13770 tokens, 12 heads. Staging dO later
 // than Q computes the row addresses twice: whole backward 4.31 -> 4.43 ms.) With the products of both kernels at a raised
 // priority (packed.h) the whole backward of 13770 tokens of 12 heads takes 4.26 ms, not 4.40, of 8192 causal tokens of 24 heads
-// over 8 1611 us, not 1661, at D = 64 1063, not 1076.
+// over 8 1611 us, not 1661, at D = 64 1063, not 1076. Not in bwd_q with a bias, whose vector work is the longer part (2303 tokens
+// of 24 heads, D = 64, whole backward 82.5 us without, 85.5 with).
 template <int D, bool BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(BwdArgs a) {
   constexpr int NKS = D / 16, NDB = D / 32, ROW = D * 2, TILE_BYTES = BK * ROW, NI = D / 32, LPR = D / 8;
@@ -401,12 +402,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
         if (8 * (r / 4) + r % 4 >= left) x[r] = -INFINITY;
     }
     // (dP's products run under the exponentials)
-    __builtin_amdgcn_s_setprio(1);
+    if (!BIAS) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) dp = emfma(elds16(vt, koff ^ (32 * ks)), dreg[ks], dp);
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = exp2f_fast(fmaf(x[r], sc, cb - ls));
-    __builtin_amdgcn_s_setprio(0);
+    if (!BIAS) __builtin_amdgcn_s_setprio(0);
   };
   // the chunk's rows of K, read before the next chunk's transfers are issued: S then finds its operands ready
   auto read_k = [&](const char* kt, ev8 (&kf)[NKS]) {
@@ -519,14 +520,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
         }
       }
       const ev8 sa = epack8(&ds[0]), sb8 = epack8(&ds[8]);
-      __builtin_amdgcn_s_setprio(1);
+      if (!BIAS) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
         const int t0 = toff0 ^ (64 * db), t1 = toff1 ^ (64 * db);
         dq[db] = emfma(ecat_tr(lds_read_tr(kt, t0), lds_read_tr(kt, t1)), sa, dq[db]);
         dq[db] = emfma(ecat_tr(lds_read_tr(kt + TILE_BYTES / 4, t0), lds_read_tr(kt + TILE_BYTES / 4, t1)), sb8, dq[db]);
       }
-      __builtin_amdgcn_s_setprio(0);
+      if (!BIAS) __builtin_amdgcn_s_setprio(0);
     }
     sb ^= 1;
     dma_wait();
