@@ -14,6 +14,7 @@
 #include <torch/library.h>
 
 #include <tuple>
+#include <utility>
 
 namespace {
 
@@ -182,6 +183,8 @@ using BackwardSignature = std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tenso
 using ForwardSignature = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
                                                     const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool,
                                                     double);
+using SharedSignature = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                   const Tensor&, double);
 
 OptTensor maybe(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
@@ -256,6 +259,24 @@ std::tuple<Tensor, Tensor> packed_forward_autograd(const Tensor& q, const Tensor
   return {r[0], r[1]};
 }
 
+// no derivative of either mode: refused rather than left out (packed.py refuses requires_grad by itself, but a tangent is seen
+// here only)
+std::tuple<Tensor, Tensor> shared_forward_autograd(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& k,
+                                                   const Tensor& v, const Tensor& lens, double scale) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("echosparse_gfx950::shared_prefix_attention", "")
+                             .typed<SharedSignature>();
+  const bool grad = at::GradMode::is_enabled();
+  for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"q", q}, {"k_prefix", kp}, {"v_prefix", vp}, {"k", k},
+                                {"v", v}}) {
+    TORCH_CHECK(!t._fw_grad(0).defined(), "shared_prefix_attention has no forward-mode derivative, and ", name,
+                " has a tangent");
+    TORCH_CHECK(!grad || !t.requires_grad(), "shared_prefix_attention has no backward, and ", name, " requires a gradient");
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, kp, vp, k, v, lens, scale);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(echosparse_gfx950, m) {
@@ -279,4 +300,5 @@ TORCH_LIBRARY_IMPL(echosparse_gfx950, Meta, m) {
 TORCH_LIBRARY_IMPL(echosparse_gfx950, Autograd, m) {
   m.impl("packed_attention", TORCH_FN(packed_forward_autograd));
   m.impl("packed_attention_backward", TORCH_FN(packed_backward_autograd));
+  m.impl("shared_prefix_attention", TORCH_FN(shared_forward_autograd));
 }

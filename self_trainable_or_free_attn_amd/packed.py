@@ -214,7 +214,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     aligned to 16 bytes. scale: 1 / sqrt(D) if None.
 
     Returns out like q, with return_lse also the natural-log LSE [B, n, H] in float32; a token without keys gives zeros and
-    -inf. There is no backward: tensors that require a gradient are refused unless gradients are off."""
+    -inf. There is no derivative: tensors that require a gradient are refused unless gradients are off, tensors that
+    carry a forward-mode tangent always."""
     if q.dim() != 4 or k.dim() != 4 or k_prefix.dim() != 3:
         raise ValueError("q must be [B, n, H, D], k and v [B, S, Hk, D], k_prefix and v_prefix [P, Hk, D]")
     named = (("k_prefix", k_prefix), ("v_prefix", v_prefix), ("k", k), ("v", v))
