@@ -25,8 +25,8 @@
 // TFLOP/s of its four (51 %; it waits the most, for its transfers and at the tile's barrier, with two workgroups a CU at 255
 // registers); causal prompts of 1 to 6553 tokens, 24 heads over 8: 0.65 and 0.90 ms. What bounds short ones is the chain of a tile's few chunks:
 // transfers, two products, exponentials, two products.
-// dS is rounded to the token type without the softmax scale (applied to the finished sums), which keeps it about ten times
-// further from the subnormal range of fp16.
+// dS is rounded to the token type without the softmax scale (applied to the finished sums). In fp16 it is rounded times a power
+// of two of its row (dQ) or key (dK), see fit.
 #include "packed.h"
 
 #include <algorithm>
@@ -37,13 +37,43 @@ namespace es {
 namespace {
 
 // fp16: the probabilities of dV = P^T dO are taken 2^14 higher, out of the type's subnormal range for all down to 2^-28; dS
-// and the finished sum take the factor back exactly
+// and the finished sum take the factor back exactly. dS follows dO and V, which may be of any size (scaled losses), so it is
+// taken times 2^DS_LOG2 at first and `fit` keeps it in range.
 #ifdef ES_ELEM_F16
+constexpr bool DS_SCALED = true;
 constexpr float P_SHIFT = 14.0f, P_BACK = 1.0f / 16384.0f;
+constexpr int DS_LOG2 = 40;
 #else
+constexpr bool DS_SCALED = false;
 constexpr float P_SHIFT = 0.0f, P_BACK = 1.0f;
+constexpr int DS_LOG2 = 0;
 #endif
 constexpr int EXACT_CHUNKS = 8;
+
+// A lane's dS as fp16 operands: values times 2^e, e of its row or key and the same in both half waves. Where one passes 2^15, e
+// falls so that the largest comes to 2^7 .. 2^8, and the sums so far fall with it (exact in float32). So no operand overflows
+// whose sum float32 holds, and the type's subnormal steps (2^-24, half of one a rounding) put a dS off by no more than 2^-32 of
+// the lane's largest, or, where e is still 40, by 2^-65. The 2^7 between the two borders make a change rare: in the first tile,
+// then only for values 128 times as large. P 2^40 |dP - delta| stays below 2^80. An infinite dS (from an infinite dO) stays one.
+// (Whole backward in fp16 without and with it, us: 13770 tokens of 12 heads 4320 and 4610, 8192 causal of 24 over 8 1490 and
+// 1560, of 16 heads at D = 64 1019 and 1089, 500 of 24 heads with a bias at D = 64 41.8 and 43.1.)
+template <int N>
+__device__ __forceinline__ bool fit(float (&ds)[16], f32x16 (&acc)[N], int& change) {
+  float mx = fabsf(ds[0]);
+#pragma unroll
+  for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fabsf(ds[r]));
+  mx = max_xor32(mx);
+  if (!(mx > 32768.0f)) return false;
+  change = 8 - __builtin_amdgcn_frexp_expf(mx);
+  const float f = __builtin_ldexpf(1.0f, change);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) ds[r] *= f;
+#pragma unroll
+  for (int db = 0; db < N; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[db][r] *= f;
+  return true;
+}
 
 struct BwdArgs {
   const e16_t *q, *k, *v, *dout, *out;
@@ -159,8 +189,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
   if (BIAS) fill_bias(tab, a.bias, a.buckets, a.num_buckets, a.R, a.G, a.H, hk);
   dma_wait();
   __syncthreads();
-  // masked key columns: every row's lse2 becomes +inf for this lane, so P = 2^(s - inf) = 0 without a branch
-  const float kmask = kvalid ? 0.0f : INFINITY;
+  float ds_mul = ldexpf(P_BACK, DS_LOG2);  // acc_k sums dS Q times ds_mul / P_BACK
+  // (lanes past the last key: whatever they sum up belongs to their own column and is not stored)
   for (int i = beg; i < end; ++i) {
     const int sb = (i - beg) & 1;
     // the rows of Q are read before the next tile's transfers are issued: S then finds its operands ready
@@ -223,7 +253,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
         }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[4 * g + e] = exp2f_fast(fmaf(p[4 * g + e], a.scale_log2, -(l4[e] + kmask)));
+      for (int e = 0; e < 4; ++e) p[4 * g + e] = exp2f_fast(fmaf(p[4 * g + e], a.scale_log2, -l4[e]));
     }
     {
       float x[16];
@@ -240,12 +270,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
     for (int g = 0; g < 4; ++g) {
       const f32x4 d4 = *reinterpret_cast<const f32x4*>(&st_s[sb][1][32 * qh + 8 * g + 4 * hi]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[4 * g + e] = p[4 * g + e] * fmaf(dp[4 * g + e], P_BACK, -d4[e]);
+      for (int e = 0; e < 4; ++e) p[4 * g + e] = (DS_SCALED ? p[4 * g + e] * ds_mul : p[4 * g + e]) * (dp[4 * g + e] - d4[e]);
     }
     {
       float x[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = p[r];
+      int change;
+      if (DS_SCALED && fit(x, acc_k, change)) ds_mul = ldexpf(ds_mul, change);
       __builtin_amdgcn_s_setprio(1);
       product(qt, epack8(&x[0]), epack8(&x[8]), acc_k);
       __builtin_amdgcn_s_setprio(0);
@@ -256,6 +288,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
 
   // the second row half hands its sums over through the staging buffers: [key half][dV | dK][register][lane]
   float* xch = reinterpret_cast<float*>(&qd_s[0][0][0]) + kh * (2 * NDB * 16 * 64);
+  if (DS_SCALED) {
+    const float back = P_BACK / ds_mul;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc_k[db][r] *= back;
+  }
   if (qh == 1) {
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
@@ -377,8 +416,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
   for (int db = 0; db < NDB; ++db) dq[db] = f32x16{};
   float far_lo = 0.0f, far_hi = 0.0f;  // dS at distances of -R and below, of R and beyond
 
-  // P and dP of keys key0 .. key0 + 31 (near: by distance, neither all at -R and below nor all at R and beyond)
-  auto scores = [&](const ev8 (&kf)[NKS], const char* vt, int key0, f32x16& x, f32x16& dp, bool& near) {
+  // P (against the statistic ls) and dP of keys key0 .. key0 + 31 (near: by distance, neither all at -R and below nor all at R
+  // and beyond)
+  auto scores = [&](const ev8 (&kf)[NKS], const char* vt, int key0, float ls, f32x16& x, f32x16& dp, bool& near) {
     x = f32x16{};
     dp = f32x16{};
 #pragma unroll
@@ -428,7 +468,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
       if (c * BK + 32 * kh < seen_max) {
         f32x16 p, dp;
         bool near;
-        scores(kf, kv_s[sb][1], c * BK + 32 * kh, p, dp, near);
+        scores(kf, kv_s[sb][1], c * BK + 32 * kh, ls, p, dp, near);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           num = fmaf(p[r], dp[r], num);
@@ -446,13 +486,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
   }
   if (valid && kh == 0 && hi == 0) {
     a.lse2[list] = ls - P_SHIFT;
-    a.delta[list] = dl * P_BACK;
+    a.delta[list] = dl;
   }
   if (BIAS) {
     __syncthreads();
     for (int i = tid; i < 4 * BIAS_ROWS; i += 256) (&hist[0][0])[i] = 0.0f;
     __syncthreads();
   }
+  int ds_log2 = DS_LOG2;  // dS and dq are taken times 2^ds_log2
+  float ds_ls = ls - (float)DS_LOG2;
   for (int c = 0; c < end; ++c) {
     ev8 kf[NKS];
     read_k(kv_s[sb][0], kf);
@@ -463,7 +505,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
     if (key0 < seen_max) {
       f32x16 x, dp;
       bool near;
-      scores(kf, vt, key0, x, dp, near);
+      scores(kf, vt, key0, ds_ls, x, dp, near);
       const int d0 = key0 + 4 * hi - pos;
       float ds[16];
 #pragma unroll
@@ -473,10 +515,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
           float sum = 0.0f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) sum += ds[r];
+          if (DS_SCALED) sum = ldexpf(sum, -ds_log2);
           if (key0 - high >= a.R) far_hi += sum;
           else far_lo += sum;
         } else {
           float* h = hist[wv] + g * width + a.R;
+          float one[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) one[r] = DS_SCALED ? ldexpf(ds[r], -ds_log2) : ds[r];
           if (a.G == 1) {
             // The run's diagonals, in a 64-lane shift register: row q's dS for key e enters at lane q and moves up a lane
             // a key, so that all of one distance meet; after key 31 lane i holds distance key0 + 31 - (first row) - i. Keys
@@ -489,7 +535,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
               unsigned up[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(ds[4 * n + e]), 0u, false, false);
+                const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(one[4 * n + e]), 0u, false, false);
                 v = dpp_f<0x138>(v) + __uint_as_float(two[0]);
                 up[e] = two[1];
               }
@@ -508,16 +554,21 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int e = 8 * (r / 4) + r % 4, d = d0 + e;
-              far_lo += d <= -a.R ? ds[r] : 0.0f;
-              far_hi += d >= a.R && d > -a.R ? ds[r] : 0.0f;
+              far_lo += d <= -a.R ? one[r] : 0.0f;
+              far_hi += d >= a.R && d > -a.R ? one[r] : 0.0f;
               const bool in = valid && d > -a.R && d < a.R;
-              if (in && hi == 0) lds_add(h + e, ds[r]);
+              if (in && hi == 0) lds_add(h + e, one[r]);
               __builtin_amdgcn_wave_barrier();  // (keeps the compiler from making one instruction of the two)
-              if (in && hi == 1) lds_add(h + e, ds[r]);
+              if (in && hi == 1) lds_add(h + e, one[r]);
               __builtin_amdgcn_wave_barrier();
             }
           }
         }
+      }
+      int change;
+      if (DS_SCALED && fit(ds, dq, change)) {
+        ds_log2 += change;
+        ds_ls -= (float)change;
       }
       const ev8 sa = epack8(&ds[0]), sb8 = epack8(&ds[8]);
       if (!BIAS) __builtin_amdgcn_s_setprio(1);
@@ -543,6 +594,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_q_kernel(BwdA
         hist[wv][i * width + 2 * a.R] += up;
       }
     }
+  }
+  if (DS_SCALED) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[db][r] = ldexpf(dq[db][r], -ds_log2);
   }
   // the second key half hands its sums over through the staging buffers
   float* xq = reinterpret_cast<float*>(&kv_s[0][0][0]) + rg * (NDB * 16 * 64);

@@ -139,7 +139,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: Op
     or -inf, which masks; finite ones are held to +-131072.
 
     Returns out like q, with return_lse also the natural-log LSE [Tq, H] ([B, Lq, H]) in float32 (no gradient). Gradients
-    are deterministic, and those of a bias are summed in float32; the backward itself is not differentiable."""
+    are deterministic, and those of a bias are summed in float32; the backward itself is not differentiable. With fp16 tensors
+    the output's gradient may be of any size (a scaled loss): a gradient overflows or vanishes only where fp16 cannot hold it."""
     dims = q.dim()
     if dims not in (3, 4) or k.dim() != dims or v.dim() != dims:
         raise ValueError("q, k and v must be [T, H, D], or all [B, L, H, D]")
