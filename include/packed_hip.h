@@ -16,8 +16,9 @@
  * to its position; its score against key j is scale * q.k + bias[buckets[clamp(j - position, -R, R) + R]][h].
  * Rows that see no key get out = 0 and lse = -inf and give no gradient. Rows behind the last sequence are such rows;
  * key rows behind it get zero gradients, and their values are never used.
- * Scores are float32 and must stay below 2^22 in magnitude. (H / Hk) * (2 * R + 1) is at most ES_PACKED_BIAS_ROWS. Bias values are finite or -inf (which masks); finite ones beyond
- * +-ES_PACKED_BIAS_MAX count as that. Calls of about 2^24 / Hk sequences and more are refused.
+ * Scores are float32 and must stay below 2^22 in magnitude. (H / Hk) * (2 * R + 1) is at most ES_PACKED_BIAS_ROWS. Bias
+ * values are finite or -inf (which masks); finite ones beyond +-ES_PACKED_BIAS_MAX count as that, and their dbias is 0. Calls
+ * of about 2^24 / Hk sequences and more are refused.
  */
 #pragma once
 #include "echosparse_hip.h"

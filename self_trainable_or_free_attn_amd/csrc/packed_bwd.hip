@@ -664,7 +664,9 @@ __global__ __launch_bounds__(1024) void bias_sums_kernel(BwdArgs a) {
     for (int d = threadIdx.x & 63; d < width; d += 64)
       if (which[d] == n) sum += (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
     sum = wave_sum_dpp(sum);
-    if ((threadIdx.x & 63) == 0) a.dbias[(size_t)n * a.H + h] = sum;
+    // (a value that fill_bias holds to its limit does not move the scores)
+    const size_t at = (size_t)n * a.H + h;
+    if ((threadIdx.x & 63) == 0) a.dbias[at] = fabsf(a.bias[at]) > BIAS_MAX ? 0.0f : sum;
   }
 }
 

@@ -136,7 +136,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: Op
     the keys up to that position. A row that sees no key gives zeros and an LSE of -inf, and no gradient. scale: 1 / sqrt(D)
     if None. bias [num_buckets, H] with buckets (`relative_buckets`, int32 [2 R + 1]) adds bias[buckets[d + R], h] to the
     score of a key at distance d from the query, d clamped to -R .. R; (H // Hk) * (2 R + 1) is at most 784. Its values are finite
-    or -inf, which masks; finite ones are held to +-131072.
+    or -inf, which masks; finite ones are held to +-131072 (and get no gradient beyond that).
 
     Returns out like q, with return_lse also the natural-log LSE [Tq, H] ([B, Lq, H]) in float32 (no gradient). Gradients
     are deterministic, and those of a bias are summed in float32; the backward itself is not differentiable. With fp16 tensors
