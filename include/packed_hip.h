@@ -31,7 +31,8 @@ extern "C" {
 #define ES_PACKED_BIAS_MAX 131072.0f
 
 /* Forward. workspace: es_packed_fwd_workspace bytes (0: none needed; NULL / 0 is then accepted), for batches of few query
- * rows against many keys, whose keys are cut into ranges that run side by side and are merged in a fixed order. */
+ * rows against many keys, whose keys are cut into ranges that run side by side and are merged in a fixed order. (Without cu_k
+ * the lengths are known, and a call that cuts nothing takes NULL / 0 where one of the same sizes with cu_k does not.) */
 size_t es_packed_fwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D);
 int es_packed_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, const float* bias,
                   const int* buckets, int num_buckets, int R, void* out, float* lse, void* workspace,

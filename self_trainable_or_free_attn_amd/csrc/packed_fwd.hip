@@ -20,6 +20,7 @@
 #include "packed.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace es {
@@ -804,21 +805,32 @@ using namespace es;
 static int resident(int D) { return D == 64 ? 768 : 512; }
 // Items a head of a ranged launch: at most one a tile more than the ranges' chunks fill.
 static long long range_items(long long tiles, int Hk, int D) { return tiles + resident(D) / Hk + 1; }
-// Key ranges are worth a second launch where the tiles do not fill the GPU and a tile may have many chunks.
-// Single tokens and the like (up to 32 rows a sequence on average, whose partials are small): from 1024 keys on.
-// One sequence, or no more keys than rows (then the longest sequence has the most tiles): a launch of whole tiles takes about
-// 0.77 us a chunk of the longest one, ranges 0.0024 us a chunk and item and 15 us more for their plan, partials and merge. (us in
-// ranges and whole, D = 128, causal: 200 tokens of 32 heads over 8 against 1000 keys 24 and 19, 2000 keys 26 and 31, 4000 keys
-// 34 and 54; 2000 tokens of 2 heads over one 24 and 29, of 8 heads 36 and 31; 3000 of 8 58 and 45; 5000 of 4 heads 61 and 67,
-// of 8 heads over 8 117 and 77; 1500 of 10 over 2 35 and 25.)
-// Otherwise some sequences may have most of the keys and few of the tiles: from 4096 keys, from 1792 where the tiles take a
-// quarter of the GPU's places or fewer.
-static bool ranged(long long tiles, int B, int Tq, int Tk, int H, int Hk, int D) {
-  const long long items = tiles * Hk, chunks = Tk / BK;
+// Key ranges are worth a second launch where the tiles do not fill the GPU and a tile may have many chunks. `equal`: the keys
+// divide into B equal sequences; otherwise the host knows their sum alone, and the longest may have anything from Tk / B of them
+// to all. It is taken to have Tk / sqrt(B) then, halfway in the logarithm: with all of them batches of short sequences
+// went to ranges that cut nothing (us whole and in ranges, D = 128, causal: 8 x 512 tokens of 4 heads 13 and 23, 100 x 64 of one
+// head 7.5 and 16, 4 x 1024 of 4 heads 18 and 31; 32 tokens against 40 keys each 8 and 10-12), with Tk / B a long
+// sequence among short ones is not cut (8000 + 7 x 64 tokens of one head 91 and 46; tokens against 8000 + 31 x 40 keys 69 and 14).
+// Single tokens and the like (up to 32 rows a sequence on average, whose partials are small): from 1024 keys on. (8 tokens, 8 heads
+// over 2, against 300 keys each 8 and 12, 1000 12.4 and 12.9; 2000 + 31 x 40 20 and 12.) From 64 sequences on the plan is read
+// once a pass, so the longest one has to be longer (64 tokens against 256 keys 7 and 17, 128 against 2000 + 127 x 20 19 and 31).
+// One sequence, or no more keys than rows (then the longest sequence has the most tiles): a launch of whole tiles takes
+// WHOLE_CHUNK_US a chunk of the longest one, ranges RANGE_CHUNK_US a chunk and item and RANGE_US more for their plan, partials and
+// merge. (us in ranges and whole, D = 128, causal: 200 tokens of 32 heads over 8 against 1000 keys 24 and 19, 2000 keys 26 and 31,
+// 4000 keys 34 and 54; 2000 tokens of 2 heads over one 24 and 29, of 8 heads 36 and 31; 3000 of 8 58 and 45; 5000 of 4 heads 61 and
+// 67, of 8 heads over 8 117 and 77; 1500 of 10 over 2 35 and 25. At D = 64 all three are about 3 / 4 of that.)
+// Otherwise some sequences may have most of the keys and few of the tiles: from 4096 keys in all (equal sequences: each), or
+// where the tiles take a quarter of the GPU's places or fewer from 1280 of the longest. (us whole and in ranges, 64 tokens each of
+// 8 heads: against 4000 + 3 x 100 keys 49 and 20, 2500 + 2 x 80 34 and 23, 4 x 2000 29 and 22, 4 x 1000 17 and 21, 4 x 500 12 and 19,
+// 16 x 300 11 and 17, 4000 + 15 x 100 51 and 21.)
+constexpr double WHOLE_CHUNK_US = 0.77, RANGE_CHUNK_US = 0.003125, RANGE_US = 15.0;
+static bool ranged(long long tiles, int B, int Tq, int Tk, int H, int Hk, int D, bool equal) {
+  const long long items = tiles * Hk;
+  const double chunks = (double)(Tk / BK), longest = equal ? chunks / B : chunks / std::sqrt((double)B);
   if (items >= 2 * resident(D)) return false;
-  if ((long long)Tq * (H / Hk) <= 32LL * B) return chunks >= 16;
-  if (B == 1 || Tk <= Tq) return items < 246 && chunks * (246 - items) >= 4800;
-  return chunks >= (4 * items <= resident(D) ? 28 : 64);
+  if ((long long)Tq * (H / Hk) <= 32LL * B) return longest >= (B < 64 ? 16.0 : 0.625 * B);
+  if (B == 1 || Tk <= Tq) return longest * WHOLE_CHUNK_US >= RANGE_US + longest * RANGE_CHUNK_US * (double)items;
+  return 4 * items <= resident(D) ? longest >= 20.0 : (equal ? longest : chunks) >= 64.0;
 }
 
 // Tiles of 64 rows instead of 128, which take about two thirds of the time each and are twice as many, as long as the GPU holds
@@ -858,7 +870,9 @@ static Layout shared_layout(int B, int n, int H, int Hk, int D) {
 extern "C" size_t es_packed_fwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D) {
   if (B <= 0 || Tq <= 0 || Tk < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
   const long long tiles = tile_numbers<TILE>(B, Tq, H / Hk);
-  return ranged(tiles, B, Tq, Tk, H, Hk, D) ? packed_layout(tiles, B, Hk, D).bytes : 0;
+  // (for either kind of running lengths: NULL or given)
+  return ranged(tiles, B, Tq, Tk, H, Hk, D, false) || ranged(tiles, B, Tq, Tk, H, Hk, D, true)
+             ? packed_layout(tiles, B, Hk, D).bytes : 0;
 }
 extern "C" size_t es_shared_prefix_workspace(int B, int n, int P, int S, int H, int Hk, int D) {
   if (B <= 0 || n <= 0 || P < 0 || S < 0 || H <= 0 || Hk <= 0 || H % Hk) return 0;
@@ -897,7 +911,7 @@ extern "C" int ES_VSA_API(es_packed_fwd)(const void* q, const void* k, const voi
   a.scale = scale * LOG2E;
   a.tiles = (int)tile_numbers<TILE>(B, Tq, a.G);
   ES_REQUIRE((long long)a.tiles * Hk < MAX_GRID, ES_ERR_UNSUPPORTED, "packed: too many sequences");
-  if (ranged(a.tiles, B, Tq, Tk, H, Hk, D)) {
+  if (ranged(a.tiles, B, Tq, Tk, H, Hk, D, cu_k == nullptr)) {
     ES_REQUIRE(workspace && workspace_bytes >= es_packed_fwd_workspace(B, Tq, Tk, H, Hk, D), ES_ERR_INVALID,
                "packed: workspace too small");
     a.part = (float*)workspace;
