@@ -12,6 +12,7 @@
 #pragma once
 #include "../../include/packed_hip.h"
 #include "elem.h"
+#include "packed_rules.h"
 
 #include <initializer_list>
 
@@ -29,27 +30,13 @@ constexpr int BIAS_PAD = 64, BIAS_TABLE = BIAS_ROWS + 2 * BIAS_PAD;
 constexpr float BIAS_MAX = ES_PACKED_BIAS_MAX;
 constexpr long long MAX_GRID = 1LL << 24;  // workgroups of a launch: its threads are counted in 32 bits
 
-// x / d for 0 <= x < 2^31 by one multiplication: mul = ceil(2^(32 + sh) / d) with 2^sh < d <= 2^(sh + 1), whose error
-// mul * d - 2^(32 + sh) < d <= 2^(sh + 1) keeps x * error under 2^(32 + sh). d = 1: mul = 0.
-struct FastDiv {
-  unsigned mul;
-  int sh;
-};
-static inline FastDiv fast_div(int d) {
-  if (d <= 1) return FastDiv{0u, 0};
-  int sh = 0;
-  while ((2 << sh) < d) ++sh;
-  return FastDiv{(unsigned)(((1ull << (32 + sh)) + d - 1) / d), sh};
-}
-__device__ __forceinline__ int divide(FastDiv f, int x) { return f.mul == 0 ? x : (int)(__umulhi((unsigned)x, f.mul) >> f.sh); }
-
 // rows of sequence b in one of the token tensors
 __device__ __forceinline__ int seq_start(const int* cu, int b, int B, int T) {
   if (cu == nullptr) return b >= B ? T : b * (T / B);
   return b <= 0 ? 0 : min(max(cu[b], 0), T);
 }
 
-// The sequence of tile number w where sequence b's numbers start at floor(start_b * G / M) + b; every lane of the wave
+// The sequence of tile number w (numbers by first_tile); every lane of the wave
 // calls it, one load a lane for 64 sequences.
 template <int M>
 __device__ __forceinline__ int seq_of_tile(const int* cu, int B, int T, int G, int w) {
@@ -57,16 +44,12 @@ __device__ __forceinline__ int seq_of_tile(const int* cu, int B, int T, int G, i
   int count = 0;
   for (int b0 = 0; b0 <= B; b0 += 64) {
     const int b = b0 + l;
-    const bool in = b <= B && seq_start(cu, min(b, B), B, T) * G / M + b <= w;
+    const bool in = b <= B && first_tile<M>(seq_start(cu, min(b, B), B, T), G, b) <= w;
     const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
     count += __builtin_popcountll(m);
     if (m != ~0ull) break;
   }
   return __builtin_amdgcn_readfirstlane(max(count - 1, 0));
-}
-template <int M>
-__host__ __device__ __forceinline__ long long tile_numbers(int B, int T, int G) {
-  return (long long)T * G / M + B + 1;
 }
 
 struct Seq {
@@ -123,7 +106,7 @@ __device__ __forceinline__ bool tile_of(const int* cu_q, const int* cu_k, int B,
     s.nk = Tk - s.k0;
     s.nq = 0;
   }
-  t = w - ((KEYS ? s.k0 : s.q0 * G) / M + b);
+  t = w - (KEYS ? first_tile<M>(s.k0, 1, b) : first_tile<M>(s.q0, G, b));
   return t >= 0 && t * M < (KEYS ? s.nk : s.nq * G);
 }
 

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
   // up to G + 63, G up to 4096, the nearest border 1 / (2 G) away). Few registers matter here: with more the compiler spills
   // some, and a reload in this loop waits for every transfer before it (a tile's transfers took 2970 cycles instead of 920).
   constexpr int RPT = 64 / LPR, XOR = D == 128 ? 16 : 32;
-  auto token_in_tile = [&](int row) { return (int)(((float)row + 0.5f) * a.inv_g); };  // of rows since the first token's
+  auto token_in_tile = [&](int row) { return token_of((float)row + 0.5f, a.inv_g); };  // of rows since the first token's
   int lane_at = (wv * 16 + l / LPR) * ROW + (((l % LPR) ^ swizzle<D>(l / LPR)) << 4);
   auto issue = [&](int i, int sb) {
     const int t0 = divide(a.div_g, i * BK), toks = min(s.nq - t0, BK + 1), rel = i * BK - t0 * a.G;
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_kv_kernel(Bwd
     const unsigned qd = lds_q + (unsigned)sb * (2u * TILE_BYTES);
 #pragma unroll
     for (int r = 0; r < NI; ++r) {
-      const unsigned tok = (unsigned)(((float)(lane_at / ROW) + (first + (float)(RPT * r))) * a.inv_g);
+      const unsigned tok = (unsigned)token_of((float)(lane_at / ROW) + (first + (float)(RPT * r)), a.inv_g);
       const unsigned at = __umul24(tok, gap) + (unsigned)((lane_at ^ (XOR * r)) + (RPT * r + rel) * ROW);
       dma16_at(rq, qd + r * 1024, at, 0u);
       dma16_at(rd, qd + TILE_BYTES + r * 1024, at, 0u);

@@ -524,18 +524,10 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// ceil(x / y) of positive values by a reciprocal: up to one in 2^22 off on either side, which moves a range's border but
-// leaves the plan the same on every wave
-__device__ __forceinline__ float parts(float x, float y) { return ceilf(x * __builtin_amdgcn_rcpf(y) - 1e-5f); }
-
-// A list's ranges a tile and chunks a range.
-struct Cut {
-  float ranges, size;
-  __device__ __forceinline__ Cut(const ListShape& x, float per) {
-    ranges = fmaxf(parts((float)x.chunks, fmaxf(per, x.rows <= 32 ? 4.0f : 8.0f)), 1.0f);
-    size = x.tiles > 0 ? parts((float)x.chunks, ranges) : 0.0f;
-  }
+struct Reciprocal {
+  __device__ __forceinline__ float operator()(float x) const { return __builtin_amdgcn_rcpf(x); }
 };
+__device__ __forceinline__ Cut cut(const ListShape& x, float per) { return Cut(x.tiles, x.chunks, x.rows, per, Reciprocal()); }
 
 // The shapes of the lists, a lane each; up to 64 are read once.
 template <class F>
@@ -559,17 +551,17 @@ struct Lists {
       sum += wave_sum_dpp((float)x.tiles * (float)x.chunks);
       most = fmaxf(most, wave_max_dpp(x.tiles > 0 ? (float)x.chunks : 0.0f));
     }
-    const float fair = fmaxf(ceilf(sum * a.inv_slots), 1.0f);
-    const int near = (int)parts(most, fair);
+    const float fair = fair_share(sum, a.inv_slots);
+    const int near = (int)parts(most, __builtin_amdgcn_rcpf(fair));
     float best = fair, least = INFINITY;
     longest_item = most;
     for (int n = max(near - 2, 1); n <= near; ++n) {
-      const float per = fmaxf(parts(most, (float)n), fair);
+      const float per = fmaxf(parts(most, __builtin_amdgcn_rcpf((float)n)), fair);
       float size = 0.0f, big = 0.0f, work = 0.0f;
-      for (int i0 = 0; i0 < lists; i0 += 64) size = fmaxf(size, wave_max_dpp(Cut(at(i0), per).size));
+      for (int i0 = 0; i0 < lists; i0 += 64) size = fmaxf(size, wave_max_dpp(cut(at(i0), per).size));
       for (int i0 = 0; i0 < lists; i0 += 64) {
         const ListShape x = at(i0);
-        const Cut c(x, per);
+        const Cut c = cut(x, per);
         const float items = (float)x.tiles * c.ranges;
         big += wave_sum_dpp(2.0f * c.size > size ? items : 0.0f);
         work += wave_sum_dpp(items * c.size);
@@ -593,7 +585,7 @@ struct Lists {
     Ranges found = {0, 0, 0};
     for (int i0 = 0; i0 < lists; i0 += 64) {
       const ListShape x = at(i0);
-      const Cut c(x, per);
+      const Cut c = cut(x, per);
       const int i = i0 + lane_id(), ranges = (int)c.ranges, items = i < lists ? x.tiles * ranges : 0;
       const bool late = lists <= 64 && 2.0f * c.size <= longest;
       const int early_upto = wave_scan(late ? 0 : items), early = __builtin_amdgcn_readlane(early_upto, 63);
@@ -639,8 +631,8 @@ __device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Range
   const int i = w - r.item0, range = i % r.ranges;
   j.r0 = i / r.ranges * TILE;
   const int chunks = tile_chunks<TILE>(a, j);
-  j.c0 = (int)((long long)chunks * range / r.ranges);
-  j.c1 = (int)((long long)chunks * (range + 1) / r.ranges);
+  j.c0 = range_begin(chunks, range, r.ranges);
+  j.c1 = range_begin(chunks, range + 1, r.ranges);
 }
 
 // Partial `item` of a launch, all kv heads of an item side by side. Shared prefix: the prefix's items have a part of their own,
@@ -736,7 +728,7 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
     const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, list);
     q0 = s.q0;
     nq = s.nq;
-    t = w - (q0 * a.G / TILE + list);
+    t = w - first_tile<TILE>(q0, a.G, list);
     if (t < 0 || t * TILE + (int)blockIdx.y * RPB >= nq * a.G) return;
     own = planned(a, list);
     if (own.ranges == 1) return;  // (finished by its only range)
@@ -800,11 +792,6 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
 
 using namespace es;
 
-// Workgroups of a ranged launch that the GPU holds at once: 256 CUs, two workgroups each at D = 128 (64 KB of staging), three
-// at D = 64 (134 registers: at 128, for four, the wide loop reloads spilled ones).
-static int resident(int D) { return D == 64 ? 768 : 512; }
-// Items a head of a ranged launch: at most one a tile more than the ranges' chunks fill.
-static long long range_items(long long tiles, int Hk, int D) { return tiles + resident(D) / Hk + 1; }
 // Key ranges are worth a second launch where the tiles do not fill the GPU and a tile may have many chunks. `equal`: the keys
 // divide into B equal sequences; otherwise the host knows their sum alone, and the longest may have anything from Tk / B of them
 // to all. It is taken to have Tk / sqrt(B) then, halfway in the logarithm: with all of them batches of short sequences
