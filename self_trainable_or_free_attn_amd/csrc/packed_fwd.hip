@@ -10,7 +10,8 @@
 //     always in flight.
 // What bounds them: wide tiles the matrix units and what runs beside them on long sequences (32760 causal tokens of 24 heads over
 // 8, D = 128: 5.94 ms, 1110 TFLOP/s; 57 % of the cycles issue a matrix instruction, 55 % vector work, LDS 29 %, no bank
-// conflicts), the transfers where many tiles stream different keys from HBM, and on sequences of a few hundred rows the chain
+// conflicts), at D = 64 the vector work (as many exponentials for half the products: 8192 causal tokens of 32 heads 0.33 ms, 830
+// TFLOP/s, 44 % matrix, 77 % vector), the transfers where many tiles stream different keys from HBM, and on sequences of a few hundred rows the chain
 // of a tile's few chunks. Narrow tiles: HBM (8 tokens, 40 heads over 8, caches of 513 to 75600 keys: 654 MB in 137 us, 4.8
 // TB/s, what a large copy reaches).
 // 128 rows a wide tile and not 256 on eight waves: those read K and V half as often, but stop at their barriers together (32760
@@ -138,7 +139,8 @@ struct Rows {
   }
 
   // Where a maximum passes the one that the terms are taken against by more than SLACK, that one moves up, by whole powers of
-  // two (exact for what is scaled). Returns whether this lane's did; alpha: its factor.
+  // two: exact for the float32 sums, and for held probabilities but those that become subnormal in fp16 (below 2^-21 of the
+  // row's largest term; half a step there is 2^-32 of it). Returns whether this lane's did; alpha: its factor.
   __device__ __forceinline__ bool raise(float mx, float& alpha) {
     if (!(mx > mrun + SLACK)) return false;
     const float next = mrun == -INFINITY ? mx : mrun + ceilf(mx - mrun);
@@ -264,7 +266,9 @@ __device__ __forceinline__ void wide_tile(const FwdArgs& a, const Job& j, char* 
       // probabilities are held back over the second's test of the maximum, and scaled with O where that one moves. Against
       // both S first and each run's exponentials before its own products: 32760 causal tokens, 24 heads 6.39 -> 6.08 ms, 8192
       // at D = 64, 32 heads 345 -> 318 us.) Products run at a raised priority (packed.h): 32760 causal tokens 6.08 -> 5.94
-      // ms, 13770 of 12 heads without a mask 1332 -> 1225 us, 8192 causal of 32 heads 541 -> 522 (at D = 64 324 -> 326).
+      // ms, 13770 of 12 heads without a mask 1332 -> 1225 us, 8192 causal of 32 heads 541 -> 522. At D = 64 it gains without a
+      // mask (13770 of 12 heads 720 -> 705, 4096 of 16 92 -> 84) and loses with one (8192 causal of 32 heads 327 -> 332, 4096 of
+      // 24 heads with a bias 78 -> 84): the mask is known at run time only, so both have it.
       const bool masked = (c + 1) * BK > seen_min;
       float sc, c0, c1, alpha;
       ev8 pa, pb, qa, qb;
@@ -671,7 +675,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_ranges_kernel(Fwd
 }
 
 // A tile of the prefix's list holds rows of several sequences, so a prefix is read once for 128 rows of the batch and not once a
-// sequence. Single tokens are HBM bound (the prefix is read once, every cache once), more of them matrix bound.
+// sequence. Single tokens are HBM bound (the prefix is read once, every cache once). More of them are bound by the matrix work
+// of places that are not always filled: 16 samples of 16 tokens, prefix 32760, 40 heads over 8 issue a matrix instruction in 37 % of
+// the cycles at 1.43 of 2 waves a SIMD (long whole tiles 57 % at 1.92), though the items' chunks are spread within 2 %.
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
