@@ -23,9 +23,10 @@
 // Bounds: the matrix units on long sequences. Clips of 13770, 11880 and 4096 tokens without a mask, 12 heads, D = 128: bwd_q
 // 2.87 ms, 1120 TFLOP/s of its three products (61 % of the cycles issue a matrix instruction, LDS 31 %), bwd_kv 4.13 ms, 1030
 // TFLOP/s of its four (51 %; it waits the most, for its transfers and at the tile's barrier, with two workgroups a CU at 255
-// registers), in fp16 3.20 and 4.62 ms; causal prompts of 1 to 6553 tokens, 24 heads over 8: 0.65 and 0.88 ms. At D = 64 as many
-// exponentials go with half the products: the clips take 1.50 and 2.21 ms, 64 and 51 % matrix issue beside 74 and 62 % vector work.
-// What bounds short sequences is the chain of a tile's few chunks: transfers, two products, exponentials, two products.
+// registers), in fp16 3.20 and 4.62 ms; causal prompts of 1 to 6553 tokens, 24 heads over 8: 0.65 and 0.88 ms. At D = 64 as
+// many exponentials go with half the products: the clips take 1.50 and 2.21 ms, 64 and 51 % matrix issue beside 74 and 62 %
+// vector work. What bounds short sequences is the chain of a tile's few chunks: transfers, two products, exponentials, two
+// products.
 // dS is rounded to the token type without the softmax scale (applied to the finished sums). In fp16 it is rounded times a power
 // of two of its row (dQ) or key (dK), see fit.
 #include "packed.h"

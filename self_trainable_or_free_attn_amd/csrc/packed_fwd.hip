@@ -1,19 +1,20 @@
 // Forward of attention over packed sequences and over a shared prefix (gfx950, MFMA 32x32x16, bf16 / fp16).
 //
-// One workgroup of four waves owns a tile of up to 128 (small grids: 64) rows of (token, head in group) (packed.h) and streams the keys its
-// rows see in 64-key chunks, online softmax: S^T = K Q^T, so that exp(S^T) is the B operand of O^T += V^T P^T.
+// One workgroup of four waves owns a tile of up to 128 (small grids: 64) rows of (token, head in group) (packed.h) and
+// streams the keys its rows see in 64-key chunks, online softmax: S^T = K Q^T, so that exp(S^T) is the B operand of O^T +=
+// V^T P^T.
 //   wide tiles (more than 32 rows): each wave has 32 rows; a chunk is staged once in LDS for all four, the next one's
 //     transfers in flight under its products. With 64 rows two waves share 32 rows and take half of each chunk's keys.
 //   narrow tiles (up to 32 rows: single tokens with their head group): every wave has the same 32 rows and takes every
 //     fourth run of 32 keys, staged in its own quarter of LDS without a barrier; the four softmax states are merged at the
 //     end. The next K run is requested when this one's products have read it, the next V run likewise, so one of them is
 //     always in flight.
-// What bounds them: wide tiles the matrix units and what runs beside them on long sequences (32760 causal tokens of 24 heads over
-// 8, D = 128: 5.94 ms, 1110 TFLOP/s; 57 % of the cycles issue a matrix instruction, 55 % vector work, LDS 29 %, no bank
-// conflicts), at D = 64 the vector work (as many exponentials for half the products: 8192 causal tokens of 32 heads 0.33 ms, 830
-// TFLOP/s, 44 % matrix, 77 % vector), the transfers where many tiles stream different keys from HBM, and on sequences of a few hundred rows the chain
-// of a tile's few chunks. Narrow tiles: HBM (8 tokens, 40 heads over 8, caches of 513 to 75600 keys: 654 MB in 137 us, 4.8
-// TB/s, what a large copy reaches).
+// What bounds them: wide tiles the matrix units and what runs beside them on long sequences (32760 causal tokens of 24 heads
+// over 8, D = 128: 5.94 ms, 1110 TFLOP/s; 57 % of the cycles issue a matrix instruction, 55 % vector work, LDS 29 %, no bank
+// conflicts), at D = 64 the vector work (as many exponentials for half the products: 8192 causal tokens of 32 heads 0.33 ms,
+// 830 TFLOP/s, 44 % matrix, 77 % vector), the transfers where many tiles stream different keys from HBM, and on sequences of
+// a few hundred rows the chain of a tile's few chunks. Narrow tiles: HBM (8 tokens, 40 heads over 8, caches of 513 to 75600
+// keys: 654 MB in 137 us, 4.8 TB/s, what a large copy reaches).
 // 128 rows a wide tile and not 256 on eight waves: those read K and V half as often, but stop at their barriers together (32760
 // causal tokens 6.57 -> 6.95 ms; 13770 of 12 heads without a mask 1433 -> 1360 us).
 // Key ranges: with few tiles the chunks of a tile are cut into ranges, one workgroup each, that leave unnormalised partials
@@ -674,10 +675,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_ranges_kernel(Fwd
   run_tile<D, BIAS, TILE>(a, j, lds, stats, tab);
 }
 
-// A tile of the prefix's list holds rows of several sequences, so a prefix is read once for 128 rows of the batch and not once a
-// sequence. Single tokens are HBM bound (the prefix is read once, every cache once). More of them are bound by the matrix work
-// of places that are not always filled: 16 samples of 16 tokens, prefix 32760, 40 heads over 8 issue a matrix instruction in 37 % of
-// the cycles at 1.43 of 2 waves a SIMD (long whole tiles 57 % at 1.92), though the items' chunks are spread within 2 %.
+// A tile of the prefix's list holds rows of several sequences, so a prefix is read once for 128 rows of the batch and not
+// once a sequence. Single tokens are HBM bound (the prefix is read once, every cache once). More of them are bound by the
+// matrix work of places that are not always filled: 16 samples of 16 tokens, prefix 32760, 40 heads over 8 issue a matrix
+// instruction in 37 % of the cycles at 1.43 of 2 waves a SIMD (long whole tiles 57 % at 1.92), though the items' chunks are
+// spread within 2 %.
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * BK * D * 2];
@@ -799,23 +801,26 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
 using namespace es;
 
 // Key ranges are worth a second launch where the tiles do not fill the GPU and a tile may have many chunks. `equal`: the keys
-// divide into B equal sequences; otherwise the host knows their sum alone, and the longest may have anything from Tk / B of them
-// to all. It is taken to have Tk / sqrt(B) then, halfway in the logarithm: with all of them batches of short sequences
-// went to ranges that cut nothing (us whole and in ranges, D = 128, causal: 8 x 512 tokens of 4 heads 13 and 23, 100 x 64 of one
-// head 7.5 and 16, 4 x 1024 of 4 heads 18 and 31; 32 tokens against 40 keys each 8 and 10-12), with Tk / B a long
-// sequence among short ones is not cut (8000 + 7 x 64 tokens of one head 91 and 46; tokens against 8000 + 31 x 40 keys 69 and 14).
-// Single tokens and the like (up to 32 rows a sequence on average, whose partials are small): from 1024 keys on. (8 tokens, 8 heads
-// over 2, against 300 keys each 8 and 12, 1000 12.4 and 12.9; 2000 + 31 x 40 20 and 12.) From 64 sequences on the plan is read
-// once a pass, so the longest one has to be longer (64 tokens against 256 keys 7 and 17, 128 against 2000 + 127 x 20 19 and 31).
+// divide into B equal sequences; otherwise the host knows their sum alone, and the longest may have anything from Tk / B of
+// them to all. It is taken to have Tk / sqrt(B) then, halfway in the logarithm: with all of them batches of short sequences
+// went to ranges that cut nothing (us whole and in ranges, D = 128, causal: 8 x 512 tokens of 4 heads 13 and 23, 100 x 64 of
+// one head 7.5 and 16, 4 x 1024 of 4 heads 18 and 31; 32 tokens against 40 keys each 8 and 10-12), with Tk / B a long
+// sequence among short ones is not cut (8000 + 7 x 64 tokens of one head 91 and 46; tokens against 8000 + 31 x 40 keys 69 and
+// 14).
+// Single tokens and the like (up to 32 rows a sequence on average, whose partials are small): from 1024 keys on. (8 tokens, 8
+// heads over 2, against 300 keys each 8 and 12, 1000 12.4 and 12.9; 2000 + 31 x 40 20 and 12.) From 64 sequences on the plan
+// is read once a pass, so the longest one has to be longer (64 tokens against 256 keys 7 and 17, 128 against 2000 + 127 x 20
+// 19 and 31).
 // One sequence, or no more keys than rows (then the longest sequence has the most tiles): a launch of whole tiles takes
-// WHOLE_CHUNK_US a chunk of the longest one, ranges RANGE_CHUNK_US a chunk and item and RANGE_US more for their plan, partials and
-// merge. (us in ranges and whole, D = 128, causal: 200 tokens of 32 heads over 8 against 1000 keys 24 and 19, 2000 keys 26 and 31,
-// 4000 keys 34 and 54; 2000 tokens of 2 heads over one 24 and 29, of 8 heads 36 and 31; 3000 of 8 58 and 45; 5000 of 4 heads 61 and
-// 67, of 8 heads over 8 117 and 77; 1500 of 10 over 2 35 and 25. At D = 64 all three are about 3 / 4 of that.)
+// WHOLE_CHUNK_US a chunk of the longest one, ranges RANGE_CHUNK_US a chunk and item and RANGE_US more for their plan,
+// partials and merge. (us in ranges and whole, D = 128, causal: 200 tokens of 32 heads over 8 against 1000 keys 24 and 19,
+// 2000 keys 26 and 31, 4000 keys 34 and 54; 2000 tokens of 2 heads over one 24 and 29, of 8 heads 36 and 31; 3000 of 8 58 and
+// 45; 5000 of 4 heads 61 and 67, of 8 heads over 8 117 and 77; 1500 of 10 over 2 35 and 25. At D = 64 all three are about 3 /
+// 4 of that.)
 // Otherwise some sequences may have most of the keys and few of the tiles: from 4096 keys in all (equal sequences: each), or
-// where the tiles take a quarter of the GPU's places or fewer from 1280 of the longest. (us whole and in ranges, 64 tokens each of
-// 8 heads: against 4000 + 3 x 100 keys 49 and 20, 2500 + 2 x 80 34 and 23, 4 x 2000 29 and 22, 4 x 1000 17 and 21, 4 x 500 12 and 19,
-// 16 x 300 11 and 17, 4000 + 15 x 100 51 and 21.)
+// where the tiles take a quarter of the GPU's places or fewer from 1280 of the longest. (us whole and in ranges, 64 tokens
+// each of 8 heads: against 4000 + 3 x 100 keys 49 and 20, 2500 + 2 x 80 34 and 23, 4 x 2000 29 and 22, 4 x 1000 17 and 21, 4
+// x 500 12 and 19, 16 x 300 11 and 17, 4000 + 15 x 100 51 and 21.)
 constexpr double WHOLE_CHUNK_US = 0.77, RANGE_CHUNK_US = 0.003125, RANGE_US = 15.0;
 static bool ranged(long long tiles, int B, int Tq, int Tk, int H, int Hk, int D, bool equal) {
   const long long items = tiles * Hk;
