@@ -138,6 +138,11 @@ def _grid_turns(grid, dim):
 SMALLEST, LARGEST = {"bf16": -120, "fp16": -13}, {"bf16": 120, "fp16": 13}
 
 
+def _power(e):
+    """2^e in float64, from the exponent's bits: exact, which powers by a function need not be."""
+    return (e.long() + 1023 << 52).view(torch.float64)
+
+
 def _quantise(x, dtype):
     """(codes uint8 [..., D / 2], exponents + 127 uint8 [..., D / 32]) of float32 x [..., D]."""
     x = x.unflatten(-1, (-1, 32))
@@ -145,7 +150,7 @@ def _quantise(x, dtype):
     frac, e = torch.frexp(top)                        # top = frac 2^e, 0.5 <= frac < 1
     e = torch.where(frac > 0.875, e - 2, e - 3)       # 7 s >= top: s = 2^(e - 3) holds up to 0.875 2^e
     e = torch.where(top == 0, SMALLEST[dtype], e).clamp(SMALLEST[dtype], LARGEST[dtype])
-    y = torch.ldexp(x.double(), -e[..., None])        # exact
+    y = x.double() * _power(-e)[..., None]            # exact
     a = y.abs()
     borders = ((0.25, False), (0.75, True), (1.25, False), (1.75, True), (2.5, False), (3.5, True), (5.0, False))
     code = torch.zeros_like(a, dtype=torch.uint8)
@@ -284,7 +289,7 @@ def _values(codes, scales):
     """The float32 values of 4-bit rows."""
     table = torch.tensor(VALUES + tuple(-x for x in VALUES), device="cuda")
     x = table[torch.stack([codes & 15, codes >> 4], -1).flatten(-2).long()]
-    return (x.unflatten(-1, (-1, 32)) * torch.exp2(scales.float() - 127)[..., None]).flatten(-2)
+    return (x.unflatten(-1, (-1, 32)) * _power(scales.int() - 127).float()[..., None]).flatten(-2)
 
 
 def _places(state):
@@ -393,11 +398,18 @@ def _rotated64(x, w, cs, halves):
     return torch.cat([torch.view_as_real(z).flatten(-2), x[..., R:]], -1)
 
 
+def _powers64(e):
+    """2^e for whole e from -127 to 128."""
+    return torch.tensor([2.0 ** i for i in range(-127, 129)], dtype=torch.float64, device="cuda")[e.long() + 127]
+
+
 def _held64(x, dtype):
     """The 4-bit values nearest to x, by steps of a power of two: 0.5 s below 2 s, s from there to 4 s, 2 s above."""
     g = x.unflatten(-1, (-1, 32))
     top = g.abs().amax(-1, keepdim=True)
-    s = torch.exp2(torch.ceil(torch.log2(top / 7).clamp(SMALLEST[dtype], LARGEST[dtype])))
+    s = _powers64(torch.log2(top / 7).ceil().clamp(SMALLEST[dtype], LARGEST[dtype]))
+    s = torch.where(top > 7 * s, 2 * s, torch.where(top <= 3.5 * s, s / 2, s))      # (a logarithm that is a last bit off)
+    s = s.clamp(2.0 ** SMALLEST[dtype], 2.0 ** LARGEST[dtype])
     a = g.abs() / s
     step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
     return (torch.sign(g) * (torch.round(a / step) * step).clamp(max=6) * s).flatten(-2)
@@ -407,8 +419,8 @@ def _decoded64(codes, scales):
     """Sign, two bits of exponent, one of mantissa."""
     n = torch.stack([codes % 16, codes // 16], -1).flatten(-2).long()
     e, m = n // 2 % 4, (n % 2).double()
-    a = torch.where(e == 0, m / 2, torch.ldexp(1 + m / 2, e - 1)) * (1 - 2 * (n // 8)).double()
-    return torch.ldexp(a, scales.long().repeat_interleave(32, -1) - 127)
+    a = torch.where(e == 0, m / 2, (1 + m / 2) * _powers64(e - 1)) * (1 - 2 * (n // 8)).double()
+    return a * _powers64(scales.long() - 127).repeat_interleave(32, -1)
 
 
 def exact(case, seed):
