@@ -1,5 +1,5 @@
-"""Bindings of the C ABI in include/echosparse_hip.h, include/vsa_hip.h and include/packed_hip.h (libechosparse_hip.so,
-built in-tree by build_lib).
+"""Bindings of the C ABI in include/echosparse_hip.h, include/vsa_hip.h, include/packed_hip.h and include/paged_hip.h
+(libechosparse_hip.so, built in-tree by build_lib).
 
 Kernel calls (`call`) go through the torch operators torch.ops.echosparse_gfx950.<entry point> (torch_ops.py,
 lib/libechosparse_torch.so): arguments are tensors (None = NULL) and Python scalars in the header's order, and each
@@ -79,20 +79,28 @@ SIGNATURES = {
     "es_packed_fwd": [P, P, P, P, P, P, P, I, I, P, P, P, Z, I, I, I, I, I, I, I, F],
     "es_packed_bwd": [P, P, P, P, P, P, P, P, P, P, I, I, P, P, P, P, P, Z, I, I, I, I, I, I, I, F],
     "es_shared_prefix_fwd": [P, P, P, P, P, P, P, P, P, Z, I, I, I, I, I, I, I, F],
+    # include/paged_hip.h
+    "es_norm_rotate": [P] * 8 + [I] * 9 + [DB, LL, LL],
+    "es_norm_rotate_bwd": [P] * 13 + [Z] + [I] * 9 + [DB, LL, LL],
+    "es_append_paged": [P] * 12 + [I] * 12 + [DB] + [LL] * 6,
+    "es_append_paged4": [P] * 14 + [I] * 12 + [DB] + [LL] * 3,
+    "es_paged_rows": [P] * 7 + [I] * 7 + [LL] * 3,
+    "es_paged_rows4": [P] * 9 + [I] * 7,
 }
-# the fp16 twins (suffix _f16) of the VSA and packed-sequence entry points that take token tensors, same arguments
+# the fp16 twins (suffix _f16) of the VSA, packed-sequence and paged-cache entry points that take token tensors, same arguments
 F16_TWINS = ("vsa_pool", "vsa_fuse_fwd", "vsa_fuse_bwd", "vsa_finalize", "vsa_attn_fwd", "vsa_attn_fwd_tasks",
              "vsa_attn_bwd_kv", "vsa_attn_bwd_kv_tasks", "vsa_attn_bwd_q", "vsa_attn_bwd_q_tasks", "vsa_block_scores",
              "vsa_route_rows", "vsa_row_topk", "vsa_router_lse", "vsa_router_scores", "vsa_split_merge_fwd",
              "vsa_split_merge_sum", "vsa_rep_build", "vsa_rep_build_kmeans", "vsa_rep_attn_fwd", "vsa_rep_attn_bwd_q", "vsa_rep_bwd_tables",
              "vsa_rep_bwd_both_tables", "vsa_rep_unpool", "vsa_row_dot", "es_packed_fwd", "es_packed_bwd",
-             "es_shared_prefix_fwd")
+             "es_shared_prefix_fwd", "es_norm_rotate", "es_norm_rotate_bwd", "es_append_paged", "es_append_paged4",
+             "es_paged_rows", "es_paged_rows4")
 SIGNATURES.update({n + "_f16": SIGNATURES[n] for n in F16_TWINS})
 NO_STREAM = {"es_representatives_workspace": ([I, I, I], Z), "es_dense_attention_workspace": ([I, I, I], Z),
              "es_representatives_noalloc_limit": ([], Z), "es_last_error_string": ([], ctypes.c_char_p),
              "es_abi_version": ([], I), "vsa_topk_workspace": ([I, I], Z),
              "es_packed_fwd_workspace": ([I] * 6, Z), "es_packed_bwd_workspace": ([I] * 9, Z),
-             "es_shared_prefix_workspace": ([I] * 7, Z)}
+             "es_shared_prefix_workspace": ([I] * 7, Z), "es_norm_rotate_workspace": ([I] * 4, Z)}
 
 _lib = None
 _ops = None

@@ -1,6 +1,7 @@
 """Torch operator registration of the C ABI: every stream-taking entry point of include/echosparse_hip.h,
-include/vsa_hip.h and include/packed_hip.h becomes the operator torch.ops.echosparse_gfx950.<entry point>, with the header's argument names
-and order (the stream is torch's current HIP stream of the tensors' device).
+include/vsa_hip.h, include/packed_hip.h and include/paged_hip.h becomes the operator
+torch.ops.echosparse_gfx950.<entry point>, with the header's argument names and order (the stream is torch's current HIP stream
+of the tensors' device).
 
 The C++ registration (csrc/torch/ops.cpp) is generated from the headers, so the operator set can not drift from
 the ABI:
@@ -10,8 +11,8 @@ the ABI:
     type is refused (no silent wrap)
   * every tensor must be contiguous (a strided view would hand the kernel the wrong rows) and of the dtype its C
     type names: float* float32, int* / unsigned* int32 (or uint32), uint8_t* uint8 (or bool), const void* bf16
-    or float16 (the token tensors), void* also float32 (outputs some entry points write in fp32 on request), and
-    a void* named workspace any dtype
+    or float16 (the token tensors), void* also float32 (outputs some entry points write in fp32 on request), as do
+    the weights of a norm (const void* ..._weight), and a void* named workspace any dtype
   * every operator returns nothing, like the C functions; a failing status raises RuntimeError with
     es_last_error_string(), a host tensor is refused before any launch
   * implementations for the CUDA (HIP) dispatch key, CPU (which only refuses host tensors) and Meta (no work, for
@@ -19,7 +20,8 @@ the ABI:
 The reference registers its native op set as a pybind11 module (csrc/vsa/vsa2_api.cpp:904-941); here the same role
 is played by torch.library (TORCH_LIBRARY), loaded with torch.ops.load_library.
 
-csrc/torch/packed.cpp adds written operators in the same namespace: the packed-sequence calls with their outputs and gradient.
+csrc/torch/packed.cpp and paged.cpp add written operators in the same namespace: the packed-sequence and paged-cache calls with
+their outputs and gradients.
 
 The library is built by build_lib.build() (g++, host code only) into lib/libechosparse_torch.so. It does not link
 libechosparse_hip.so: its C symbols resolve against the copy the ctypes binding loaded with RTLD_GLOBAL, so an
@@ -32,9 +34,10 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-HEADERS = [os.path.join(ROOT, "include", h) for h in ("echosparse_hip.h", "vsa_hip.h", "packed_hip.h")]
+HEADERS = [os.path.join(ROOT, "include", h) for h in ("echosparse_hip.h", "vsa_hip.h", "packed_hip.h", "paged_hip.h")]
 SOURCE = os.path.join(HERE, "csrc", "torch", "ops.cpp")
-WRITTEN = [os.path.join(HERE, "csrc", "torch", "packed.cpp")]     # operators with outputs and a gradient of their own
+# operators with outputs and a gradient of their own
+WRITTEN = [os.path.join(HERE, "csrc", "torch", f) for f in ("packed.cpp", "paged.cpp")]
 LIB = os.path.join(HERE, "lib", "libechosparse_torch.so")
 NAMESPACE = "echosparse_gfx950"
 
@@ -80,6 +83,8 @@ def _dtype_kind(ctype, pname):
     if base == "void":
         if pname == "workspace":
             return "ES_ANY"
+        if pname.endswith("_weight"):
+            return "ES_OUT"
         # a written token tensor may be an fp32 output (out_fp32 / accumulate variants)
         return "ES_HALF" if ctype.startswith("const") else "ES_OUT"
     return {"float": "ES_F32", "int": "ES_I32", "unsigned": "ES_I32", "uint8_t": "ES_U8"}[base]
@@ -121,10 +126,11 @@ def source():
     """The generated C++ registration."""
     eps = entry_points()
     lines = [
-        "// Generated by self_trainable_or_free_attn_amd/torch_ops.py from include/echosparse_hip.h, include/vsa_hip.h and",
-        "// include/packed_hip.h: one torch operator per stream-taking C entry point. Do not edit by hand.",
+        "// Generated by self_trainable_or_free_attn_amd/torch_ops.py from include/echosparse_hip.h, include/vsa_hip.h,",
+        "// include/packed_hip.h and include/paged_hip.h: one torch operator per stream-taking C entry point. Do not edit by hand.",
         '#include "../../../include/vsa_hip.h"',
         '#include "../../../include/packed_hip.h"',
+        '#include "../../../include/paged_hip.h"',
         "",
         "#include <ATen/core/Tensor.h>",
         "#include <c10/core/DeviceGuard.h>",
