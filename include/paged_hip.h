@@ -97,6 +97,29 @@ int es_paged_rows4_f16(const uint8_t* k_codes, const uint8_t* k_scales, const ui
                        const int* pages, const int* lens, const int* cu, void* k, void* v, int B, int T, int max_pages,
                        int num_pages, int page_size, int Hk, int D, hipStream_t stream);
 
+/* Attention of new tokens q (Tq, H, D) over the cache: token i of n new ones of sequence b sees all its lens[b] keys, with causal
+ * != 0 those up to its own position; out (Tq, H, D), lse (Tq, H) float32 as in packed_hip.h. Keys of pages that the cache does not
+ * have are left out. Rows that see no key, and rows behind the last sequence, get out = 0 and lse = -inf. Values of the keys in
+ * use must be finite (of a cache of 4 bits within the token type), scores below 2^22 in magnitude.
+ * workspace: es_paged_workspace bytes (0: none needed; NULL / 0 is then accepted); bits: 16 or 4. */
+size_t es_paged_workspace(int B, int Tq, int max_pages, int page_size, int H, int Hk, int D, int bits);
+int es_paged_fwd(const void* q, const void* k_pages, const void* v_pages, const int* pages, const int* lens, const int* cu,
+                 void* out, float* lse, void* workspace, size_t workspace_bytes, int B, int Tq, int max_pages, int num_pages,
+                 int page_size, int H, int Hk, int D, int causal, float scale, long long page_stride, long long head_stride,
+                 long long row_stride, hipStream_t stream);
+int es_paged_fwd_f16(const void* q, const void* k_pages, const void* v_pages, const int* pages, const int* lens, const int* cu,
+                     void* out, float* lse, void* workspace, size_t workspace_bytes, int B, int Tq, int max_pages,
+                     int num_pages, int page_size, int H, int Hk, int D, int causal, float scale, long long page_stride,
+                     long long head_stride, long long row_stride, hipStream_t stream);
+int es_paged4_fwd(const void* q, const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
+                  const uint8_t* v_scales, const int* pages, const int* lens, const int* cu, void* out, float* lse,
+                  void* workspace, size_t workspace_bytes, int B, int Tq, int max_pages, int num_pages, int page_size, int H,
+                  int Hk, int D, int causal, float scale, hipStream_t stream);
+int es_paged4_fwd_f16(const void* q, const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
+                      const uint8_t* v_scales, const int* pages, const int* lens, const int* cu, void* out, float* lse,
+                      void* workspace, size_t workspace_bytes, int B, int Tq, int max_pages, int num_pages, int page_size,
+                      int H, int Hk, int D, int causal, float scale, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

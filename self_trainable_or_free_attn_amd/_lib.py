@@ -86,6 +86,8 @@ SIGNATURES = {
     "es_append_paged4": [P] * 14 + [I] * 12 + [DB] + [LL] * 3,
     "es_paged_rows": [P] * 7 + [I] * 7 + [LL] * 3,
     "es_paged_rows4": [P] * 9 + [I] * 7,
+    "es_paged_fwd": [P] * 9 + [Z] + [I] * 9 + [F] + [LL] * 3,
+    "es_paged4_fwd": [P] * 11 + [Z] + [I] * 9 + [F],
 }
 # the fp16 twins (suffix _f16) of the VSA, packed-sequence and paged-cache entry points that take token tensors, same arguments
 F16_TWINS = ("vsa_pool", "vsa_fuse_fwd", "vsa_fuse_bwd", "vsa_finalize", "vsa_attn_fwd", "vsa_attn_fwd_tasks",
@@ -94,13 +96,14 @@ F16_TWINS = ("vsa_pool", "vsa_fuse_fwd", "vsa_fuse_bwd", "vsa_finalize", "vsa_at
              "vsa_split_merge_sum", "vsa_rep_build", "vsa_rep_build_kmeans", "vsa_rep_attn_fwd", "vsa_rep_attn_bwd_q", "vsa_rep_bwd_tables",
              "vsa_rep_bwd_both_tables", "vsa_rep_unpool", "vsa_row_dot", "es_packed_fwd", "es_packed_bwd",
              "es_shared_prefix_fwd", "es_norm_rotate", "es_norm_rotate_bwd", "es_append_paged", "es_append_paged4",
-             "es_paged_rows", "es_paged_rows4")
+             "es_paged_rows", "es_paged_rows4", "es_paged_fwd", "es_paged4_fwd")
 SIGNATURES.update({n + "_f16": SIGNATURES[n] for n in F16_TWINS})
 NO_STREAM = {"es_representatives_workspace": ([I, I, I], Z), "es_dense_attention_workspace": ([I, I, I], Z),
              "es_representatives_noalloc_limit": ([], Z), "es_last_error_string": ([], ctypes.c_char_p),
              "es_abi_version": ([], I), "vsa_topk_workspace": ([I, I], Z),
              "es_packed_fwd_workspace": ([I] * 6, Z), "es_packed_bwd_workspace": ([I] * 9, Z),
-             "es_shared_prefix_workspace": ([I] * 7, Z), "es_norm_rotate_workspace": ([I] * 4, Z)}
+             "es_shared_prefix_workspace": ([I] * 7, Z), "es_norm_rotate_workspace": ([I] * 4, Z),
+             "es_paged_workspace": ([I] * 8, Z)}
 
 _lib = None
 _ops = None

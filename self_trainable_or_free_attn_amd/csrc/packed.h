@@ -72,10 +72,11 @@ __device__ __forceinline__ Seq sequence(const int* cu_q, const int* cu_k, int B,
 // Tile number w of a launch without ranges: the sequences in descending order of their other length (keys where tiles are of
 // rows, rows where KEYS), so that the tiles with the most work start first and those that start last are short (workgroups are
 // dispatched in order), each with its tiles. Up to 64 sequences (the rows behind the last one included): each lane takes one
-// and adds up the tiles of those before it. More: their own order, by seq_of_tile. false: no tile has this number.
+// and adds up the tiles of those before it. More: their own order, by seq_of_tile. false: no tile has this number. lens: the
+// keys of each sequence, held to `cap`, in the place of cu_k.
 template <int M, bool KEYS>
 __device__ __forceinline__ bool tile_of(const int* cu_q, const int* cu_k, int B, int Tq, int Tk, int G, int w, Seq& s, int& b,
-                                        int& t) {
+                                        int& t, const int* lens = nullptr, int cap = 0) {
   if (B < 64) {
     const int l = min(lane_id(), B), last = KEYS ? Tk : Tq;
     Seq x;
@@ -83,6 +84,7 @@ __device__ __forceinline__ bool tile_of(const int* cu_q, const int* cu_k, int B,
     x.k0 = seq_start(cu_k, l, B, Tk);
     x.nq = l < B ? max(seq_start(cu_q, l + 1, B, Tq) - x.q0, 0) : 0;
     x.nk = l < B ? max(seq_start(cu_k, l + 1, B, Tk) - x.k0, 0) : 0;
+    if (lens != nullptr) x.nk = l < B ? min(max(lens[l], 0), cap) : 0;
     if (l == B) (KEYS ? x.nk : x.nq) = last - (KEYS ? x.k0 : x.q0);
     const int tiles = ((KEYS ? x.nk : x.nq * G) + M - 1) / M, weight = KEYS ? x.nq : x.nk;
     int base = 0;
@@ -102,6 +104,7 @@ __device__ __forceinline__ bool tile_of(const int* cu_q, const int* cu_k, int B,
   }
   b = KEYS ? seq_of_tile<M>(cu_k, B, Tk, 1, w) : seq_of_tile<M>(cu_q, B, Tq, G, w);
   s = sequence(cu_q, cu_k, B, Tq, Tk, b);
+  if (lens != nullptr) s.nk = b < B ? __builtin_amdgcn_readfirstlane(min(max(lens[b], 0), cap)) : 0;
   if (KEYS && b >= B) {
     s.nk = Tk - s.k0;
     s.nq = 0;

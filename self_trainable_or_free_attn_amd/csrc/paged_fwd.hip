@@ -1,0 +1,609 @@
+// Attention of new tokens over paged caches of 16 and 4 bits (gfx950, bf16 / fp16): where the tiles of packed_tiles.h get their keys
+// from, and tiles of their own for few rows over a cache of 4 bits.
+//
+// Page numbers: a page holds 16 rows or a multiple of that, so sixteen keys that start at a multiple of sixteen stand in one page.
+// Each lane of a wave holds the page number of one such group, a window of 64 groups (the next window's numbers are on their way),
+// and the wave takes the one that it needs by a lane read: no load stands between a chunk and its transfers.
+// Groups whose page number is outside the cache are missing: their scores become -inf, their values zeros.
+#include "packed_tiles.h"
+#include "paged.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace es {
+
+namespace {
+
+__device__ __forceinline__ int cached_keys(const FwdArgs& a, int b) {
+  return b >= a.B ? 0 : __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.paged.cap));
+}
+
+// Page numbers of 64 groups of sixteen keys, a lane each: narrow tiles, whose waves take every fourth run of 32 keys, hold those of
+// 32 runs of their own, wide ones those of sixteen chunks. -1: missing; 0 where the sequence has no keys.
+struct PageWindow {
+  int cur, next, first, step;  // the window's first run or chunk, and how many it spans
+  unsigned long long gone;
+  bool narrow;
+
+  __device__ __forceinline__ int fetch(const FwdArgs& a, const Job& j, int from) const {
+    const int l = lane_id(), g = narrow ? 2 * (from + 4 * (l >> 1)) + (l & 1) : 4 * from + l;
+    if (16 * g >= j.nk) return 0;
+    const int p = j.table[(16 * g) >> a.paged.shift];
+    return p >= 0 && p < a.paged.num_pages ? p : -1;
+  }
+  __device__ __forceinline__ void start(const FwdArgs& a, const Job& j, int from, bool narrow_) {
+    narrow = narrow_;
+    step = narrow ? 128 : 16;
+    first = from;
+    cur = fetch(a, j, first);
+    next = fetch(a, j, first + step);
+    gone = __builtin_amdgcn_ballot_w64(cur < 0);
+  }
+  // moves on to the window that holds run (chunk) x, which is in this one or the first of the next; its slot
+  __device__ __forceinline__ int slot(const FwdArgs& a, const Job& j, int x) {
+    if (x - first >= step) {
+      first += step;
+      cur = next;
+      gone = __builtin_amdgcn_ballot_w64(cur < 0);
+      next = fetch(a, j, first + step);
+    }
+    return narrow ? (x - first) >> 2 : x - first;
+  }
+  // page number of group i of the window
+  __device__ __forceinline__ int page(int i) const { return __builtin_amdgcn_readlane(cur, i); }
+  __device__ __forceinline__ unsigned missing(int i, unsigned mask) const { return (unsigned)(gone >> i) & mask; }
+};
+
+// the scores of missing groups of sixteen keys; bits: two groups
+__device__ __forceinline__ void mask_groups(f32x16& s, unsigned bits) {
+  if (bits == 0) return;
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (bits >> (r / 8) & 1) s[r] = -INFINITY;
+}
+
+// 16 bits: transfers of sixteen rows each from their page, rows past the sequence's keys and of missing pages read as zeros
+template <int D>
+struct Pages {
+  static constexpr bool HOLES = true, STAGED = false;
+  static constexpr int LPR = D / 8, NI = D / 32;  // NI transfers of 64 / LPR rows: sixteen rows
+  PageWindow window;
+  unsigned src[2 * NI], stride, now, then;
+  int wv;
+  __device__ __forceinline__ Pages(const FwdArgs& a, const Job& j, int l, int wave, bool narrow) : now(0), then(0), wv(wave) {
+    stride = (unsigned)a.paged.row_stride * 2;
+#pragma unroll
+    for (int i = 0; i < 2 * NI; ++i) {  // (the row within its group; its place in LDS goes by the row within the tile)
+      const int R = i * (64 / LPR) + l / LPR, at = (narrow ? 0 : 16 * wv) + R;
+      src[i] = (unsigned)(R & 15) * stride + (unsigned)(((l % LPR) ^ swizzle<D>(at)) * 16);
+    }
+    window.start(a, j, narrow ? 2 * j.c0 + wv : j.c0, narrow);
+  }
+  // group g of the sequence in page `page`: what holds it, and the bytes of it that are there
+  __device__ __forceinline__ size_t group(const FwdArgs& a, const Job& j, int g, int page, unsigned& bytes) const {
+    const int left = min(16, j.nk - 16 * g);
+    bytes = page < 0 || left <= 0 ? 0u : (unsigned)(left - 1) * stride + D * 2;
+    return (size_t)max(page, 0) * a.paged.page_stride +
+           (size_t)((16 * g) & ((1 << a.paged.shift) - 1)) * a.paged.row_stride;
+  }
+  __device__ __forceinline__ void wide(const FwdArgs& a, const Job& j, int c, unsigned dst) {
+    const int slot = window.slot(a, j, c);
+    then = window.missing(4 * slot, 15u);
+    unsigned bytes;
+    const size_t at = group(a, j, 4 * c + wv, window.page(4 * slot + wv), bytes);
+    const srd_t rk = make_srd(j.k + at, bytes), rv = make_srd(j.v + at, bytes);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma16_at(rk, dst + i * 1024, src[i], 0u);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma16_at(rv, dst + BK * D * 2 + i * 1024, src[i], 0u);
+  }
+  __device__ __forceinline__ void settle(char*) {}
+  __device__ __forceinline__ void run(const FwdArgs& a, const Job& j, bool v, int u, unsigned dst) {
+    const int slot = window.slot(a, j, u);
+    then = window.missing(2 * slot, 3u);
+    const e16_t* base = v ? j.v : j.k;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      unsigned bytes;
+      const size_t at = group(a, j, 2 * u + t, window.page(2 * slot + t), bytes);
+      const srd_t r = make_srd(base + at, bytes);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) dma16_at(r, dst + (NI * t + i) * 1024, src[NI * t + i], 0u);
+    }
+  }
+  __device__ __forceinline__ void enter() { now = then; }
+  __device__ __forceinline__ void enter_run(int) { now = then; }  // (called before the next run's transfers)
+  __device__ __forceinline__ void mask(f32x16& s, int run) const { mask_groups(s, now >> (2 * run) & 3u); }
+};
+
+// 4 bits, wide tiles: a thread loads 32 codes of a row and their scale a chunk ahead (D = 128: of keys and of values) and writes
+// them as token values where the transfers of 16 bits would have put them
+template <int D>
+struct Codes {
+  static constexpr bool HOLES = true, STAGED = true;
+  static constexpr int PARTS = D == 128 ? 2 : 1, TPR = D / 32;  // threads a row
+  PageWindow window;
+  uint4 code[PARTS];
+  unsigned scale[PARTS], now, then;
+  int tensor, row, part, wv;  // D = 64: two waves have the keys, two the values
+  __device__ __forceinline__ Codes(const FwdArgs& a, const Job& j, int l, int wave, bool) : now(0), then(0), wv(wave) {
+    tensor = D == 128 ? 0 : wv >> 1;
+    row = D == 128 ? 16 * wv + (l >> 2) : 32 * (wv & 1) + (l >> 1);
+    part = l % TPR;
+    window.start(a, j, j.c0, false);
+  }
+  __device__ __forceinline__ void wide(const FwdArgs& a, const Job& j, int c, unsigned) {
+    const int slot = window.slot(a, j, c);
+    then = window.missing(4 * slot, 15u);
+    int page = window.page(4 * slot + (D == 128 ? wv : 2 * (wv & 1)));
+    if (D == 64) page = row & 16 ? window.page(4 * slot + 2 * (wv & 1) + 1) : page;
+    const int key = BK * c + row;
+    const bool there = key < j.nk && page >= 0;
+    const size_t at = (((size_t)max(page, 0) * a.Hk + j.hk) << a.paged.shift) + (key & ((1 << a.paged.shift) - 1));
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      const uint8_t* codes = tensor + p ? a.paged.codes[1] : a.paged.codes[0];
+      const uint8_t* scales = tensor + p ? a.paged.scales[1] : a.paged.scales[0];
+      code[p] = make_uint4(0, 0, 0, 0);
+      scale[p] = 127;
+      if (there) {
+        code[p] = *reinterpret_cast<const uint4*>(codes + at * (D / 2) + 16 * part);
+        scale[p] = scales[at * (D / 32) + part];
+      }
+    }
+  }
+  __device__ __forceinline__ void settle(char* base) const {
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      char* tile = base + (tensor + p) * BK * D * 2;
+      const float s = __uint_as_float(scale[p] << 23);
+      const unsigned w[4] = {code[p].x, code[p].y, code[p].z, code[p].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<ev8*>(tile + tile_at<D>(row, 4 * part + i)) = decode8(w[i], s);
+    }
+  }
+  __device__ __forceinline__ void enter() { now = then; }
+  __device__ __forceinline__ void mask(f32x16& s, int run) const { mask_groups(s, now >> (2 * run) & 3u); }
+};
+
+// ------------------------------------------------------------------------------------------------ few rows over 4 bits
+// MFMA 16x16x32. Operand layouts (checked on the GPU): A (16x32): lane l holds A[l % 16][8 (l / 16) + 0..7], B (32x16): lane l holds
+// B[8 (l / 16) + 0..7][l % 16], C (16x16): lane l, register r holds C[4 (l / 16) + r][l % 16].
+__device__ __forceinline__ f32x4 emfma16(ev8 a, ev8 b, f32x4 c) {
+#ifdef ES_ELEM_F16
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+#else
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+#endif
+}
+
+// sums and maxima over the four lanes l % 16 + 16 i
+__device__ __forceinline__ float2 lane_pair16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_rows16(float x) {
+  const float2 h = lane_pair16(x);
+  return max_xor32(fmaxf(h.x, h.y));
+}
+__device__ __forceinline__ float sum_rows16(float x) {
+  const float2 h = lane_pair16(x);
+  return sum_xor32(h.x + h.y);
+}
+
+// Up to 16 NR rows; every wave has the same rows and takes every fourth run of 32 keys, the four states are merged at the end.
+// S^T = K Q^T of two groups of sixteen keys, channels in the order in which a lane's bytes hold them: lane (key l % 16, quarter
+// l / 16) loads a quarter of its key's row in one piece and feeds it to the products without LDS. The exponentials of both groups
+// are the B operand of O^T += V^T P^T with the keys in the order 4 q + 0..3, 16 + 4 q + 0..3 of quarter q. V goes through the
+// wave's own LDS as token values, from where it is read transposed. No barrier in the loop.
+template <int D, int NR>
+__device__ __forceinline__ void narrow4_tile(const FwdArgs& a, const Job& j, char* lds, float* stats) {
+  constexpr int NKS = D / 32, NDB = D / 16, ROW = D * 2, WORDS = D / 32;  // words of 8 codes a lane and group
+  constexpr int LDS_WAVE = NR * 32 * ROW;
+  const int tid = threadIdx.x, l = tid & 63, c = l & 15, g = l >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rows = j.nq * a.G, last = min(j.r0 + 16 * NR, rows) - 1;
+  const int seen_min = keys_seen(a, j, j.r0), seen_max = keys_seen(a, j, last);
+
+  ev8 q[NR][NKS];
+  f32x4 o[NR][NDB];
+  float lsum[NR], mrun[NR];
+  int seen[NR];
+  size_t at[NR];
+  bool valid[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int r = j.r0 + 16 * n + c;
+    valid[n] = r < rows;
+    const int tok = divide(a.div_g, r), head = r - tok * a.G;
+    at[n] = ((size_t)(j.q0 + (valid[n] ? tok : 0)) * a.Hk + j.hk) * a.G + (valid[n] ? head : 0);
+    seen[n] = valid[n] ? keys_seen(a, j, r) : 0;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const ev8 z = {};
+      q[n][ks] = valid[n] ? *reinterpret_cast<const ev8*>(a.q + at[n] * D + (D / 4) * g + 8 * ks) : z;
+    }
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[n][db] = f32x4{};
+    lsum[n] = 0.0f;
+    mrun[n] = -INFINITY;
+  }
+
+  PageWindow window;
+  const int end = min(2 * j.c1, (seen_max + 31) / 32);
+  int u = 2 * j.c0 + wv;
+  window.start(a, j, u, true);
+  typedef typename std::conditional<D == 128, uint4, uint2>::type Piece;  // a lane's codes of a group
+  Piece kc[2], vc[2];
+  unsigned ks8[2], vs8[2];
+  const int k_at = c * (D / 2) + g * (D / 8), ks_at = c * (D / 32) + (D == 128 ? g : g >> 1);
+  const int v_at = l * (D / 8), vs_at = (l >> 2) * (D / 32) + (D == 128 ? l & 3 : (l & 3) >> 1);
+  size_t at16[2];  // a run's groups: the first row in the cache
+  unsigned missing = 0, missing_next = 0;
+  auto places = [&](int u) {
+    const int slot = window.slot(a, j, u);
+    missing_next = window.missing(2 * slot, 3u);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      at16[t] = (((size_t)max(window.page(2 * slot + t), 0) * a.Hk + j.hk) << a.paged.shift) +
+                ((32 * u + 16 * t) & ((1 << a.paged.shift) - 1));
+  };
+  auto load_k = [&]() {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      kc[t] = *reinterpret_cast<const Piece*>(a.paged.codes[0] + at16[t] * (D / 2) + k_at);
+      ks8[t] = a.paged.scales[0][at16[t] * (D / 32) + ks_at];
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      vc[t] = *reinterpret_cast<const Piece*>(a.paged.codes[1] + at16[t] * (D / 2) + v_at);
+      vs8[t] = a.paged.scales[1][at16[t] * (D / 32) + vs_at];
+    }
+  };
+  char* vb = lds + wv * LDS_WAVE;
+  const int tr = tile_at<D>(4 * g + (c >> 2), (c & 3) >> 1) + (c & 1) * 8, tr16 = tile_at<D>(16 + 4 * g + (c >> 2), (c & 3) >> 1) + (c & 1) * 8;
+  if (u < end) {
+    places(u);
+    load_k();
+    load_v();
+  }
+  for (; u < end; u += 4) {
+    const bool more = u + 4 < end;
+    missing = missing_next;
+    f32x4 s[NR][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float scale = __uint_as_float(ks8[t] << 23);
+      unsigned w[WORDS];
+      __builtin_memcpy(w, &kc[t], sizeof(w));
+#pragma unroll
+      for (int n = 0; n < NR; ++n) s[n][t] = f32x4{};
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        const ev8 k = decode8(w[ks], scale);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[n][t] = emfma16(k, q[n][ks], s[n][t]);
+      }
+    }
+    // V of this run to LDS, then the next run's loads
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = 32 * u + 16 * t + (l >> 2);
+      const bool there = key < j.nk && !(missing >> t & 1);
+      const float scale = __uint_as_float((there ? vs8[t] : 127u) << 23);
+      unsigned w[WORDS];
+      __builtin_memcpy(w, &vc[t], sizeof(w));
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i)
+        *reinterpret_cast<ev8*>(vb + tile_at<D>(16 * t + (l >> 2), WORDS * (l & 3) + i)) = decode8(w[i], scale);
+    }
+    asm volatile("" ::: "memory");
+    if (more) {
+      places(u + 4);
+      load_k();
+      load_v();
+    }
+    ev8 p[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      if (missing || 32 * (u + 1) > seen_min) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int left = missing >> t & 1 ? 0 : seen[n] - 32 * u - 16 * t - 4 * g;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r >= left) s[n][t][r] = -INFINITY;
+        }
+      }
+      float mx = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
+                       fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+      mx = max_rows16(mx) * a.scale;
+      if (mx > mrun[n] + SLACK) {  // (as in Rows::raise)
+        const float next = mrun[n] == -INFINITY ? mx : mrun[n] + ceilf(mx - mrun[n]), alpha = exp2f_fast(mrun[n] - next);
+        lsum[n] *= alpha;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[n][db] *= alpha;
+        mrun[n] = next;
+      }
+      const float shift = P_SHIFT - (mrun[n] == -INFINITY ? 0.0f : mrun[n]);
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = exp2f_fast(fmaf(s[n][i >> 2][i & 3], a.scale, shift));
+      p[n] = epack8(e);
+      lsum[n] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    }
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const ev8 v = ecat_tr(lds_read_tr(vb, tr ^ (32 * db)), lds_read_tr(vb, tr16 ^ (32 * db)));
+#pragma unroll
+      for (int n = 0; n < NR; ++n) o[n][db] = emfma16(v, p[n], o[n][db]);
+    }
+    asm volatile("" ::: "memory");
+  }
+
+  // merge of the four waves' states: each wave finishes a quarter of the channels
+  static_assert(NR * NDB * 4 * 64 * 4 <= LDS_WAVE, "a wave's O fits its LDS");
+  float* mine = reinterpret_cast<float*>(vb);
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+#pragma unroll
+    for (int i = 0; i < NDB * 4; ++i) mine[(n * NDB * 4 + i) * 64 + l] = o[n][i >> 2][i & 3];
+    const float sum = sum_rows16(lsum[n]);
+    if (g == 0) {
+      stats[((wv * NR + n) * 2) * 16 + c] = mrun[n];
+      stats[((wv * NR + n) * 2 + 1) * 16 + c] = sum;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    float w[4], top = -INFINITY, tot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, stats[((i * NR + n) * 2) * 16 + c]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float m = stats[((i * NR + n) * 2) * 16 + c];
+      w[i] = m == -INFINITY ? 0.0f : exp2f_fast(m - top);
+      tot += w[i] * stats[((i * NR + n) * 2 + 1) * 16 + c];
+    }
+    const float inv = j.part != nullptr ? 1.0f : tot == 0.0f ? 0.0f : 1.0f / tot;
+    const int r = 16 * n + c;
+#pragma unroll
+    for (int x = 0; x < NDB / 4; ++x) {
+      const int db = wv * (NDB / 4) + x, col = 16 * db + 4 * g;
+      f32x4 acc = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* other = reinterpret_cast<const float*>(lds + i * LDS_WAVE);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(w[i], other[(n * NDB * 4 + 4 * db + e) * 64 + l], acc[e]);
+      }
+      if (j.part != nullptr) *reinterpret_cast<f32x4*>(j.part + 2 * j.part_rows + r * D + col) = acc;
+      else if (valid[n]) store_row<D>(a, at[n], col, acc * inv);
+    }
+    if (wv == 0 && g == 0) {
+      if (j.part != nullptr) {
+        j.part[r] = top;
+        j.part[j.part_rows + r] = tot;
+      } else if (valid[n]) {
+        a.lse[at[n]] = tot == 0.0f ? -INFINITY : (top - P_SHIFT + log2f(tot)) * PK_LN2;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ kernels
+// rows a tile of a launch: TOKENS = 16 (single tokens over 4 bits), else 64 or 128 with up to 32 rows as narrow tiles
+constexpr int TOKENS = 16;
+
+template <int D, int BITS, int M>
+__device__ __forceinline__ void paged_tile(const FwdArgs& a, const Job& j, char* lds, float* stats) {
+  if constexpr (M == TOKENS) {
+    narrow4_tile<D, 1>(a, j, lds, stats);
+  } else if constexpr (BITS == 16) {
+    run_tile<D, false, M, Pages<D>>(a, j, lds, stats, nullptr);
+  } else {
+    if (j.nq * a.G - j.r0 <= 32) narrow4_tile<D, 2>(a, j, lds, stats);
+    else wide_tile<D, false, M, Codes<D>>(a, j, lds, stats, nullptr);
+  }
+}
+
+// the job of a tile of sequence b, its keys and rows
+template <int D, int BITS>
+__device__ __forceinline__ void paged_job(const FwdArgs& a, Job& j, const Seq& s, int b, int nk, int hk) {
+  j.table = a.paged.table + (size_t)(b < a.B ? b : 0) * a.paged.max_pages;
+  if (BITS == 16) {
+    j.k = a.paged.k + (size_t)hk * a.paged.head_stride;
+    j.v = a.paged.v + (size_t)hk * a.paged.head_stride;
+  }
+  j.q0 = s.q0;
+  j.nq = s.nq;
+  j.nk = nk;
+  j.hk = hk;
+  j.causal = a.causal;
+}
+
+// LDS: wide tiles two chunks of keys and values, TOKENS a run of values a wave
+template <int D, int M>
+constexpr int paged_lds() { return M == TOKENS ? 4 * 32 * D * 2 : 4 * BK * D * 2; }
+// whole tiles: grid tiles * Hk, a tile's heads on neighbouring workgroups
+template <int D, int BITS, int M>
+__global__ __launch_bounds__(256, M == TOKENS ? 4 : D == 64 ? 3 : 2) void paged_whole_kernel(FwdArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[paged_lds<D, M>()];
+  __shared__ float stats[4 * 128];
+  const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
+  int b, t;
+  Seq s;
+  Job j;
+  if (!tile_of<M, false>(a.cu_q, nullptr, a.B, a.Tq, 0, a.G, w, s, b, t, a.lens, a.paged.cap)) return;
+  j.r0 = ((s.nq * a.G + M - 1) / M - 1 - t) * M;
+  paged_job<D, BITS>(a, j, s, b, s.nk, hk);
+  j.part = nullptr;
+  j.c0 = 0;
+  j.c1 = tile_chunks<M>(a, j);
+  paged_tile<D, BITS, M>(a, j, lds, stats);
+}
+
+// packed sequences over a paged cache: list b, the rows behind the last sequence being list B
+template <int M>
+struct PagedLists {
+  const FwdArgs& a;
+  __device__ __forceinline__ ListShape operator()(int b) const {
+    const int rows = list_rows(a.cu_q, a.B, a.Tq, a.G, b), nk = b >= a.B ? 0 : min(max(a.lens[b], 0), a.paged.cap);
+    return ListShape{(rows + M - 1) / M, (nk + BK - 1) / BK, rows};
+  }
+};
+
+// key ranges (packed_tiles.h): grid items * Hk
+template <int D, int BITS, int M>
+__global__ __launch_bounds__(256, M == TOKENS ? 4 : D == 64 ? 3 : 2) void paged_ranges_kernel(FwdArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[paged_lds<D, M>()];
+  __shared__ float stats[4 * 128];
+  const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
+  const PagedLists<M> shape{a};
+  const Lists<PagedLists<M>> lists(shape, a.B + 1);
+  const Ranges r = lists.find(a, w);
+  if (r.ranges == 0) return;
+  const Seq s = sequence(a.cu_q, nullptr, a.B, a.Tq, 0, r.list);
+  Job j;
+  paged_job<D, BITS>(a, j, s, r.list, cached_keys(a, r.list), hk);
+  take_range<M>(a, j, r, w);
+  j.part_rows = M;
+  j.part = r.ranges == 1 ? nullptr : partial<D>(a.part, M, a, w, hk);
+  paged_tile<D, BITS, M>(a, j, lds, stats);
+}
+
+}  // namespace
+
+// What a call launches: tiles of M rows, whole or cut into key ranges.
+struct PagedPlan {
+  int M, slots;  // rows a tile, workgroups that the GPU holds
+  bool ranged;
+  long long tiles, items;
+  size_t plan, bytes;  // workspace: partials, plan
+};
+
+// `cap`: the keys that a sequence can have. equal: B sequences of Tq / B tokens.
+static PagedPlan paged_plan(int B, int Tq, int cap, int H, int Hk, int D, int bits, bool equal) {
+  PagedPlan p = {};
+  const int G = H / Hk;
+  // single tokens (with running counts: no more tokens than sequences) and the like whose rows fit one tile of sixteen
+  const bool tokens = bits == 4 && (equal ? (long long)(Tq / B) * G : Tq <= B ? G : 17) <= 16;
+  p.M = tokens ? TOKENS : TILE;
+  p.slots = 256 * (tokens ? 4 : D == 64 ? 3 : 2);
+  p.tiles = tokens ? tile_numbers<TOKENS>(B, Tq, G) : tile_numbers<TILE>(B, Tq, G);
+  p.ranged = p.tiles * Hk < 2 * p.slots && cap >= 1024;
+  if (!p.ranged) return p;
+  p.items = p.tiles + p.slots / Hk + 1;
+  p.plan = (size_t)p.items * Hk * part_floats(p.M, D) * sizeof(float);
+  p.bytes = p.plan + (size_t)(B + 1) * sizeof(int2);
+  return p;
+}
+
+#ifndef ES_ELEM_F16
+extern "C" size_t es_paged_workspace(int B, int Tq, int max_pages, int page_size, int H, int Hk, int D, int bits) {
+  if (B <= 0 || Tq <= 0 || max_pages < 0 || page_size <= 0 || H <= 0 || Hk <= 0 || H % Hk || (D != 64 && D != 128)) return 0;
+  const int cap = (int)std::min<long long>((long long)max_pages * page_size, 1LL << 30);
+  const size_t a = paged_plan(B, Tq, cap, H, Hk, D, bits, false).bytes;  // (with and without running counts)
+  return std::max(a, paged_plan(B, Tq, cap, H, Hk, D, bits, true).bytes);
+}
+#endif
+
+static int paged_fwd(FwdArgs& a, const void* q, const int* pages, const int* lens, const int* cu, void* out, float* lse,
+                     void* workspace, size_t workspace_bytes, int B, int Tq, int max_pages, int num_pages, int page_size, int H,
+                     int Hk, int D, int causal, float scale, int bits, hipStream_t stream) {
+  if (int st = places_check(pages, lens, cu, B, Tq, max_pages, num_pages, page_size, Hk)) return st;
+  if (int st = packed_check(q, nullptr, nullptr, cu, lens, nullptr, nullptr, 0, 0, B, Tq, 0, H, Hk, D, scale)) return st;
+  if (Tq == 0) return ES_OK;
+  ES_REQUIRE(out && lse, ES_ERR_INVALID, "paged: null out / lse");
+  ES_REQUIRE(aligned16({q, out, workspace}), ES_ERR_INVALID, "paged: tensors must be aligned to 16 bytes");
+  a.q = (const e16_t*)q;
+  a.cu_q = cu;
+  a.out = (e16_t*)out;
+  a.lse = lse;
+  a.lens = lens;
+  a.B = B;
+  a.Tq = Tq;
+  a.H = H;
+  a.Hk = Hk;
+  a.G = H / Hk;
+  a.div_g = fast_div(a.G);
+  a.causal = causal != 0;
+  a.scale = scale * LOG2E;
+  a.paged.table = pages;
+  a.paged.max_pages = max_pages;
+  a.paged.num_pages = num_pages;
+  a.paged.shift = log2_of(page_size);
+  a.paged.cap = num_pages > 0 ? max_pages * page_size : 0;  // (without pages no sequence has keys)
+  const PagedPlan p = paged_plan(B, Tq, max_pages * page_size, H, Hk, D, bits, cu == nullptr);
+  a.tiles = (int)p.tiles;
+  ES_REQUIRE(p.tiles * Hk < MAX_GRID && p.items * Hk < MAX_GRID, ES_ERR_UNSUPPORTED, "paged: too many sequences");
+  ES_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes), ES_ERR_INVALID, "paged: workspace too small");
+  auto launch = [&](auto dim, auto bit, auto rows) {
+    constexpr int d = decltype(dim)::value, n = decltype(bit)::value, m = decltype(rows)::value;
+    if (p.ranged) {
+      a.part = (float*)workspace;
+      a.plan = (int2*)((char*)workspace + p.plan);
+      a.inv_slots = (float)Hk / (float)p.slots;
+      a.items = (int)p.items;
+      hipLaunchKernelGGL((paged_ranges_kernel<d, n, m>), dim3((unsigned)(p.items * Hk)), dim3(256), 0, stream, a);
+      const long long rows_most = std::min<long long>((long long)Tq * a.G, m);
+      hipLaunchKernelGGL((merge_kernel<d, false, m>), dim3((unsigned)(p.tiles * Hk), (unsigned)((rows_most * d / 4 + 255) / 256)),
+                         dim3(256), 0, stream, a);
+    } else {
+      hipLaunchKernelGGL((paged_whole_kernel<d, n, m>), dim3((unsigned)(p.tiles * Hk)), dim3(256), 0, stream, a);
+    }
+  };
+  using std::integral_constant;
+  auto with_rows = [&](auto dim, auto bit) {
+    if constexpr (decltype(bit)::value == 4) {
+      if (p.M == TOKENS) {
+        launch(dim, bit, integral_constant<int, TOKENS>{});
+        return;
+      }
+    }
+    launch(dim, bit, integral_constant<int, TILE>{});
+  };
+  auto with_bits = [&](auto dim) {
+    if (bits == 16) with_rows(dim, integral_constant<int, 16>{});
+    else with_rows(dim, integral_constant<int, 4>{});
+  };
+  if (D == 64) with_bits(integral_constant<int, 64>{});
+  else with_bits(integral_constant<int, 128>{});
+  return check_launch("es_paged_fwd");
+}
+
+}  // namespace es
+
+using namespace es;
+
+extern "C" int ES_VSA_API(es_paged_fwd)(const void* q, const void* k_pages, const void* v_pages, const int* pages,
+                                        const int* lens, const int* cu, void* out, float* lse, void* workspace,
+                                        size_t workspace_bytes, int B, int Tq, int max_pages, int num_pages, int page_size, int H,
+                                        int Hk, int D, int causal, float scale, long long page_stride, long long head_stride,
+                                        long long row_stride, hipStream_t stream) {
+  if (int st = cache_check(k_pages, v_pages, num_pages, page_size, Hk, D, page_stride, head_stride, row_stride)) return st;
+  FwdArgs a = {};
+  a.paged.k = (const e16_t*)k_pages;
+  a.paged.v = (const e16_t*)v_pages;
+  a.paged.page_stride = page_stride, a.paged.head_stride = head_stride, a.paged.row_stride = row_stride;
+  return paged_fwd(a, q, pages, lens, cu, out, lse, workspace, workspace_bytes, B, Tq, max_pages, num_pages, page_size, H, Hk, D,
+                   causal, scale, 16, stream);
+}
+
+extern "C" int ES_VSA_API(es_paged4_fwd)(const void* q, const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
+                                         const uint8_t* v_scales, const int* pages, const int* lens, const int* cu, void* out,
+                                         float* lse, void* workspace, size_t workspace_bytes, int B, int Tq, int max_pages,
+                                         int num_pages, int page_size, int H, int Hk, int D, int causal, float scale,
+                                         hipStream_t stream) {
+  if (int st = cache4_check(k_codes, k_scales, v_codes, v_scales, num_pages)) return st;
+  FwdArgs a = {};
+  a.paged.codes[0] = k_codes, a.paged.codes[1] = v_codes;
+  a.paged.scales[0] = k_scales, a.paged.scales[1] = v_scales;
+  return paged_fwd(a, q, pages, lens, cu, out, lse, workspace, workspace_bytes, B, Tq, max_pages, num_pages, page_size, H, Hk, D,
+                   causal, scale, 4, stream);
+}

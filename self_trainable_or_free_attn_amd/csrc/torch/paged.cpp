@@ -1,6 +1,6 @@
 // Torch operators of norms with rotation and of paged caches with their outputs, workspaces and gradient:
-// echosparse_gfx950::norm_rotate, ::append_paged and ::paged_rows, called by rotary.py and paged.py, which check the arguments
-// against the documentation.
+// echosparse_gfx950::norm_rotate, ::append_paged, ::paged_rows and ::paged_attention, called by rotary.py and paged.py, which check
+// the arguments against the documentation.
 //
 // Every operator checks what the C entry points rely on (device, dtype, layout, sizes), so a direct call cannot reach them with
 // other pointers than it names.
@@ -244,7 +244,39 @@ std::tuple<Tensor, Tensor> rows_forward(const Tensor& kp, const Tensor& vp, cons
   return {k, v};
 }
 
+std::tuple<Tensor, Tensor> attention_forward(const Tensor& q_, const Tensor& kp, const Tensor& vp, const OptTensor& ks,
+                                             const OptTensor& vs, const Tensor& pages, const Tensor& lens, const OptTensor& cu,
+                                             bool causal, double scale) {
+  const c10::OptionalDeviceGuard guard(q_.device());
+  const bool f16 = half_type(q_.scalar_type());
+  check_on("q", q_, q_);
+  TORCH_CHECK(q_.dim() == 3 && q_.is_contiguous(), "q must be a contiguous [T, heads, D] tensor");
+  const Cache c(kp, vp, ks, vs, pages, lens, cu, q_.scalar_type(), q_.size(0));
+  check_on("the cache", kp, q_);
+  TORCH_CHECK(q_.size(2) == c.D, "q and the cache do not go together");
+  const Tensor q = q_.numel() ? aligned(q_) : q_;
+  const int H = as_int(q.size(1));
+  Tensor out = at::empty_like(q), lse = at::empty({c.T, H}, q.options().dtype(at::kFloat));
+  const size_t bytes = es_paged_workspace(c.B, c.T, c.max_pages, c.page_size, H, c.Hk, c.D, c.four ? 4 : 16);
+  const Tensor ws = bytes ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : Tensor();
+  float* l = static_cast<float*>(data(lse));
+  if (c.four)
+    check_status("es_paged4_fwd", (f16 ? es_paged4_fwd_f16 : es_paged4_fwd)(
+        data(q), c.bytes(kp), c.bytes(c.ks), c.bytes(vp), c.bytes(c.vs), ints(pages), ints(lens), ints(c.cu), data(out), l, data(ws),
+        bytes, c.B, c.T, c.max_pages, c.num_pages, c.page_size, H, c.Hk, c.D, causal, static_cast<float>(scale), stream_of(q)));
+  else
+    check_status("es_paged_fwd", (f16 ? es_paged_fwd_f16 : es_paged_fwd)(
+        data(q), data(kp), data(vp), ints(pages), ints(lens), ints(c.cu), data(out), l, data(ws), bytes, c.B, c.T, c.max_pages,
+        c.num_pages, c.page_size, H, c.Hk, c.D, causal, static_cast<float>(scale), c.page_stride(), c.head_stride(), c.row_stride(),
+        stream_of(q)));
+  return {out, lse};
+}
+
 // ------------------------------------------------------------------------------------------------ shapes alone
+std::tuple<Tensor, Tensor> attention_meta(const Tensor& q, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&,
+                                          const Tensor&, const Tensor&, const OptTensor&, bool, double) {
+  return {at::empty_like(q), at::empty_symint({q.sym_size(0), q.sym_size(1)}, q.options().dtype(at::kFloat))};
+}
 std::tuple<Tensor, Tensor> rotate_meta(const Tensor& q, const Tensor& k, const OptTensor&, const OptTensor&, const OptTensor&,
                                        const OptTensor&, int64_t, bool, double) {
   return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint(k.sym_sizes(), k.options())};
@@ -379,6 +411,18 @@ std::tuple<Tensor, Tensor> rows_autograd(const Tensor& kp, const Tensor& vp, con
   return op.call(kp, vp, ks, vs, pages, lens, cu, count, dtype);
 }
 
+using AttentionSignature = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                                                      const OptTensor&, const Tensor&, const Tensor&, const OptTensor&, bool,
+                                                      double);
+std::tuple<Tensor, Tensor> attention_autograd(const Tensor& q, const Tensor& kp, const Tensor& vp, const OptTensor& ks,
+                                              const OptTensor& vs, const Tensor& pages, const Tensor& lens, const OptTensor& cu,
+                                              bool causal, double scale) {
+  static const auto op = find<AttentionSignature>("echosparse_gfx950::paged_attention");
+  refuse_derivatives("paged_attention", {{"q", q}, {"cache.k", kp}, {"cache.v", vp}});
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, kp, vp, ks, vs, pages, lens, cu, causal, scale);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(echosparse_gfx950, m) {
@@ -391,22 +435,27 @@ TORCH_LIBRARY_FRAGMENT(echosparse_gfx950, m) {
         "bool halves, float eps) -> Tensor");
   m.def("paged_rows(Tensor k_pages, Tensor v_pages, Tensor? k_scales, Tensor? v_scales, Tensor pages, Tensor lens, Tensor? cu, "
         "int rows, ScalarType dtype) -> (Tensor, Tensor)");
+  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? k_scales, Tensor? v_scales, Tensor pages, "
+        "Tensor lens, Tensor? cu, bool causal, float scale) -> (Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(echosparse_gfx950, CUDA, m) {
   m.impl("norm_rotate", TORCH_FN(rotate_forward));
   m.impl("norm_rotate_backward", TORCH_FN(rotate_backward));
   m.impl("append_paged", TORCH_FN(append_forward));
   m.impl("paged_rows", TORCH_FN(rows_forward));
+  m.impl("paged_attention", TORCH_FN(attention_forward));
 }
 TORCH_LIBRARY_IMPL(echosparse_gfx950, Meta, m) {
   m.impl("norm_rotate", TORCH_FN(rotate_meta));
   m.impl("norm_rotate_backward", TORCH_FN(rotate_backward_meta));
   m.impl("append_paged", TORCH_FN(append_meta));
   m.impl("paged_rows", TORCH_FN(rows_meta));
+  m.impl("paged_attention", TORCH_FN(attention_meta));
 }
 TORCH_LIBRARY_IMPL(echosparse_gfx950, Autograd, m) {
   m.impl("norm_rotate", TORCH_FN(rotate_autograd));
   m.impl("norm_rotate_backward", TORCH_FN(rotate_backward_autograd));
   m.impl("append_paged", TORCH_FN(append_autograd));
   m.impl("paged_rows", TORCH_FN(rows_autograd));
+  m.impl("paged_attention", TORCH_FN(attention_autograd));
 }

@@ -1,8 +1,9 @@
-"""Paged caches of keys and values in 16 or 4 bits: new tokens into one, rows back out of one
+"""Paged caches of keys and values in 16 or 4 bits: new tokens into one, their attention over it, rows back out of it
 (include/paged_hip.h; the reference has no counterpart).
 
   PagedCache, paged_cache   the tensors of a cache, and an empty one
   append_paged              new tokens' keys and values into a cache, normed and rotated on the way, with their queries
+  paged_attention           new tokens over all that the cache holds of their sequences, causal or not, grouped heads
   paged_rows                what a cache holds of its sequences' last tokens, as packed tokens
 
 Sequences grow in pages of 16 to 4096 rows that stand anywhere in the cache: `pages` [B, max_pages] names those of each
@@ -15,7 +16,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .packed import _check_gpu, _check_ints, _check_tokens, _ops
+from .packed import _check_gpu, _check_heads, _check_ints, _check_tokens, _ops, _scale
 from .rotary import _check_turn
 
 
@@ -196,3 +197,42 @@ def paged_rows(cache: PagedCache, pages: torch.Tensor, lens: torch.Tensor, cu: O
     _check_places(pages, lens, cu, size, rows, device)
     _check_gpu(cache.k)
     return _ops().paged_rows(cache.k, cache.v, cache.k_scales, cache.v_scales, pages, lens, cu, int(rows), dtype)
+
+
+def paged_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, lens: torch.Tensor, cu: Optional[torch.Tensor] = None,
+                    *, causal: bool = True, scale: Optional[float] = None, return_lse: bool = False):
+    """Attention of new tokens over a cache that holds their own keys already (`append_paged`).
+
+    q [T, H, D], H a multiple of the cache's heads, packed: sequence b has rows cu[b] to cu[b + 1] - 1 (int32 [B + 1]), without cu
+    T / B each, also as [B, n, H, D]. pages and lens as in `append_paged`: lens[b] keys, the n new tokens' own the last of them. Token
+    i sees them all, with causal those up to its position lens[b] - n + i. Single tokens, pieces of prompts and whole ones may
+    share a call. scale: 1 / sqrt(D) if None.
+
+    Keys of pages outside the cache are left out. Cache rows from lens[b] on are never used; the values in use must be finite
+    (those of a 4-bit cache within q's type), scores below 2^22 in magnitude. Values of 4 bits are used exactly as they are held.
+
+    Returns out like q, with return_lse also the natural-log LSE [T, H] ([B, n, H]) in float32; a token that sees no key, and rows
+    behind the last sequence, give zeros and -inf. The same inputs give the same bits. There is no derivative: tensors that require a
+    gradient are refused unless gradients are off."""
+    dims = q.dim()
+    if dims not in (3, 4):
+        raise ValueError(f"q must be [T, H, D] or [B, n, H, D], got {tuple(q.shape)}")
+    _check_tokens(q, ())
+    device, shape = q.device, q.shape
+    heads, size, D = _check_cache(cache, q.dtype, device, "q")
+    if shape[-1] != D:
+        raise ValueError(f"the cache holds heads of {D} channels, q has {shape[-1]}")
+    _check_heads(shape[-2], heads)
+    rows = shape[0] if dims == 3 else shape[0] * shape[1]
+    B = _check_places(pages, lens, cu, size, rows, device)
+    if dims == 4 and (cu is not None or shape[0] != B):
+        raise ValueError(f"[B, n, H, D] tensors go without cu and with {B} sequences")
+    scale = _scale(scale, D)
+    _check_gpu(q)
+    q = q.contiguous()
+    if dims == 4:
+        q = q.flatten(0, 1)
+    out, lse = _ops().paged_attention(q, cache.k, cache.v, cache.k_scales, cache.v_scales, pages, lens, cu, bool(causal), scale)
+    if dims == 4:
+        out, lse = out.view(shape), lse.view(shape[:-1])
+    return (out, lse) if return_lse else out

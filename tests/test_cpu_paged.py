@@ -8,7 +8,8 @@ import re
 import pytest
 import torch
 
-from self_trainable_or_free_attn_amd import (PagedCache, _lib, append_paged, norm_rotate, paged_cache, paged_rows, rotary_table)
+from self_trainable_or_free_attn_amd import (PagedCache, _lib, append_paged, norm_rotate, paged_attention, paged_cache, paged_rows,
+                                            rotary_table)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 BF, FP = torch.bfloat16, torch.float16
@@ -175,6 +176,34 @@ def test_paged_rows_refuses(kw, error):
         paged_rows(_c(), _i(3, 4), _i(3), **kw)
 
 
+def _attend(q=None, cache=None, pages=None, lens=None, cu=None, **kw):
+    return paged_attention(_t(6, 4, 64) if q is None else q, _c() if cache is None else cache, _i(3, 4) if pages is None else pages,
+                           _i(3) if lens is None else lens, cu, **kw)
+
+
+@pytest.mark.parametrize("kw, error", [
+    (dict(q=_t(6, 64)), ValueError), (dict(q=_t(6, 3, 64)), ValueError), (dict(q=_t(6, 0, 64)), ValueError),
+    (dict(q=_t(6, 8192, 64)), ValueError), (dict(q=_t(6, 4, 128)), ValueError), (dict(q=_t(7, 4, 64)), ValueError),
+    (dict(q=_t(6, 4, 64, dtype=FP)), TypeError), (dict(q=_t(6, 4, 64, dtype=torch.float32)), TypeError),
+    (dict(q=_t(2, 3, 4, 64)), ValueError), (dict(q=_t(3, 2, 4, 64), cu=_i(4)), ValueError),
+    (dict(pages=_t(3, 4, dtype=torch.int64)), TypeError), (dict(pages=_i(0, 4)), ValueError), (dict(lens=_i(4)), ValueError),
+    (dict(cu=_i(5)), ValueError), (dict(scale=0.0), ValueError), (dict(scale=math.inf), ValueError), (dict(scale=math.nan), ValueError),
+    (dict(cache=_c(4)._replace(v_scales=None)), ValueError), (dict(cache=_c(dim=128)), ValueError),
+    (dict(cache=PagedCache(_t(8, 2, 16, 64), _t(8, 2, 16, 64, dtype=FP))), TypeError),
+])
+def test_paged_attention_refuses(kw, error):
+    with pytest.raises(error):
+        _attend(**kw)
+
+
+def test_paged_attention_shapes():
+    for cache, dtype in ((_c(), BF), (_c(4), BF), (_c(4), FP)):
+        out, lse = _attend(q=_t(6, 4, 64, dtype=dtype), cache=cache, cu=_i(4), return_lse=True)
+        assert out.shape == (6, 4, 64) and lse.shape == (6, 4) and out.dtype == dtype and lse.dtype == torch.float32
+        out, lse = _attend(q=_t(3, 2, 6, 64, dtype=dtype), cache=cache, return_lse=True, causal=False)
+        assert out.shape == (3, 2, 6, 64) and lse.shape == (3, 2, 6)
+
+
 # ------------------------------------------------------------------ derivatives
 def test_derivatives_that_do_not_exist_are_refused():
     k = _t(6, 2, 64).requires_grad_()
@@ -186,6 +215,8 @@ def test_derivatives_that_do_not_exist_are_refused():
         _append(k_weight=_t(64).requires_grad_())
     with pytest.raises(RuntimeError, match="no backward"):
         paged_rows(PagedCache(_t(8, 2, 16, 64).requires_grad_(), _t(8, 2, 16, 64)), _i(3, 4), _i(3), rows=6)
+    with pytest.raises(RuntimeError, match="no backward"):
+        _attend(q=_t(6, 4, 64).requires_grad_())
     with pytest.raises(RuntimeError, match="table"):
         _rotate(table=_t(6, 32, 2, dtype=torch.float32).requires_grad_())
     import torch.autograd.forward_ad as fw
@@ -264,7 +295,15 @@ def test_c_cache_calls_refuse():
     append4 = dict(items[:at] + [("kc", P16), ("ks", P16), ("vc", P16), ("vs", P16)] + items[at:])
     common = [dict(B=0), dict(T=5), dict(T=-1), dict(page=24), dict(page=8), dict(page=8192), dict(max_pages=1 << 26), dict(lens=None),
               dict(pages=None), dict(D=96), dict(Hk=0), dict(num=-1), dict(max_pages=-1), dict(B=1 << 24, T=1 << 24)]
+    fwd = dict(q=P16, kp=P16, vp=P16, pages=P16, lens=P16, cu=None, out=P16, lse=P16, ws=P16, bytes=1 << 30, **CACHE, H=4, Hk=2, D=64,
+               causal=1, scale=0.1, ps=2048, hs=1024, rs=64)
+    fwd4 = dict(q=P16, kc=P16, ks=P16, vc=P16, vs=P16, pages=P16, lens=P16, cu=None, out=P16, lse=P16, ws=P16, bytes=1 << 30, **CACHE,
+                H=4, Hk=2, D=64, causal=1, scale=0.1)
+    attend = [dict(H=5), dict(H=0), dict(H=8194), dict(q=None), dict(out=None), dict(lse=None), dict(out=odd), dict(q=odd), dict(scale=0.0),
+              dict(scale=math.nan), dict(max_pages=4096, ws=None), dict(max_pages=4096, bytes=64)]
     for name, base, more in (
+            ("es_paged_fwd", fwd, attend + [dict(kp=None), dict(vp=odd), dict(rs=32)]),
+            ("es_paged4_fwd", fwd4, attend + [dict(kc=None), dict(vs=None), dict(ks=odd)]),
             ("es_paged_rows", rows, [dict(kp=None), dict(vp=odd), dict(rs=60), dict(rs=32), dict(hs=-8), dict(ps=4), dict(k=None),
                                      dict(v=odd), dict(rs=1 << 30)]),
             ("es_paged_rows4", rows4, [dict(kc=None), dict(vs=None), dict(ks=odd), dict(k=None)]),
@@ -276,7 +315,7 @@ def test_c_cache_calls_refuse():
             for suffix in ("", "_f16"):
                 assert _call(name + suffix, change, base) in (1, 2), (name, change)
     # nothing to do: no launch, no error
-    for name, base in (("es_paged_rows", rows), ("es_paged_rows4", rows4), ("es_append_paged", append), ("es_append_paged4", append4)):
+    for name, base in (("es_paged_fwd", fwd), ("es_paged4_fwd", fwd4), ("es_paged_rows", rows), ("es_paged_rows4", rows4), ("es_append_paged", append), ("es_append_paged4", append4)):
         assert _call(name, dict(T=0), base) == 0
 
 
