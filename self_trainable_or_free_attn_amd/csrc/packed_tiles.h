@@ -66,6 +66,9 @@ struct FwdArgs {
   int n, P, S;
   int part_rows;  // rows of a sequence's partial
   PagedArgs paged;
+  // paged caches (paged_fwd.hip): shares of a head, the least cost of one, units of cost a chunk
+  int shares, least_share;
+  float cost_unit;
 };
 
 // What one workgroup computes: the tile from row r0 on of the list of nq * G rows that starts at token q0, against key rows
@@ -542,27 +545,38 @@ struct Reciprocal {
 };
 __device__ __forceinline__ Cut cut(const ListShape& x, float per) { return Cut(x.tiles, x.chunks, x.rows, per, Reciprocal()); }
 
-// The shapes of the lists, a lane each; up to 64 are read once.
-template <class F>
+// The shapes of the lists, K one behind the other a lane; up to 64 K are read once.
+template <class F, int K = 1>
 struct Lists {
   const F& shape;
   int lists;
-  ListShape mine;
-  __device__ __forceinline__ Lists(const F& f, int n) : shape(f), lists(n), mine{0, 0, 0} {
-    if (lane_id() < n) mine = f(lane_id());
+  ListShape mine[K];
+  __device__ __forceinline__ Lists(const F& f, int n) : shape(f), lists(n) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      mine[k] = ListShape{0, 0, 0};
+      if (lane_id() * K + k < n) mine[k] = f(lane_id() * K + k);
+    }
   }
-  __device__ __forceinline__ ListShape at(int i0) const {
-    if (i0 == 0) return mine;
-    return i0 + lane_id() < lists ? shape(i0 + lane_id()) : ListShape{0, 0, 0};
+  __device__ __forceinline__ ListShape at(int i0, int k) const {
+    if (i0 == 0) return mine[k];
+    const int i = i0 + lane_id() * K + k;
+    return i < lists ? shape(i) : ListShape{0, 0, 0};
   }
 
   // `per`, and the longest item's chunks. (Sums in float32: every wave computes the same ones.)
   __device__ __forceinline__ float range_chunks(const FwdArgs& a, float& longest_item) const {
     float sum = 0.0f, most = 0.0f;
-    for (int i0 = 0; i0 < lists; i0 += 64) {
-      const ListShape x = at(i0);
-      sum += wave_sum_dpp((float)x.tiles * (float)x.chunks);
-      most = fmaxf(most, wave_max_dpp(x.tiles > 0 ? (float)x.chunks : 0.0f));
+    for (int i0 = 0; i0 < lists; i0 += 64 * K) {
+      float s = 0.0f, m = 0.0f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const ListShape x = at(i0, k);
+        s += (float)x.tiles * (float)x.chunks;
+        m = fmaxf(m, x.tiles > 0 ? (float)x.chunks : 0.0f);
+      }
+      sum += wave_sum_dpp(s);
+      most = fmaxf(most, wave_max_dpp(m));
     }
     const float fair = fair_share(sum, a.inv_slots);
     const int near = (int)parts(most, __builtin_amdgcn_rcpf(fair));
@@ -571,13 +585,24 @@ struct Lists {
     for (int n = max(near - 2, 1); n <= near; ++n) {
       const float per = fmaxf(parts(most, __builtin_amdgcn_rcpf((float)n)), fair);
       float size = 0.0f, big = 0.0f, work = 0.0f;
-      for (int i0 = 0; i0 < lists; i0 += 64) size = fmaxf(size, wave_max_dpp(cut(at(i0), per).size));
-      for (int i0 = 0; i0 < lists; i0 += 64) {
-        const ListShape x = at(i0);
-        const Cut c = cut(x, per);
-        const float items = (float)x.tiles * c.ranges;
-        big += wave_sum_dpp(2.0f * c.size > size ? items : 0.0f);
-        work += wave_sum_dpp(items * c.size);
+      for (int i0 = 0; i0 < lists; i0 += 64 * K) {
+        float m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) m = fmaxf(m, cut(at(i0, k), per).size);
+        size = fmaxf(size, wave_max_dpp(m));
+      }
+      for (int i0 = 0; i0 < lists; i0 += 64 * K) {
+        float s = 0.0f, m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const ListShape x = at(i0, k);
+          const Cut c = cut(x, per);
+          const float items = (float)x.tiles * c.ranges;
+          m += 2.0f * c.size > size ? items : 0.0f;
+          s += items * c.size;
+        }
+        big += wave_sum_dpp(m);
+        work += wave_sum_dpp(s);
       }
       const float time = fmaxf(ceilf(big * a.inv_slots) * size, work * a.inv_slots);
       if (time < 0.98f * least) {  // (more ranges for a shorter schedule only)
@@ -596,19 +621,34 @@ struct Lists {
     const bool leave = blockIdx.x == 0 && threadIdx.x < 64;
     int first = 0;
     Ranges found = {0, 0, 0};
-    for (int i0 = 0; i0 < lists; i0 += 64) {
-      const ListShape x = at(i0);
-      const Cut c = cut(x, per);
-      const int i = i0 + lane_id(), ranges = (int)c.ranges, items = i < lists ? x.tiles * ranges : 0;
-      const bool late = lists <= 64 && 2.0f * c.size <= longest;
-      const int early_upto = wave_scan(late ? 0 : items), early = __builtin_amdgcn_readlane(early_upto, 63);
-      const int late_upto = wave_scan(late ? items : 0);
-      const int item0 = first + (late ? early + late_upto : early_upto) - items;
-      if (leave && i < lists) a.plan[i] = make_int2(ranges, item0);
-      const unsigned long long hit = __builtin_amdgcn_ballot_w64(item0 <= w && w < item0 + items);
+    for (int i0 = 0; i0 < lists; i0 += 64 * K) {
+      int ranges[K], items[K], early_items = 0, late_items = 0;
+      bool late[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const ListShape x = at(i0, k);
+        const Cut c = cut(x, per);
+        ranges[k] = (int)c.ranges;
+        items[k] = i0 + lane_id() * K + k < lists ? x.tiles * ranges[k] : 0;
+        late[k] = lists <= 64 * K && 2.0f * c.size <= longest;
+        (late[k] ? late_items : early_items) += items[k];
+      }
+      const int early_upto = wave_scan(early_items), early = __builtin_amdgcn_readlane(early_upto, 63);
+      const int late_upto = wave_scan(late_items);
+      int next_early = first + early_upto - early_items, next_late = first + early + late_upto - late_items;
+      int list = -1, list_ranges = 0, list_item0 = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int i = i0 + lane_id() * K + k, item0 = late[k] ? next_late : next_early;
+        (late[k] ? next_late : next_early) += items[k];
+        if (leave && i < lists) a.plan[i] = make_int2(ranges[k], item0);
+        if (item0 <= w && w < item0 + items[k]) list = i, list_ranges = ranges[k], list_item0 = item0;
+      }
+      const unsigned long long hit = __builtin_amdgcn_ballot_w64(list >= 0);
       if (hit) {
         const int from = __builtin_ctzll(hit);
-        found = Ranges{i0 + from, __builtin_amdgcn_readlane(ranges, from), __builtin_amdgcn_readlane(item0, from)};
+        found = Ranges{__builtin_amdgcn_readlane(list, from), __builtin_amdgcn_readlane(list_ranges, from),
+                       __builtin_amdgcn_readlane(list_item0, from)};
         if (!leave) break;
       }
       first += early + __builtin_amdgcn_readlane(late_upto, 63);
@@ -639,14 +679,17 @@ struct SharedLists {
   }
 };
 
-// item w of a list: its job's tile (of M rows) and chunks
-template <int M = TILE>
-__device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Ranges& r, int w) {
-  const int i = w - r.item0, range = i % r.ranges;
-  j.r0 = i / r.ranges * M;
-  const int chunks = tile_chunks<M>(a, j);
+// item w of a list: its job's tile and chunks. LAST_FIRST: the list's last tiles first, which see the most keys under a causal mask
+// (partials stay in the order of the tiles); returns the partial's number.
+template <bool LAST_FIRST = false>
+__device__ __forceinline__ int take_range(const FwdArgs& a, Job& j, const Ranges& r, int w) {
+  const int i = w - r.item0, range = i % r.ranges, tiles = (j.nq * a.G + TILE - 1) / TILE;
+  const int tile = LAST_FIRST ? tiles - 1 - i / r.ranges : i / r.ranges;
+  j.r0 = tile * TILE;
+  const int chunks = tile_chunks<TILE>(a, j);
   j.c0 = range_begin(chunks, range, r.ranges);
   j.c1 = range_begin(chunks, range + 1, r.ranges);
+  return r.item0 + tile * r.ranges + range;
 }
 
 // Partial `item` of a launch, all kv heads of an item side by side. Shared prefix: the prefix's items have a part of their own,
@@ -661,7 +704,7 @@ __device__ __forceinline__ float* partial(float* base, int rows, const FwdArgs& 
 // O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's partials in order: D / 4 lanes a row, which first take one
 // partial's m and l each and then, eight partials in flight, four channels each. SHARED: a row's prefix partials, then those
 // of its own cache. Grid: (tile numbers * Hk, merge_rows). Latency bound: 4 to 12 us.
-template <int D, bool SHARED, int M = TILE>
+template <int D, bool SHARED>
 __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
   constexpr int LPR = D / 4, RPB = 256 / LPR;
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
@@ -677,19 +720,19 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
     own = planned(a, list);
     pre = planned(a, 0);
   } else {
-    list = seq_of_tile<M>(a.cu_q, a.B, a.Tq, a.G, w);
+    list = seq_of_tile<TILE>(a.cu_q, a.B, a.Tq, a.G, w);
     const Seq s = sequence(a.cu_q, a.cu_k, a.B, a.Tq, a.Tk, list);
     q0 = s.q0;
     nq = s.nq;
-    t = w - first_tile<M>(q0, a.G, list);
-    if (t < 0 || t * M + (int)blockIdx.y * RPB >= nq * a.G) return;
+    t = w - first_tile<TILE>(q0, a.G, list);
+    if (t < 0 || t * TILE + (int)blockIdx.y * RPB >= nq * a.G) return;
     own = planned(a, list);
     if (own.ranges == 1) return;  // (finished by its only range)
   }
-  const int rows = min(nq * a.G - t * M, M), lane = threadIdx.x % LPR, c = lane * 4, n = pre.ranges + own.ranges;
-  const int own_rows = SHARED ? a.part_rows : M;
+  const int rows = min(nq * a.G - t * TILE, TILE), lane = threadIdx.x % LPR, c = lane * 4, n = pre.ranges + own.ranges;
+  const int own_rows = SHARED ? a.part_rows : TILE;
   for (int r = blockIdx.y * RPB + threadIdx.x / LPR; r < rows; r += gridDim.y * RPB) {
-    const int all = q0 * a.G + t * M + r, rp = SHARED ? all % TILE : 0;  // the row among all rows of the batch
+    const int all = q0 * a.G + t * TILE + r, rp = SHARED ? all % TILE : 0;  // the row among all rows of the batch
     // a row's partial i: m at [row], l at [rows + row], O behind them
     auto part = [&](int i, int& stored, int& row) -> const float* {
       const bool p = SHARED && i < pre.ranges;
@@ -699,14 +742,14 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
                : partial<D>(a.part, own_rows, a, own.item0 + t * own.ranges + i - pre.ranges, hk);
     };
     int stored, row;
-    float top = -INFINITY;
+    float M = -INFINITY;
     for (int i = lane; i < n; i += LPR) {
       const float* p = part(i, stored, row);
-      top = fmaxf(top, p[row]);
+      M = fmaxf(M, p[row]);
     }
 #pragma unroll
-    for (int m = LPR / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-    const float msub = top == -INFINITY ? 0.0f : top;
+    for (int m = LPR / 2; m >= 1; m >>= 1) M = fmaxf(M, __shfl_xor(M, m, 64));
+    const float msub = M == -INFINITY ? 0.0f : M;
     f32x4 acc = {};
     float sum = 0.0f;
     for (int i0 = 0; i0 < n; i0 += LPR) {
@@ -732,10 +775,10 @@ __global__ __launch_bounds__(256) void merge_kernel(FwdArgs a) {
         }
       }
     }
-    const int lrow = t * M + r, tok = divide(a.div_g, lrow);
+    const int lrow = t * TILE + r, tok = divide(a.div_g, lrow);
     const size_t at = ((size_t)(q0 + tok) * a.Hk + hk) * a.G + (lrow - tok * a.G);
     store_row<D>(a, at, c, acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
-    if (c == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top - P_SHIFT + log2f(sum)) * PK_LN2;
+    if (c == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (M - P_SHIFT + log2f(sum)) * PK_LN2;
   }
 }
 

@@ -397,15 +397,19 @@ __device__ __forceinline__ void narrow4_tile(const FwdArgs& a, const Job& j, cha
 }
 
 // ------------------------------------------------------------------------------------------------ kernels
-// rows a tile of a launch: TOKENS = 16 (single tokens over 4 bits), else 64 or 128 with up to 32 rows as narrow tiles
-constexpr int TOKENS = 16;
+// Rows a tile of a launch: TOKENS, up to sixteen (4 bits) or 32 (16 bits) rows, which are narrow tiles, or 128 (64), of which those
+// with up to 32 rows are.
+template <int BITS>
+constexpr int TOKENS = BITS == 4 ? 16 : 32;
 
 template <int D, int BITS, int M>
 __device__ __forceinline__ void paged_tile(const FwdArgs& a, const Job& j, char* lds, float* stats) {
-  if constexpr (M == TOKENS) {
-    narrow4_tile<D, 1>(a, j, lds, stats);
+  if constexpr (BITS == 16 && M == TOKENS<16>) {
+    narrow_tile<D, false, Pages<D>>(a, j, lds, stats, nullptr);
   } else if constexpr (BITS == 16) {
     run_tile<D, false, M, Pages<D>>(a, j, lds, stats, nullptr);
+  } else if constexpr (M == TOKENS<4>) {
+    narrow4_tile<D, 1>(a, j, lds, stats);
   } else {
     if (j.nq * a.G - j.r0 <= 32) narrow4_tile<D, 2>(a, j, lds, stats);
     else wide_tile<D, false, M, Codes<D>>(a, j, lds, stats, nullptr);
@@ -427,12 +431,16 @@ __device__ __forceinline__ void paged_job(const FwdArgs& a, Job& j, const Seq& s
   j.causal = a.causal;
 }
 
-// LDS: wide tiles two chunks of keys and values, TOKENS a run of values a wave
+// LDS: two chunks (16 bits, narrow: a run a wave) of keys and values; 4 bits, TOKENS: a run of values a wave
 template <int D, int M>
-constexpr int paged_lds() { return M == TOKENS ? 4 * 32 * D * 2 : 4 * BK * D * 2; }
+constexpr int paged_lds() { return M == TOKENS<4> ? 4 * 32 * D * 2 : 4 * BK * D * 2; }
+// Workgroups that a CU holds. (TOKENS over 4 bits: 163 registers; at 128, for four, the loop reloads spilled ones, and 48 tokens
+// against 8000 keys, 32 heads over 8, take 107 us instead of 88.)
+#define ES_PAGED_RESIDENT(D, M) ((M) == 16 || (D) == 64 ? 3 : 2)
+
 // whole tiles: grid tiles * Hk, a tile's heads on neighbouring workgroups
 template <int D, int BITS, int M>
-__global__ __launch_bounds__(256, M == TOKENS ? 4 : D == 64 ? 3 : 2) void paged_whole_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_whole_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[paged_lds<D, M>()];
   __shared__ float stats[4 * 128];
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
@@ -448,59 +456,319 @@ __global__ __launch_bounds__(256, M == TOKENS ? 4 : D == 64 ? 3 : 2) void paged_
   paged_tile<D, BITS, M>(a, j, lds, stats);
 }
 
-// packed sequences over a paged cache: list b, the rows behind the last sequence being list B
+// ------------------------------------------------------------------------------------------------ tokens: equal shares
+// Launches of narrow tiles are bound by HBM, and a workgroup reads keys as fast as any other: all tiles of a head, sequence by
+// sequence, laid end to end by the chunks that they read, are cut into as many equal shares as the GPU holds workgroups. Each
+// workgroup does its share: the rest of a tile, whole tiles, the beginning of a tile. Whole tiles are finished by it, pieces leave
+// partials (two a share at most) that a second launch adds in order. So one long history among short ones takes what it costs and
+// not the time of one workgroup (200 tokens against 1 to 40000 keys, 32 heads over 8: 16 bits 766 us whole tiles, 704 key ranges,
+// 561 shares; 4 bits 468, 256, 178).
+// Every wave derives its share's borders from the lengths by itself, so they stay on the device: costs are whole numbers (units of
+// 1 / cost_unit chunks, TILE_COST more for a tile's beginning and end), and a border is a function of its place alone, so all waves
+// agree on it. A border near a tile's own (SNAP of a share) moves there, which saves a partial; where all tiles are about as long
+// as a share or shorter and no share needs more than one, all of them do. A lane has LISTS sequences one behind the other, so up to
+// 255 are read once.
+struct Share {
+  int tile, chunk;  // tile number as in packed.h (first_tile of its sequence and its place there), chunk within it
+};
+constexpr int END = 0x7fffffff;
+constexpr int LISTS = 4;
+constexpr float TILE_COST = 2.0f, SNAP = 0.1f, WHOLE = 1.3f;
+
+// rows and keys of sequence b (b == B: the rows behind the last one, without keys)
+__device__ __forceinline__ int paged_rows_of(const FwdArgs& a, int b) { return list_rows(a.cu_q, a.B, a.Tq, a.G, b); }
+__device__ __forceinline__ int paged_keys_of(const FwdArgs& a, int b) {
+  return b >= a.B ? 0 : min(max(a.lens[min(b, a.B - 1)], 0), a.paged.cap);
+}
+
 template <int M>
-struct PagedLists {
+struct Shares {
   const FwdArgs& a;
-  __device__ __forceinline__ ListShape operator()(int b) const {
-    const int rows = list_rows(a.cu_q, a.B, a.Tq, a.G, b), nk = b >= a.B ? 0 : min(max(a.lens[b], 0), a.paged.cap);
-    return ListShape{(rows + M - 1) / M, (nk + BK - 1) / BK, rows};
+  int mine[LISTS], upto, from;  // of the first 64 * LISTS sequences: costs of this lane's, their sum with and without them
+  int share, count;             // cost of a share; shares
+  bool whole;                   // no tile is cut
+
+  // a tile's cost, and the tiles, of sequence b. (Causal tiles of more rows than one tile has count as if they saw all keys: these
+  // are sequences of several tiles, which launches of tokens rarely have.)
+  __device__ __forceinline__ int cost(int b, int& tiles) const {
+    if (b > a.B) return tiles = 0;
+    tiles = (paged_rows_of(a, b) + M - 1) / M;
+    return max((int)(((float)((paged_keys_of(a, b) + BK - 1) / BK) + TILE_COST) * a.cost_unit), 1);
+  }
+
+  __device__ __forceinline__ Shares(const FwdArgs& args) : a(args) {
+    int total = 0, all_tiles = 0;
+    float most = 0.0f;
+    for (int b0 = 0; b0 <= a.B; b0 += 64 * LISTS) {
+      int x[LISTS], sum = 0;
+#pragma unroll
+      for (int k = 0; k < LISTS; ++k) {
+        int tiles;
+        const int each = cost(b0 + lane_id() * LISTS + k, tiles);
+        x[k] = each * tiles;
+        most = fmaxf(most, tiles > 0 ? (float)each : 0.0f);
+        all_tiles += tiles;
+        sum += x[k];
+      }
+      const int scan = total + wave_scan(sum);
+      if (b0 == 0) {
+#pragma unroll
+        for (int k = 0; k < LISTS; ++k) mine[k] = x[k];
+        upto = scan;
+        from = scan - sum;
+      }
+      total = __builtin_amdgcn_readlane(scan, 63);
+    }
+    most = wave_max_dpp(most);
+    share = max((total + a.shares - 1) / a.shares, a.least_share);
+    count = total > 0 ? (total + share - 1) / share : 1;
+    whole = most <= WHOLE * (float)share && __builtin_amdgcn_readlane(wave_scan(all_tiles), 63) <= a.shares;
+  }
+
+  // the border in front of share w, its sequence and place there
+  __device__ __forceinline__ Share border(int w, int& seq, int& place) const {
+    seq = place = 0;
+    if (w <= 0) return Share{first_tile<M>(0, a.G, 0), 0};
+    if (w >= count) return Share{END, 0};
+    const int x = w * share;
+    int lane_from = from, lane_upto = upto, y = 0, front = 0, tiles;
+    int each[LISTS];
+#pragma unroll
+    for (int k = 0; k < LISTS; ++k) each[k] = mine[k];
+    for (int b0 = 0; b0 <= a.B; b0 += 64 * LISTS) {
+      if (b0 > 0) {
+        int sum = 0;
+#pragma unroll
+        for (int k = 0; k < LISTS; ++k) {
+          each[k] = cost(b0 + lane_id() * LISTS + k, tiles);
+          each[k] *= tiles;
+          sum += each[k];
+        }
+        lane_upto = front + wave_scan(sum);
+        lane_from = lane_upto - sum;
+      }
+      const unsigned long long past = __builtin_amdgcn_ballot_w64(lane_upto > x);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        int at = lane_from, k = 0;  // the lane's sequence that x falls into
+#pragma unroll
+        for (int i = 0; i < LISTS - 1; ++i)
+          if (k == i && at + each[i] <= x) {
+            at += each[i];
+            k = i + 1;
+          }
+        seq = b0 + l * LISTS + __builtin_amdgcn_readlane(k, l);
+        y = x - __builtin_amdgcn_readlane(at, l);
+        break;
+      }
+      front = __builtin_amdgcn_readlane(lane_upto, 63);
+    }
+    const int tile_cost = cost(seq, tiles);
+    place = min(y / tile_cost, tiles - 1);
+    y -= place * tile_cost;
+    const int number = first_tile<M>(seq_start(a.cu_q, seq, a.B, a.Tq), a.G, seq) + place;
+    const float snap = SNAP * (float)share;
+    if (whole ? 2 * y <= tile_cost : (float)y < snap) return Share{number, 0};
+    if (whole || (float)(tile_cost - y) < snap) {
+      ++place;
+      return Share{number + 1, 0};
+    }
+    const int rows = paged_rows_of(a, seq), nk = paged_keys_of(a, seq), nq = divide(a.div_g, rows);
+    const int last = min((place + 1) * M, rows) - 1;
+    const int seen = a.causal ? min(max(divide(a.div_g, last) + 1 + nk - nq, 0), nk) : nk;
+    const int chunks = (seen + BK - 1) / BK;
+    return Share{number, max(min((int)((float)y / (float)tile_cost * (float)chunks), chunks - 1), 0)};
   }
 };
 
-// key ranges (packed_tiles.h): grid items * Hk
+// grid: shares * Hk, a share's heads on neighbouring workgroups (workgroup i runs on XCD i % 8: with eight kv heads each XCD's L2
+// then holds one head's keys)
 template <int D, int BITS, int M>
-__global__ __launch_bounds__(256, M == TOKENS ? 4 : D == 64 ? 3 : 2) void paged_ranges_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_shares_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[paged_lds<D, M>()];
   __shared__ float stats[4 * 128];
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
-  const PagedLists<M> shape{a};
-  const Lists<PagedLists<M>> lists(shape, a.B + 1);
+  const Shares<M> shares(a);
+  int seq, place, other_seq, other_place;
+  const Share from = shares.border(w, seq, place), to = shares.border(w + 1, other_seq, other_place);
+  if (hk == 0 && threadIdx.x == 0) {
+    int4* borders = reinterpret_cast<int4*>(a.plan);
+    borders[w] = make_int4(from.tile, from.chunk, seq, place);
+    if (w == a.shares - 1) borders[w + 1] = make_int4(END, 0, 0, 0);
+  }
+  int tile = __builtin_amdgcn_readfirstlane(from.tile), chunk = __builtin_amdgcn_readfirstlane(from.chunk);
+  const int last_tile = __builtin_amdgcn_readfirstlane(to.tile), last_chunk = __builtin_amdgcn_readfirstlane(to.chunk);
+  if (tile == END) return;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  place = __builtin_amdgcn_readfirstlane(place);
+  while (seq <= a.B && (tile < last_tile || (tile == last_tile && chunk < last_chunk))) {
+    const Seq s = sequence(a.cu_q, nullptr, a.B, a.Tq, 0, seq);
+    if (place * M >= s.nq * a.G) {
+      ++seq;
+      place = chunk = 0;
+      if (seq <= a.B) tile = first_tile<M>(__builtin_amdgcn_readfirstlane(seq_start(a.cu_q, seq, a.B, a.Tq)), a.G, seq);
+      continue;
+    }
+    Job j;
+    paged_job<D, BITS>(a, j, s, seq, cached_keys(a, seq), hk);
+    j.r0 = place * M;
+    const int chunks = tile_chunks<M>(a, j);
+    j.c0 = min(chunk, chunks);
+    j.c1 = tile == last_tile ? min(last_chunk, chunks) : chunks;
+    j.part_rows = M;
+    j.part = j.c0 == 0 && j.c1 == chunks ? nullptr : partial<D>(a.part, M, a, 2 * w + (j.c0 == 0), hk);
+    if (j.part == nullptr || j.c0 < j.c1) {
+      paged_tile<D, BITS, M>(a, j, lds, stats);
+      __syncthreads();
+    }
+    ++place;
+    ++tile;
+    chunk = 0;
+  }
+}
+
+// O of tiles that were cut: sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over the pieces. D / 4 lanes a row and piece, SIDE pieces
+// of a row side by side (one after the other 75600 keys, a half of the shares, took 8 us), whose sums are added in order. Grid:
+// (borders * Hk, rows of a tile / rows of a workgroup): the first border within a tile has it merged, so the launch does not grow
+// with the sequences, most of whose tiles are whole.
+template <int D, int M>
+__global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
+  constexpr int LPR = D / 4, SIDE = 4, RPB = 256 / (LPR * SIDE);
+  const int w = blockIdx.x / a.Hk + 1, hk = blockIdx.x - (w - 1) * a.Hk;
+  const int4* borders = reinterpret_cast<const int4*>(a.plan);
+  const int4 here = borders[w], before = borders[w - 1];
+  if (here.y == 0 || (before.x == here.x && before.y > 0)) return;
+  const int seq = __builtin_amdgcn_readfirstlane(here.z), t = __builtin_amdgcn_readfirstlane(here.w), r0 = blockIdx.y * RPB;
+  const Seq s = sequence(a.cu_q, nullptr, a.B, a.Tq, 0, seq);
+  const int rows = min(s.nq * a.G - t * M, M);
+  if (r0 >= rows) return;
+  // the shares that have a piece of it, in order: the one before the border the beginning, in its second slot, the others in their
+  // first; two borders may stand at one place
+  __shared__ int pieces[256 * ES_PAGED_RESIDENT(D, M) + 1];
+  if (threadIdx.x == 0) pieces[0] = w - 1;
+  int n = 1;
+  for (int i0 = w; i0 < a.shares; i0 += 64) {
+    const int i = i0 + lane_id();
+    const int4 x = borders[min(i, a.shares)], y = borders[min(i + 1, a.shares)];
+    const bool within = i < a.shares && x.x == here.x, mine = within && (y.x != x.x || y.y > x.y);
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(mine);
+    if (mine && threadIdx.x < 64) pieces[n + __builtin_popcountll(hit & ((1ull << lane_id()) - 1))] = i;
+    n += __builtin_popcountll(hit);
+    if (!__builtin_amdgcn_readlane((int)within, 63)) break;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x % LPR, c = lane * 4, side = threadIdx.x / LPR % SIDE, local = threadIdx.x / (LPR * SIDE);
+  const int r = min(r0 + local, rows - 1);
+  auto part = [&](int i) { return partial<D>(a.part, M, a, 2 * pieces[i] + (i == 0), hk); };
+  float top = -INFINITY;
+  for (int i = lane; i < n; i += LPR) top = fmaxf(top, part(i)[r]);
+#pragma unroll
+  for (int m = LPR / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  const float msub = top == -INFINITY ? 0.0f : top;
+  f32x4 acc = {};
+  float sum = 0.0f;
+  for (int i = side; i < n; i += 4 * SIDE) {  // (four pieces in flight)
+    f32x4 x[4];
+    float f[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool in = i + e * SIDE < n;
+      const float* p = part(in ? i + e * SIDE : i);
+      x[e] = *reinterpret_cast<const f32x4*>(p + 2 * M + r * D + c);
+      f[e] = in ? exp2f_fast(p[r] - msub) : 0.0f;
+      l[e] = p[M + r];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc += f[e] * x[e];
+      sum = fmaf(f[e], l[e], sum);
+    }
+  }
+  __shared__ f32x4 sums[SIDE][RPB][LPR];
+  __shared__ float weights[SIDE][RPB];
+  sums[side][local][lane] = acc;
+  if (lane == 0) weights[side][local] = sum;
+  __syncthreads();
+  if (side != 0 || r0 + local >= rows) return;
+#pragma unroll
+  for (int i = 1; i < SIDE; ++i) {
+    acc += sums[i][local][lane];
+    sum += weights[i][local];
+  }
+  const int row = t * M + r, tok = divide(a.div_g, row);
+  const size_t at = ((size_t)(s.q0 + tok) * a.Hk + hk) * a.G + (row - tok * a.G);
+  store_row<D>(a, at, c, acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
+  if (c == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top - P_SHIFT + log2f(sum)) * PK_LN2;
+}
+
+// ------------------------------------------------------------------------------------------------ wide tiles: key ranges
+// Launches with wide tiles are bound by the matrix units, and tiles that read the same keys side by side have them from L2: these
+// are cut into ranges as in packed_tiles.h, the last tiles of a sequence first. (Equal shares, whose pieces start anywhere: 4096
+// tokens of 32 heads over 8 alone 228 us, ranges 168; 32760 of 24 heads 7100 and 6480, whole tiles 6170. 4096 tokens beside one that
+// sees 75600 keys: whole tiles 572, ranges 224.) List i: the rows of sequence i, list B: those behind the last one.
+struct PagedLists {
+  const FwdArgs& a;
+  __device__ __forceinline__ ListShape operator()(int b) const {
+    const int rows = paged_rows_of(a, b), nk = paged_keys_of(a, b);
+    return ListShape{(rows + TILE - 1) / TILE, (nk + BK - 1) / BK, rows};
+  }
+};
+
+// grid: items * Hk
+template <int D, int BITS>
+__global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, TILE)) void paged_ranges_kernel(FwdArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[paged_lds<D, TILE>()];
+  __shared__ float stats[4 * 128];
+  const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
+  const PagedLists shape{a};
+  const Lists<PagedLists, LISTS> lists(shape, a.B + 1);
   const Ranges r = lists.find(a, w);
   if (r.ranges == 0) return;
   const Seq s = sequence(a.cu_q, nullptr, a.B, a.Tq, 0, r.list);
   Job j;
   paged_job<D, BITS>(a, j, s, r.list, cached_keys(a, r.list), hk);
-  take_range<M>(a, j, r, w);
-  j.part_rows = M;
-  j.part = r.ranges == 1 ? nullptr : partial<D>(a.part, M, a, w, hk);
-  paged_tile<D, BITS, M>(a, j, lds, stats);
+  const int number = take_range<true>(a, j, r, w);
+  j.part_rows = TILE;
+  j.part = r.ranges == 1 ? nullptr : partial<D>(a.part, TILE, a, number, hk);
+  paged_tile<D, BITS, TILE>(a, j, lds, stats);
 }
 
 }  // namespace
 
-// What a call launches: tiles of M rows, whole or cut into key ranges.
+// What a call launches.
+enum PagedForm { WHOLE_TILES, SHARES, RANGES };
 struct PagedPlan {
-  int M, slots;  // rows a tile, workgroups that the GPU holds
-  bool ranged;
-  long long tiles, items;
-  size_t plan, bytes;  // workspace: partials, plan
+  PagedForm form;
+  int M;               // rows a tile
+  long long tiles;     // tile numbers of a head
+  int shares, items;   // a head: SHARES, RANGES
+  size_t plan, bytes;  // workspace: partials, then borders (SHARES) or ranges (RANGES)
 };
 
-// `cap`: the keys that a sequence can have. equal: B sequences of Tq / B tokens.
+// `cap`: the keys that a sequence can have. equal: B sequences of Tq / B tokens. Up to 1024 keys a tile is short enough for one
+// workgroup, and a second launch would take as long again.
 static PagedPlan paged_plan(int B, int Tq, int cap, int H, int Hk, int D, int bits, bool equal) {
   PagedPlan p = {};
-  const int G = H / Hk;
-  // single tokens (with running counts: no more tokens than sequences) and the like whose rows fit one tile of sixteen
-  const bool tokens = bits == 4 && (equal ? (long long)(Tq / B) * G : Tq <= B ? G : 17) <= 16;
-  p.M = tokens ? TOKENS : TILE;
-  p.slots = 256 * (tokens ? 4 : D == 64 ? 3 : 2);
-  p.tiles = tokens ? tile_numbers<TOKENS>(B, Tq, G) : tile_numbers<TILE>(B, Tq, G);
-  p.ranged = p.tiles * Hk < 2 * p.slots && cap >= 1024;
-  if (!p.ranged) return p;
-  p.items = p.tiles + p.slots / Hk + 1;
-  p.plan = (size_t)p.items * Hk * part_floats(p.M, D) * sizeof(float);
-  p.bytes = p.plan + (size_t)(B + 1) * sizeof(int2);
+  const int G = H / Hk, narrow = bits == 4 ? TOKENS<4> : TOKENS<16>;
+  // single tokens (with running counts: no more tokens than sequences) and the like whose rows fit a narrow tile
+  const bool tokens = (equal ? (long long)(Tq / B) * G : Tq <= B ? G : narrow + 1) <= narrow;
+  p.M = tokens ? narrow : TILE;
+  p.tiles = !tokens ? tile_numbers<TILE>(B, Tq, G) : bits == 4 ? tile_numbers<TOKENS<4>>(B, Tq, G) : tile_numbers<TOKENS<16>>(B, Tq, G);
+  p.form = cap <= 1024 ? WHOLE_TILES : tokens ? SHARES : RANGES;
+  if (p.form == WHOLE_TILES && !tokens && p.tiles * Hk <= (D == 64 ? 768 : 384)) {  // (as for packed sequences)
+    p.M = TILE / 2;
+    p.tiles = tile_numbers<TILE / 2>(B, Tq, G);
+  }
+  const int slots = 256 * ES_PAGED_RESIDENT(D, p.M);
+  if (p.form == SHARES) {
+    p.shares = std::max(slots / Hk, 1);
+    p.plan = (size_t)2 * p.shares * Hk * part_floats(p.M, D) * sizeof(float);
+    p.bytes = p.plan + (size_t)(p.shares + 1) * sizeof(int4);
+  } else if (p.form == RANGES) {
+    p.items = (int)(p.tiles + slots / Hk + 1);  // (as range_items)
+    p.plan = (size_t)p.items * Hk * part_floats(p.M, D) * sizeof(float);
+    p.bytes = p.plan + (size_t)(B + 1) * sizeof(int2);
+  }
   return p;
 }
 
@@ -541,36 +809,48 @@ static int paged_fwd(FwdArgs& a, const void* q, const int* pages, const int* len
   a.paged.cap = num_pages > 0 ? max_pages * page_size : 0;  // (without pages no sequence has keys)
   const PagedPlan p = paged_plan(B, Tq, max_pages * page_size, H, Hk, D, bits, cu == nullptr);
   a.tiles = (int)p.tiles;
-  ES_REQUIRE(p.tiles * Hk < MAX_GRID && p.items * Hk < MAX_GRID, ES_ERR_UNSUPPORTED, "paged: too many sequences");
+  ES_REQUIRE(p.tiles * Hk < MAX_GRID && (long long)p.items * Hk < MAX_GRID, ES_ERR_UNSUPPORTED, "paged: too many sequences");
   ES_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes), ES_ERR_INVALID, "paged: workspace too small");
+  a.part = (float*)workspace;
+  a.plan = (int2*)((char*)workspace + p.plan);
+  a.items = p.form == SHARES ? 2 * p.shares : p.items;
+  a.shares = p.shares;
+  a.inv_slots = (float)Hk / (float)(256 * ES_PAGED_RESIDENT(D, p.M));
+  // sixteenths of a chunk, or as much more as it takes for all costs of a head to stay below 2^29
+  a.cost_unit = (float)std::min(16.0, (double)(1 << 29) / ((double)p.tiles * ((double)a.paged.cap / BK + 4.0)));
+  a.least_share = std::max((int)(4.0f * a.cost_unit), 1);
+  const long long rows_most = std::min<long long>((long long)Tq * a.G, p.M);
   auto launch = [&](auto dim, auto bit, auto rows) {
     constexpr int d = decltype(dim)::value, n = decltype(bit)::value, m = decltype(rows)::value;
-    if (p.ranged) {
-      a.part = (float*)workspace;
-      a.plan = (int2*)((char*)workspace + p.plan);
-      a.inv_slots = (float)Hk / (float)p.slots;
-      a.items = (int)p.items;
-      hipLaunchKernelGGL((paged_ranges_kernel<d, n, m>), dim3((unsigned)(p.items * Hk)), dim3(256), 0, stream, a);
-      const long long rows_most = std::min<long long>((long long)Tq * a.G, m);
-      hipLaunchKernelGGL((merge_kernel<d, false, m>), dim3((unsigned)(p.tiles * Hk), (unsigned)((rows_most * d / 4 + 255) / 256)),
-                         dim3(256), 0, stream, a);
-    } else {
-      hipLaunchKernelGGL((paged_whole_kernel<d, n, m>), dim3((unsigned)(p.tiles * Hk)), dim3(256), 0, stream, a);
-    }
-  };
-  using std::integral_constant;
-  auto with_rows = [&](auto dim, auto bit) {
-    if constexpr (decltype(bit)::value == 4) {
-      if (p.M == TOKENS) {
-        launch(dim, bit, integral_constant<int, TOKENS>{});
+    if constexpr (m == TOKENS<n>) {
+      if (p.form == SHARES) {
+        hipLaunchKernelGGL((paged_shares_kernel<d, n, m>), dim3((unsigned)(p.shares * Hk)), dim3(256), 0, stream, a);
+        if (p.shares > 1)
+          hipLaunchKernelGGL((merge_shares_kernel<d, m>), dim3((unsigned)((p.shares - 1) * Hk), (unsigned)((rows_most * d + 255) / 256)),
+                             dim3(256), 0, stream, a);
+        return;
+      }
+    } else if constexpr (m == TILE) {
+      if (p.form == RANGES) {
+        hipLaunchKernelGGL((paged_ranges_kernel<d, n>), dim3((unsigned)(p.items * Hk)), dim3(256), 0, stream, a);
+        // (a workgroup for 8 rows at D = 128, more where there are many tiles, most of which are then whole)
+        const long long most = (rows_most * d / 4 + 255) / 256, few = std::max<long long>(4096 / (p.tiles * Hk), 1);
+        hipLaunchKernelGGL((merge_kernel<d, false>), dim3((unsigned)(p.tiles * Hk), (unsigned)std::min(most, few)), dim3(256), 0,
+                           stream, a);
         return;
       }
     }
-    launch(dim, bit, integral_constant<int, TILE>{});
+    hipLaunchKernelGGL((paged_whole_kernel<d, n, m>), dim3((unsigned)(p.tiles * Hk)), dim3(256), 0, stream, a);
   };
+  using std::integral_constant;
   auto with_bits = [&](auto dim) {
-    if (bits == 16) with_rows(dim, integral_constant<int, 16>{});
-    else with_rows(dim, integral_constant<int, 4>{});
+    auto with_rows = [&](auto bit) {
+      if (p.M == TILE) launch(dim, bit, integral_constant<int, TILE>{});
+      else if (p.M == TILE / 2) launch(dim, bit, integral_constant<int, TILE / 2>{});
+      else launch(dim, bit, integral_constant<int, TOKENS<decltype(bit)::value>>{});
+    };
+    if (bits == 16) with_rows(integral_constant<int, 16>{});
+    else with_rows(integral_constant<int, 4>{});
   };
   if (D == 64) with_bits(integral_constant<int, 64>{});
   else with_bits(integral_constant<int, 128>{});
