@@ -153,14 +153,20 @@ struct Codes {
       }
     }
   }
+  // (Rows that the tile's swizzle puts into the same banks write their four chunks in another order, number i ^ turn in step i: four
+  // rows of 16 lanes then touch every bank once instead of four times.)
   __device__ __forceinline__ void settle(char* base) const {
+    const int turn = D == 128 ? row & 3 : row & 2, at = tile_at<D>(row, 4 * part + turn);
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
       char* tile = base + (tensor + p) * BK * D * 2;
       const float s = __uint_as_float(scale[p] << 23);
-      const unsigned w[4] = {code[p].x, code[p].y, code[p].z, code[p].w};
+      unsigned w[4] = {code[p].x, code[p].y, code[p].z, code[p].w};
+      const bool odd = turn & 1, upper = turn & 2;
+      const unsigned a0 = odd ? w[1] : w[0], a1 = odd ? w[0] : w[1], a2 = odd ? w[3] : w[2], a3 = odd ? w[2] : w[3];
+      w[0] = upper ? a2 : a0, w[1] = upper ? a3 : a1, w[2] = upper ? a0 : a2, w[3] = upper ? a1 : a3;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<ev8*>(tile + tile_at<D>(row, 4 * part + i)) = decode8(w[i], s);
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<ev8*>(tile + (at ^ (16 * i))) = decode8(w[i], s);
     }
   }
   __device__ __forceinline__ void enter() { now = then; }
@@ -190,6 +196,18 @@ __device__ __forceinline__ float max_rows16(float x) {
 __device__ __forceinline__ float sum_rows16(float x) {
   const float2 h = lane_pair16(x);
   return sum_xor32(h.x + h.y);
+}
+
+// V rows of a run in a wave's LDS: 16-byte chunk c of row r at c ^ values_swizzle(r). Sixteen lanes write four rows, each lane a chunk
+// of its own quarter, and read four rows at two neighbouring chunks: both touch every bank once (with the swizzle of the wide tiles
+// the writes met four times: LDS busy 58 % of the time, 48 tokens against 8000 keys, 32 heads over 8, 89 us).
+template <int D>
+__device__ __forceinline__ int values_swizzle(int row) {
+  return D == 128 ? (row & 3) | (row & 1) << 2 | (row >> 2 & 1) << 3 : (row >> 1 & 1) * 3 | (row >> 2 & 1) << 2;
+}
+template <int D>
+__device__ __forceinline__ int values_at(int row, int c) {
+  return row * (D * 2) + ((c ^ values_swizzle<D>(row)) << 4);
 }
 
 // Up to 16 NR rows; every wave has the same rows and takes every fourth run of 32 keys, the four states are merged at the end.
@@ -264,7 +282,7 @@ __device__ __forceinline__ void narrow4_tile(const FwdArgs& a, const Job& j, cha
     }
   };
   char* vb = lds + wv * LDS_WAVE;
-  const int tr = tile_at<D>(4 * g + (c >> 2), (c & 3) >> 1) + (c & 1) * 8, tr16 = tile_at<D>(16 + 4 * g + (c >> 2), (c & 3) >> 1) + (c & 1) * 8;
+  const int tr = values_at<D>(4 * g + (c >> 2), (c & 3) >> 1) + (c & 1) * 8, put = values_at<D>(l >> 2, WORDS * (l & 3));
   if (u < end) {
     places(u);
     load_k();
@@ -299,7 +317,7 @@ __device__ __forceinline__ void narrow4_tile(const FwdArgs& a, const Job& j, cha
       __builtin_memcpy(w, &vc[t], sizeof(w));
 #pragma unroll
       for (int i = 0; i < WORDS; ++i)
-        *reinterpret_cast<ev8*>(vb + tile_at<D>(16 * t + (l >> 2), WORDS * (l & 3) + i)) = decode8(w[i], scale);
+        *reinterpret_cast<ev8*>(vb + 16 * t * ROW + (put ^ (16 * i))) = decode8(w[i], scale);
     }
     asm volatile("" ::: "memory");
     if (more) {
@@ -338,7 +356,7 @@ __device__ __forceinline__ void narrow4_tile(const FwdArgs& a, const Job& j, cha
     }
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
-      const ev8 v = ecat_tr(lds_read_tr(vb, tr ^ (32 * db)), lds_read_tr(vb, tr16 ^ (32 * db)));
+      const ev8 v = ecat_tr(lds_read_tr(vb, tr ^ (32 * db)), lds_read_tr(vb + 16 * ROW, tr ^ (32 * db)));
 #pragma unroll
       for (int n = 0; n < NR; ++n) o[n][db] = emfma16(v, p[n], o[n][db]);
     }
