@@ -134,20 +134,25 @@ __global__ __launch_bounds__(256) void rotate_bwd_kernel(RotateArgs a) {
   }
 }
 
-// dw: grid (D / 16, 2), 16 channels a workgroup, each by 16 lanes' runs of the workgroups' sums
-__global__ __launch_bounds__(256) void weight_sums_kernel(const float* sums, int blocks_q, int blocks_k, int D, void* dq_weight,
-                                                          void* dk_weight, int f32) {
+// dw: grid (D / 16, 2), 16 channels a workgroup, each by 64 lanes' runs of the workgroups' sums (16 lanes each took 15 us for 1024
+// sums, these XX)
+__global__ __launch_bounds__(1024) void weight_sums_kernel(const float* sums, int blocks_q, int blocks_k, int D, void* dq_weight,
+                                                           void* dk_weight, int f32) {
   const int which = blockIdx.y, n = which ? blocks_k : blocks_q;
   const int c = blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4;
   const float* p = sums + (size_t)(which ? blocks_q : 0) * D + c;
   float s = 0.0f;
-  for (int i = run; i < n; i += 16) s += p[(size_t)i * D];
-  __shared__ float lds[16][16];
+#pragma unroll 4
+  for (int i = run; i < n; i += 64) s += p[(size_t)i * D];
+  __shared__ float lds[64][16];
   lds[run][threadIdx.x & 15] = s;
-  __syncthreads();
+  for (int m = 32; m >= 1; m >>= 1) {
+    __syncthreads();
+    if (run < m) lds[run][threadIdx.x & 15] += lds[run + m][threadIdx.x & 15];
+  }
   void* out = which ? dk_weight : dq_weight;
   if (run != 0 || out == nullptr) return;
-  for (int i = 1; i < 16; ++i) s += lds[i][threadIdx.x];
+  s = lds[0][threadIdx.x];
   if (f32) reinterpret_cast<float*>(out)[c] = s;
   else reinterpret_cast<e16_t*>(out)[c] = f2e(s);
 }
@@ -257,7 +262,7 @@ extern "C" int ES_VSA_API(es_norm_rotate_bwd)(const void* q, const void* k, cons
     });
   }
   if (norm)
-    hipLaunchKernelGGL(weight_sums_kernel, dim3(D / 16, 2), dim3(256), 0, stream, a.sums, a.blocks[0], a.blocks[1], D,
+    hipLaunchKernelGGL(weight_sums_kernel, dim3(D / 16, 2), dim3(1024), 0, stream, a.sums, a.blocks[0], a.blocks[1], D,
                        dq_weight, dk_weight, weight_f32);
   return check_launch("es_norm_rotate_bwd");
 }

@@ -103,19 +103,27 @@ struct Rotation {
   int T, H, Hk, D;
   bool f16;
   Rotation(const Tensor& q_, const Tensor& k_, const OptTensor& qw, const OptTensor& kw, const OptTensor& table,
-           const OptTensor& positions_)
+           const OptTensor& positions_, int64_t L)
       : q(rows("q", q_, q_)), k(rows("k", k_, q_)), positions(given(positions_)), turn(q_, q_.size(2), qw, kw, table),
         f16(half_type(q_.scalar_type())) {
     TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2), "q and k do not go together");
     T = as_int(q.size(0)), H = as_int(q.size(1)), D = as_int(q.size(2)), Hk = as_int(k.size(1));
-    if (positions.defined()) check_ints("positions", positions, q, {q.size(0)});
+    TORCH_CHECK(H > 0 && Hk > 0, "q and k must have heads");
+    TORCH_CHECK(turn.q_weight.defined() == turn.k_weight.defined(), "q_weight and k_weight go together");
+    TORCH_CHECK(turn.q_weight.defined() || turn.table.defined(), "norm_rotate needs weights, a table or both");
+    if (positions.defined()) {
+      TORCH_CHECK(turn.table.defined(), "positions go with a table");
+      check_ints("positions", positions, q, {q.size(0)});
+    } else {
+      TORCH_CHECK(!turn.table.defined() || turn.P >= L, "the table has ", turn.P, " positions for ", L, " rows");
+    }
   }
 };
 
 std::tuple<Tensor, Tensor> rotate_forward(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw,
                                           const OptTensor& table, const OptTensor& positions, int64_t L, bool halves, double eps) {
   const c10::OptionalDeviceGuard guard(q.device());
-  const Rotation a(q, k, qw, kw, table, positions);
+  const Rotation a(q, k, qw, kw, table, positions, L);
   Tensor qo = at::empty(a.q.sizes(), q.options()), ko = at::empty(a.k.sizes(), q.options());
   check_status("es_norm_rotate", (a.f16 ? es_norm_rotate_f16 : es_norm_rotate)(
       data(a.q), data(a.k), data(a.turn.q_weight), data(a.turn.k_weight), a.turn.angles(), ints(a.positions), data(qo), data(ko),
@@ -129,7 +137,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rotate_backward(const Tensor& dqo_, c
                                                            const OptTensor& table, const OptTensor& positions, int64_t L,
                                                            bool halves, double eps) {
   const c10::OptionalDeviceGuard guard(q.device());
-  const Rotation a(q, k, qw, kw, table, positions);
+  const Rotation a(q, k, qw, kw, table, positions, L);
   auto gradient = [&](const char* name, const Tensor& d, const Tensor& x) {
     check_on(name, d, x);
     TORCH_CHECK(d.scalar_type() == x.scalar_type() && d.sizes() == x.sizes(), name, " must be like its output");
@@ -180,6 +188,9 @@ struct Cache {
       TORCH_CHECK(k.scalar_type() == dtype && v.scalar_type() == dtype, "a cache of 16 bits must have the tokens' dtype (got ",
                   k.scalar_type(), " and ", v.scalar_type(), ")");
       TORCH_CHECK(k.strides() == v.strides() && k.stride(3) == 1, "k and v of a cache must have the same strides, channels 1 apart");
+      for (int i = 0; i < 3; ++i)
+        TORCH_CHECK(k.size(i) <= 1 || (k.stride(i) >= D && k.stride(i) % 8 == 0),
+                    "rows of a cache must not overlap, their strides be multiples of 8");
     }
     for (const Tensor* t : {&k, &v, (const Tensor*)&ks, (const Tensor*)&vs})
       TORCH_CHECK(!t->defined() || t->numel() == 0 || !misaligned(*t), "the cache must be aligned to 16 bytes");
@@ -208,7 +219,9 @@ Tensor append_forward(const OptTensor& q_, const Tensor& k_, const Tensor& v_, c
   TORCH_CHECK(k.sizes() == v.sizes() && k.size(1) == c.Hk && k.size(2) == c.D &&
                   (!q.defined() || (q.size(0) == k.size(0) && q.size(2) == c.D)),
               "q, k, v and the cache do not go together");
-  const Turn turn(k_, c.D, q.defined() ? qw : OptTensor(), kw, table);
+  TORCH_CHECK(q.defined() ? q.size(1) > 0 && qw.has_value() == kw.has_value() : !qw.has_value(),
+              "q_weight goes with q and k_weight, q has heads");
+  const Turn turn(k_, c.D, qw, kw, table);
   const int H = q.defined() ? as_int(q.size(1)) : 0;
   Tensor out = q.defined() ? at::empty(q.sizes(), q.options()) : at::empty({0}, k.options());
   void* qo = q.defined() ? data(out) : nullptr;
@@ -368,8 +381,17 @@ struct RotateForward : torch::autograd::Function<RotateForward> {
 std::tuple<Tensor, Tensor> rotate_autograd(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw,
                                            const OptTensor& table, const OptTensor& positions, int64_t L, bool halves,
                                            double eps) {
-  TORCH_CHECK(!table.has_value() || !at::GradMode::is_enabled() || !table->requires_grad(),
-              "norm_rotate has no gradient of its table");
+  const bool grad = at::GradMode::is_enabled();
+  auto wants = [](const OptTensor& t) { return t.has_value() && t->requires_grad(); };
+  TORCH_CHECK(!grad || !wants(table), "norm_rotate has no gradient of its table");
+  auto tangent = [](const OptTensor& t) { return t.has_value() && t->_fw_grad(0).defined(); };
+  TORCH_CHECK(!tangent(q) && !tangent(k) && !tangent(qw) && !tangent(kw) && !tangent(table),
+              "norm_rotate has no forward-mode derivative");
+  if (!grad || !(q.requires_grad() || k.requires_grad() || wants(qw) || wants(kw))) {  // (nothing to keep: a third of a short call)
+    static const auto op = find<RotateSignature>("echosparse_gfx950::norm_rotate");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(q, k, qw, kw, table, positions, L, halves, eps);
+  }
   auto r = RotateForward::apply(q, k, qw, kw, table, positions, L, halves, eps);
   return {r[0], r[1]};
 }

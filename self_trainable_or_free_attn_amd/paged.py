@@ -120,27 +120,8 @@ def _check_places(pages, lens, cu, page_size, rows, device):
     return B
 
 
-def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor,
-                 cu: Optional[torch.Tensor] = None, *, q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
-                 k_weight: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None, eps: float = 1e-6,
-                 halves: bool = False) -> Optional[torch.Tensor]:
-    """Keys and values of new tokens into the cache, in place, and with q their queries normed and rotated, returned: one launch.
-
-    k, v [T, Hk, D] and q [T, H, D]: packed tokens (column ranges of a projection's rows are read where they are), those of
-    sequence b from cu[b] to cu[b + 1] - 1 (int32 [B + 1], running counts from 0); without cu T / B each, also as [B, n, heads, D].
-    pages int32 [B, max_pages], lens int32 [B]: the sequence's tokens with the new ones, so token i of n has position
-    lens[b] - n + i, which is held in row position % page_size of page pages[b, position // page_size]. Weights, table, eps and
-    halves as in `norm_rotate`, for k (and q) at that position (past the table's last: as the last); without them k and q stay
-    as they are.
-
-    4 bits: keys are normed and rotated in 64 bits and rounded to float32, then every 32 channels of keys and values take the
-    smallest power of two s with max |x| <= 7 s (2^-120 .. 2^120, for fp16 2^-13 .. 2^13) and the nearest of their values, ties
-    to the even code. Values must be finite.
-
-    Nothing is written for tokens behind the last sequence, of negative positions, past the named pages, or whose page number is
-    outside the cache; q's rows of the first two are zeros. A row that two tokens of a call share gets one of them: pages may be
-    shared for reading only. Returns the new q, contiguous and shaped like q, or None without q. There is no derivative: tensors
-    that require a gradient are refused unless gradients are off."""
+def _check_append(cache, k, v, pages, lens, cu, q, q_weight, k_weight, table, eps):
+    """The arguments of append_paged; eps."""
     dims = k.dim()
     if dims not in (3, 4) or k.shape != v.shape:
         raise ValueError(f"k and v must be [T, Hk, D], or both [B, n, Hk, D], got {tuple(k.shape)} and {tuple(v.shape)}")
@@ -166,18 +147,43 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, pages: tor
             raise ValueError("q_weight and k_weight go together")
     elif q_weight is not None:
         raise ValueError("q_weight goes with q")
-    eps = _check_turn(k, D, q_weight, k_weight, table, eps)
+    return _check_turn(k, D, q_weight, k_weight, table, eps)
+
+
+def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor,
+                 cu: Optional[torch.Tensor] = None, *, q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 halves: bool = False) -> Optional[torch.Tensor]:
+    """Keys and values of new tokens into the cache, in place, and with q their queries normed and rotated, returned: one launch.
+
+    k, v [T, Hk, D] and q [T, H, D]: packed tokens (column ranges of a projection's rows are read where they are), those of
+    sequence b from cu[b] to cu[b + 1] - 1 (int32 [B + 1], running counts from 0); without cu T / B each, also as [B, n, heads, D].
+    pages int32 [B, max_pages], lens int32 [B]: the sequence's tokens with the new ones, so token i of n has position
+    lens[b] - n + i, which is held in row position % page_size of page pages[b, position // page_size]. Weights, table, eps and
+    halves as in `norm_rotate`, for k (and q) at that position (past the table's last: as the last); without them k and q stay
+    as they are.
+
+    4 bits: keys are normed and rotated in 64 bits and rounded to float32, then every 32 channels of keys and values take the
+    smallest power of two s with max |x| <= 7 s (2^-120 .. 2^120, for fp16 2^-13 .. 2^13) and the nearest of their values, ties
+    to the even code. Values must be finite.
+
+    Nothing is written for tokens behind the last sequence, of negative positions, past the named pages, or whose page number is
+    outside the cache; q's rows of the first two are zeros. A row that two tokens of a call share gets one of them: pages may be
+    shared for reading only. Returns the new q, contiguous and shaped like q, or None without q. There is no derivative: tensors
+    that require a gradient are refused unless gradients are off."""
+    if k.is_cuda and k.dim() == 3:      # the operator checks everything itself; what it refuses is named by the checks below
+        try:
+            out = _ops().append_paged(q, k, v, q_weight, k_weight, table, pages, lens, cu, *cache, bool(halves), eps)
+        except (RuntimeError, TypeError):
+            _check_append(cache, k, v, pages, lens, cu, q, q_weight, k_weight, table, eps)
+            raise
+        return None if q is None else out
+    eps = _check_append(cache, k, v, pages, lens, cu, q, q_weight, k_weight, table, eps)
     _check_gpu(k)
-    if dims == 4:
-        k, v = k.flatten(0, 1), v.flatten(0, 1)
-        q_rows = None if q is None else q.flatten(0, 1)
-    else:
-        q_rows = q
-    out = _ops().append_paged(q_rows, k, v, q_weight, k_weight, table, pages, lens, cu, cache.k, cache.v, cache.k_scales,
-                              cache.v_scales, bool(halves), eps)
-    if q is None:
-        return None
-    return out.view(shape) if dims == 4 else out
+    flat = (lambda x: x) if k.dim() == 3 else lambda x: x.flatten(0, 1)
+    out = _ops().append_paged(None if q is None else flat(q), flat(k), flat(v), q_weight, k_weight, table, pages, lens, cu, *cache,
+                              bool(halves), eps)
+    return None if q is None else out.view(q.shape)
 
 
 def paged_rows(cache: PagedCache, pages: torch.Tensor, lens: torch.Tensor, cu: Optional[torch.Tensor] = None, *, rows: int,
@@ -199,6 +205,24 @@ def paged_rows(cache: PagedCache, pages: torch.Tensor, lens: torch.Tensor, cu: O
     return _ops().paged_rows(cache.k, cache.v, cache.k_scales, cache.v_scales, pages, lens, cu, int(rows), dtype)
 
 
+def _check_attention(q, cache, pages, lens, cu, scale):
+    """The arguments of paged_attention; the scale."""
+    dims = q.dim()
+    if dims not in (3, 4):
+        raise ValueError(f"q must be [T, H, D] or [B, n, H, D], got {tuple(q.shape)}")
+    _check_tokens(q, ())
+    device, shape = q.device, q.shape
+    heads, size, D = _check_cache(cache, q.dtype, device, "q")
+    if shape[-1] != D:
+        raise ValueError(f"the cache holds heads of {D} channels, q has {shape[-1]}")
+    _check_heads(shape[-2], heads)
+    rows = shape[0] if dims == 3 else shape[0] * shape[1]
+    B = _check_places(pages, lens, cu, size, rows, device)
+    if dims == 4 and (cu is not None or shape[0] != B):
+        raise ValueError(f"[B, n, H, D] tensors go without cu and with {B} sequences")
+    return _scale(scale, D)
+
+
 def paged_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, lens: torch.Tensor, cu: Optional[torch.Tensor] = None,
                     *, causal: bool = True, scale: Optional[float] = None, return_lse: bool = False):
     """Attention of new tokens over a cache that holds their own keys already (`append_paged`).
@@ -214,25 +238,18 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, len
     Returns out like q, with return_lse also the natural-log LSE [T, H] ([B, n, H]) in float32; a token that sees no key, and rows
     behind the last sequence, give zeros and -inf. The same inputs give the same bits. There is no derivative: tensors that require a
     gradient are refused unless gradients are off."""
-    dims = q.dim()
-    if dims not in (3, 4):
-        raise ValueError(f"q must be [T, H, D] or [B, n, H, D], got {tuple(q.shape)}")
-    _check_tokens(q, ())
-    device, shape = q.device, q.shape
-    heads, size, D = _check_cache(cache, q.dtype, device, "q")
-    if shape[-1] != D:
-        raise ValueError(f"the cache holds heads of {D} channels, q has {shape[-1]}")
-    _check_heads(shape[-2], heads)
-    rows = shape[0] if dims == 3 else shape[0] * shape[1]
-    B = _check_places(pages, lens, cu, size, rows, device)
-    if dims == 4 and (cu is not None or shape[0] != B):
-        raise ValueError(f"[B, n, H, D] tensors go without cu and with {B} sequences")
-    scale = _scale(scale, D)
+    if q.is_cuda and q.dim() == 3:      # the operator checks everything itself; what it refuses is named by the checks below
+        try:
+            out = _ops().paged_attention(q.contiguous(), *cache, pages, lens, cu, bool(causal),
+                                         q.shape[2] ** -0.5 if scale is None else scale)
+        except (RuntimeError, TypeError):
+            _check_attention(q, cache, pages, lens, cu, scale)
+            raise
+        return out if return_lse else out[0]
+    scale = _check_attention(q, cache, pages, lens, cu, scale)
     _check_gpu(q)
+    shape = q.shape
     q = q.contiguous()
-    if dims == 4:
-        q = q.flatten(0, 1)
-    out, lse = _ops().paged_attention(q, cache.k, cache.v, cache.k_scales, cache.v_scales, pages, lens, cu, bool(causal), scale)
-    if dims == 4:
-        out, lse = out.view(shape), lse.view(shape[:-1])
+    out, lse = _ops().paged_attention(q if len(shape) == 3 else q.flatten(0, 1), *cache, pages, lens, cu, bool(causal), scale)
+    out, lse = out.view(shape), lse.view(shape[:-1])
     return (out, lse) if return_lse else out

@@ -69,19 +69,8 @@ def _check_turn(x, D, q_weight, k_weight, table, eps):
     return eps
 
 
-def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
-                k_weight: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
-                positions: Optional[torch.Tensor] = None, *, eps: float = 1e-6, halves: bool = False):
-    """Queries and keys normed and rotated in one pass, with gradients for q, k and the weights.
-
-    q [T, H, D] and k [T, Hk, D] (or [B, L, H, D] and [B, L, Hk, D]), bf16 or fp16, D 64 or 128; column ranges of a projection's
-    rows are read where they are. With weights ([D], the tokens' type or float32, both or neither) a head's row x becomes
-    x / sqrt(mean x^2 + eps) * weight. With a table (`rotary_table`) its first R channels are then turned in pairs by the angles
-    of the row's position, channels 2 i and 2 i + 1, with halves i and i + R / 2. positions: int32 [T] ([B, L]) rows of the
-    table, clamped to it; None: a row's place in q (in its sequence of the batch).
-
-    Returns the new q and k, contiguous. All arithmetic is float32, rounded once at the end. Gradients are deterministic and those
-    of the weights are summed in float32; the backward itself is not differentiable, and a table gets no gradient."""
+def _check_rotate(q, k, q_weight, k_weight, table, positions, eps):
+    """The arguments of norm_rotate; eps and the positions of all rows."""
     dims = q.dim()
     if dims not in (3, 4) or k.dim() != dims:
         raise ValueError("q and k must be [T, H, D], or both [B, L, H, D]")
@@ -108,8 +97,33 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tenso
         _check_ints("positions", positions, q.device)
     elif table is not None and table.shape[0] < L:
         raise ValueError(f"the table has {table.shape[0]} positions for {L} rows")
+    return eps, positions
+
+
+def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                k_weight: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
+                positions: Optional[torch.Tensor] = None, *, eps: float = 1e-6, halves: bool = False):
+    """Queries and keys normed and rotated in one pass, with gradients for q, k and the weights.
+
+    q [T, H, D] and k [T, Hk, D] (or [B, L, H, D] and [B, L, Hk, D]), bf16 or fp16, D 64 or 128; column ranges of a projection's
+    rows are read where they are. With weights ([D], the tokens' type or float32, both or neither) a head's row x becomes
+    x / sqrt(mean x^2 + eps) * weight. With a table (`rotary_table`) its first R channels are then turned in pairs by the angles
+    of the row's position, channels 2 i and 2 i + 1, with halves i and i + R / 2. positions: int32 [T] ([B, L]) rows of the
+    table, clamped to it; None: a row's place in q (in its sequence of the batch).
+
+    Returns the new q and k, contiguous. All arithmetic is float32, rounded once at the end. Gradients are deterministic and those
+    of the weights are summed in float32; the backward itself is not differentiable, and a table gets no gradient."""
+    if q.is_cuda and q.dim() == 3:      # the operator checks everything itself; what it refuses is named by the checks below
+        try:
+            return _ops().norm_rotate(q, k, q_weight, k_weight, table, positions, max(q.shape[0], 1), bool(halves), eps)
+        except (RuntimeError, TypeError):
+            _check_rotate(q, k, q_weight, k_weight, table, positions, eps)
+            raise
+    eps, positions = _check_rotate(q, k, q_weight, k_weight, table, positions, eps)
     _check_gpu(q)
-    if dims == 4:
-        q, k = q.flatten(0, 1), k.flatten(0, 1)
-    q, k = _ops().norm_rotate(q, k, q_weight, k_weight, table, positions, max(L, 1), bool(halves), eps)
-    return (q.view(shape), k.view(kshape)) if dims == 4 else (q, k)
+    if q.dim() == 3:
+        return _ops().norm_rotate(q, k, q_weight, k_weight, table, positions, max(q.shape[0], 1), bool(halves), eps)
+    shape, kshape = q.shape, k.shape
+    q, k = _ops().norm_rotate(q.flatten(0, 1), k.flatten(0, 1), q_weight, k_weight, table, positions, max(shape[1], 1), bool(halves),
+                              eps)
+    return q.view(shape), k.view(kshape)

@@ -72,7 +72,7 @@ W = _t(64)
 TABLE = _t(6, 32, 2, dtype=torch.float32)
 
 
-@pytest.mark.parametrize("kw, error", [
+ROTATE_REFUSED = [
     (dict(), ValueError), (dict(qw=W), ValueError), (dict(kw=W), ValueError),
     (dict(q=_t(6, 4, 64, dtype=torch.float32), table=TABLE), TypeError), (dict(k=_t(6, 2, 64, dtype=FP), table=TABLE), TypeError),
     (dict(q=_t(6, 4, 96), k=_t(6, 2, 96), table=TABLE), ValueError), (dict(k=_t(5, 2, 64), table=TABLE), ValueError),
@@ -88,7 +88,10 @@ TABLE = _t(6, 32, 2, dtype=torch.float32)
     (dict(table=TABLE, positions=_t(6, dtype=torch.int64)), TypeError), (dict(table=TABLE, positions=_i(5)), ValueError),
     (dict(qw=W, kw=W, positions=_i(6)), ValueError),
     (dict(qw=W, kw=W, eps=-1e-6), ValueError), (dict(qw=W, kw=W, eps=math.nan), ValueError), (dict(qw=W, kw=W, eps=math.inf), ValueError),
-])
+]
+
+
+@pytest.mark.parametrize("kw, error", ROTATE_REFUSED)
 def test_norm_rotate_refuses(kw, error):
     with pytest.raises(error):
         _rotate(**kw)
@@ -181,7 +184,7 @@ def _attend(q=None, cache=None, pages=None, lens=None, cu=None, **kw):
                            _i(3) if lens is None else lens, cu, **kw)
 
 
-@pytest.mark.parametrize("kw, error", [
+ATTEND_REFUSED = [
     (dict(q=_t(6, 64)), ValueError), (dict(q=_t(6, 3, 64)), ValueError), (dict(q=_t(6, 0, 64)), ValueError),
     (dict(q=_t(6, 8192, 64)), ValueError), (dict(q=_t(6, 4, 128)), ValueError), (dict(q=_t(7, 4, 64)), ValueError),
     (dict(q=_t(6, 4, 64, dtype=FP)), TypeError), (dict(q=_t(6, 4, 64, dtype=torch.float32)), TypeError),
@@ -190,7 +193,10 @@ def _attend(q=None, cache=None, pages=None, lens=None, cu=None, **kw):
     (dict(cu=_i(5)), ValueError), (dict(scale=0.0), ValueError), (dict(scale=math.inf), ValueError), (dict(scale=math.nan), ValueError),
     (dict(cache=_c(4)._replace(v_scales=None)), ValueError), (dict(cache=_c(dim=128)), ValueError),
     (dict(cache=PagedCache(_t(8, 2, 16, 64), _t(8, 2, 16, 64, dtype=FP))), TypeError),
-])
+]
+
+
+@pytest.mark.parametrize("kw, error", ATTEND_REFUSED)
 def test_paged_attention_refuses(kw, error):
     with pytest.raises(error):
         _attend(**kw)
