@@ -96,12 +96,8 @@ __device__ __forceinline__ float quad_max(float x) {
 }
 
 __device__ __forceinline__ ev8 load8(const e16_t* p) { return *reinterpret_cast<const ev8*>(p); }
-template <class A>
-__device__ __forceinline__ void store8(e16_t* p, const A* x) {
-  ev8 r;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = (elem_t)(float)x[e];
-  *reinterpret_cast<ev8*>(p) = r;
+__device__ __forceinline__ void store8(e16_t* p, const float* x) {
+  *reinterpret_cast<ev8*>(p) = epack8(x);
 }
 
 // how the channels are paired: neighbours, the two halves of a row, the two halves of its first R < D channels
@@ -140,28 +136,27 @@ struct Angles {
   }
 
   // x[0 .. 7] and x[8 .. 15]: the lane's chunks; y: their partners (PART_HALVES only). back: by the negative angles.
-  template <class A>
-  __device__ __forceinline__ void apply(A* x, const A* y, bool back, const bool* second) const {
+  __device__ __forceinline__ void apply(float* x, const float* y, bool back, const bool* second) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (PAIRS == NEIGHBOURS) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const A cc = c[4 * i + e], ss = back ? -s[4 * i + e] : s[4 * i + e];
-          const A a = x[8 * i + 2 * e], b = x[8 * i + 2 * e + 1];
+          const float cc = c[4 * i + e], ss = back ? -s[4 * i + e] : s[4 * i + e];
+          const float a = x[8 * i + 2 * e], b = x[8 * i + 2 * e + 1];
           if (turn[i]) x[8 * i + 2 * e] = a * cc - b * ss, x[8 * i + 2 * e + 1] = a * ss + b * cc;
         }
       } else if (PAIRS == HALVES) {
         if (i == 1) break;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const A cc = c[e], ss = back ? -s[e] : s[e], a = x[e], b = x[8 + e];
+          const float cc = c[e], ss = back ? -s[e] : s[e], a = x[e], b = x[8 + e];
           x[e] = a * cc - b * ss, x[8 + e] = a * ss + b * cc;
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const A cc = c[(8 * i + e) % N], ss = back != second[i] ? s[(8 * i + e) % N] : -s[(8 * i + e) % N];
+          const float cc = c[(8 * i + e) % N], ss = back != second[i] ? s[(8 * i + e) % N] : -s[(8 * i + e) % N];
           if (turn[i]) x[8 * i + e] = x[8 * i + e] * cc + y[8 * i + e] * ss;
         }
       }
@@ -215,38 +210,82 @@ struct RawRow {
       }
     }
   }
-  template <class A>
-  __device__ __forceinline__ void get(A* x) const {
+  __device__ __forceinline__ void get(float* x) const {
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[8 * i + e] = (A)(float)v[i][e];
+      for (int e = 0; e < 8; ++e) x[8 * i + e] = (float)v[i][e];
   }
 };
 
-__device__ __forceinline__ float inverse_root(float x) { return rsqrtf(x); }
-__device__ __forceinline__ double inverse_root(double x) { return 1.0 / sqrt(x); }
-
 // 1 / sqrt(mean x^2 + eps) of a row
-template <int D, class A>
-__device__ __forceinline__ A inverse_rms(const A* x, A eps) {
-  A sum = x[0] * x[0];
+template <int D>
+__device__ __forceinline__ float inverse_rms(const float* x, float eps) {
+  float sum = x[0] * x[0];
 #pragma unroll
   for (int e = 1; e < 16; ++e) sum += x[e] * x[e];
-  return inverse_root(lanes_sum<D / 16>(sum) * (A)(1.0f / D) + eps);
+  return rsqrtf(lanes_sum<D / 16>(sum) * (1.0f / D) + eps);
 }
 
-// x (16 values of the lane, under PART_HALVES with their partners' behind them): normed and rotated in the arithmetic of A
-template <int D, int PAIRS, bool NORM, class A>
-__device__ __forceinline__ void norm_rotate_row(A* x, const Weights<D, PAIRS>& w, const Angles<D, PAIRS>& angles, int j, int R,
-                                                A eps) {
+// x (16 values of the lane, under PART_HALVES with their partners' behind them), normed and rotated
+template <int D, int PAIRS, bool NORM>
+__device__ __forceinline__ void norm_rotate_row(float* x, const Weights<D, PAIRS>& w, const Angles<D, PAIRS>& angles, int j, int R,
+                                                float eps) {
   if (NORM) {
-    const A r = inverse_rms<D>(x, eps);
+    const float r = inverse_rms<D>(x, eps);
 #pragma unroll
-    for (int e = 0; e < Weights<D, PAIRS>::N; ++e) x[e] = x[e] * r * (A)w.w[e];
+    for (int e = 0; e < Weights<D, PAIRS>::N; ++e) x[e] = x[e] * r * w.w[e];
   }
   const bool second[2] = {j >= R / 16, j + D / 16 >= R / 16};
   angles.apply(x, x + (PAIRS == PART_HALVES ? 16 : 0), false, second);
+}
+
+// The same in 64 bits, rounded to float32: a pair at a time, so that few values are held in 64 bits.
+template <int D, int PAIRS, bool NORM>
+__device__ __forceinline__ void norm_rotate_exact(const RawRow<D, PAIRS>& raw, const Weights<D, PAIRS>& w,
+                                                  const Angles<D, PAIRS>& angles, int j, int R, double eps, float* y) {
+  double r = 1.0;
+  if (NORM) {
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float x = (float)raw.v[e / 8][e % 8];
+      sum += (double)(x * x);  // (exact in float32: 11 bits each)
+    }
+    r = 1.0 / sqrt(lanes_sum<D / 16>(sum) * (1.0 / D) + eps);
+  }
+  auto value = [&](int e) {
+    const double x = (double)(float)raw.v[e / 8][e % 8];
+    return NORM ? x * r * (double)w.w[e] : x;
+  };
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (PAIRS == NEIGHBOURS) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = 8 * i + 2 * e;
+        const double a = value(k), b = value(k + 1), c = angles.c[4 * i + e], s = angles.s[4 * i + e];
+        y[k] = (float)(angles.turn[i] ? a * c - b * s : a);
+        y[k + 1] = (float)(angles.turn[i] ? a * s + b * c : b);
+      }
+    } else if (PAIRS == HALVES) {
+      if (i == 1) break;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double a = value(e), b = value(8 + e), c = angles.c[e], s = angles.s[e];
+        y[e] = (float)(a * c - b * s);
+        y[8 + e] = (float)(a * s + b * c);
+      }
+    } else {
+      const bool second = j + i * (D / 16) >= R / 16;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int k = 8 * i + e, n = k % Angles<D, PAIRS>::N;
+        const double a = value(k), b = value((16 + k) % (8 * RawRow<D, PAIRS>::N)), s = second ? angles.s[n] : -angles.s[n];
+        y[k] = (float)(angles.turn[i] ? a * (double)angles.c[n] + b * s : a);
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ 4 bits

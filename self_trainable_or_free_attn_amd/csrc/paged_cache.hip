@@ -5,7 +5,8 @@
 // single tokens is bound by launches and by the chain of loads from the running lengths to the page number and the angles.
 // 4 bits: a lane's 8 channels are a quarter of the 32 that share a scale. Keys are normed and rotated in 64 bits there: a code then
 // follows from the formula alone and not from the order of float32 operations, which moves values that stand next to a border of
-// two codes by a whole step. (Twice the vector work of keys, which the transfers hide.)
+// two codes by a whole step. They take one head a lane group: the angles and weights of UNIT heads would be held in 64 bits (171
+// registers a lane instead of 106, and 5696 tokens of 40 heads over 8 take 44.7 us instead of 37.9).
 #include "paged.h"
 
 #include <type_traits>
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   int part = (int)(u < last ? u : last) - t * units;
   const int which = part < a.units[0] ? 0 : part < a.units[0] + a.units[1] ? 1 : 2;
   part -= which == 0 ? 0 : which == 1 ? a.units[0] : a.units[0] + a.units[1];
-  const int head0 = part * UNIT, heads = min(a.heads[which] - head0, UNIT);
+  const int step = BITS == 4 && which == 1 ? 1 : UNIT, head0 = part * step, heads = min(a.heads[which] - head0, step);
   const e16_t* x = a.x[which] + (size_t)t * a.stride[which] + (size_t)head0 * D;
   RawRow<D, PAIRS> raw[UNIT];
 #pragma unroll
@@ -73,34 +74,33 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   }
   Angles<D, PAIRS> angles;
   if (which < 2) angles.load(a.table + (size_t)(a.R ? min(place.position, a.P - 1) : 0) * a.R, j, a.R);
+  auto hold = [&](const float* v, int head) {
+    const size_t row = (((size_t)place.page * a.Hk + head) << a.places.shift) + place.row;
+    uint8_t* codes = a.codes[which - 1] + row * (D / 2);
+    uint8_t* scales = a.scales[which - 1] + row * (D / 32);
+    hold4(v, codes, scales, j, j);
+    hold4(v + 8, codes, scales, j + D / 16, j);
+  };
+  if (BITS == 4 && which == 1) {
+    float v[16];
+    norm_rotate_exact<D, PAIRS, NORM>(raw[0], w, angles, j, a.R, a.eps, v);
+    hold(v, head0);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < UNIT; ++i) {
     if (i >= heads) break;
     const int head = head0 + i;
     float v[8 * RawRow<D, PAIRS>::N];
-    if (BITS == 4 && which == 1) {
-      double d[8 * RawRow<D, PAIRS>::N];
-      raw[i].get(d);
-      norm_rotate_row<D, PAIRS, NORM>(d, w, angles, j, a.R, a.eps);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = (float)d[e];
-    } else {
-      raw[i].get(v);
-      if (which < 2) norm_rotate_row<D, PAIRS, NORM>(v, w, angles, j, a.R, (float)a.eps);
-    }
-    e16_t* y = nullptr;
-    if (which == 0) {
-      y = a.q_out + ((size_t)t * a.heads[0] + head) * D;
-    } else if (BITS == 16) {
-      y = a.pages[which - 1] + (size_t)place.page * a.page_stride + (size_t)head * a.head_stride + (size_t)place.row * a.row_stride;
-    } else {
-      const size_t row = (((size_t)place.page * a.Hk + head) << a.places.shift) + place.row;
-      uint8_t* codes = a.codes[which - 1] + row * (D / 2);
-      uint8_t* scales = a.scales[which - 1] + row * (D / 32);
-      hold4(v, codes, scales, j, j);
-      hold4(v + 8, codes, scales, j + D / 16, j);
+    raw[i].get(v);
+    if (which < 2) norm_rotate_row<D, PAIRS, NORM>(v, w, angles, j, a.R, (float)a.eps);
+    if (BITS == 4 && which > 0) {
+      hold(v, head);
       continue;
     }
+    e16_t* y = which == 0 ? a.q_out + ((size_t)t * a.heads[0] + head) * D
+                          : a.pages[which - 1] + (size_t)place.page * a.page_stride + (size_t)head * a.head_stride +
+                                (size_t)place.row * a.row_stride;
     store8(y + 8 * j, v);
     store8(y + 8 * (j + D / 16), v + 8);
   }
@@ -112,34 +112,44 @@ struct RowsArgs {
   e16_t* out[2];
   Places places;
   long long page_stride, head_stride, row_stride;
-  FastDiv div_heads;
-  int T, Hk;
+  FastDiv div_units;
+  int T, Hk, units;  // units of UNIT heads
 };
 
-// D / 8 lanes a row, rows in the order (token, keys or values, head)
+// D / 8 lanes a row; a lane group takes UNIT heads of a token's keys or values (one head a group looked the token's place up as often
+// as it moved a row: 5696 tokens of 8 heads from 4 bits 11.0 us, so 7.4)
 template <int D, int BITS>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   constexpr int LPR = D / 8;
-  const int c = threadIdx.x % LPR, heads = 2 * a.Hk;
-  const long long u = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR, last = (long long)a.T * heads - 1;
-  const int t = divide(a.div_heads, (int)(u < last ? u : last));
-  int head = (int)(u < last ? u : last) - t * heads;
-  const int which = head >= a.Hk;
-  head -= which ? a.Hk : 0;
+  const int c = threadIdx.x % LPR, units = 2 * a.units;
+  const long long u = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR, last = (long long)a.T * units - 1;
+  const int t = divide(a.div_units, (int)(u < last ? u : last));
+  int part = (int)(u < last ? u : last) - t * units;
+  const int which = part >= a.units, head0 = (part - (which ? a.units : 0)) * UNIT, heads = min(a.Hk - head0, UNIT);
   const Place place = place_of(a.places, t);
   if (u > last) return;
-  ev8 x = {};
+  ev8 x[UNIT] = {};
   if (place.page >= 0) {
     if (BITS == 16) {
-      x = load8(a.pages[which] + (size_t)place.page * a.page_stride + (size_t)head * a.head_stride +
-                (size_t)place.row * a.row_stride + 8 * c);
+      const e16_t* p = a.pages[which] + (size_t)place.page * a.page_stride + (size_t)place.row * a.row_stride + 8 * c;
+#pragma unroll
+      for (int i = 0; i < UNIT; ++i) x[i] = load8(p + (size_t)(head0 + min(i, heads - 1)) * a.head_stride);
     } else {
-      const size_t row = (((size_t)place.page * a.Hk + head) << a.places.shift) + place.row;
-      const unsigned codes = *reinterpret_cast<const unsigned*>(a.codes[which] + row * (D / 2) + 4 * c);
-      x = decode8(codes, __uint_as_float((unsigned)a.scales[which][row * (D / 32) + c / 4] << 23));
+      unsigned codes[UNIT], scales[UNIT];
+#pragma unroll
+      for (int i = 0; i < UNIT; ++i) {
+        const size_t row = (((size_t)place.page * a.Hk + head0 + min(i, heads - 1)) << a.places.shift) + place.row;
+        codes[i] = *reinterpret_cast<const unsigned*>(a.codes[which] + row * (D / 2) + 4 * c);
+        scales[i] = a.scales[which][row * (D / 32) + c / 4];
+      }
+#pragma unroll
+      for (int i = 0; i < UNIT; ++i) x[i] = decode8(codes[i], __uint_as_float(scales[i] << 23));
     }
   }
-  *reinterpret_cast<ev8*>(a.out[which] + ((size_t)t * a.Hk + head) * D + 8 * c) = x;
+  e16_t* out = a.out[which] + ((size_t)t * a.Hk + head0) * D + 8 * c;
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i)
+    if (i < heads) *reinterpret_cast<ev8*>(out + i * D) = x[i];
 }
 
 }  // namespace
@@ -162,7 +172,7 @@ static int append(AppendArgs& a, const void* q, const void* k, const void* v, co
   a.places = make_places(pages, lens, cu, B, T, max_pages, num_pages, page_size);
   a.stride[0] = q_stride, a.stride[1] = k_stride, a.stride[2] = v_stride;
   a.heads[0] = H, a.heads[1] = a.heads[2] = Hk;
-  for (int i = 0; i < 3; ++i) a.units[i] = (a.heads[i] + UNIT - 1) / UNIT;
+  for (int i = 0; i < 3; ++i) a.units[i] = bits == 4 && i == 1 ? Hk : (a.heads[i] + UNIT - 1) / UNIT;
   const int units = a.units[0] + a.units[1] + a.units[2];
   a.div_units = fast_div(units);
   a.T = T, a.Hk = Hk, a.R = R, a.P = P, a.f32 = weight_f32;
@@ -186,10 +196,10 @@ static int paged_rows(RowsArgs& a, const int* pages, const int* lens, const int*
   ES_REQUIRE(k && v && all_aligned16({k, v}), ES_ERR_INVALID, "paged rows: outputs must be given and aligned to 16 bytes");
   a.out[0] = (e16_t*)k, a.out[1] = (e16_t*)v;
   a.places = make_places(pages, lens, cu, B, T, max_pages, num_pages, page_size);
-  a.div_heads = fast_div(2 * Hk);
-  a.T = T, a.Hk = Hk;
-  const long long rows = 256 / (D / 8), blocks = ((long long)T * 2 * Hk + rows - 1) / rows;
-  ES_REQUIRE((long long)T * 2 * Hk < (1LL << 30) && blocks < PAGED_GRID, ES_ERR_UNSUPPORTED, "paged rows: too many rows");
+  a.T = T, a.Hk = Hk, a.units = (Hk + UNIT - 1) / UNIT;
+  a.div_units = fast_div(2 * a.units);
+  const long long groups = 256 / (D / 8), blocks = ((long long)T * 2 * a.units + groups - 1) / groups;
+  ES_REQUIRE((long long)T * 2 * a.units < (1LL << 30) && blocks < PAGED_GRID, ES_ERR_UNSUPPORTED, "paged rows: too many rows");
   if (D == 64) {
     if (bits == 16) hipLaunchKernelGGL((rows_kernel<64, 16>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((rows_kernel<64, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, a);

@@ -611,7 +611,8 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_shares_ker
   const Share from = shares.border(w, seq, place), to = shares.border(w + 1, other_seq, other_place);
   if (hk == 0 && threadIdx.x == 0) {
     int4* borders = reinterpret_cast<int4*>(a.plan);
-    borders[w] = make_int4(from.tile, from.chunk, seq, place);
+    const int rows = from.chunk > 0 ? min(paged_rows_of(a, seq) - place * M, M) : 0;  // (of a cut tile)
+    borders[w] = make_int4(from.tile, from.chunk, seq_start(a.cu_q, seq, a.B, a.Tq), 64 * place + rows);
     if (w == a.shares - 1) borders[w + 1] = make_int4(END, 0, 0, 0);
   }
   int tile = __builtin_amdgcn_readfirstlane(from.tile), chunk = __builtin_amdgcn_readfirstlane(from.chunk);
@@ -646,75 +647,88 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_shares_ker
 }
 
 // O of tiles that were cut: sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over the pieces. D / 4 lanes a row and piece, SIDE pieces
-// of a row side by side (one after the other 75600 keys, a half of the shares, took 8 us), whose sums are added in order. Grid:
-// (borders * Hk, rows of a tile / rows of a workgroup): the first border within a tile has it merged, so the launch does not grow
-// with the sequences, most of whose tiles are whole.
+// of a row side by side, each side with a maximum of its own, the sides added in order. Grid: (borders * Hk, rows of a tile / rows
+// of a workgroup): the first border within a tile has it merged, so the launch does not grow with the sequences, most of whose tiles
+// are whole, and a border says all that is to be known of its tile: one load a lane, then the pieces' (256 tokens against 2000 keys, 32
+// heads over 8: 397 us with a workgroup a tile, 365 so; 75600 keys, a half of the shares, piece after piece 8 us, so XX).
 template <int D, int M>
 __global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
   constexpr int LPR = D / 4, SIDE = 4, RPB = 256 / (LPR * SIDE);
-  const int w = blockIdx.x / a.Hk + 1, hk = blockIdx.x - (w - 1) * a.Hk;
+  const int w = blockIdx.x / a.Hk + 1, hk = blockIdx.x - (w - 1) * a.Hk, l = lane_id();
   const int4* borders = reinterpret_cast<const int4*>(a.plan);
-  const int4 here = borders[w], before = borders[w - 1];
-  if (here.y == 0 || (before.x == here.x && before.y > 0)) return;
-  const int seq = __builtin_amdgcn_readfirstlane(here.z), t = __builtin_amdgcn_readfirstlane(here.w), r0 = blockIdx.y * RPB;
-  const Seq s = sequence(a.cu_q, nullptr, a.B, a.Tq, 0, seq);
-  const int rows = min(s.nq * a.G - t * M, M);
+  int4 x = borders[min(w - 1 + l, a.shares)];
+  const int tile = __builtin_amdgcn_readlane(x.x, 1), r0 = blockIdx.y * RPB;
+  if (__builtin_amdgcn_readlane(x.y, 1) == 0 || (__builtin_amdgcn_readlane(x.x, 0) == tile && __builtin_amdgcn_readlane(x.y, 0) > 0))
+    return;
+  const int q0 = __builtin_amdgcn_readlane(x.z, 1), place = __builtin_amdgcn_readlane(x.w, 1), rows = place % 64, t = place / 64;
   if (r0 >= rows) return;
   // the shares that have a piece of it, in order: the one before the border the beginning, in its second slot, the others in their
   // first; two borders may stand at one place
   __shared__ int pieces[256 * ES_PAGED_RESIDENT(D, M) + 1];
   if (threadIdx.x == 0) pieces[0] = w - 1;
   int n = 1;
-  for (int i0 = w; i0 < a.shares; i0 += 64) {
-    const int i = i0 + lane_id();
-    const int4 x = borders[min(i, a.shares)], y = borders[min(i + 1, a.shares)];
-    const bool within = i < a.shares && x.x == here.x, mine = within && (y.x != x.x || y.y > x.y);
+  for (int i0 = w - 1;; i0 += 62) {  // (lanes 1 to 62, which see the next border)
+    if (i0 >= w) x = borders[min(i0 + l, a.shares)];
+    const int next = __shfl(x.x, min(l + 1, 63), 64), next_chunk = __shfl(x.y, min(l + 1, 63), 64);
+    const bool within = l >= 1 && l <= 62 && i0 + l < a.shares && x.x == tile;
+    const bool mine = within && (next != tile || next_chunk > x.y);
     const unsigned long long hit = __builtin_amdgcn_ballot_w64(mine);
-    if (mine && threadIdx.x < 64) pieces[n + __builtin_popcountll(hit & ((1ull << lane_id()) - 1))] = i;
+    if (mine && threadIdx.x < 64) pieces[n + __builtin_popcountll(hit & ((1ull << l) - 1))] = i0 + l;
     n += __builtin_popcountll(hit);
-    if (!__builtin_amdgcn_readlane((int)within, 63)) break;
+    if (!__builtin_amdgcn_readlane((int)within, 62)) break;
   }
   __syncthreads();
   const int lane = threadIdx.x % LPR, c = lane * 4, side = threadIdx.x / LPR % SIDE, local = threadIdx.x / (LPR * SIDE);
   const int r = min(r0 + local, rows - 1);
-  auto part = [&](int i) { return partial<D>(a.part, M, a, 2 * pieces[i] + (i == 0), hk); };
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += LPR) top = fmaxf(top, part(i)[r]);
-#pragma unroll
-  for (int m = LPR / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-  const float msub = top == -INFINITY ? 0.0f : top;
+  float top = -INFINITY, sum = 0.0f;
   f32x4 acc = {};
-  float sum = 0.0f;
   for (int i = side; i < n; i += 4 * SIDE) {  // (four pieces in flight)
-    f32x4 x[4];
-    float f[4], l[4];
+    f32x4 o[4];
+    float m[4], z[4], most = top;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const bool in = i + e * SIDE < n;
-      const float* p = part(in ? i + e * SIDE : i);
-      x[e] = *reinterpret_cast<const f32x4*>(p + 2 * M + r * D + c);
-      f[e] = in ? exp2f_fast(p[r] - msub) : 0.0f;
-      l[e] = p[M + r];
+      const int k = min(i + e * SIDE, n - 1);
+      const float* p = partial<D>(a.part, M, a, 2 * pieces[k] + (k == 0), hk);
+      o[e] = *reinterpret_cast<const f32x4*>(p + 2 * M + r * D + c);
+      m[e] = i + e * SIDE < n ? p[r] : -INFINITY;
+      z[e] = p[M + r];
     }
 #pragma unroll
+    for (int e = 0; e < 4; ++e) most = fmaxf(most, m[e]);
+    if (most == -INFINITY) continue;
+    const float old = exp2f_fast(top - most);
+    acc *= old;
+    sum *= old;
+#pragma unroll
     for (int e = 0; e < 4; ++e) {
-      acc += f[e] * x[e];
-      sum = fmaf(f[e], l[e], sum);
+      const float f = exp2f_fast(m[e] - most);
+      acc += f * o[e];
+      sum = fmaf(f, z[e], sum);
     }
+    top = most;
   }
   __shared__ f32x4 sums[SIDE][RPB][LPR];
-  __shared__ float weights[SIDE][RPB];
+  __shared__ float2 weights[SIDE][RPB];  // maximum, sum
   sums[side][local][lane] = acc;
-  if (lane == 0) weights[side][local] = sum;
+  if (lane == 0) weights[side][local] = make_float2(top, sum);
   __syncthreads();
   if (side != 0 || r0 + local >= rows) return;
+  float2 s[SIDE];
 #pragma unroll
-  for (int i = 1; i < SIDE; ++i) {
-    acc += sums[i][local][lane];
-    sum += weights[i][local];
+  for (int i = 0; i < SIDE; ++i) {
+    s[i] = weights[i][local];
+    top = fmaxf(top, s[i].x);
+  }
+  acc = f32x4{};
+  sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < SIDE; ++i) {
+    const float f = s[i].x == -INFINITY ? 0.0f : exp2f_fast(s[i].x - top);
+    acc += f * sums[i][local][lane];
+    sum = fmaf(f, s[i].y, sum);
   }
   const int row = t * M + r, tok = divide(a.div_g, row);
-  const size_t at = ((size_t)(s.q0 + tok) * a.Hk + hk) * a.G + (row - tok * a.G);
+  const size_t at = ((size_t)(q0 + tok) * a.Hk + hk) * a.G + (row - tok * a.G);
   store_row<D>(a, at, c, acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
   if (c == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top - P_SHIFT + log2f(sum)) * PK_LN2;
 }

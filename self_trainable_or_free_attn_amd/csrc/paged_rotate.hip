@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void rotate_bwd_kernel(RotateArgs a) {
 }
 
 // dw: grid (D / 16, 2), 16 channels a workgroup, each by 64 lanes' runs of the workgroups' sums (16 lanes each took 15 us for 1024
-// sums, these XX)
+// sums, these 4)
 __global__ __launch_bounds__(1024) void weight_sums_kernel(const float* sums, int blocks_q, int blocks_k, int D, void* dq_weight,
                                                            void* dk_weight, int f32) {
   const int which = blockIdx.y, n = which ? blocks_k : blocks_q;
