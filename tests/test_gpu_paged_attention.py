@@ -187,6 +187,53 @@ def test_many_sequences(dev, bits, B, most):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("most", [1, 2])
+@pytest.mark.parametrize("B", [300, 600])
+def test_more_sequences_than_a_wave_reads_at_once(dev, bits, most, B):
+    """255 at a time: single tokens in shares, more of them in ranges; a few long histories among short ones, some without keys."""
+    lens = [(5 * i) % (most + 1) if most > 1 else 1 for i in range(B)]
+    keys = [n + (13 * i) % 30 + (4000 if i % 97 == 5 else 0) if i % 11 else 0 for i, n in enumerate(lens)]
+    _case(dev, lens, keys, 4, 2, 64, BF, 16, bits, seed=21, pad=2 if most > 1 else 0)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("G", [1, 4])
+@pytest.mark.parametrize("lens", [[200] + [0] * 199, [0] * 30 + [7, 90] + [1] * 100, [33] + [1] * 40 + [0] * 32])
+def test_few_sequences_have_most_of_the_tokens(dev, bits, G, lens):
+    """No more tokens than sequences, so the call takes them for single ones, but some sequences have many: tiles of few rows whose
+    pieces under a causal mask see a part of the keys, next to empty sequences."""
+    for extra in (0, 3000):
+        keys = [n + (extra if n > 1 else 5 * i % 70) if n else 0 for i, n in enumerate(lens)]
+        for causal in (True, False):
+            _case(dev, lens, keys, 2 * G, 2, 64, FP, 32, bits, seed=22, causal=causal, width=200)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches(dev, seed):
+    """Any mix of tokens, pieces and prompts, heads, pages and holes, tables of pages longer than needed (so that the call cuts)."""
+    import random
+    rng = random.Random(seed)
+    log = lambda lo, hi: int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+    B = log(1, 90)
+    single = rng.random() < 0.6
+    lens = [1 if single or rng.random() < 0.7 else log(1, 300) for _ in range(B)]
+    if rng.random() < 0.3:
+        lens[rng.randrange(B)] = 0
+    keys = [0 if rng.random() < 0.05 else max(0, n + log(1, 6000) - (rng.random() < 0.1) * n) for n in lens]
+    Hk = rng.choice([1, 2, 3, 8, 40])
+    H, D, page = Hk * rng.choice([1, 2, 4, 5, 8]), rng.choice([64, 128]), rng.choice([16, 32, 64, 256])
+    used = [(b, i) for b, m in enumerate(keys) for i in range(-(-m // page))]
+    holes = rng.sample(used, min(len(used), rng.choice([0, 0, 3])))
+    while sum(n * m for n, m in zip(lens, keys)) * H > 40_000_000:      # (the 64-bit result's time)
+        i = max(range(B), key=lambda b: lens[b] * keys[b])
+        lens[i] = max(1, lens[i] // 2)
+        if lens[i] == 1:
+            break
+    _case(dev, lens, keys, H, Hk, D, rng.choice([BF, FP]), page, rng.choice([16, 4]), seed=100 + seed, causal=rng.random() < 0.8,
+          pad=rng.choice([0, 3]), holes=holes, width=-(-max(max(keys), 1) // page) + rng.choice([0, 1, 100]))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("lens", [[1, 1, 1, 1], [40, 1, 100, 20]])
 @pytest.mark.parametrize("width", [None, 200])
 def test_pages_that_do_not_exist(dev, bits, lens, width):

@@ -153,6 +153,50 @@ def test_batches_and_broadcast_gradients(dev):
     assert torch.equal(g1, g2)
 
 
+def test_more_than_2_31_values(dev):
+    """The last rows of a tensor whose offsets pass 32 bits, forward and backward, are what they are alone."""
+    api, T, H, D = _api(), 136_000, 128, 128
+    g = torch.Generator(device=dev).manual_seed(14)
+    q = torch.empty(T, H, D, device=dev, dtype=BF)
+    tail = torch.randn(50, H, D, device=dev, generator=g).to(BF)
+    q[:-50] = 0
+    q[-50:] = tail
+    k = torch.zeros(T, 1, D, device=dev, dtype=BF)
+    w = torch.ones(D, device=dev, dtype=BF)
+    table = api.rotary_table(1000, D, device=dev)
+    pos = torch.arange(T, device=dev, dtype=torch.int32) % 1000
+    q.requires_grad_()
+    out, _ = api.norm_rotate(q, k, w, w, table, pos)
+    few = tail.clone().requires_grad_()
+    want, _ = api.norm_rotate(few, k[-50:], w, w, table, pos[-50:].clone())
+    assert torch.equal(out[-50:], want)
+    dq, = torch.autograd.grad(out, q, torch.ones_like(out))
+    dwant, = torch.autograd.grad(want, few, torch.ones_like(want))
+    assert torch.equal(dq[-50:], dwant)
+
+
+def test_gradients_of_broadcast_heads(dev):
+    """One head's rows expanded to several, and a weight that queries and keys share."""
+    api, T, D = _api(), 30, 64
+    g = torch.Generator(device=dev).manual_seed(15)
+    one = torch.randn(T, 1, D, device=dev, generator=g).to(BF).requires_grad_()
+    w = torch.ones(D, device=dev, requires_grad=True)
+    table = api.rotary_table(T, D, device=dev)
+    q, k = api.norm_rotate(one.expand(T, 4, D), one, w, w, table)
+    dy = torch.randn(T, 4, D, device=dev, generator=g).to(BF)
+    dk = torch.randn(T, 1, D, device=dev, generator=g).to(BF)
+    dx, dw = torch.autograd.grad((q, k), (one, w), (dy, dk))
+    many, key = one.detach().expand(T, 4, D).contiguous().requires_grad_(), one.detach().clone().requires_grad_()
+    wq, wk = (w.detach().clone().requires_grad_() for _ in "qk")
+    each = torch.autograd.grad(api.norm_rotate(many, key, wq, wk, table), (many, key, wq, wk), (dy, dk))
+    heads = each[0].double().sum(1, keepdim=True)
+    total = heads + each[1].double()
+    # the heads' sum and the keys' gradient beside it are each rounded to the token type (sums of five float32 values: 2^-21)
+    bound = (2.0 ** -8 + 2.0 ** -21) * (heads.abs() + total.abs()) + 2.0 ** -21 * each[0].double().abs().sum(1, keepdim=True)
+    ref.check("dx", dx, total, bound)
+    ref.check("dw", dw, (each[2].double() + each[3].double()), 2.0 ** -23 * (each[2].double().abs() + each[3].double().abs()))
+
+
 def test_positions_are_held_to_the_table(dev):
     api, D = _api(), 64
     x = torch.randn(4, 1, D, device=dev).to(BF)
