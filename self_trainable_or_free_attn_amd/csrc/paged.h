@@ -296,8 +296,8 @@ constexpr int SCALE_MIN = -13, SCALE_MAX = 13;
 constexpr int SCALE_MIN = -120, SCALE_MAX = 120;
 #endif
 
-// The scale of 32 channels whose largest magnitude is `top`, as its float bits >> 23 (= exponent + 127): the smallest power of two s
-// with top <= 7 s. (7 and not 6, the largest value: what lies between is off by at most half the step from 4 to 6, and the other
+// The scale of 32 channels whose largest magnitude is `top`, as its float bits >> 23 (= exponent + 127): the smallest power of two
+// s with top <= 7 s. (7 and not 6, the largest value: what lies between is off by at most half the step from 4 to 6, and the other
 // 31 keep twice the resolution that the next power would leave them.)
 __device__ __forceinline__ int scale_of(float top) {
   const unsigned bits = __float_as_uint(top);

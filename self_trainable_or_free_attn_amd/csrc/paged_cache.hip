@@ -116,8 +116,8 @@ struct RowsArgs {
   int T, Hk, units;  // units of UNIT heads
 };
 
-// D / 8 lanes a row; a lane group takes UNIT heads of a token's keys or values (one head a group looked the token's place up as often
-// as it moved a row: 5696 tokens of 8 heads from 4 bits 11.0 us, so 7.4)
+// D / 8 lanes a row; a lane group takes UNIT heads of a token's keys or values (one head a group looked the token's place up as
+// often as it moved a row: 5696 tokens of 8 heads from 4 bits 11.0 us, so 7.4)
 template <int D, int BITS>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   constexpr int LPR = D / 8;

@@ -1,5 +1,5 @@
-// Attention of new tokens over paged caches of 16 and 4 bits (gfx950, bf16 / fp16): where the tiles of packed_tiles.h get their keys
-// from, and tiles of their own for few rows over a cache of 4 bits.
+// Attention of new tokens over paged caches of 16 and 4 bits (gfx950, bf16 / fp16): where the tiles of packed_tiles.h get their
+// keys from, and tiles of their own for few rows over a cache of 4 bits.
 //
 // Page numbers: a page holds 16 rows or a multiple of that, so sixteen keys that start at a multiple of sixteen stand in one page.
 // Each lane of a wave holds the page number of one such group, a window of 64 groups (the next window's numbers are on their way),
@@ -118,19 +118,22 @@ struct Pages {
 };
 
 // 4 bits, wide tiles: a thread loads 32 codes of a row and their scale a chunk ahead (D = 128: of keys and of values) and writes
-// them as token values where the transfers of 16 bits would have put them
+// them as token values where the transfers of 16 bits would have put them. Lanes have the rows in an order in which eight
+// neighbours write to different banks (in the order of memory, a row to four lanes, 1.5e7 cycles of conflicts instead of 7e5, and 32760
+// tokens, 24 heads, 7180 us instead of 7110).
 template <int D>
 struct Codes {
   static constexpr bool HOLES = true, STAGED = true;
-  static constexpr int PARTS = D == 128 ? 2 : 1, TPR = D / 32;  // threads a row
+  static constexpr int PARTS = D == 128 ? 2 : 1;
   PageWindow window;
   uint4 code[PARTS];
   unsigned scale[PARTS], now, then;
   int tensor, row, part, wv;  // D = 64: two waves have the keys, two the values
   __device__ __forceinline__ Codes(const FwdArgs& a, const Job& j, int l, int wave, bool) : now(0), then(0), wv(wave) {
     tensor = D == 128 ? 0 : wv >> 1;
-    row = D == 128 ? 16 * wv + (l >> 2) : 32 * (wv & 1) + (l >> 1);
-    part = l % TPR;
+    row = D == 128 ? 16 * wv + ((l & 1) | (l >> 1 & 3) << 2 | (l >> 3 & 1) << 1)
+                   : 32 * (wv & 1) + (2 * (l & 7) | (l >> 3 & 1) | (l & 16));
+    part = l >> (D == 128 ? 4 : 5);
     window.start(a, j, j.c0, false);
   }
   __device__ __forceinline__ void wide(const FwdArgs& a, const Job& j, int c, unsigned) {
@@ -153,18 +156,13 @@ struct Codes {
       }
     }
   }
-  // (Rows that the tile's swizzle puts into the same banks write their four chunks in another order, number i ^ turn in step i: four
-  // rows of 16 lanes then touch every bank once instead of four times.)
   __device__ __forceinline__ void settle(char* base) const {
-    const int turn = D == 128 ? row & 3 : row & 2, at = tile_at<D>(row, 4 * part + turn);
+    const int at = tile_at<D>(row, 4 * part);
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
       char* tile = base + (tensor + p) * BK * D * 2;
       const float s = __uint_as_float(scale[p] << 23);
-      unsigned w[4] = {code[p].x, code[p].y, code[p].z, code[p].w};
-      const bool odd = turn & 1, upper = turn & 2;
-      const unsigned a0 = odd ? w[1] : w[0], a1 = odd ? w[0] : w[1], a2 = odd ? w[3] : w[2], a3 = odd ? w[2] : w[3];
-      w[0] = upper ? a2 : a0, w[1] = upper ? a3 : a1, w[2] = upper ? a0 : a2, w[3] = upper ? a1 : a3;
+      const unsigned w[4] = {code[p].x, code[p].y, code[p].z, code[p].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) *reinterpret_cast<ev8*>(tile + (at ^ (16 * i))) = decode8(w[i], s);
     }
@@ -174,8 +172,8 @@ struct Codes {
 };
 
 // ------------------------------------------------------------------------------------------------ few rows over 4 bits
-// MFMA 16x16x32. Operand layouts (checked on the GPU): A (16x32): lane l holds A[l % 16][8 (l / 16) + 0..7], B (32x16): lane l holds
-// B[8 (l / 16) + 0..7][l % 16], C (16x16): lane l, register r holds C[4 (l / 16) + r][l % 16].
+// MFMA 16x16x32. Operand layouts (checked on the GPU): A (16x32): lane l holds A[l % 16][8 (l / 16) + 0..7], B (32x16): lane l
+// holds B[8 (l / 16) + 0..7][l % 16], C (16x16): lane l, register r holds C[4 (l / 16) + r][l % 16].
 __device__ __forceinline__ f32x4 emfma16(ev8 a, ev8 b, f32x4 c) {
 #ifdef ES_ELEM_F16
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -198,12 +196,12 @@ __device__ __forceinline__ float sum_rows16(float x) {
   return sum_xor32(h.x + h.y);
 }
 
-// V rows of a run in a wave's LDS: 16-byte chunk c of row r at c ^ values_swizzle(r). Sixteen lanes write four rows, each lane a chunk
-// of its own quarter, and read four rows at two neighbouring chunks: both touch every bank once (with the swizzle of the wide tiles
-// the writes met four times: LDS busy 58 % of the time, 48 tokens against 8000 keys, 32 heads over 8, 89 us).
+// V rows of a run in a wave's LDS: 16-byte chunk c of row r at c ^ values_swizzle(r). Eight lanes write a chunk each of eight rows,
+// and sixteen lanes read four rows at two neighbouring chunks: both touch every bank once. (With the rows of the wide tiles and a
+// row to four lanes, LDS was busy 58 % of the time, 48 tokens against 8000 keys, 32 heads over 8; so 20 %.)
 template <int D>
 __device__ __forceinline__ int values_swizzle(int row) {
-  return D == 128 ? (row & 3) | (row & 1) << 2 | (row >> 2 & 1) << 3 : (row >> 1 & 1) * 3 | (row >> 2 & 1) << 2;
+  return (row & 3) << 1 | (row >> 2 & 1) | (D == 128 ? row & 8 : 0);
 }
 template <int D>
 __device__ __forceinline__ int values_at(int row, int c) {
@@ -255,8 +253,8 @@ __device__ __forceinline__ void narrow4_tile(const FwdArgs& a, const Job& j, cha
   typedef typename std::conditional<D == 128, uint4, uint2>::type Piece;  // a lane's codes of a group
   Piece kc[2], vc[2];
   unsigned ks8[2], vs8[2];
+  // a lane's quarter of its key's row: K as the products take it, V as it is written
   const int k_at = c * (D / 2) + g * (D / 8), ks_at = c * (D / 32) + (D == 128 ? g : g >> 1);
-  const int v_at = l * (D / 8), vs_at = (l >> 2) * (D / 32) + (D == 128 ? l & 3 : (l & 3) >> 1);
   size_t at16[2];  // a run's groups: the first row in the cache
   unsigned missing = 0, missing_next = 0;
   auto places = [&](int u) {
@@ -277,12 +275,12 @@ __device__ __forceinline__ void narrow4_tile(const FwdArgs& a, const Job& j, cha
   auto load_v = [&]() {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      vc[t] = *reinterpret_cast<const Piece*>(a.paged.codes[1] + at16[t] * (D / 2) + v_at);
-      vs8[t] = a.paged.scales[1][at16[t] * (D / 32) + vs_at];
+      vc[t] = *reinterpret_cast<const Piece*>(a.paged.codes[1] + at16[t] * (D / 2) + k_at);
+      vs8[t] = a.paged.scales[1][at16[t] * (D / 32) + ks_at];
     }
   };
   char* vb = lds + wv * LDS_WAVE;
-  const int tr = values_at<D>(4 * g + (c >> 2), (c & 3) >> 1) + (c & 1) * 8, put = values_at<D>(l >> 2, WORDS * (l & 3));
+  const int tr = values_at<D>(4 * g + (c >> 2), (c & 3) >> 1) + (c & 1) * 8, put = values_at<D>(c, WORDS * g);
   if (u < end) {
     places(u);
     load_k();
@@ -310,7 +308,7 @@ __device__ __forceinline__ void narrow4_tile(const FwdArgs& a, const Job& j, cha
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int key = 32 * u + 16 * t + (l >> 2);
+      const int key = 32 * u + 16 * t + c;
       const bool there = key < j.nk && !(missing >> t & 1);
       const float scale = __uint_as_float((there ? vs8[t] : 127u) << 23);
       unsigned w[WORDS];
@@ -648,9 +646,10 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_shares_ker
 
 // O of tiles that were cut: sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over the pieces. D / 4 lanes a row and piece, SIDE pieces
 // of a row side by side, each side with a maximum of its own, the sides added in order. Grid: (borders * Hk, rows of a tile / rows
-// of a workgroup): the first border within a tile has it merged, so the launch does not grow with the sequences, most of whose tiles
-// are whole, and a border says all that is to be known of its tile: one load a lane, then the pieces' (256 tokens against 2000 keys, 32
-// heads over 8: 397 us with a workgroup a tile, 365 so; 75600 keys, a half of the shares, piece after piece 8 us, so XX).
+// of a workgroup): the first border within a tile has it merged, so the launch does not grow with the sequences, most of whose
+// tiles are whole, and a border says all that is to be known of its tile: one load a lane, then the pieces' (256 tokens against
+// 2000 keys, 32 heads over 8: attention 397 us with a workgroup a tile, 349 so; one sequence of 75600 keys among 49, whose tile has
+// half of the borders: 8 us piece after piece, 4.7 so).
 template <int D, int M>
 __global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
   constexpr int LPR = D / 4, SIDE = 4, RPB = 256 / (LPR * SIDE);
@@ -658,8 +657,8 @@ __global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
   const int4* borders = reinterpret_cast<const int4*>(a.plan);
   int4 x = borders[min(w - 1 + l, a.shares)];
   const int tile = __builtin_amdgcn_readlane(x.x, 1), r0 = blockIdx.y * RPB;
-  if (__builtin_amdgcn_readlane(x.y, 1) == 0 || (__builtin_amdgcn_readlane(x.x, 0) == tile && __builtin_amdgcn_readlane(x.y, 0) > 0))
-    return;
+  const bool again = __builtin_amdgcn_readlane(x.x, 0) == tile && __builtin_amdgcn_readlane(x.y, 0) > 0;
+  if (__builtin_amdgcn_readlane(x.y, 1) == 0 || again) return;
   const int q0 = __builtin_amdgcn_readlane(x.z, 1), place = __builtin_amdgcn_readlane(x.w, 1), rows = place % 64, t = place / 64;
   if (r0 >= rows) return;
   // the shares that have a piece of it, in order: the one before the border the beginning, in its second slot, the others in their
@@ -736,8 +735,8 @@ __global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
 // ------------------------------------------------------------------------------------------------ wide tiles: key ranges
 // Launches with wide tiles are bound by the matrix units, and tiles that read the same keys side by side have them from L2: these
 // are cut into ranges as in packed_tiles.h, the last tiles of a sequence first. (Equal shares, whose pieces start anywhere: 4096
-// tokens of 32 heads over 8 alone 228 us, ranges 168; 32760 of 24 heads 7100 and 6480, whole tiles 6170. 4096 tokens beside one that
-// sees 75600 keys: whole tiles 572, ranges 224.) List i: the rows of sequence i, list B: those behind the last one.
+// tokens of 32 heads over 8 alone 228 us, ranges 168; 32760 of 24 heads 7100 and 6480, whole tiles 6170. 4096 tokens beside one
+// that sees 75600 keys: whole tiles 572, ranges 224.) List i: the rows of sequence i, list B: those behind the last one.
 struct PagedLists {
   const FwdArgs& a;
   __device__ __forceinline__ ListShape operator()(int b) const {
@@ -785,7 +784,9 @@ static PagedPlan paged_plan(int B, int Tq, int cap, int H, int Hk, int D, int bi
   // single tokens (with running counts: no more tokens than sequences) and the like whose rows fit a narrow tile
   const bool tokens = (equal ? (long long)(Tq / B) * G : Tq <= B ? G : narrow + 1) <= narrow;
   p.M = tokens ? narrow : TILE;
-  p.tiles = !tokens ? tile_numbers<TILE>(B, Tq, G) : bits == 4 ? tile_numbers<TOKENS<4>>(B, Tq, G) : tile_numbers<TOKENS<16>>(B, Tq, G);
+  p.tiles = !tokens     ? tile_numbers<TILE>(B, Tq, G)
+            : bits == 4 ? tile_numbers<TOKENS<4>>(B, Tq, G)
+                        : tile_numbers<TOKENS<16>>(B, Tq, G);
   p.form = cap <= 1024 ? WHOLE_TILES : tokens ? SHARES : RANGES;
   if (p.form == WHOLE_TILES && !tokens && p.tiles * Hk <= (D == 64 ? 768 : 384)) {  // (as for packed sequences)
     p.M = TILE / 2;
@@ -858,8 +859,8 @@ static int paged_fwd(FwdArgs& a, const void* q, const int* pages, const int* len
       if (p.form == SHARES) {
         hipLaunchKernelGGL((paged_shares_kernel<d, n, m>), dim3((unsigned)(p.shares * Hk)), dim3(256), 0, stream, a);
         if (p.shares > 1)
-          hipLaunchKernelGGL((merge_shares_kernel<d, m>), dim3((unsigned)((p.shares - 1) * Hk), (unsigned)((rows_most * d + 255) / 256)),
-                             dim3(256), 0, stream, a);
+          hipLaunchKernelGGL((merge_shares_kernel<d, m>),
+                             dim3((unsigned)((p.shares - 1) * Hk), (unsigned)((rows_most * d + 255) / 256)), dim3(256), 0, stream, a);
         return;
       }
     } else if constexpr (m == TILE) {

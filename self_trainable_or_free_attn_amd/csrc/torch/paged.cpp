@@ -48,8 +48,8 @@ void check_on(const char* name, const Tensor& t, const Tensor& like) {
 }
 void check_ints(const char* name, const Tensor& t, const Tensor& like, at::IntArrayRef shape) {
   check_on(name, t, like);
-  TORCH_CHECK(t.scalar_type() == at::kInt && t.sizes() == shape && t.is_contiguous(), name, " must be a contiguous int32 tensor of ",
-              shape);
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.sizes() == shape && t.is_contiguous(), name,
+              " must be a contiguous int32 tensor of ", shape);
 }
 
 // [T, heads, D] rows of one stride: as they are, or copied where the kernels' loads do not take their layout
@@ -187,7 +187,8 @@ struct Cache {
     } else {
       TORCH_CHECK(k.scalar_type() == dtype && v.scalar_type() == dtype, "a cache of 16 bits must have the tokens' dtype (got ",
                   k.scalar_type(), " and ", v.scalar_type(), ")");
-      TORCH_CHECK(k.strides() == v.strides() && k.stride(3) == 1, "k and v of a cache must have the same strides, channels 1 apart");
+      TORCH_CHECK(k.strides() == v.strides() && k.stride(3) == 1,
+                  "k and v of a cache must have the same strides, channels 1 apart");
       for (int i = 0; i < 3; ++i)
         TORCH_CHECK(k.size(i) <= 1 || (k.stride(i) >= D && k.stride(i) % 8 == 0),
                     "rows of a cache must not overlap, their strides be multiples of 8");
@@ -275,8 +276,8 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor& q_, const Tensor& kp,
   float* l = static_cast<float*>(data(lse));
   if (c.four)
     check_status("es_paged4_fwd", (f16 ? es_paged4_fwd_f16 : es_paged4_fwd)(
-        data(q), c.bytes(kp), c.bytes(c.ks), c.bytes(vp), c.bytes(c.vs), ints(pages), ints(lens), ints(c.cu), data(out), l, data(ws),
-        bytes, c.B, c.T, c.max_pages, c.num_pages, c.page_size, H, c.Hk, c.D, causal, static_cast<float>(scale), stream_of(q)));
+        data(q), c.bytes(kp), c.bytes(c.ks), c.bytes(vp), c.bytes(c.vs), ints(pages), ints(lens), ints(c.cu), data(out), l,
+        data(ws), bytes, c.B, c.T, c.max_pages, c.num_pages, c.page_size, H, c.Hk, c.D, causal, static_cast<float>(scale), stream_of(q)));
   else
     check_status("es_paged_fwd", (f16 ? es_paged_fwd_f16 : es_paged_fwd)(
         data(q), data(kp), data(vp), ints(pages), ints(lens), ints(c.cu), data(out), l, data(ws), bytes, c.B, c.T, c.max_pages,

@@ -228,16 +228,16 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, len
     """Attention of new tokens over a cache that holds their own keys already (`append_paged`).
 
     q [T, H, D], H a multiple of the cache's heads, packed: sequence b has rows cu[b] to cu[b + 1] - 1 (int32 [B + 1]), without cu
-    T / B each, also as [B, n, H, D]. pages and lens as in `append_paged`: lens[b] keys, the n new tokens' own the last of them. Token
-    i sees them all, with causal those up to its position lens[b] - n + i. Single tokens, pieces of prompts and whole ones may
-    share a call. scale: 1 / sqrt(D) if None.
+    T / B each, also as [B, n, H, D]. pages and lens as in `append_paged`: lens[b] keys, the n new tokens' own the last of them.
+    Token i sees them all, with causal those up to its position lens[b] - n + i. Single tokens, pieces of prompts and whole ones
+    may share a call. scale: 1 / sqrt(D) if None.
 
     Keys of pages outside the cache are left out. Cache rows from lens[b] on are never used; the values in use must be finite
     (those of a 4-bit cache within q's type), scores below 2^22 in magnitude. Values of 4 bits are used exactly as they are held.
 
     Returns out like q, with return_lse also the natural-log LSE [T, H] ([B, n, H]) in float32; a token that sees no key, and rows
-    behind the last sequence, give zeros and -inf. The same inputs give the same bits. There is no derivative: tensors that require a
-    gradient are refused unless gradients are off."""
+    behind the last sequence, give zeros and -inf. The same inputs give the same bits. There is no derivative: tensors that require
+    a gradient are refused unless gradients are off."""
     if q.is_cuda and q.dim() == 3:      # the operator checks everything itself; what it refuses is named by the checks below
         try:
             out = _ops().paged_attention(q.contiguous(), *cache, pages, lens, cu, bool(causal),

@@ -124,6 +124,6 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tenso
     if q.dim() == 3:
         return _ops().norm_rotate(q, k, q_weight, k_weight, table, positions, max(q.shape[0], 1), bool(halves), eps)
     shape, kshape = q.shape, k.shape
-    q, k = _ops().norm_rotate(q.flatten(0, 1), k.flatten(0, 1), q_weight, k_weight, table, positions, max(shape[1], 1), bool(halves),
-                              eps)
+    q, k = _ops().norm_rotate(q.flatten(0, 1), k.flatten(0, 1), q_weight, k_weight, table, positions, max(shape[1], 1),
+                              bool(halves), eps)
     return q.view(shape), k.view(kshape)
