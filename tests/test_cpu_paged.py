@@ -8,6 +8,7 @@ import re
 import pytest
 import torch
 
+import test_cpu_dma_wait_states as waits
 from self_trainable_or_free_attn_amd import (PagedCache, _lib, append_paged, norm_rotate, paged_attention, paged_cache, paged_rows,
                                             rotary_table)
 
@@ -330,3 +331,12 @@ def test_direct_operator_calls_check_their_tensors():
     x = torch.zeros(2, 2, 64, dtype=BF)
     with pytest.raises((RuntimeError, NotImplementedError)):
         ops.norm_rotate(x, x, None, None, rotary_table(2, 64), None, 2, False, 1e-6)
+
+
+# ------------------------------------------------------------------ transfers into LDS
+@pytest.mark.skipif(not os.path.exists(waits.HIPCC), reason="hipcc not installed")
+@pytest.mark.parametrize("extra", [[], ["-DES_ELEM_F16"], ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]])
+def test_transfers_keep_their_wait_states(extra):
+    asm = waits._compile("paged_fwd.hip", extra)
+    n = sum(1 for s in waits._instructions(asm) if s.split()[0].startswith("buffer_load") and s.endswith(" lds"))
+    assert n > 40 and not waits.violations(asm)
