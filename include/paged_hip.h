@@ -12,8 +12,7 @@
  *   table (P, R / 2, 2) float32     cosine and sine of each position and pair, R a multiple of 16 up to D; NULL (R = 0): no
  *                                   rotation. halves == 0: pair i is channels 2 i and 2 i + 1, otherwise i and i + R / 2.
  *                                   Positions past the last row take that row's angles, negative ones the first row's.
- *   pages (B, max_pages) int32      page numbers of a sequence; lens (B) int32: the tokens that it holds with the new ones,
- *                                   clamped to 0 .. max_pages * page_size
+ *   pages (B, max_pages) int32      page numbers of a sequence; lens (B) int32: its tokens with the new ones (below 0: 0)
  *   cu (B + 1) int32                running counts of new tokens as in packed_hip.h; NULL: T / B each
  *   cache, 16 bits                  k_pages, v_pages: (num_pages, Hk, page_size, D) with the strides page_stride, head_stride and
  *                                   row_stride (values) that both have
@@ -58,7 +57,7 @@ int es_norm_rotate_bwd_f16(const void* q, const void* k, const void* dq_out, con
 
 /* New tokens into the cache: k normed (k_weight) and rotated, v as it is; with q (T, H, D) also q_out (T, H, D) contiguous, q
  * normed and rotated at the same positions (q NULL, H 0: none). q_out rows of tokens without a position (behind the last
- * sequence, or negative) are zeros. Rows that two tokens of a call are held in get one of them. */
+ * sequence, or negative) are zeros. What two tokens of a call are held in at once is not defined. */
 int es_append_paged(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight, const float* table,
                     const int* pages, const int* lens, const int* cu, void* q_out, void* k_pages, void* v_pages, int B, int T,
                     int max_pages, int num_pages, int page_size, int H, int Hk, int D, int R, int P, int halves, int weight_f32,

@@ -76,6 +76,7 @@ struct FwdArgs {
 struct Job {
   const e16_t *k, *v;
   int q0, nq, nk, hk, r0, c0, c1, causal;
+  int over = 0;      // paged: tokens of the sequence past its last page, whose keys nothing holds
   const int* table;  // paged: the sequence's page numbers
   float* part;  // a partial of `part_rows` rows; nullptr: finished rows go to out / lse
   int part_rows;
@@ -86,7 +87,7 @@ __host__ __device__ constexpr int part_floats(int rows, int D) { return rows * (
 
 // keys that row r of the job's list sees
 __device__ __forceinline__ int keys_seen(const FwdArgs& a, const Job& j, int r) {
-  return j.causal ? min(max(divide(a.div_g, r) + 1 + j.nk - j.nq, 0), j.nk) : j.nk;
+  return j.causal ? min(max(divide(a.div_g, r) + 1 - j.nq + j.nk + j.over, 0), j.nk) : j.nk;
 }
 // chunks that any of the M rows of the job's tile sees
 template <int M>

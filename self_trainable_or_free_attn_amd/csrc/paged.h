@@ -55,13 +55,13 @@ __device__ __forceinline__ Place place_of(const Places& a, int t) {
   Place p = {-1, -1, 0};
   const int b = sequence_of(a, t);
   if (b >= a.B || t >= a.T) return p;
-  const int len = min((long long)max(a.lens[b], 0), (long long)a.max_pages << a.shift);
+  const int len = max(a.lens[b], 0);
   p.position = len - start_of(a, b + 1) + t;
   if (p.position < 0 || p.position >= len) {
     p.position = -1;
     return p;
   }
-  const int page = a.pages[(size_t)b * a.max_pages + (p.position >> a.shift)];
+  const int entry = p.position >> a.shift, page = entry < a.max_pages ? a.pages[(size_t)b * a.max_pages + entry] : -1;
   p.page = page >= 0 && page < a.num_pages ? page : -1;
   p.row = p.position & ((1 << a.shift) - 1);
   return p;

@@ -18,6 +18,10 @@ namespace {
 __device__ __forceinline__ int cached_keys(const FwdArgs& a, int b) {
   return b >= a.B ? 0 : __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.paged.cap));
 }
+// tokens that stand past the last page
+__device__ __forceinline__ int keys_over(const FwdArgs& a, int b) {
+  return b >= a.B ? 0 : __builtin_amdgcn_readfirstlane(max(a.lens[b], a.paged.cap)) - a.paged.cap;
+}
 
 // Page numbers of 64 groups of sixteen keys, a lane each: narrow tiles, whose waves take every fourth run of 32 keys, hold those of
 // 32 runs of their own, wide ones those of sixteen chunks. -1: missing; 0 where the sequence has no keys.
@@ -443,6 +447,7 @@ __device__ __forceinline__ void paged_job(const FwdArgs& a, Job& j, const Seq& s
   j.q0 = s.q0;
   j.nq = s.nq;
   j.nk = nk;
+  j.over = keys_over(a, b);
   j.hk = hk;
   j.causal = a.causal;
 }
@@ -590,8 +595,8 @@ struct Shares {
       return Share{number + 1, 0};
     }
     const int rows = paged_rows_of(a, seq), nk = paged_keys_of(a, seq), nq = divide(a.div_g, rows);
-    const int last = min((place + 1) * M, rows) - 1;
-    const int seen = a.causal ? min(max(divide(a.div_g, last) + 1 + nk - nq, 0), nk) : nk;
+    const int len = seq < a.B ? max(a.lens[seq], 0) : 0, last = min((place + 1) * M, rows) - 1;
+    const int seen = a.causal ? min(max(divide(a.div_g, last) + 1 - nq + len, 0), nk) : nk;
     const int chunks = (seen + BK - 1) / BK;
     return Share{number, max(min((int)((float)y / (float)tile_cost * (float)chunks), chunks - 1), 0)};
   }
@@ -648,7 +653,7 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_shares_ker
 // of a row side by side, each side with a maximum of its own, the sides added in order. Grid: (borders * Hk, rows of a tile / rows
 // of a workgroup): the first border within a tile has it merged, so the launch does not grow with the sequences, most of whose
 // tiles are whole, and a border says all that is to be known of its tile: one load a lane, then the pieces' (256 tokens against
-// 2000 keys, 32 heads over 8: attention 397 us with a workgroup a tile, 349 so; one sequence of 75600 keys among 49, whose tile has
+// 2000 keys, 32 heads over 8: attention 397 us with a workgroup a tile, 365 so; one sequence of 75600 keys among 49, whose tile has
 // half of the borders: 8 us piece after piece, 4.7 so).
 template <int D, int M>
 __global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {

@@ -168,8 +168,8 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, pages: tor
     to the even code. Values must be finite.
 
     Nothing is written for tokens behind the last sequence, of negative positions, past the named pages, or whose page number is
-    outside the cache; q's rows of the first two are zeros. A row that two tokens of a call share gets one of them: pages may be
-    shared for reading only. Returns the new q, contiguous and shaped like q, or None without q. There is no derivative: tensors
+    outside the cache; q's rows of the first two are zeros. What a row holds that two tokens of a call share is not defined: pages
+    may be shared for reading only. Returns the new q, contiguous and shaped like q, or None without q. There is no derivative: tensors
     that require a gradient are refused unless gradients are off."""
     if k.is_cuda and k.dim() == 3:      # the operator checks everything itself; what it refuses is named by the checks below
         try:
@@ -190,7 +190,8 @@ def paged_rows(cache: PagedCache, pages: torch.Tensor, lens: torch.Tensor, cu: O
                dtype: Optional[torch.dtype] = None):
     """(k, v) [rows, Hk, D]: what the cache holds of each sequence's last tokens, packed: cu[b + 1] - cu[b] of sequence b (int32
     [B + 1]), without cu rows / B. pages and lens as in `append_paged`; with running counts of lens it returns every sequence
-    whole. Zeros for rows behind the last sequence, tokens of negative positions and pages outside the cache. dtype: of the
+    whole. Zeros for rows behind the last sequence, tokens of negative positions or past the named pages, and pages outside the
+    cache. dtype: of the
     result, bf16 or fp16, the cache's own by default and at 16 bits."""
     four = cache.k_scales is not None
     dtype = dtype if dtype is not None else torch.bfloat16 if four else cache.k.dtype
@@ -232,7 +233,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, len
     Token i sees them all, with causal those up to its position lens[b] - n + i. Single tokens, pieces of prompts and whole ones
     may share a call. scale: 1 / sqrt(D) if None.
 
-    Keys of pages outside the cache are left out. Cache rows from lens[b] on are never used; the values in use must be finite
+    Keys past the named pages and of pages outside the cache are left out. Cache rows from lens[b] on are never used; the values in use must be finite
     (those of a 4-bit cache within q's type), scores below 2^22 in magnitude. Values of 4 bits are used exactly as they are held.
 
     Returns out like q, with return_lse also the natural-log LSE [T, H] ([B, n, H]) in float32; a token that sees no key, and rows

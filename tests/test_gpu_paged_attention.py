@@ -254,7 +254,7 @@ def test_an_empty_cache(dev, bits):
         out, lse = api.paged_attention(q, cache, pages, _ints([5, 0, 40], dev), return_lse=True)
         assert not out.any() and bool((lse == -math.inf).all())
         x = torch.randn(3, 2, 64, device=dev).to(BF)
-        assert torch.equal(api.append_paged(cache, x, x, pages, _ints([5, 1, 40], dev), q=q)[:1].any(), torch.tensor(width > 0, device=dev))
+        assert torch.equal(api.append_paged(cache, x, x, pages, _ints([5, 1, 40], dev), q=q), q)    # (nowhere held, all the same)
         k, v = api.paged_rows(cache, pages, _ints([5, 0, 40], dev), rows=3)
         assert not k.any() and not v.any()
     out = api.paged_attention(q[:0], cache, torch.zeros(1, 3, dtype=torch.int32, device=dev), _ints([5], dev))
@@ -272,6 +272,25 @@ def test_lengths_past_the_pages(dev, bits):
     far = api.paged_attention(q, cache, pages, _ints([10 ** 9, -5], dev), return_lse=True)
     want = api.paged_attention(q, cache, pages, _ints([32, 0], dev), return_lse=True)
     assert all(torch.equal(a, b) for a, b in zip(far, want))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n, width", [(1, 2), (7, 2), (40, 2), (90, 3), (1, 100), (5, 90), (300, 90)])
+def test_tokens_past_the_pages(dev, bits, causal, n, width):
+    """Sequences that have outgrown their rows of pages: each token keeps its position and sees what is held."""
+    api, page, H, D = _api(), 16, 4, 64
+    cap = width * page
+    g = torch.Generator(device=dev).manual_seed(15)
+    lens, keys = [n] * 5, [cap, cap + 1, cap + n, cap + n + 50, cap + n // 2]
+    cache = _filled(5 * width, 1, D, page, bits, BF, dev, g)
+    pages = torch.randperm(5 * width, device=dev, generator=g).to(torch.int32).view(5, width)
+    longer = torch.nn.functional.pad(pages, (0, -(-(n + 50) // page)), value=-1)
+    q = torch.randn(5 * n, H, D, device=dev, generator=g).to(BF)
+    out, lse = api.paged_attention(q, cache, pages, _ints(keys, dev), causal=causal, return_lse=True)
+    want_out, want_lse = _want(q, cache, longer, lens, keys, page, causal, D ** -0.5, BF)
+    packed_ref.check("out", out, *want_out)
+    packed_ref.check("lse", lse, *want_lse)
 
 
 @pytest.mark.parametrize("D, dtype", [(64, BF), (128, FP)])

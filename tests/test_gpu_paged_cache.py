@@ -226,6 +226,36 @@ def test_decoding_every_code(dev):
         assert torch.equal(k.double(), want) and torch.equal(v.double(), want), dtype
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_tokens_past_the_pages(dev, bits, n):
+    """Sequences that have outgrown their rows of pages: tokens past them go nowhere, and their queries keep their positions."""
+    api, page, D, width = _api(), 16, 64, 3
+    cap, g = width * page, torch.Generator(device=dev).manual_seed(16)
+    keys = [cap, cap + 1, cap + n // 2, cap + n, cap + n + 50, 2 ** 31 - 1]
+    B = len(keys)
+    q, k, v = (torch.randn(B * n, h, D, device=dev, generator=g).to(BF) for h in (4, 2, 2))
+    pages = torch.randperm(B * width, device=dev, generator=g).to(torch.int32).view(B, width)
+    cache = _noise(api.paged_cache(B * width, 2, D, page_size=page, bits=bits, device=dev), g)
+    before = [None if c is None else c.clone() for c in cache]
+    table = api.rotary_table(cap + n + 50, D, device=dev)
+    out = api.append_paged(cache, k, v, pages, _ints(keys, dev), q=q, table=table)
+    pos = torch.cat([torch.arange(m - n, m, device=dev) for m in keys])
+    ref.check("q", out, *ref.rotate(q, None, table[pos.clamp(max=len(table) - 1)], 1e-6, False)["y"])
+    new = pos < cap
+    at = pages.long()[torch.arange(B, device=dev).repeat_interleave(n)[new], pos[new] // page]
+    held = _values(cache, BF)
+    want = v[new].double() if bits == 16 else ref.held4(v[new].float(), BF)[0]
+    assert torch.equal(held[1][at, :, pos[new] % page], want)
+    touched = torch.zeros(B * width, page, dtype=torch.bool, device=dev)
+    touched[at, pos[new] % page] = True
+    for c, old in zip(cache, before):
+        if c is not None:
+            assert torch.equal(c.transpose(1, 2)[~touched], old.transpose(1, 2)[~touched])
+    rows_k, rows_v = api.paged_rows(cache, pages, _ints(keys, dev), rows=B * n, dtype=BF)
+    assert torch.equal(rows_v[new].double(), want) and not rows_k[~new].any() and not rows_v[~new].any()
+
+
 def test_layouts_of_a_cache(dev):
     """Rows of all heads side by side, keys and values in one allocation, pages far apart: the same contents."""
     api, Hk, D, page, keys = _api(), 3, 64, 16, [50, 20]
