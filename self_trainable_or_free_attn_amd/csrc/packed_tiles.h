@@ -546,38 +546,27 @@ struct Reciprocal {
 };
 __device__ __forceinline__ Cut cut(const ListShape& x, float per) { return Cut(x.tiles, x.chunks, x.rows, per, Reciprocal()); }
 
-// The shapes of the lists, K one behind the other a lane; up to 64 K are read once.
-template <class F, int K = 1>
+// The shapes of the lists, a lane each; up to 64 are read once.
+template <class F>
 struct Lists {
   const F& shape;
   int lists;
-  ListShape mine[K];
-  __device__ __forceinline__ Lists(const F& f, int n) : shape(f), lists(n) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      mine[k] = ListShape{0, 0, 0};
-      if (lane_id() * K + k < n) mine[k] = f(lane_id() * K + k);
-    }
+  ListShape mine;
+  __device__ __forceinline__ Lists(const F& f, int n) : shape(f), lists(n), mine{0, 0, 0} {
+    if (lane_id() < n) mine = f(lane_id());
   }
-  __device__ __forceinline__ ListShape at(int i0, int k) const {
-    if (i0 == 0) return mine[k];
-    const int i = i0 + lane_id() * K + k;
-    return i < lists ? shape(i) : ListShape{0, 0, 0};
+  __device__ __forceinline__ ListShape at(int i0) const {
+    if (i0 == 0) return mine;
+    return i0 + lane_id() < lists ? shape(i0 + lane_id()) : ListShape{0, 0, 0};
   }
 
   // `per`, and the longest item's chunks. (Sums in float32: every wave computes the same ones.)
   __device__ __forceinline__ float range_chunks(const FwdArgs& a, float& longest_item) const {
     float sum = 0.0f, most = 0.0f;
-    for (int i0 = 0; i0 < lists; i0 += 64 * K) {
-      float s = 0.0f, m = 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const ListShape x = at(i0, k);
-        s += (float)x.tiles * (float)x.chunks;
-        m = fmaxf(m, x.tiles > 0 ? (float)x.chunks : 0.0f);
-      }
-      sum += wave_sum_dpp(s);
-      most = fmaxf(most, wave_max_dpp(m));
+    for (int i0 = 0; i0 < lists; i0 += 64) {
+      const ListShape x = at(i0);
+      sum += wave_sum_dpp((float)x.tiles * (float)x.chunks);
+      most = fmaxf(most, wave_max_dpp(x.tiles > 0 ? (float)x.chunks : 0.0f));
     }
     const float fair = fair_share(sum, a.inv_slots);
     const int near = (int)parts(most, __builtin_amdgcn_rcpf(fair));
@@ -586,24 +575,13 @@ struct Lists {
     for (int n = max(near - 2, 1); n <= near; ++n) {
       const float per = fmaxf(parts(most, __builtin_amdgcn_rcpf((float)n)), fair);
       float size = 0.0f, big = 0.0f, work = 0.0f;
-      for (int i0 = 0; i0 < lists; i0 += 64 * K) {
-        float m = 0.0f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) m = fmaxf(m, cut(at(i0, k), per).size);
-        size = fmaxf(size, wave_max_dpp(m));
-      }
-      for (int i0 = 0; i0 < lists; i0 += 64 * K) {
-        float s = 0.0f, m = 0.0f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const ListShape x = at(i0, k);
-          const Cut c = cut(x, per);
-          const float items = (float)x.tiles * c.ranges;
-          m += 2.0f * c.size > size ? items : 0.0f;
-          s += items * c.size;
-        }
-        big += wave_sum_dpp(m);
-        work += wave_sum_dpp(s);
+      for (int i0 = 0; i0 < lists; i0 += 64) size = fmaxf(size, wave_max_dpp(cut(at(i0), per).size));
+      for (int i0 = 0; i0 < lists; i0 += 64) {
+        const ListShape x = at(i0);
+        const Cut c = cut(x, per);
+        const float items = (float)x.tiles * c.ranges;
+        big += wave_sum_dpp(2.0f * c.size > size ? items : 0.0f);
+        work += wave_sum_dpp(items * c.size);
       }
       const float time = fmaxf(ceilf(big * a.inv_slots) * size, work * a.inv_slots);
       if (time < 0.98f * least) {  // (more ranges for a shorter schedule only)
@@ -622,34 +600,19 @@ struct Lists {
     const bool leave = blockIdx.x == 0 && threadIdx.x < 64;
     int first = 0;
     Ranges found = {0, 0, 0};
-    for (int i0 = 0; i0 < lists; i0 += 64 * K) {
-      int ranges[K], items[K], early_items = 0, late_items = 0;
-      bool late[K];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const ListShape x = at(i0, k);
-        const Cut c = cut(x, per);
-        ranges[k] = (int)c.ranges;
-        items[k] = i0 + lane_id() * K + k < lists ? x.tiles * ranges[k] : 0;
-        late[k] = lists <= 64 * K && 2.0f * c.size <= longest;
-        (late[k] ? late_items : early_items) += items[k];
-      }
-      const int early_upto = wave_scan(early_items), early = __builtin_amdgcn_readlane(early_upto, 63);
-      const int late_upto = wave_scan(late_items);
-      int next_early = first + early_upto - early_items, next_late = first + early + late_upto - late_items;
-      int list = -1, list_ranges = 0, list_item0 = 0;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int i = i0 + lane_id() * K + k, item0 = late[k] ? next_late : next_early;
-        (late[k] ? next_late : next_early) += items[k];
-        if (leave && i < lists) a.plan[i] = make_int2(ranges[k], item0);
-        if (item0 <= w && w < item0 + items[k]) list = i, list_ranges = ranges[k], list_item0 = item0;
-      }
-      const unsigned long long hit = __builtin_amdgcn_ballot_w64(list >= 0);
+    for (int i0 = 0; i0 < lists; i0 += 64) {
+      const ListShape x = at(i0);
+      const Cut c = cut(x, per);
+      const int i = i0 + lane_id(), ranges = (int)c.ranges, items = i < lists ? x.tiles * ranges : 0;
+      const bool late = lists <= 64 && 2.0f * c.size <= longest;
+      const int early_upto = wave_scan(late ? 0 : items), early = __builtin_amdgcn_readlane(early_upto, 63);
+      const int late_upto = wave_scan(late ? items : 0);
+      const int item0 = first + (late ? early + late_upto : early_upto) - items;
+      if (leave && i < lists) a.plan[i] = make_int2(ranges, item0);
+      const unsigned long long hit = __builtin_amdgcn_ballot_w64(item0 <= w && w < item0 + items);
       if (hit) {
         const int from = __builtin_ctzll(hit);
-        found = Ranges{__builtin_amdgcn_readlane(list, from), __builtin_amdgcn_readlane(list_ranges, from),
-                       __builtin_amdgcn_readlane(list_item0, from)};
+        found = Ranges{i0 + from, __builtin_amdgcn_readlane(ranges, from), __builtin_amdgcn_readlane(item0, from)};
         if (!leave) break;
       }
       first += early + __builtin_amdgcn_readlane(late_upto, 63);
@@ -680,17 +643,13 @@ struct SharedLists {
   }
 };
 
-// item w of a list: its job's tile and chunks. LAST_FIRST: the list's last tiles first, which see the most keys under a causal mask
-// (partials stay in the order of the tiles); returns the partial's number.
-template <bool LAST_FIRST = false>
-__device__ __forceinline__ int take_range(const FwdArgs& a, Job& j, const Ranges& r, int w) {
-  const int i = w - r.item0, range = i % r.ranges, tiles = (j.nq * a.G + TILE - 1) / TILE;
-  const int tile = LAST_FIRST ? tiles - 1 - i / r.ranges : i / r.ranges;
-  j.r0 = tile * TILE;
+// item w of a list: its job's tile and chunks
+__device__ __forceinline__ void take_range(const FwdArgs& a, Job& j, const Ranges& r, int w) {
+  const int i = w - r.item0, range = i % r.ranges;
+  j.r0 = i / r.ranges * TILE;
   const int chunks = tile_chunks<TILE>(a, j);
   j.c0 = range_begin(chunks, range, r.ranges);
   j.c1 = range_begin(chunks, range + 1, r.ranges);
-  return r.item0 + tile * r.ranges + range;
 }
 
 // Partial `item` of a launch, all kv heads of an item side by side. Shared prefix: the prefix's items have a part of their own,

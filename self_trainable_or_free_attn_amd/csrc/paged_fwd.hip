@@ -7,6 +7,7 @@
 // Groups whose page number is outside the cache are missing: their scores become -inf, their values zeros.
 #include "packed_tiles.h"
 #include "paged.h"
+#include "paged_rules.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -123,8 +124,8 @@ struct Pages {
 
 // 4 bits, wide tiles: a thread loads 32 codes of a row and their scale a chunk ahead (D = 128: of keys and of values) and writes
 // them as token values where the transfers of 16 bits would have put them. Lanes have the rows in an order in which eight
-// neighbours write to different banks (in the order of memory, a row to four lanes, 1.5e7 cycles of conflicts instead of 7e5, and 32760
-// tokens, 24 heads, 7180 us instead of 7110).
+// neighbours write to different banks (in the order of memory, a row to four lanes, 1.5e7 cycles of conflicts instead of 7e5, and
+// 32760 tokens, 24 heads, 7180 us instead of 7110).
 template <int D>
 struct Codes {
   static constexpr bool HOLES = true, STAGED = true;
@@ -438,16 +439,16 @@ __device__ __forceinline__ void paged_tile(const FwdArgs& a, const Job& j, char*
 
 // the job of a tile of sequence b, its keys and rows
 template <int D, int BITS>
-__device__ __forceinline__ void paged_job(const FwdArgs& a, Job& j, const Seq& s, int b, int nk, int hk) {
+__device__ __forceinline__ void paged_job(const FwdArgs& a, Job& j, int q0, int nq, int b, int nk, int over, int hk) {
   j.table = a.paged.table + (size_t)(b < a.B ? b : 0) * a.paged.max_pages;
   if (BITS == 16) {
     j.k = a.paged.k + (size_t)hk * a.paged.head_stride;
     j.v = a.paged.v + (size_t)hk * a.paged.head_stride;
   }
-  j.q0 = s.q0;
-  j.nq = s.nq;
+  j.q0 = q0;
+  j.nq = nq;
   j.nk = nk;
-  j.over = keys_over(a, b);
+  j.over = over;
   j.hk = hk;
   j.causal = a.causal;
 }
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_whole_kern
   Job j;
   if (!tile_of<M, false>(a.cu_q, nullptr, a.B, a.Tq, 0, a.G, w, s, b, t, a.lens, a.paged.cap)) return;
   j.r0 = ((s.nq * a.G + M - 1) / M - 1 - t) * M;
-  paged_job<D, BITS>(a, j, s, b, s.nk, hk);
+  paged_job<D, BITS>(a, j, s.q0, s.nq, b, s.nk, keys_over(a, b), hk);
   j.part = nullptr;
   j.c0 = 0;
   j.c1 = tile_chunks<M>(a, j);
@@ -632,7 +633,7 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_shares_ker
       continue;
     }
     Job j;
-    paged_job<D, BITS>(a, j, s, seq, cached_keys(a, seq), hk);
+    paged_job<D, BITS>(a, j, s.q0, s.nq, seq, cached_keys(a, seq), keys_over(a, seq), hk);
     j.r0 = place * M;
     const int chunks = tile_chunks<M>(a, j);
     j.c0 = min(chunk, chunks);
@@ -649,39 +650,13 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_shares_ker
   }
 }
 
-// O of tiles that were cut: sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over the pieces. D / 4 lanes a row and piece, SIDE pieces
-// of a row side by side, each side with a maximum of its own, the sides added in order. Grid: (borders * Hk, rows of a tile / rows
-// of a workgroup): the first border within a tile has it merged, so the launch does not grow with the sequences, most of whose
-// tiles are whole, and a border says all that is to be known of its tile: one load a lane, then the pieces' (256 tokens against
-// 2000 keys, 32 heads over 8: attention 397 us with a workgroup a tile, 365 so; one sequence of 75600 keys among 49, whose tile has
-// half of the borders: 8 us piece after piece, 4.7 so).
-template <int D, int M>
-__global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
-  constexpr int LPR = D / 4, SIDE = 4, RPB = 256 / (LPR * SIDE);
-  const int w = blockIdx.x / a.Hk + 1, hk = blockIdx.x - (w - 1) * a.Hk, l = lane_id();
-  const int4* borders = reinterpret_cast<const int4*>(a.plan);
-  int4 x = borders[min(w - 1 + l, a.shares)];
-  const int tile = __builtin_amdgcn_readlane(x.x, 1), r0 = blockIdx.y * RPB;
-  const bool again = __builtin_amdgcn_readlane(x.x, 0) == tile && __builtin_amdgcn_readlane(x.y, 0) > 0;
-  if (__builtin_amdgcn_readlane(x.y, 1) == 0 || again) return;
-  const int q0 = __builtin_amdgcn_readlane(x.z, 1), place = __builtin_amdgcn_readlane(x.w, 1), rows = place % 64, t = place / 64;
-  if (r0 >= rows) return;
-  // the shares that have a piece of it, in order: the one before the border the beginning, in its second slot, the others in their
-  // first; two borders may stand at one place
-  __shared__ int pieces[256 * ES_PAGED_RESIDENT(D, M) + 1];
-  if (threadIdx.x == 0) pieces[0] = w - 1;
-  int n = 1;
-  for (int i0 = w - 1;; i0 += 62) {  // (lanes 1 to 62, which see the next border)
-    if (i0 >= w) x = borders[min(i0 + l, a.shares)];
-    const int next = __shfl(x.x, min(l + 1, 63), 64), next_chunk = __shfl(x.y, min(l + 1, 63), 64);
-    const bool within = l >= 1 && l <= 62 && i0 + l < a.shares && x.x == tile;
-    const bool mine = within && (next != tile || next_chunk > x.y);
-    const unsigned long long hit = __builtin_amdgcn_ballot_w64(mine);
-    if (mine && threadIdx.x < 64) pieces[n + __builtin_popcountll(hit & ((1ull << l) - 1))] = i0 + l;
-    n += __builtin_popcountll(hit);
-    if (!__builtin_amdgcn_readlane((int)within, 62)) break;
-  }
-  __syncthreads();
+// O of rows r0 + 0 .. of a tile that was cut: sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over the n pieces, whose partials (M
+// rows each) are numbered in `pieces`. D / 4 lanes a row and piece, SIDE pieces of a row side by side, each side with a maximum of
+// its own, the sides added in order. A workgroup does merge_rows_of(D, SIDE) rows.
+constexpr int merge_rows_of(int D, int side) { return 256 / (D / 4 * side); }
+template <int D, int M, int SIDE>
+__device__ __forceinline__ void merge_rows(const FwdArgs& a, const int* pieces, int n, int hk, int q0, int row0, int r0, int rows) {
+  constexpr int LPR = D / 4, RPB = merge_rows_of(D, SIDE);
   const int lane = threadIdx.x % LPR, c = lane * 4, side = threadIdx.x / LPR % SIDE, local = threadIdx.x / (LPR * SIDE);
   const int r = min(r0 + local, rows - 1);
   float top = -INFINITY, sum = 0.0f;
@@ -691,10 +666,13 @@ __global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
     float m[4], z[4], most = top;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int k = min(i + e * SIDE, n - 1);
-      const float* p = partial<D>(a.part, M, a, 2 * pieces[k] + (k == 0), hk);
+      o[e] = f32x4{};
+      m[e] = -INFINITY;
+      z[e] = 0.0f;
+      if (i + e * SIDE >= n) continue;
+      const float* p = partial<D>(a.part, M, a, pieces[i + e * SIDE], hk);
       o[e] = *reinterpret_cast<const f32x4*>(p + 2 * M + r * D + c);
-      m[e] = i + e * SIDE < n ? p[r] : -INFINITY;
+      m[e] = p[r];
       z[e] = p[M + r];
     }
 #pragma unroll
@@ -711,74 +689,344 @@ __global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
     }
     top = most;
   }
-  __shared__ f32x4 sums[SIDE][RPB][LPR];
-  __shared__ float2 weights[SIDE][RPB];  // maximum, sum
-  sums[side][local][lane] = acc;
-  if (lane == 0) weights[side][local] = make_float2(top, sum);
-  __syncthreads();
-  if (side != 0 || r0 + local >= rows) return;
-  float2 s[SIDE];
+  if constexpr (SIDE > 1) {
+    __shared__ f32x4 sums[SIDE][RPB][LPR];
+    __shared__ float2 weights[SIDE][RPB];  // maximum, sum
+    sums[side][local][lane] = acc;
+    if (lane == 0) weights[side][local] = make_float2(top, sum);
+    __syncthreads();
+    if (side != 0) return;
+    float2 s[SIDE];
 #pragma unroll
-  for (int i = 0; i < SIDE; ++i) {
-    s[i] = weights[i][local];
-    top = fmaxf(top, s[i].x);
-  }
-  acc = f32x4{};
-  sum = 0.0f;
+    for (int i = 0; i < SIDE; ++i) {
+      s[i] = weights[i][local];
+      top = fmaxf(top, s[i].x);
+    }
+    acc = f32x4{};
+    sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < SIDE; ++i) {
-    const float f = s[i].x == -INFINITY ? 0.0f : exp2f_fast(s[i].x - top);
-    acc += f * sums[i][local][lane];
-    sum = fmaf(f, s[i].y, sum);
+    for (int i = 0; i < SIDE; ++i) {
+      const float f = s[i].x == -INFINITY ? 0.0f : exp2f_fast(s[i].x - top);
+      acc += f * sums[i][local][lane];
+      sum = fmaf(f, s[i].y, sum);
+    }
   }
-  const int row = t * M + r, tok = divide(a.div_g, row);
+  if (r0 + local >= rows) return;
+  const int row = row0 + r, tok = divide(a.div_g, row);
   const size_t at = ((size_t)(q0 + tok) * a.Hk + hk) * a.G + (row - tok * a.G);
   store_row<D>(a, at, c, acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
   if (c == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top - P_SHIFT + log2f(sum)) * PK_LN2;
 }
 
-// ------------------------------------------------------------------------------------------------ wide tiles: key ranges
-// Launches with wide tiles are bound by the matrix units, and tiles that read the same keys side by side have them from L2: these
-// are cut into ranges as in packed_tiles.h, the last tiles of a sequence first. (Equal shares, whose pieces start anywhere: 4096
-// tokens of 32 heads over 8 alone 228 us, ranges 168; 32760 of 24 heads 7100 and 6480, whole tiles 6170. 4096 tokens beside one
-// that sees 75600 keys: whole tiles 572, ranges 224.) List i: the rows of sequence i, list B: those behind the last one.
-struct PagedLists {
+// Tiles that were cut. Grid: (borders * Hk, rows of a tile / rows of a workgroup): the first border within a tile has it merged,
+// so the launch does not grow with the sequences, most of whose tiles are whole, and a border says all that is to be known of its
+// tile: one load a lane, then the pieces' (256 tokens against 2000 keys, 32 heads over 8: attention 397 us with a workgroup a tile,
+// 365 so; one sequence of 75600 keys among 49, whose tile has half of the borders: 8 us piece after piece, 4.7 so).
+template <int D, int M>
+__global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
+  constexpr int RPB = merge_rows_of(D, 4);
+  const int w = blockIdx.x / a.Hk + 1, hk = blockIdx.x - (w - 1) * a.Hk, l = lane_id();
+  const int4* borders = reinterpret_cast<const int4*>(a.plan);
+  int4 x = borders[min(w - 1 + l, a.shares)];
+  const int tile = __builtin_amdgcn_readlane(x.x, 1), r0 = blockIdx.y * RPB;
+  const bool again = __builtin_amdgcn_readlane(x.x, 0) == tile && __builtin_amdgcn_readlane(x.y, 0) > 0;
+  if (__builtin_amdgcn_readlane(x.y, 1) == 0 || again) return;
+  const int q0 = __builtin_amdgcn_readlane(x.z, 1), place = __builtin_amdgcn_readlane(x.w, 1), rows = place % 64, t = place / 64;
+  if (r0 >= rows) return;
+  // the shares that have a piece of it, in order: the one before the border the beginning, in its second slot, the others in their
+  // first; two borders may stand at one place
+  __shared__ int pieces[256 * ES_PAGED_RESIDENT(D, M) + 1];
+  if (threadIdx.x == 0) pieces[0] = 2 * (w - 1) + 1;
+  int n = 1;
+  for (int i0 = w - 1;; i0 += 62) {  // (lanes 1 to 62, which see the next border)
+    if (i0 >= w) x = borders[min(i0 + l, a.shares)];
+    const int next = __shfl(x.x, min(l + 1, 63), 64), next_chunk = __shfl(x.y, min(l + 1, 63), 64);
+    const bool within = l >= 1 && l <= 62 && i0 + l < a.shares && x.x == tile;
+    const bool mine = within && (next != tile || next_chunk > x.y);
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(mine);
+    if (mine && threadIdx.x < 64) pieces[n + __builtin_popcountll(hit & ((1ull << l) - 1))] = 2 * (i0 + l);
+    n += __builtin_popcountll(hit);
+    if (!__builtin_amdgcn_readlane((int)within, 62)) break;
+  }
+  __syncthreads();
+  merge_rows<D, M, 4>(a, pieces, n, hk, q0, t * M, r0, rows);
+}
+
+// ------------------------------------------------------------------------------------------------ wide tiles: pieces
+// Launches with wide tiles are bound by the matrix units, and tiles that read the same keys side by side have them from L2: tiles
+// are cut into pieces (paged_rules.h) that fill the GPU about once, one level of all tiles after the other. (Equal shares, whose
+// pieces start anywhere: 4096 tokens of 32 heads over 8 alone 228 us, pieces 155. One count of ranges for all tiles of a sequence,
+// as packed_tiles.h has it, which takes a causal prompt for twice its work: prompts of 3923, 938 and 3440 tokens, 8 heads of 64
+// over one, 114 us, pieces 79; 256 and 512 tokens over 9000 and 512 keys beside two small ones, 24 heads over 8, 65 and 56.)
+// Every wave derives the cut from the lengths by itself, so they stay on the device: of sizes from the fair share on the one with
+// the shortest schedule, by a model of it. Items over three quarters of the largest come first, then those over a half, over a
+// quarter and the rest, since workgroups are dispatched in order. Lanes have LISTS sequences each, 64 apart; more than 64 * LISTS
+// are read once a pass and keep their order.
+struct WideItem {
+  int list, tile, level, piece;  // list < 0: none
+};
+// What the first workgroup leaves for the merge, behind it (first item, first cut tile) of each list.
+struct WidePlan {
+  int per, above, cut_tiles, pad;
+};
+struct Wide {
+  WideList x;
+  int q0, nq;
+  __device__ __forceinline__ int keys(const FwdArgs& a) const { return min(nq - x.behind, a.paged.cap); }
+  __device__ __forceinline__ int over(const FwdArgs& a) const { return nq - x.behind - keys(a); }
+};
+__device__ __forceinline__ Wide wide_of(const FwdArgs& a, int b) {
+  Wide w;
+  w.q0 = seq_start(a.cu_q, b, a.B, a.Tq);
+  w.nq = max((b < a.B ? seq_start(a.cu_q, b + 1, a.B, a.Tq) : a.Tq) - w.q0, 0);
+  const int rows = w.nq * a.G, len = b < a.B ? max(a.lens[b], 0) : 0, head = divide(a.div_g, max(min(rows, TILE) - 1, 0)) + 1;
+  w.x = wide_list(rows, w.nq, len, min(len, a.paged.cap), head, a.causal);
+  return w;
+}
+// lane `from`'s
+__device__ __forceinline__ Wide wide_at(const Wide& w, int from) {
+  auto at = [&](int v) { return __builtin_amdgcn_readlane(v, from); };
+  return Wide{WideList{at(w.x.rows), at(w.x.tiles), at(w.x.chunks), at(w.x.behind), at(w.x.first)}, at(w.q0), at(w.nq)};
+}
+// sums of a row of sixteen lanes, on its last one
+__device__ __forceinline__ float row_sum(float x) {
+  x += __int_as_float(dpp_i<0x111>(__float_as_int(x)));
+  x += __int_as_float(dpp_i<0x112>(__float_as_int(x)));
+  x += __int_as_float(dpp_i<0x114>(__float_as_int(x)));
+  return x + __int_as_float(dpp_i<0x118>(__float_as_int(x)));
+}
+constexpr int CUTS = 16;  // sizes of pieces that are looked at
+// A plan, page numbers and first keys take about 8 us, a chunk 2.1, with D = 64 1.1; a merge 5 more where tiles are cut.
+template <int D>
+constexpr float START = D == 128 ? 3.5f : 7.0f;
+template <int D>
+struct WideLists {
   const FwdArgs& a;
-  __device__ __forceinline__ ListShape operator()(int b) const {
-    const int rows = paged_rows_of(a, b), nk = paged_keys_of(a, b);
-    return ListShape{(rows + TILE - 1) / TILE, (nk + BK - 1) / BK, rows};
+  int lists, classes;
+  bool few;  // a row of sixteen lanes has all lists, each row the same
+  Wide mine[LISTS];
+
+  __device__ __forceinline__ Wide load(int i) const { return i < lists ? wide_of(a, i) : Wide{}; }
+  __device__ __forceinline__ explicit WideLists(const FwdArgs& args)
+      : a(args), lists(args.B + 1), classes(lists <= 64 * LISTS ? 4 : 1), few(lists <= 16) {
+    mine[0] = load(few ? lane_id() & 15 : lane_id());
+#pragma unroll
+    for (int k = 1; k < LISTS; ++k) mine[k] = 64 * k < lists ? load(64 * k + lane_id()) : Wide{};
+  }
+  // each list once
+  __device__ __forceinline__ WideList at(int i0, int k) const {
+    if (i0 > 0) return load(i0 + 64 * k + lane_id()).x;
+    return few && lane_id() >= 16 ? WideList{} : mine[k].x;
+  }
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i0 = 0; i0 < lists; i0 += 64 * LISTS) {
+#pragma unroll
+      for (int k = 0; k < LISTS; ++k)
+        if (i0 + 64 * k < lists) f(at(i0, k));
+    }
+  }
+  // items of at most this many chunks are in a class behind class k
+  __device__ __forceinline__ int bound(int longest, int k) const { return classes == 1 ? -1 : longest * (3 - k) / 4; }
+
+  struct Load {
+    float big, small, later;  // items of class 0, the others' time, pieces above level 0
+  };
+  __device__ __forceinline__ void add(Load& s, const WideList& x, int per) const {
+    const int rest = tiles_within(x, a.G, a.causal, bound(per, 0)), more = later_pieces(x, a.G, a.causal, piece_of(x, per));
+    s.big += (float)(x.tiles - rest + more);
+    s.small += (float)rest * (0.5f * (float)(min(x.first, x.chunks) + min(x.chunks, bound(per, 0))) + START<D>);
+    s.later += (float)more;
+  }
+
+  // Chunks a piece. The waves look at some sizes each, with up to 16 lists each row of lanes at one. times: [CUTS] in LDS.
+  __device__ __forceinline__ int cut(float* times) const {
+    float sum = 0.0f, top = 0.0f;
+    each([&](const WideList& x) {
+      sum += (float)x.tiles * (0.5f * (float)(x.first + x.chunks) + 0.5f);
+      top = fmaxf(top, x.tiles > 0 ? (float)x.chunks : 0.0f);
+    });
+    const int most = max((int)wave_max_dpp(top), 1);
+    const float mean = wave_sum_dpp(sum) * a.inv_slots;
+    const int least = max((int)ceilf(fminf(mean, (float)most)), 4);
+    if (least >= most) return most;
+    const int wave = threadIdx.x >> 6;
+    auto size = [&](int i) { return i < CUTS - 1 ? min(least + (least * i + 11) / 12, most) : most; };  // (at last: no tile is cut)
+    auto time = [&](const Load& s, int per) {
+      const float t = wide_time(s.big, (float)per, s.small, mean, s.later > 0.0f, START<D>, a.inv_slots);
+      return s.later <= (float)(a.items - a.tiles) ? t : INFINITY;
+    };
+    if (few) {
+      const int i = 4 * wave + (lane_id() >> 4), per = size(i);
+      Load s = {};
+      add(s, mine[0].x, per);
+      s.big = row_sum(s.big);
+      s.small = row_sum(s.small);
+      s.later = row_sum(s.later);
+      if ((lane_id() & 15) == 15) times[i] = time(s, per);
+    } else {
+      for (int i = wave; i < CUTS; i += 4) {
+        const int per = size(i);
+        Load s = {};
+        each([&](const WideList& x) { add(s, x, per); });
+        s.big = wave_sum_dpp(s.big);
+        s.small = wave_sum_dpp(s.small);
+        s.later = wave_sum_dpp(s.later);
+        if (lane_id() == 0) times[i] = time(s, per);
+      }
+    }
+    __syncthreads();
+    int best = most;
+    float shortest = times[CUTS - 1];
+#pragma unroll
+    for (int i = 0; i < CUTS - 1; ++i) {
+      const float t = times[i];
+      if (t < shortest) {
+        shortest = t;
+        best = size(i);
+      }
+    }
+    return __builtin_amdgcn_readfirstlane(best);
+  }
+
+  // item w, and its list
+  __device__ __forceinline__ WideItem find(int w, float* times, Wide& own) const {
+    const int per = cut(times), l = lane_id();
+    const bool leave = blockIdx.x == 0 && threadIdx.x < 64;
+    int2* plan = a.plan + 2;
+    int first = 0, cut_tiles = 0, list = -1, kind = 0, number = 0;
+    for (int i0 = 0; i0 < lists; i0 += 64 * LISTS) {
+      int upto[LISTS][4], count[LISTS][4], base[4] = {}, all = 0;
+#pragma unroll
+      for (int k = 0; k < LISTS; ++k) {
+        if (i0 + 64 * k >= lists) continue;
+        const WideList x = at(i0, k);
+        int before = tiles_within(x, a.G, a.causal, bound(per, 0));
+        count[k][0] = x.tiles - before + later_pieces(x, a.G, a.causal, piece_of(x, per));
+#pragma unroll
+        for (int c = 1; c < 4; ++c) {
+          const int rest = c < 3 ? tiles_within(x, a.G, a.causal, bound(per, c)) : 0;
+          count[k][c] = before - rest;
+          before = rest;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          upto[k][c] = wave_scan(count[k][c]);
+          base[c] += __builtin_amdgcn_readlane(upto[k][c], 63);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int n = base[c];
+        base[c] = first + all;
+        all += n;
+      }
+#pragma unroll
+      for (int k = 0; k < LISTS; ++k) {
+        if (i0 + 64 * k >= lists) continue;
+        const int i = i0 + 64 * k + l;
+        if (leave) {
+          const WideList x = at(i0, k);
+          const int cuts = x.tiles - tiles_within(x, a.G, a.causal, piece_of(x, per)), cut_upto = wave_scan(cuts);
+          if (i < lists) plan[i] = make_int2(base[0] + upto[k][0] - count[k][0], cut_tiles + cut_upto - cuts);
+          cut_tiles += __builtin_amdgcn_readlane(cut_upto, 63);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int item0 = base[c] + upto[k][c] - count[k][c];
+          base[c] += __builtin_amdgcn_readlane(upto[k][c], 63);
+          if (item0 <= w && w < item0 + count[k][c]) list = i, kind = c, number = w - item0;
+        }
+      }
+      first += all;
+      if (!leave && __builtin_amdgcn_ballot_w64(list >= 0)) break;
+    }
+    if (leave && l == 0) *reinterpret_cast<WidePlan*>(a.plan) = WidePlan{per, bound(per, 0), cut_tiles, 0};
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(list >= 0);
+    if (hit == 0) return WideItem{-1};
+    const int from = __builtin_ctzll(hit);
+    list = __builtin_amdgcn_readlane(list, from);
+    kind = __builtin_amdgcn_readlane(kind, from);
+    number = __builtin_amdgcn_readlane(number, from);
+    if (list < 64) own = wide_at(mine[0], from);
+    else own = wide_at(wide_of(a, list), 0);
+    const int piece = piece_of(own.x, per);
+    WideItem item = {list, 0, 0};
+    if (kind > 0) item.tile = tiles_within(own.x, a.G, a.causal, bound(per, kind - 1)) - 1 - number;
+    else if (!piece_at(own.x, a.G, a.causal, piece, bound(per, 0), number, item.tile, item.level)) item.list = -1;
+    item.piece = piece;
+    return item;
   }
 };
 
 // grid: items * Hk
 template <int D, int BITS>
-__global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, TILE)) void paged_ranges_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, TILE)) void paged_pieces_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[paged_lds<D, TILE>()];
   __shared__ float stats[4 * 128];
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
-  const PagedLists shape{a};
-  const Lists<PagedLists, LISTS> lists(shape, a.B + 1);
-  const Ranges r = lists.find(a, w);
-  if (r.ranges == 0) return;
-  const Seq s = sequence(a.cu_q, nullptr, a.B, a.Tq, 0, r.list);
+  __shared__ float times[CUTS];
+  Wide own;
+  const WideItem item = WideLists<D>(a).find(w, times, own);
+  if (item.list < 0) return;
   Job j;
-  paged_job<D, BITS>(a, j, s, r.list, cached_keys(a, r.list), hk);
-  const int number = take_range<true>(a, j, r, w);
+  paged_job<D, BITS>(a, j, own.q0, own.nq, item.list, own.keys(a), own.over(a), hk);
+  j.r0 = item.tile * TILE;
+  const int chunks = tile_chunks<TILE>(a, j), n = pieces_of(chunks, item.piece);
+  j.c0 = range_begin(chunks, item.level, n);
+  j.c1 = range_begin(chunks, item.level + 1, n);
   j.part_rows = TILE;
-  j.part = r.ranges == 1 ? nullptr : partial<D>(a.part, TILE, a, number, hk);
+  j.part = n == 1 ? nullptr : partial<D>(a.part, TILE, a, w, hk);
   paged_tile<D, BITS, TILE>(a, j, lds, stats);
+}
+
+// Their tiles that were cut, numbered list by list, the last ones first. Grid: (as many as there can be * Hk, parts of their rows).
+template <int D>
+__global__ __launch_bounds__(256) void merge_pieces_kernel(FwdArgs a) {
+  constexpr int MOST = 256 * ES_PAGED_RESIDENT(D, TILE) + 2;  // pieces of a tile: as many as fill the GPU
+  const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
+  const WidePlan plan = *reinterpret_cast<const WidePlan*>(a.plan);
+  int2 first = a.plan[2 + min(lane_id(), a.B)];
+  if (w >= plan.cut_tiles) return;
+  int list = 0;
+  for (int i0 = 0; i0 <= a.B; i0 += 64) {  // the last list that starts at or before w and has cut tiles
+    if (i0 > 0) first = a.plan[2 + min(i0 + lane_id(), a.B)];
+    const unsigned long long upto = __builtin_amdgcn_ballot_w64(i0 + lane_id() <= a.B && first.y <= w);
+    if (upto == 0) break;
+    list = i0 + 63 - __builtin_clzll(upto);
+    if (!(upto >> 63)) break;
+  }
+  const int2 left = a.plan[2 + list];
+  const Wide own = wide_at(wide_of(a, list), 0);
+  const int piece = piece_of(own.x, plan.per), t = __builtin_amdgcn_readfirstlane(own.x.tiles - 1 - (w - left.y));
+  if (t < 0) return;
+  const int rows = min(own.x.rows - t * TILE, TILE), last = divide(a.div_g, t * TILE + rows - 1);
+  const int seen = a.causal ? min(max(last + 1 - own.x.behind, 0), own.keys(a)) : own.keys(a);
+  const int n = min(pieces_of((seen + BK - 1) / BK, piece), MOST);
+  __shared__ int pieces[MOST];
+  for (int i = threadIdx.x; i < n; i += 256) pieces[i] = left.x + piece_number(own.x, a.G, a.causal, piece, plan.above, t, i);
+  __syncthreads();
+  auto merge = [&](auto side) {
+    constexpr int S = decltype(side)::value, RPB = merge_rows_of(D, S);
+    for (int r0 = blockIdx.y * RPB; r0 < rows; r0 += gridDim.y * RPB) {
+      merge_rows<D, TILE, S>(a, pieces, n, hk, own.q0, t * TILE, r0, rows);
+      __syncthreads();
+    }
+  };
+  if (n <= 8) merge(std::integral_constant<int, 1>{});
+  else merge(std::integral_constant<int, 4>{});
 }
 
 }  // namespace
 
 // What a call launches.
-enum PagedForm { WHOLE_TILES, SHARES, RANGES };
+enum PagedForm { WHOLE_TILES, SHARES, PIECES };
 struct PagedPlan {
   PagedForm form;
   int M;               // rows a tile
   long long tiles;     // tile numbers of a head
-  int shares, items;   // a head: SHARES, RANGES
-  size_t plan, bytes;  // workspace: partials, then borders (SHARES) or ranges (RANGES)
+  int shares, items;   // a head: SHARES, PIECES
+  size_t plan, bytes;  // workspace: partials, then borders (SHARES) or the cut (PIECES)
 };
 
 // `cap`: the keys that a sequence can have. equal: B sequences of Tq / B tokens. Up to 1024 keys a tile is short enough for one
@@ -792,7 +1040,7 @@ static PagedPlan paged_plan(int B, int Tq, int cap, int H, int Hk, int D, int bi
   p.tiles = !tokens     ? tile_numbers<TILE>(B, Tq, G)
             : bits == 4 ? tile_numbers<TOKENS<4>>(B, Tq, G)
                         : tile_numbers<TOKENS<16>>(B, Tq, G);
-  p.form = cap <= 1024 ? WHOLE_TILES : tokens ? SHARES : RANGES;
+  p.form = cap <= 1024 ? WHOLE_TILES : tokens ? SHARES : PIECES;
   if (p.form == WHOLE_TILES && !tokens && p.tiles * Hk <= (D == 64 ? 768 : 384)) {  // (as for packed sequences)
     p.M = TILE / 2;
     p.tiles = tile_numbers<TILE / 2>(B, Tq, G);
@@ -802,10 +1050,10 @@ static PagedPlan paged_plan(int B, int Tq, int cap, int H, int Hk, int D, int bi
     p.shares = std::max(slots / Hk, 1);
     p.plan = (size_t)2 * p.shares * Hk * part_floats(p.M, D) * sizeof(float);
     p.bytes = p.plan + (size_t)(p.shares + 1) * sizeof(int4);
-  } else if (p.form == RANGES) {
-    p.items = (int)(p.tiles + slots / Hk + 1);  // (as range_items)
+  } else if (p.form == PIECES) {
+    p.items = (int)(p.tiles + slots / Hk + 1);
     p.plan = (size_t)p.items * Hk * part_floats(p.M, D) * sizeof(float);
-    p.bytes = p.plan + (size_t)(B + 1) * sizeof(int2);
+    p.bytes = p.plan + sizeof(WidePlan) + (size_t)(B + 1) * sizeof(int2);
   }
   return p;
 }
@@ -865,16 +1113,16 @@ static int paged_fwd(FwdArgs& a, const void* q, const int* pages, const int* len
         hipLaunchKernelGGL((paged_shares_kernel<d, n, m>), dim3((unsigned)(p.shares * Hk)), dim3(256), 0, stream, a);
         if (p.shares > 1)
           hipLaunchKernelGGL((merge_shares_kernel<d, m>),
-                             dim3((unsigned)((p.shares - 1) * Hk), (unsigned)((rows_most * d + 255) / 256)), dim3(256), 0, stream, a);
+                             dim3((unsigned)((p.shares - 1) * Hk), (unsigned)((rows_most * d + 255) / 256)), dim3(256), 0,
+                             stream, a);
         return;
       }
     } else if constexpr (m == TILE) {
-      if (p.form == RANGES) {
-        hipLaunchKernelGGL((paged_ranges_kernel<d, n>), dim3((unsigned)(p.items * Hk)), dim3(256), 0, stream, a);
-        // (a workgroup for 8 rows at D = 128, more where there are many tiles, most of which are then whole)
-        const long long most = (rows_most * d / 4 + 255) / 256, few = std::max<long long>(4096 / (p.tiles * Hk), 1);
-        hipLaunchKernelGGL((merge_kernel<d, false>), dim3((unsigned)(p.tiles * Hk), (unsigned)std::min(most, few)), dim3(256), 0,
-                           stream, a);
+      if (p.form == PIECES) {
+        hipLaunchKernelGGL((paged_pieces_kernel<d, n>), dim3((unsigned)(p.items * Hk)), dim3(256), 0, stream, a);
+        const long long cuts = std::min<long long>(p.tiles, p.items - p.tiles), side = merge_rows_of(d, 1);
+        hipLaunchKernelGGL((merge_pieces_kernel<d>), dim3((unsigned)(cuts * Hk), (unsigned)((rows_most + side - 1) / side)),
+                           dim3(256), 0, stream, a);
         return;
       }
     }

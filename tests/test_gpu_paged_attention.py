@@ -208,6 +208,20 @@ def test_few_sequences_have_most_of_the_tokens(dev, bits, G, lens):
             _case(dev, lens, keys, 2 * G, 2, 64, FP, 32, bits, seed=22, causal=causal, width=200)
 
 
+@pytest.mark.parametrize("D, dtype", [(64, BF), (128, FP)])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("B", [1, 2, 15, 16, 63, 64, 255, 256])
+def test_cuts_of_wide_tiles(dev, D, dtype, bits, causal, B):
+    """Prompts, pieces and single tokens of every length: tiles that are cut into none to many pieces, of as many sequences as rows
+    of lanes, waves and passes hold, the rows behind the last one among them."""
+    for many in (False, True):
+        n = lambda i: [700, 40, 1, 90][i % 4] if B < 60 or i % 40 < 2 else 1 + i % 3
+        lens = [n(i) for i in range(B)]
+        keys = [m + [0, 1500, 130, 5000][i % 4] // (1 if B < 60 or i % 20 == 3 else 50) if i % 9 < 8 else m // 2 for i, m in enumerate(lens)]
+        _case(dev, lens, keys, 6 if many else 1, 2 if many else 1, D, dtype, 32, bits, seed=23, causal=causal, pad=B % 3)
+
+
 @pytest.mark.parametrize("seed", range(24))
 def test_random_batches(dev, seed):
     """Any mix of tokens, pieces and prompts, heads, pages and holes, tables of pages longer than needed (so that the call cuts)."""
