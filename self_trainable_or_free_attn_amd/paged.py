@@ -191,10 +191,22 @@ def paged_rows(cache: PagedCache, pages: torch.Tensor, lens: torch.Tensor, cu: O
     """(k, v) [rows, Hk, D]: what the cache holds of each sequence's last tokens, packed: cu[b + 1] - cu[b] of sequence b (int32
     [B + 1]), without cu rows / B. pages and lens as in `append_paged`; with running counts of lens it returns every sequence
     whole. Zeros for rows behind the last sequence, tokens of negative positions or past the named pages, and pages outside the
-    cache. dtype: of the
-    result, bf16 or fp16, the cache's own by default and at 16 bits."""
-    four = cache.k_scales is not None
-    dtype = dtype if dtype is not None else torch.bfloat16 if four else cache.k.dtype
+    cache. dtype: of the result, bf16 or fp16, the cache's own by default and at 16 bits."""
+    if dtype is None:
+        dtype = cache.k.dtype if cache.k_scales is None else torch.bfloat16
+    if cache.k.is_cuda:      # the operator checks everything itself; what it refuses is named by the checks below
+        try:
+            return _ops().paged_rows(*cache, pages, lens, cu, rows, dtype)
+        except (RuntimeError, TypeError):
+            _check_rows(cache, pages, lens, cu, rows, dtype)
+            raise
+    _check_rows(cache, pages, lens, cu, rows, dtype)
+    _check_gpu(cache.k)
+    return _ops().paged_rows(*cache, pages, lens, cu, rows, dtype)
+
+
+def _check_rows(cache, pages, lens, cu, rows, dtype):
+    """The arguments of paged_rows."""
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise TypeError(f"dtype must be bfloat16 or float16, got {dtype}")
     device = cache.k.device
@@ -202,8 +214,6 @@ def paged_rows(cache: PagedCache, pages: torch.Tensor, lens: torch.Tensor, cu: O
     if not 0 <= rows < MAX_TOKENS:
         raise ValueError(f"rows must be 0 to {MAX_TOKENS - 1}, got {rows}")
     _check_places(pages, lens, cu, size, rows, device)
-    _check_gpu(cache.k)
-    return _ops().paged_rows(cache.k, cache.v, cache.k_scales, cache.v_scales, pages, lens, cu, int(rows), dtype)
 
 
 def _check_attention(q, cache, pages, lens, cu, scale):

@@ -85,3 +85,20 @@ def test_tensors_of_the_host_are_refused(dev):
                  lambda: norm_rotate(x, x, table=rotary_table(3, 64)), lambda: norm_rotate(x, x.cpu(), table=rotary_table(3, 64, device=dev))):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("kw, error", [
+    (dict(rows=-1), ValueError), (dict(rows=1 << 30), ValueError), (dict(rows=4), ValueError), (dict(dtype=torch.float32), TypeError),
+    (dict(dtype=torch.float16), TypeError), (dict(pages=torch.long), TypeError), (dict(lens=4), ValueError), (dict(cu=3), ValueError),
+    (dict(bits=4, dtype=torch.float32), TypeError), (dict(bits=4, rows=4), ValueError), (dict(cut="k_scales"), ValueError),
+    (dict(cut="k"), ValueError),
+])
+def test_paged_rows_refuses(dev, kw, error):
+    cache = paged_cache(8, 2, 64, page_size=16, bits=4 if "cut" in kw else kw.get("bits", 16), device=dev)
+    if "cut" in kw:
+        cache = cache._replace(**{kw["cut"]: getattr(cache, kw["cut"])[..., :1].contiguous()})
+    pages = torch.zeros(3, 4, dtype=kw.get("pages", torch.int32), device=dev)
+    lens = torch.ones(kw.get("lens", 3), dtype=torch.int32, device=dev)
+    cu = torch.zeros(kw["cu"], dtype=torch.int32, device=dev) if "cu" in kw else None
+    with pytest.raises(error):
+        paged_rows(cache, pages, lens, cu, rows=kw.get("rows", 3), dtype=kw.get("dtype"))
