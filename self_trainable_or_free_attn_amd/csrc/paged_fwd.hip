@@ -1121,9 +1121,12 @@ static int paged_fwd(FwdArgs& a, const void* q, const int* pages, const int* len
     } else if constexpr (m == TILE) {
       if (p.form == PIECES) {
         hipLaunchKernelGGL((paged_pieces_kernel<d, n>), dim3((unsigned)(p.items * Hk)), dim3(256), 0, stream, a);
-        const long long cuts = std::min<long long>(p.tiles, p.items - p.tiles), side = merge_rows_of(d, 1);
-        hipLaunchKernelGGL((merge_pieces_kernel<d>), dim3((unsigned)(cuts * Hk), (unsigned)((rows_most + side - 1) / side)),
-                           dim3(256), 0, stream, a);
+        // a tile's rows are shared out over more workgroups, down to one pass each, where the tiles are few (15 sequences of 16
+        // tokens, 16 heads over 2, up to 13269 keys: merge 10.0 us with 16 workgroups a tile, 5.0 with 64)
+        const long long cuts = std::min<long long>(p.tiles, p.items - p.tiles) * Hk;
+        const long long few = merge_rows_of(d, 4), many = merge_rows_of(d, 1);
+        const long long parts = std::min((rows_most + few - 1) / few, std::max((rows_most + many - 1) / many, 2048 / cuts));
+        hipLaunchKernelGGL((merge_pieces_kernel<d>), dim3((unsigned)cuts, (unsigned)parts), dim3(256), 0, stream, a);
         return;
       }
     }
