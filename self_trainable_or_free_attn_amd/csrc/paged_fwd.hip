@@ -484,13 +484,14 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_whole_kern
 // workgroup does its share: the rest of a tile, whole tiles, the beginning of a tile. Whole tiles are finished by it, pieces leave
 // partials (two a share at most) that a second launch adds in order. So one long history among short ones takes what it costs and
 // not the time of one workgroup (200 tokens against 1 to 40000 keys, 32 heads over 8: 16 bits 766 us whole tiles, 704 key ranges,
-// 561 shares; 4 bits 468, 256, 178).
+// 535 shares; 4 bits 468, 256, 167).
 // Every wave derives its share's borders from the lengths by itself, so they stay on the device: costs are whole numbers (units of
 // 1 / cost_unit chunks, TILE_COST more for a tile's beginning and end), and a border is a function of its place alone, so all waves
 // agree on it. A border near a tile's own (SNAP of a share) moves there, which saves a partial; where all tiles are about as long
 // as a share or shorter and no share needs more than one, all of them do. (TILE_COST 2 and shares of 4 chunks instead of LEAST = 6
 // at least: 12 tokens against 6 to 23354 keys, 3 heads, 33.0 us instead of 28.1; 100 against 1 to 40000, 16 heads of 64 over 2,
-// 47.7 instead of 43.3; the large cases above the same.) A lane has LISTS sequences one behind the other, so up to 255 are read once.
+// 47.7 instead of 43.3; the large cases above the same.) A lane has LISTS sequences one behind the other, so up to 255 are read
+// once.
 struct Share {
   int tile, chunk;  // tile number as in packed.h (first_tile of its sequence and its place there), chunk within it
 };
