@@ -379,6 +379,22 @@ struct RotateForward : torch::autograd::Function<RotateForward> {
     return res;
   }
 };
+// A captured backward hands each gradient to the stream on which its input's node was made. Where that is another one, as for a
+// leaf that an eager graph still holds, the capture cannot be ended any more: refused at the forward call.
+void refuse_other_streams(std::initializer_list<Tensor> inputs, const Tensor& like) {
+  const auto stream = c10::hip::getCurrentHIPStream(like.device().index());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status != hipStreamCaptureStatusActive) return;
+  for (const Tensor& t : inputs) {
+    if (!t.defined() || !t.requires_grad()) continue;
+    const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) continue;
+    const auto made_on = node->stream();
+    TORCH_CHECK(!made_on.has_value() || *made_on == stream.unwrap(), "norm_rotate cannot be captured with inputs whose gradients "
+                "belong to another stream: take leaves made inside the capture, or free the graphs made before it");
+  }
+}
+
 std::tuple<Tensor, Tensor> rotate_autograd(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw,
                                            const OptTensor& table, const OptTensor& positions, int64_t L, bool halves,
                                            double eps) {
@@ -393,6 +409,7 @@ std::tuple<Tensor, Tensor> rotate_autograd(const Tensor& q, const Tensor& k, con
     at::AutoDispatchBelowADInplaceOrView below;
     return op.call(q, k, qw, kw, table, positions, L, halves, eps);
   }
+  if (q.is_cuda()) refuse_other_streams({q, k, given(qw), given(kw)}, q);
   auto r = RotateForward::apply(q, k, qw, kw, table, positions, L, halves, eps);
   return {r[0], r[1]};
 }

@@ -112,7 +112,8 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tenso
     table, clamped to it; None: a row's place in q (in its sequence of the batch).
 
     Returns the new q and k, contiguous. All arithmetic is float32, rounded once at the end. Gradients are deterministic and those
-    of the weights are summed in float32; the backward itself is not differentiable, and a table gets no gradient."""
+    of the weights are summed in float32; the backward itself is not differentiable, and a table gets no gradient. A capture with
+    gradients takes leaves made inside it; those that an eager graph of another stream holds are refused."""
     if q.is_cuda and q.dim() == 3:      # the operator checks everything itself; what it refuses is named by the checks below
         try:
             return _ops().norm_rotate(q, k, q_weight, k_weight, table, positions, max(q.shape[0], 1), bool(halves), eps)

@@ -1,6 +1,6 @@
-"""Attention over paged caches of 16 and 4 bits against plain 64-bit attention over what the cache holds (packed_ref.py, which derives
-the bounds): lengths from nothing to long, page sizes, grouped heads, rows that see nothing, pages that do not exist, stale rows full of
-NaN, key ranges, streams, graphs, and a decoding loop of all operators together."""
+"""Attention over paged caches of 16 and 4 bits against plain 64-bit attention over what the cache holds (packed_ref.py, which
+derives the bounds): lengths from nothing to long, page sizes, grouped heads, rows that see nothing, pages that do not exist, stale
+rows full of NaN, tiles cut into pieces, streams, graphs, and a decoding loop of all operators together."""
 import math
 
 import pytest
@@ -218,7 +218,8 @@ def test_cuts_of_wide_tiles(dev, D, dtype, bits, causal, B):
     for many in (False, True):
         n = lambda i: [700, 40, 1, 90][i % 4] if B < 60 or i % 40 < 2 else 1 + i % 3
         lens = [n(i) for i in range(B)]
-        keys = [m + [0, 1500, 130, 5000][i % 4] // (1 if B < 60 or i % 20 == 3 else 50) if i % 9 < 8 else m // 2 for i, m in enumerate(lens)]
+        keys = [m + [0, 1500, 130, 5000][i % 4] // (1 if B < 60 or i % 20 == 3 else 50) if i % 9 < 8 else m // 2
+                for i, m in enumerate(lens)]
         _case(dev, lens, keys, 6 if many else 1, 2 if many else 1, D, dtype, 32, bits, seed=23, causal=causal, pad=B % 3)
 
 
@@ -474,6 +475,49 @@ def test_two_captured_graphs(dev, bits):
         torch.cuda.synchronize()
         for (a, la), (b, lb) in zip(res, want):
             assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_captured_chunks_side_by_side(dev, bits):
+    """Wide tiles in pieces: two graphs replayed with other lengths and counts, in turn and on two streams at once."""
+    api, B, T, H, Hk, D, page = _api(), 4, 400, 6, 2, 64, 16
+    g = torch.Generator(device=dev).manual_seed(24)
+    pages, num = ref.page_table([4000] * B, page, 0, dev, 24)
+    cache = _filled(num, Hk, D, page, bits, FP, dev, g)
+    lens, cu = _ints([400, 0, 0, 0], dev), _ints([0, T, T, T, T], dev)
+    qs = [torch.randn(T, H, D, device=dev, generator=g).to(FP) for _ in "ab"]
+    call = lambda q: api.paged_attention(q, cache, pages, lens, cu, return_lse=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call(qs[0])
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, res = [torch.cuda.CUDAGraph() for _ in qs], []
+    for graph, q in zip(graphs, qs):
+        with torch.cuda.graph(graph):
+            res.append(call(q))
+    streams = [torch.cuda.Stream() for _ in qs]
+    for counts, keys in (([400, 0, 0, 0], [400, 0, 0, 0]), ([1, 350, 1, 48], [4000, 360, 5, 3000]),
+                         ([100, 100, 100, 90], [4000, 90, 2000, 1030]), ([0, 0, 0, 400], [7, 7, 7, 4000])):
+        cu.copy_(_ints(ref.starts(counts), dev))
+        lens.copy_(_ints(keys, dev))
+        want = [call(q) for q in qs]
+        for at_once in (False, True):
+            for i, graph in enumerate(graphs):
+                for x in res[i]:
+                    x.fill_(7.0)
+                streams[i].wait_stream(torch.cuda.current_stream())
+                if not at_once:
+                    graph.replay()
+            if at_once:
+                for stream, graph in zip(streams, graphs):
+                    with torch.cuda.stream(stream):
+                        graph.replay()
+                for stream in streams:
+                    torch.cuda.current_stream().wait_stream(stream)
+            torch.cuda.synchronize()
+            for (a, la), (b, lb) in zip(res, want):
+                assert torch.equal(a, b) and torch.equal(la, lb)
 
 
 def test_strided_queries(dev):

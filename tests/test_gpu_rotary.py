@@ -263,6 +263,26 @@ def test_captured_training_step(dev):
         assert all(torch.equal(a, b) for a, b in zip(res, want))
 
 
+def test_captured_step_of_leaves_of_another_stream(dev):
+    """Leaves that an eager graph holds are refused in a capture, taken again once it is gone, and without gradients at once."""
+    api = _api()
+    t = _inputs(40, 4, 2, 64, BF, dev, 14)
+    table = api.rotary_table(40, 64, device=dev)
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "qw", "kw")]
+    eager = api.norm_rotate(*leaves, table)
+    want = [x.detach().clone() for x in eager]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="another stream"):
+            api.norm_rotate(*leaves, table)
+        with torch.no_grad():
+            res = api.norm_rotate(*leaves, table)
+        fresh = api.norm_rotate(*(x.detach().requires_grad_() for x in leaves), table)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(c.detach(), b) for a, b, c in zip(res, want, fresh))
+
+
 def test_grid_table(dev):
     """Three axes: each point's rows turn by its own coordinates."""
     api, sizes, dims = _api(), (3, 4, 5), (16, 24, 24)
