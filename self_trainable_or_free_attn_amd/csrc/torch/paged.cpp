@@ -384,7 +384,11 @@ struct RotateForward : torch::autograd::Function<RotateForward> {
 void refuse_other_streams(std::initializer_list<Tensor> inputs, const Tensor& like) {
   const auto stream = c10::hip::getCurrentHIPStream(like.device().index());
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status != hipStreamCaptureStatusActive) return;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) {  // (asked of the default stream beside a capture)
+    (void)hipGetLastError();
+    return;
+  }
+  if (status != hipStreamCaptureStatusActive) return;
   for (const Tensor& t : inputs) {
     if (!t.defined() || !t.requires_grad()) continue;
     const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
