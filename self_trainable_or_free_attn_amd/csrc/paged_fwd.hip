@@ -488,10 +488,12 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_whole_kern
 // Every wave derives its share's borders from the lengths by itself, so they stay on the device: costs are whole numbers (units of
 // 1 / cost_unit chunks, TILE_COST more for a tile's beginning and end), and a border is a function of its place alone, so all waves
 // agree on it. A border near a tile's own (SNAP of a share) moves there, which saves a partial; where all tiles are about as long
-// as a share or shorter and no share needs more than one, all of them do. (TILE_COST 2 and shares of 4 chunks instead of LEAST = 6
-// at least: 12 tokens against 6 to 23354 keys, 3 heads, 33.0 us instead of 28.1; 100 against 1 to 40000, 16 heads of 64 over 2,
-// 47.7 instead of 43.3; the large cases above the same.) A lane has LISTS sequences one behind the other, so up to 255 are read
-// once.
+// as a share or shorter and no share needs more than one, all of them do. In launches so small that shares are left over, each
+// tile has some of its own: no workgroup then has two pieces, one after the other (7 tokens against 3 to 9923 keys, 24 heads over
+// 3, 17.9 us instead of 20.4; 18 against 1 to 25716 over 4 bits, 16 heads over 2, 21.2 instead of 23.0). TILE_COST 2 and shares of
+// 4 chunks instead of LEAST = 6 at least: 12 tokens against 6 to 23354 keys, 3 heads, 33.0 us instead of 28.1; 100 against 1 to
+// 40000, 16 heads of 64 over 2, 47.7 instead of 43.3; the large cases above the same. A lane has LISTS sequences one behind the
+// other, so up to 255 are read once.
 struct Share {
   int tile, chunk;  // tile number as in packed.h (first_tile of its sequence and its place there), chunk within it
 };
@@ -510,18 +512,22 @@ struct Shares {
   const FwdArgs& a;
   int mine[LISTS], upto, from;  // of the first 64 * LISTS sequences: costs of this lane's, their sum with and without them
   int share, count;             // cost of a share; shares
-  bool whole;                   // no tile is cut
+  bool whole, even;             // no tile is cut; every tile has shares of its own
 
   // a tile's cost, and the tiles, of sequence b. (Causal tiles of more rows than one tile has count as if they saw all keys: these
   // are sequences of several tiles, which launches of tokens rarely have.)
   __device__ __forceinline__ int cost(int b, int& tiles) const {
     if (b > a.B) return tiles = 0;
     tiles = (paged_rows_of(a, b) + M - 1) / M;
-    return max((int)(((float)((paged_keys_of(a, b) + BK - 1) / BK) + TILE_COST) * a.cost_unit), 1);
+    const int each = max((int)(((float)((paged_keys_of(a, b) + BK - 1) / BK) + TILE_COST) * a.cost_unit), 1);
+    return even ? own_shares(each) * share : each;
+  }
+  __device__ __forceinline__ int own_shares(int each) const {
+    return max((int)ceilf((float)each / (float)share - (WHOLE - 1.0f)), 1);
   }
 
-  __device__ __forceinline__ Shares(const FwdArgs& args) : a(args) {
-    int total = 0, all_tiles = 0;
+  __device__ __forceinline__ Shares(const FwdArgs& args) : a(args), even(false) {
+    int total = 0, all_tiles = 0, each_of[LISTS], tiles_of[LISTS];
     float most = 0.0f;
     for (int b0 = 0; b0 <= a.B; b0 += 64 * LISTS) {
       int x[LISTS], sum = 0;
@@ -530,6 +536,8 @@ struct Shares {
         int tiles;
         const int each = cost(b0 + lane_id() * LISTS + k, tiles);
         x[k] = each * tiles;
+        each_of[k] = each;
+        tiles_of[k] = tiles;
         most = fmaxf(most, tiles > 0 ? (float)each : 0.0f);
         all_tiles += tiles;
         sum += x[k];
@@ -547,6 +555,18 @@ struct Shares {
     share = max((total + a.shares - 1) / a.shares, a.least_share);
     count = total > 0 ? (total + share - 1) / share : 1;
     whole = most <= WHOLE * (float)share && __builtin_amdgcn_readlane(wave_scan(all_tiles), 63) <= a.shares;
+    if (share > a.least_share || a.B >= 64 * LISTS) return;
+    int own = 0;
+#pragma unroll
+    for (int k = 0; k < LISTS; ++k) own += own_shares(each_of[k]) * tiles_of[k];
+    const int scan = wave_scan(own), all = __builtin_amdgcn_readlane(scan, 63);
+    if (all > a.shares) return;
+    even = true;
+    count = max(all, 1);
+    upto = scan * share;
+    from = upto - own * share;
+#pragma unroll
+    for (int k = 0; k < LISTS; ++k) mine[k] = own_shares(each_of[k]) * tiles_of[k] * share;
   }
 
   // the border in front of share w, its sequence and place there
