@@ -75,7 +75,7 @@ struct Turn {
       TORCH_CHECK(w->dim() == 1 && w->size(0) == D, name, " must be [", D, "]");
       TORCH_CHECK(w->scalar_type() == at::kFloat || w->scalar_type() == like.scalar_type(), name,
                   " must be float32 or of the tokens' dtype");
-      return aligned(w->detach().contiguous());
+      return w->is_contiguous() && !misaligned(*w) ? *w : aligned(w->contiguous());
     };
     q_weight = weight("q_weight", qw);
     k_weight = weight("k_weight", kw);
@@ -141,11 +141,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rotate_backward(const Tensor& dqo_, c
   auto gradient = [&](const char* name, const Tensor& d, const Tensor& x) {
     check_on(name, d, x);
     TORCH_CHECK(d.scalar_type() == x.scalar_type() && d.sizes() == x.sizes(), name, " must be like its output");
-    return aligned(d.contiguous());
+    return d.is_contiguous() && !misaligned(d) ? d : aligned(d.contiguous());
   };
   const Tensor dqo = gradient("the gradient of q", dqo_, a.q), dko = gradient("the gradient of k", dko_, a.k);
   Tensor dq = at::empty(a.q.sizes(), q.options()), dk = at::empty(a.k.sizes(), q.options());
-  auto like = [&](const Tensor& w) { return w.defined() ? at::empty_like(w) : at::empty({0}, q.options()); };
+  auto like = [&](const Tensor& w) { return at::empty({w.defined() ? a.D : 0}, (w.defined() ? w : q).options()); };
   Tensor dqw = like(a.turn.q_weight), dkw = like(a.turn.k_weight);
   const bool norm = a.turn.q_weight.defined();
   const size_t bytes = norm ? es_norm_rotate_workspace(a.T, a.H, a.Hk, a.D) : 0;
@@ -270,7 +270,7 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor& q_, const Tensor& kp,
   TORCH_CHECK(q_.size(2) == c.D, "q and the cache do not go together");
   const Tensor q = q_.numel() ? aligned(q_) : q_;
   const int H = as_int(q.size(1));
-  Tensor out = at::empty_like(q), lse = at::empty({c.T, H}, q.options().dtype(at::kFloat));
+  Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({c.T, H}, q.options().dtype(at::kFloat));
   const size_t bytes = es_paged_workspace(c.B, c.T, c.max_pages, c.page_size, H, c.Hk, c.D, c.four ? 4 : 16);
   const Tensor ws = bytes ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : Tensor();
   float* l = static_cast<float*>(data(lse));
