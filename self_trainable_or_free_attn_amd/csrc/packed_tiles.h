@@ -96,6 +96,14 @@ __device__ __forceinline__ int tile_chunks(const FwdArgs& a, const Job& j) {
   return (keys_seen(a, j, last) + BK - 1) / BK;
 }
 
+// eight values less their held ones, held
+__device__ __forceinline__ ev8 rest8(const float* p, const ev8& held) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = p[i] - (float)held[i];
+  return epack8(x);
+}
+
 // A lane's row, its softmax state and the exponentials of a 32-key run of S^T.
 template <int D, bool BIAS>
 struct Rows {
@@ -170,14 +178,19 @@ struct Rows {
     return true;
   }
 
-  // p = exp(s - maximum) as two B operands
-  __device__ __forceinline__ void exponentials(const f32x16& s, float sc, float c, ev8& pa, ev8& pb) {
+  // p = exp(s - maximum) as two B operands; ra, rb: what their rounding leaves, as two more
+  __device__ __forceinline__ void exponentials(const f32x16& s, float sc, float c, ev8& pa, ev8& pb, ev8* ra = nullptr,
+                                               ev8* rb = nullptr) {
     c -= (mrun == -INFINITY ? 0.0f : mrun) - P_SHIFT;
     float p[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) p[r] = exp2f_fast(fmaf(s[r], sc, c));
     pa = epack8(&p[0]);
     pb = epack8(&p[8]);
+    if (ra != nullptr) {
+      *ra = rest8(&p[0], pa);
+      *rb = rest8(&p[8], pb);
+    }
     // (the sum takes the probabilities before their rounding: the LSE is a float32 result of its own)
     float sum[4] = {p[0], p[1], p[2], p[3]};
 #pragma unroll
@@ -185,11 +198,14 @@ struct Rows {
     lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   }
 
-  // O^T += V^T P^T of sixteen keys at `v`
-  __device__ __forceinline__ void values(const char* v, int t0, int t1, const ev8& p) {
+  // O^T += V^T P^T of sixteen keys at `v`; rest: of what the rounding of P left, too
+  __device__ __forceinline__ void values(const char* v, int t0, int t1, const ev8& p, const ev8* rest = nullptr) {
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-      o[db] = emfma(ecat_tr(lds_read_tr(v, t0 ^ (64 * db)), lds_read_tr(v, t1 ^ (64 * db))), p, o[db]);
+    for (int db = 0; db < D / 32; ++db) {
+      const ev8 x = ecat_tr(lds_read_tr(v, t0 ^ (64 * db)), lds_read_tr(v, t1 ^ (64 * db)));
+      o[db] = emfma(x, p, o[db]);
+      if (rest != nullptr) o[db] = emfma(x, *rest, o[db]);
+    }
   }
 };
 
@@ -218,9 +234,10 @@ __device__ __forceinline__ void store_row(const FwdArgs& a, size_t at, int col, 
 //   settle(base)             what the transfers leave to do once they have landed (STAGED: nothing)
 //   run(a, j, v, u, dst)     narrow tiles: starts those of K (v: V) of the 32-key run u, all of them by this wave
 //   enter / mask             HOLES: keys that a sequence counts may be missing, 16 at a time; their scores become -inf
+//   FINE                     narrow tiles multiply V by what the rounding of P leaves, too
 template <int D>
 struct Rowwise {
-  static constexpr bool HOLES = false, STAGED = false;
+  static constexpr bool HOLES = false, STAGED = false, FINE = false;
   static constexpr int LPR = D / 8, NI = D / 32;
   int l, wv;
   unsigned src[2 * NI], stride;
@@ -441,15 +458,15 @@ __device__ __forceinline__ void narrow_tile(const FwdArgs& a, const Job& j, char
     for (int ks = 0; ks < NKS; ++ks) s = emfma(elds16(kb, off.k0 ^ (32 * ks)), x.q[ks], s);
     wait_lds();
     if (more) keys.run(a, j, false, u + 4, kd);
-    ev8 pa, pb;
+    ev8 pa, pb, ra, rb;
     float sc, c, alpha;
     keys.mask(s, 0);
     x.raise(x.scores(a, tab, s, 32 * u, hi, 32 * (u + 1) > seen_min, low, high, sc, c), alpha);
-    x.exponentials(s, sc, c, pa, pb);
+    x.exponentials(s, sc, c, pa, pb, KEYS::FINE ? &ra : nullptr, KEYS::FINE ? &rb : nullptr);
     if (more) wait_transfers<NI>();
     else wait_transfers<0>();
-    x.values(vb, off.t0, off.t1, pa);
-    x.values(vb + RUN / 2, off.t0, off.t1, pb);
+    x.values(vb, off.t0, off.t1, pa, KEYS::FINE ? &ra : nullptr);
+    x.values(vb + RUN / 2, off.t0, off.t1, pb, KEYS::FINE ? &rb : nullptr);
     wait_lds();
     if (more) keys.run(a, j, true, u + 4, vd);
   }
