@@ -218,10 +218,10 @@ __device__ __forceinline__ int values_at(int row, int c) {
 // l / 16) loads a quarter of its key's row in one piece and feeds it to the products without LDS. The exponentials of both groups
 // are the B operand of O^T += V^T P^T with the keys in the order 4 q + 0..3, 16 + 4 q + 0..3 of quarter q. V goes through the
 // wave's own LDS as token values, from where it is read transposed. No barrier in the loop.
-// P goes into the products as its 16-bit value and, rounded again, what that leaves (FINE in packed_tiles.h, for caches of 16 bits):
-// launches of few rows wait for HBM, and outputs then have no error but their own rounding (relative error of 48 tokens against 1 to
-// 16000 keys over 4 bits 4.7e-4 instead of 6.8e-4, with probabilities in float32 4.7e-4; 97.1 us instead of 96.4, and at most 7 %
-// more, 64 tokens against 8000 keys of 64 channels). Wide tiles, which the matrix units bound, round P once.
+// P goes into the products as its 16-bit value and, rounded again, what that leaves (FINE in packed_tiles.h, for caches of 16
+// bits): launches of few rows wait for HBM, and outputs then have no error but their own rounding (48 tokens against 1 to 16000
+// keys over 4 bits: relative error 4.7e-4 instead of 6.8e-4, with probabilities in float32 4.7e-4; 97.1 us instead of 96.4, and at
+// most 7 % more, 64 tokens against 8000 keys of 64 channels). Wide tiles, which the matrix units bound, round P once.
 template <int D, int NR>
 __device__ __forceinline__ void narrow4_tile(const FwdArgs& a, const Job& j, char* lds, float* stats) {
   constexpr int NKS = D / 32, NDB = D / 16, ROW = D * 2, WORDS = D / 32;  // words of 8 codes a lane and group
