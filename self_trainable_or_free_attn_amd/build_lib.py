@@ -2,8 +2,8 @@
 the torch operator library over it (torch_ops.py, lib/libechosparse_torch.so).
 
 Every HIP source under csrc/ is compiled to an object in parallel and linked into lib/libechosparse_hip.so; the
-VSA, packed-sequence and paged-cache sources (vsa_*.hip, packed_*.hip, paged_*.hip) are compiled a second time with -DES_ELEM_F16 for their fp16
-entry points (suffix _f16).
+VSA, packed-sequence and paged-cache sources (vsa_*.hip, packed_*.hip, paged_*.hip) are compiled a second time with
+-DES_ELEM_F16 for their fp16 entry points (suffix _f16).
 Flags: -O3, gfx950 only, and packed FP32 instructions disabled (-Xclang -target-feature -Xclang -packed-fp32-ops).
 """
 import os
