@@ -249,8 +249,8 @@ __device__ __forceinline__ void norm_rotate_exact(const RawRow<D, PAIRS>& raw, c
     double sum = 0.0;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float x = (float)raw.v[e / 8][e % 8];
-      sum += (double)(x * x);  // (exact in float32: 11 bits each)
+      const double x = (double)(float)raw.v[e / 8][e % 8];
+      sum += x * x;  // (a bf16 value's square has 16 digits, but float32 ends at values of 1.8e19 and 1e-19)
     }
     r = 1.0 / sqrt(lanes_sum<D / 16>(sum) * (1.0 / D) + eps);
   }
