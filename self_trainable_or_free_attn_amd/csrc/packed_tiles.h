@@ -66,8 +66,8 @@ struct FwdArgs {
   int n, P, S;
   int part_rows;  // rows of a sequence's partial
   PagedArgs paged;
-  // paged caches (paged_fwd.hip): shares of a head, the least cost of one, units of cost a chunk
-  int shares, least_share;
+  // paged caches (paged_fwd.hip): shares of a head, the least cost of one, units of cost a chunk; partials of a head
+  int shares, least_share, parts;
   float cost_unit;
 };
 

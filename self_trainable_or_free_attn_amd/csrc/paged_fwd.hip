@@ -796,11 +796,11 @@ __global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
 // quarter and the rest, since workgroups are dispatched in order. Lanes have LISTS sequences each, 64 apart; more than 64 * LISTS
 // are read once a pass and keep their order.
 struct WideItem {
-  int list, tile, level, piece;  // list < 0: none
+  int list, tile, level, piece, number, per;  // list < 0: none; number: within its class and list
 };
-// What the first workgroup leaves for the merge, behind it (first item, first cut tile) of each list.
+// What the first workgroup leaves for the merge, behind it (first partial, first cut tile) of each list.
 struct WidePlan {
-  int per, above, cut_tiles, pad;
+  int per, cut_tiles;
 };
 struct Wide {
   WideList x;
@@ -828,6 +828,8 @@ __device__ __forceinline__ float row_sum(float x) {
   x += __int_as_float(dpp_i<0x114>(__float_as_int(x)));
   return x + __int_as_float(dpp_i<0x118>(__float_as_int(x)));
 }
+// x, held to the workspace whatever counts a call has
+__device__ __forceinline__ int within(int x, int n) { return (int)min((unsigned)x, (unsigned)(n - 1)); }
 constexpr int CUTS = 16;  // sizes of pieces that are looked at
 // A plan, page numbers and first keys take about 8 us, a chunk 2.1, with D = 64 1.1; a merge 5 more where tiles are cut.
 template <int D>
@@ -928,12 +930,31 @@ struct WideLists {
     return __builtin_amdgcn_readfirstlane(best);
   }
 
+  __device__ __forceinline__ int cut_tiles_of(const WideList& x, int per) const {
+    return x.tiles - tiles_within(x, a.G, a.causal, piece_of(x, per));
+  }
+  __device__ __forceinline__ int parts_of(const WideList& x, int per) const {
+    return cut_tiles_of(x, per) + later_pieces(x, a.G, a.causal, piece_of(x, per));
+  }
+  // the partial of an item of a cut tile, all of which are in class 0
+  __device__ __forceinline__ int part(const WideItem& item, const WideList& own) const {
+    int front = 0;  // partials of this lane's lists in front of the item's
+    for (int i0 = 0; i0 < item.list; i0 += 64 * LISTS) {
+#pragma unroll
+      for (int k = 0; k < LISTS; ++k)
+        if (i0 + 64 * k < item.list && i0 + 64 * k + lane_id() < item.list) front += parts_of(at(i0, k), item.per);
+    }
+    const int level0 = own.tiles - tiles_within(own, a.G, a.causal, bound(item.per, 0));
+    return within(__builtin_amdgcn_readlane(wave_scan(front), 63) + partial_number(item.number, level0, cut_tiles_of(own, item.per)),
+                  a.parts);
+  }
+
   // item w, and its list
   __device__ __forceinline__ WideItem find(int w, float* times, Wide& own) const {
     const int per = cut(times), l = lane_id();
     const bool leave = blockIdx.x == 0 && threadIdx.x < 64;
-    int2* plan = a.plan + 2;
-    int first = 0, cut_tiles = 0, list = -1, kind = 0, number = 0;
+    int2* plan = a.plan + 1;
+    int first = 0, cut_tiles = 0, parts = 0, list = -1, kind = 0, number = 0;
     for (int i0 = 0; i0 < lists; i0 += 64 * LISTS) {
       int upto[LISTS][4], count[LISTS][4], base[4] = {}, all = 0;
 #pragma unroll
@@ -966,8 +987,9 @@ struct WideLists {
         const int i = i0 + 64 * k + l;
         if (leave) {
           const WideList x = at(i0, k);
-          const int cuts = x.tiles - tiles_within(x, a.G, a.causal, piece_of(x, per)), cut_upto = wave_scan(cuts);
-          if (i < lists) plan[i] = make_int2(base[0] + upto[k][0] - count[k][0], cut_tiles + cut_upto - cuts);
+          const int cuts = cut_tiles_of(x, per), cut_upto = wave_scan(cuts), own_parts = parts_of(x, per), part_upto = wave_scan(own_parts);
+          if (i < lists) plan[i] = make_int2(parts + part_upto - own_parts, cut_tiles + cut_upto - cuts);
+          parts += __builtin_amdgcn_readlane(part_upto, 63);
           cut_tiles += __builtin_amdgcn_readlane(cut_upto, 63);
         }
 #pragma unroll
@@ -980,7 +1002,7 @@ struct WideLists {
       first += all;
       if (!leave && __builtin_amdgcn_ballot_w64(list >= 0)) break;
     }
-    if (leave && l == 0) *reinterpret_cast<WidePlan*>(a.plan) = WidePlan{per, bound(per, 0), cut_tiles, 0};
+    if (leave && l == 0) *reinterpret_cast<WidePlan*>(a.plan) = WidePlan{per, cut_tiles};
     const unsigned long long hit = __builtin_amdgcn_ballot_w64(list >= 0);
     if (hit == 0) return WideItem{-1};
     const int from = __builtin_ctzll(hit);
@@ -990,7 +1012,7 @@ struct WideLists {
     if (list < 64) own = wide_at(mine[0], from);
     else own = wide_at(wide_of(a, list), 0);
     const int piece = piece_of(own.x, per);
-    WideItem item = {list, 0, 0};
+    WideItem item = {list, 0, 0, 0, number, per};
     if (kind > 0) item.tile = tiles_within(own.x, a.G, a.causal, bound(per, kind - 1)) - 1 - number;
     else if (!piece_at(own.x, a.G, a.causal, piece, bound(per, 0), number, item.tile, item.level)) item.list = -1;
     item.piece = piece;
@@ -1006,7 +1028,8 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, TILE)) void paged_pieces_
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
   __shared__ float times[CUTS];
   Wide own;
-  const WideItem item = WideLists<D>(a).find(w, times, own);
+  const WideLists<D> all(a);
+  const WideItem item = all.find(w, times, own);
   if (item.list < 0) return;
   Job j;
   paged_job<D, BITS>(a, j, own.q0, own.nq, item.list, own.keys(a), own.over(a), hk);
@@ -1015,7 +1038,7 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, TILE)) void paged_pieces_
   j.c0 = range_begin(chunks, item.level, n);
   j.c1 = range_begin(chunks, item.level + 1, n);
   j.part_rows = TILE;
-  j.part = n == 1 ? nullptr : partial<D>(a.part, TILE, a, w, hk);
+  j.part = n == 1 ? nullptr : partial<D>(a.part, TILE, a, all.part(item, own.x), hk);
   paged_tile<D, BITS, TILE>(a, j, lds, stats);
 }
 
@@ -1025,17 +1048,17 @@ __global__ __launch_bounds__(256) void merge_pieces_kernel(FwdArgs a) {
   constexpr int MOST = 256 * ES_PAGED_RESIDENT(D, TILE) + 2;  // pieces of a tile: as many as fill the GPU
   const int w = blockIdx.x / a.Hk, hk = blockIdx.x - w * a.Hk;
   const WidePlan plan = *reinterpret_cast<const WidePlan*>(a.plan);
-  int2 first = a.plan[2 + min(lane_id(), a.B)];
+  int2 first = a.plan[1 + min(lane_id(), a.B)];
   if (w >= plan.cut_tiles) return;
   int list = 0;
   for (int i0 = 0; i0 <= a.B; i0 += 64) {  // the last list that starts at or before w and has cut tiles
-    if (i0 > 0) first = a.plan[2 + min(i0 + lane_id(), a.B)];
+    if (i0 > 0) first = a.plan[1 + min(i0 + lane_id(), a.B)];
     const unsigned long long upto = __builtin_amdgcn_ballot_w64(i0 + lane_id() <= a.B && first.y <= w);
     if (upto == 0) break;
     list = i0 + 63 - __builtin_clzll(upto);
     if (!(upto >> 63)) break;
   }
-  const int2 left = a.plan[2 + list];
+  const int2 left = a.plan[1 + list];
   const Wide own = wide_at(wide_of(a, list), 0);
   const int piece = piece_of(own.x, plan.per), t = __builtin_amdgcn_readfirstlane(own.x.tiles - 1 - (w - left.y));
   if (t < 0) return;
@@ -1043,7 +1066,8 @@ __global__ __launch_bounds__(256) void merge_pieces_kernel(FwdArgs a) {
   const int seen = a.causal ? min(max(last + 1 - own.x.behind, 0), own.keys(a)) : own.keys(a);
   const int n = min(pieces_of((seen + BK - 1) / BK, piece), MOST);
   __shared__ int pieces[MOST];
-  for (int i = threadIdx.x; i < n; i += 256) pieces[i] = left.x + piece_number(own.x, a.G, a.causal, piece, plan.above, t, i);
+  for (int i = threadIdx.x; i < n; i += 256)
+    pieces[i] = within(left.x + piece_number(own.x, a.G, a.causal, piece, piece, t, i), a.parts);
   __syncthreads();
   auto merge = [&](auto side) {
     constexpr int S = decltype(side)::value, RPB = merge_rows_of(D, S);
@@ -1065,6 +1089,7 @@ struct PagedPlan {
   int M;               // rows a tile
   long long tiles;     // tile numbers of a head
   int shares, items;   // a head: SHARES, PIECES
+  int parts;           // a head: PIECES
   size_t plan, bytes;  // workspace: partials, then borders (SHARES) or the cut (PIECES)
 };
 
@@ -1090,8 +1115,12 @@ static PagedPlan paged_plan(int B, int Tq, int cap, int H, int Hk, int D, int bi
     p.plan = (size_t)2 * p.shares * Hk * part_floats(p.M, D) * sizeof(float);
     p.bytes = p.plan + (size_t)(p.shares + 1) * sizeof(int4);
   } else if (p.form == PIECES) {
-    p.items = (int)(p.tiles + slots / Hk + 1);
-    p.plan = (size_t)p.items * Hk * part_floats(p.M, D) * sizeof(float);
+    // later pieces as many as fill the GPU (WideLists::cut); only cut tiles have partials (75600 tokens of 40 heads over 8: 69 MB
+    // instead of the 1.6 GB of one for every tile)
+    const int later = slots / Hk + 1;
+    p.items = (int)(p.tiles + later);
+    p.parts = (int)most_partials(p.tiles, later);
+    p.plan = (size_t)p.parts * Hk * part_floats(p.M, D) * sizeof(float);
     p.bytes = p.plan + sizeof(WidePlan) + (size_t)(B + 1) * sizeof(int2);
   }
   return p;
@@ -1140,6 +1169,7 @@ static int paged_fwd(FwdArgs& a, const void* q, const int* pages, const int* len
   a.plan = (int2*)((char*)workspace + p.plan);
   a.items = p.form == SHARES ? 2 * p.shares : p.items;
   a.shares = p.shares;
+  a.parts = p.parts;
   a.inv_slots = (float)Hk / (float)(256 * ES_PAGED_RESIDENT(D, p.M));
   // sixteenths of a chunk, or as much more as it takes for all costs of a head to stay below 2^29
   a.cost_unit = (float)std::min(16.0, (double)(1 << 29) / ((double)p.tiles * ((double)a.paged.cap / BK + TILE_COST)));

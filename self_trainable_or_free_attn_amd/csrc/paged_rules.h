@@ -91,6 +91,13 @@ ES_RULE int piece_number(const WideList& x, int group, bool causal, int piece, i
   return n;
 }
 
+// Partials, which only the pieces of cut tiles have, are numbered in the same order without the tiles that are whole: that of
+// piece_number with `above` = piece. Of the piece with number i, of a list with `level0` pieces of level 0 and `cuts` cut tiles,
+// which are the first of them:
+ES_RULE int partial_number(int i, int level0, int cuts) { return i < level0 ? i : i - level0 + cuts; }
+// All partials of a launch of `tiles` tiles that allows `later` pieces above level 0: a cut tile has one of those at least.
+ES_RULE long long most_partials(long long tiles, long long later) { return (tiles < later ? tiles : later) + later; }
+
 // A launch's time in chunks: `big` items of `size` chunks, of which the GPU holds 1 / inv_slots, and small ones that take `small`
 // together: rounds of big ones, small ones in the places that the last round leaves and behind it. An item's start takes as long
 // as `start` chunks, a merge of tiles that are cut too. `mean`: all chunks over all places; what a CU does beside an item that is
