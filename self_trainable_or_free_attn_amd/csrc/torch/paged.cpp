@@ -292,12 +292,12 @@ std::tuple<Tensor, Tensor> attention_meta(const Tensor& q, const Tensor&, const 
   return {at::empty_like(q), at::empty_symint({q.sym_size(0), q.sym_size(1)}, q.options().dtype(at::kFloat))};
 }
 std::tuple<Tensor, Tensor> rotate_meta(const Tensor& q, const Tensor& k, const OptTensor&, const OptTensor&, const OptTensor&,
-                                       const OptTensor&, int64_t, bool, double) {
+                                       const OptTensor&, c10::SymInt, bool, double) {
   return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint(k.sym_sizes(), k.options())};
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> rotate_backward_meta(const Tensor&, const Tensor&, const Tensor& q, const Tensor& k,
                                                                 const OptTensor& qw, const OptTensor& kw, const OptTensor&,
-                                                                const OptTensor&, int64_t, bool, double) {
+                                                                const OptTensor&, c10::SymInt, bool, double) {
   auto like = [&](const OptTensor& w) { return w.has_value() ? at::empty_like(*w) : at::empty({0}, q.options()); };
   return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint(k.sym_sizes(), k.options()), like(qw), like(kw)};
 }
@@ -307,17 +307,17 @@ Tensor append_meta(const OptTensor& q, const Tensor& k, const Tensor&, const Opt
   return q.has_value() ? at::empty_symint(q->sym_sizes(), q->options()) : at::empty({0}, k.options());
 }
 std::tuple<Tensor, Tensor> rows_meta(const Tensor& kp, const Tensor&, const OptTensor& ks, const OptTensor&, const Tensor&,
-                                     const Tensor&, const OptTensor&, int64_t count, at::ScalarType dtype) {
-  Tensor k = at::empty_symint({count, kp.sym_size(1), kp.sym_size(3) * (ks.has_value() ? 2 : 1)}, kp.options().dtype(dtype));
+                                     const Tensor&, const OptTensor&, c10::SymInt count, at::ScalarType dtype) {
+  Tensor k = at::empty_symint({std::move(count), kp.sym_size(1), kp.sym_size(3) * (ks.has_value() ? 2 : 1)}, kp.options().dtype(dtype));
   return {k, at::empty_like(k)};
 }
 
 // ------------------------------------------------------------------------------------------------ gradient
 using RotateSignature = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&,
-                                                   const OptTensor&, const OptTensor&, int64_t, bool, double);
+                                                   const OptTensor&, const OptTensor&, c10::SymInt, bool, double);
 using RotateBackwardSignature = std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&,
                                                                            const Tensor&, const OptTensor&, const OptTensor&,
-                                                                           const OptTensor&, const OptTensor&, int64_t, bool,
+                                                                           const OptTensor&, const OptTensor&, c10::SymInt, bool,
                                                                            double);
 
 template <class Signature>
@@ -333,7 +333,7 @@ const c10::TypedOperatorHandle<RotateBackwardSignature>& rotate_backward_op() {
 struct RotateBackward : torch::autograd::Function<RotateBackward> {
   static variable_list forward(AutogradContext*, const Tensor& dqo, const Tensor& dko, const Tensor& q, const Tensor& k,
                                const OptTensor& qw, const OptTensor& kw, const OptTensor& table, const OptTensor& positions,
-                               int64_t L, bool halves, double eps) {
+                               c10::SymInt L, bool halves, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [dq, dk, dqw, dkw] = rotate_backward_op().call(dqo, dko, q, k, qw, kw, table, positions, L, halves, eps);
     return {dq, dk, dqw, dkw};
@@ -345,7 +345,7 @@ struct RotateBackward : torch::autograd::Function<RotateBackward> {
 std::tuple<Tensor, Tensor, Tensor, Tensor> rotate_backward_autograd(const Tensor& dqo, const Tensor& dko, const Tensor& q,
                                                                     const Tensor& k, const OptTensor& qw, const OptTensor& kw,
                                                                     const OptTensor& table, const OptTensor& positions,
-                                                                    int64_t L, bool halves, double eps) {
+                                                                    c10::SymInt L, bool halves, double eps) {
   if (!at::GradMode::is_enabled()) {  // (a backward without create_graph: no node to make)
     at::AutoDispatchBelowADInplaceOrView below;
     return rotate_backward_op().call(dqo, dko, q, k, qw, kw, table, positions, L, halves, eps);
@@ -356,7 +356,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rotate_backward_autograd(const Tensor
 
 struct RotateForward : torch::autograd::Function<RotateForward> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw,
-                               const OptTensor& table, const OptTensor& positions, int64_t L, bool halves, double eps) {
+                               const OptTensor& table, const OptTensor& positions, c10::SymInt L, bool halves, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = find<RotateSignature>("echosparse_gfx950::norm_rotate");
     auto [qo, ko] = op.call(q, k, qw, kw, table, positions, L, halves, eps);
@@ -370,7 +370,7 @@ struct RotateForward : torch::autograd::Function<RotateForward> {
     variable_list res(9);
     const auto s = ctx->get_saved_variables();
     auto [dq, dk, dqw, dkw] = rotate_backward_op().call(grads[0], grads[1], s[0], s[1], maybe(s[2]), maybe(s[3]), maybe(s[4]),
-                                                        maybe(s[5]), ctx->saved_data["L"].toInt(),
+                                                        maybe(s[5]), ctx->saved_data["L"].toSymInt(),
                                                         ctx->saved_data["halves"].toBool(), ctx->saved_data["eps"].toDouble());
     res[0] = dq;
     res[1] = dk;
@@ -400,7 +400,7 @@ void refuse_other_streams(std::initializer_list<Tensor> inputs, const Tensor& li
 }
 
 std::tuple<Tensor, Tensor> rotate_autograd(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw,
-                                           const OptTensor& table, const OptTensor& positions, int64_t L, bool halves,
+                                           const OptTensor& table, const OptTensor& positions, c10::SymInt L, bool halves,
                                            double eps) {
   const bool grad = at::GradMode::is_enabled();
   auto wants = [](const OptTensor& t) { return t.has_value() && t->requires_grad(); };
@@ -445,9 +445,9 @@ Tensor append_autograd(const OptTensor& q, const Tensor& k, const Tensor& v, con
 }
 
 using RowsSignature = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const Tensor&,
-                                                 const Tensor&, const OptTensor&, int64_t, at::ScalarType);
+                                                 const Tensor&, const OptTensor&, c10::SymInt, at::ScalarType);
 std::tuple<Tensor, Tensor> rows_autograd(const Tensor& kp, const Tensor& vp, const OptTensor& ks, const OptTensor& vs,
-                                         const Tensor& pages, const Tensor& lens, const OptTensor& cu, int64_t count,
+                                         const Tensor& pages, const Tensor& lens, const OptTensor& cu, c10::SymInt count,
                                          at::ScalarType dtype) {
   static const auto op = find<RowsSignature>("echosparse_gfx950::paged_rows");
   refuse_derivatives("paged_rows", {{"cache.k", kp}, {"cache.v", vp}});
@@ -470,15 +470,15 @@ std::tuple<Tensor, Tensor> attention_autograd(const Tensor& q, const Tensor& kp,
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(echosparse_gfx950, m) {
-  m.def("norm_rotate(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? table, Tensor? positions, int L, "
+  m.def("norm_rotate(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? table, Tensor? positions, SymInt L, "
         "bool halves, float eps) -> (Tensor, Tensor)");
   m.def("norm_rotate_backward(Tensor dq_out, Tensor dk_out, Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, "
-        "Tensor? table, Tensor? positions, int L, bool halves, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
+        "Tensor? table, Tensor? positions, SymInt L, bool halves, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("append_paged(Tensor? q, Tensor k, Tensor v, Tensor? q_weight, Tensor? k_weight, Tensor? table, Tensor pages, "
         "Tensor lens, Tensor? cu, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scales, Tensor(d!)? v_scales, "
         "bool halves, float eps) -> Tensor");
   m.def("paged_rows(Tensor k_pages, Tensor v_pages, Tensor? k_scales, Tensor? v_scales, Tensor pages, Tensor lens, Tensor? cu, "
-        "int rows, ScalarType dtype) -> (Tensor, Tensor)");
+        "SymInt rows, ScalarType dtype) -> (Tensor, Tensor)");
   m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? k_scales, Tensor? v_scales, Tensor pages, "
         "Tensor lens, Tensor? cu, bool causal, float scale) -> (Tensor, Tensor)");
 }
