@@ -85,7 +85,7 @@ def _check_cache(cache, dtype, device, like):
     else:
         if k.dtype is not dtype or v.dtype is not dtype:
             raise TypeError(f"a cache of 16 bits must be {dtype} like the tokens, got {k.dtype} and {v.dtype}")
-        if k.stride() != v.stride() or k.stride(3) != 1 or any(s % 8 for s in k.stride()[:3]):
+        if k.stride() != v.stride() or k.stride(3) != 1 or any(n > 1 and s % 8 for n, s in zip(k.shape[:3], k.stride())):
             raise ValueError(f"cache.k and cache.v must have the same strides, channels 1 apart and the others multiples of 8, got "
                              f"{k.stride()} and {v.stride()}")
         if any(n > 1 and s < dim for n, s in zip(k.shape[:3], k.stride())):

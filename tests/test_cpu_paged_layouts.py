@@ -1,0 +1,37 @@
+"""Layouts of paged caches that the operators of paged.py take and refuse, on meta tensors. (The tests of the same name on the GPU
+make the calls whose tensors the native operators check.)"""
+import pytest
+import torch
+
+from self_trainable_or_free_attn_amd import PagedCache, append_paged, paged_attention, paged_rows
+
+BF = torch.bfloat16
+
+
+def strided(shape, strides, device="meta"):
+    """A tensor of these strides over as much memory as they span."""
+    size = 1 + sum((n - 1) * s for n, s in zip(shape, strides))
+    return torch.zeros(size, dtype=BF, device=device).as_strided(shape, strides)
+
+
+def _i(*shape):
+    return torch.empty(*shape, dtype=torch.int32, device="meta")
+
+
+def _calls(cache, n=2):
+    """All calls with one sequence, whose tokens Python checks (a batch) on meta tensors."""
+    Hk, D = cache.k.shape[1], cache.k.shape[3]
+    x = torch.empty(1, n, Hk, D, dtype=BF, device="meta")
+    return [lambda: append_paged(cache, x, x, _i(1, 1), _i(1)), lambda: paged_attention(x, cache, _i(1, 1), _i(1)),
+            lambda: paged_rows(cache, _i(1, 1), _i(1), rows=n)]
+
+
+# (pages, heads, rows of a page, channels) and strides; a dimension of one may have any stride
+ONES = [((1, 2, 16, 64), (3, 1024, 64, 1)), ((8, 1, 16, 64), (1024, 5, 64, 1)), ((8, 1, 16, 64), (1024, 0, 64, 1)),
+        ((1, 1, 32, 128), (7, 9, 136, 1)), ((1, 3, 16, 64), (1, 64, 192, 1))]
+
+
+@pytest.mark.parametrize("shape, strides", ONES)
+def test_dimensions_of_one_have_any_stride(shape, strides):
+    for call in _calls(PagedCache(strided(shape, strides), strided(shape, strides))):
+        call()
