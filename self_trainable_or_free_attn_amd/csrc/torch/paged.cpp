@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <tuple>
 #include <utility>
@@ -189,9 +190,15 @@ struct Cache {
                   k.scalar_type(), " and ", v.scalar_type(), ")");
       TORCH_CHECK(k.strides() == v.strides() && k.stride(3) == 1,
                   "k and v of a cache must have the same strides, channels 1 apart");
-      for (int i = 0; i < 3; ++i)
-        TORCH_CHECK(k.size(i) <= 1 || (k.stride(i) >= D && k.stride(i) % 8 == 0),
-                    "rows of a cache must not overlap, their strides be multiples of 8");
+      // each dimension steps over all that those of smaller strides hold (a dimension of one may have any stride)
+      int order[3] = {2, 1, 0};
+      std::sort(order, order + 3, [&](int i, int j) { return k.stride(i) < k.stride(j); });
+      int64_t span = D;
+      for (int i : order) {
+        if (k.size(i) <= 1) continue;
+        TORCH_CHECK(k.stride(i) >= span && k.stride(i) % 8 == 0, "rows of a cache must not overlap, their strides be multiples of 8");
+        span += (k.size(i) - 1) * k.stride(i);
+      }
     }
     for (const Tensor* t : {&k, &v, (const Tensor*)&ks, (const Tensor*)&vs})
       TORCH_CHECK(!t->defined() || t->numel() == 0 || !misaligned(*t), "the cache must be aligned to 16 bytes");

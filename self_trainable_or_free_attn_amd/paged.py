@@ -60,6 +60,12 @@ PAGE_SIZES = frozenset(1 << i for i in range(4, 13))
 MAX_TOKENS = 1 << 30      # that a row of `pages` can name
 
 
+def _rows_apart(shape, strides, dim):
+    """Whether rows of `dim` channels stand apart: each dimension steps over all that those of smaller strides hold."""
+    dims = [(s, n) for n, s in zip(shape, strides) if n > 1]
+    return all(s >= dim + sum((m - 1) * r for j, (r, m) in enumerate(dims) if j != i and r <= s) for i, (s, _) in enumerate(dims))
+
+
 def _check_cache(cache, dtype, device, like):
     """(heads, page_size, dim) of a cache that holds tokens of `dtype`."""
     k, v, ks, vs = cache
@@ -88,7 +94,7 @@ def _check_cache(cache, dtype, device, like):
         if k.stride() != v.stride() or k.stride(3) != 1 or any(n > 1 and s % 8 for n, s in zip(k.shape[:3], k.stride())):
             raise ValueError(f"cache.k and cache.v must have the same strides, channels 1 apart and the others multiples of 8, got "
                              f"{k.stride()} and {v.stride()}")
-        if any(n > 1 and s < dim for n, s in zip(k.shape[:3], k.stride())):
+        if not _rows_apart(k.shape[:3], k.stride(), dim):
             raise ValueError(f"rows of the cache must not overlap, got strides {k.stride()}")
     if dim not in (64, 128):
         raise ValueError(f"head dim must be 64 or 128, got {dim}")

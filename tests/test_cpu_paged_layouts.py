@@ -35,3 +35,23 @@ ONES = [((1, 2, 16, 64), (3, 1024, 64, 1)), ((8, 1, 16, 64), (1024, 5, 64, 1)), 
 def test_dimensions_of_one_have_any_stride(shape, strides):
     for call in _calls(PagedCache(strided(shape, strides), strided(shape, strides))):
         call()
+
+
+# rows that share values, though every stride is as long as a row
+OVERLAPPING = [((8, 2, 16, 64), (256, 64, 128, 1)), ((8, 2, 16, 64), (1024, 128, 64, 1)), ((2, 3, 16, 64), (64, 96, 384, 1)),
+               ((4, 2, 16, 128), (4096, 2048, 64, 1)), ((3, 2, 16, 64), (2048, 1024, 0, 1))]
+APART = [((8, 2, 16, 64), (2048, 64, 128, 1)), ((8, 2, 16, 64), (64, 512, 1024, 1)), ((2, 3, 16, 64), (80, 160, 480, 1)),
+         ((4, 2, 16, 128), (10000, 5000, 136, 1)), ((1, 2, 16, 64), (0, 64, 128, 1))]
+
+
+@pytest.mark.parametrize("shape, strides", OVERLAPPING)
+def test_rows_that_overlap_are_refused(shape, strides):
+    for call in _calls(PagedCache(strided(shape, strides), strided(shape, strides))):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+
+
+@pytest.mark.parametrize("shape, strides", APART)
+def test_rows_apart_in_any_order(shape, strides):
+    for call in _calls(PagedCache(strided(shape, strides), strided(shape, strides))):
+        call()

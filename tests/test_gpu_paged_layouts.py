@@ -29,3 +29,27 @@ def test_dimensions_of_one_have_any_stride(dev, shape, strides):
     for other in res[1:]:
         assert all(torch.equal(a, b) for a, b in zip(res[0], other))
     assert torch.equal(odd.k[num - 1].transpose(0, 1)[:9], k) and torch.equal(odd.v[num - 1].transpose(0, 1)[:9], v)
+
+
+@pytest.mark.parametrize("shape, strides", cases.OVERLAPPING)
+def test_rows_that_overlap_are_refused(dev, shape, strides):
+    cache = PagedCache(*(cases.strided(shape, strides, dev) for _ in "kv"))
+    pages, lens = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    x = torch.zeros(2, shape[1], shape[3], dtype=BF, device=dev)
+    for call in (lambda: append_paged(cache, x, x, pages, lens), lambda: paged_attention(x, cache, pages, lens),
+                 lambda: paged_rows(cache, pages, lens, rows=2)):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+
+
+@pytest.mark.parametrize("shape, strides", cases.APART)
+def test_rows_apart_in_any_order(dev, shape, strides):
+    num, Hk, page, D = shape
+    g = torch.Generator(device=dev).manual_seed(2)
+    odd = PagedCache(*(cases.strided(shape, strides, dev) for _ in "kv"))
+    n = num * page - 3
+    pages, lens = torch.randperm(num, device=dev, generator=g).to(torch.int32)[None], torch.tensor([n], dtype=torch.int32, device=dev)
+    k, v = torch.randn(2, n, Hk, D, device=dev, generator=g).to(BF)
+    append_paged(odd, k, v, pages, lens)
+    rows = paged_rows(odd, pages, lens, rows=n)
+    assert torch.equal(rows[0], k) and torch.equal(rows[1], v)
