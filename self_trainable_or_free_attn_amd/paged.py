@@ -258,7 +258,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, len
     if q.is_cuda and q.dim() == 3:      # the operator checks everything itself; what it refuses is named by the checks below
         try:
             out = _ops().paged_attention(q.contiguous(), *cache, pages, lens, cu, bool(causal),
-                                         q.shape[2] ** -0.5 if scale is None else scale)
+                                         max(q.shape[2], 1) ** -0.5 if scale is None else scale)
         except (RuntimeError, TypeError):
             _check_attention(q, cache, pages, lens, cu, scale)
             raise

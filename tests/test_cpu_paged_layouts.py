@@ -55,3 +55,19 @@ def test_rows_that_overlap_are_refused(shape, strides):
 def test_rows_apart_in_any_order(shape, strides):
     for call in _calls(PagedCache(strided(shape, strides), strided(shape, strides))):
         call()
+
+
+def test_heads_without_channels_are_refused():
+    q, cache = torch.empty(2, 2, 0, dtype=BF, device="meta"), PagedCache(*(torch.empty(8, 2, 16, 64, dtype=BF, device="meta"),) * 2)
+    with pytest.raises(ValueError, match="head dim"):
+        paged_attention(q, cache, _i(2, 3), _i(2))
+
+
+def test_the_default_scale_needs_no_channels():
+    """Tensors that claim to be on a GPU, whose calls only the native operator checks: no arithmetic of Python's fails before."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        t = lambda *s, dtype=BF: torch.empty(*s, dtype=dtype, device="cuda")
+        out = paged_attention(t(2, 2, 0), PagedCache(t(8, 2, 16, 64), t(8, 2, 16, 64)), t(2, 3, dtype=torch.int32),
+                              t(2, dtype=torch.int32))
+        assert out.shape == (2, 2, 0)

@@ -53,3 +53,11 @@ def test_rows_apart_in_any_order(dev, shape, strides):
     append_paged(odd, k, v, pages, lens)
     rows = paged_rows(odd, pages, lens, rows=n)
     assert torch.equal(rows[0], k) and torch.equal(rows[1], v)
+
+
+@pytest.mark.parametrize("scale", [None, 0.1])
+def test_heads_without_channels_are_refused(dev, scale):
+    cache = PagedCache(*(torch.zeros(8, 2, 16, 64, dtype=BF, device=dev) for _ in "kv"))
+    pages, lens = torch.zeros(2, 3, dtype=torch.int32, device=dev), torch.ones(2, dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError, match="head dim"):
+        paged_attention(torch.zeros(2, 2, 0, dtype=BF, device=dev), cache, pages, lens, scale=scale)
