@@ -612,14 +612,14 @@ struct Shares {
             at += each[i];
             k = i + 1;
           }
-        seq = b0 + l * LISTS + __builtin_amdgcn_readlane(k, l);
+        seq = min(b0 + l * LISTS + __builtin_amdgcn_readlane(k, l), a.B);
         y = x - __builtin_amdgcn_readlane(at, l);
         break;
       }
       front = __builtin_amdgcn_readlane(lane_upto, 63);
     }
     const int tile_cost = cost(seq, tiles);
-    place = min(y / tile_cost, tiles - 1);
+    place = place_in(y, tile_cost, tiles);
     y -= place * tile_cost;
     const int number = first_tile<M>(seq_start(a.cu_q, seq, a.B, a.Tq), a.G, seq) + place;
     const float snap = SNAP * (float)share;
@@ -945,8 +945,8 @@ struct WideLists {
         if (i0 + 64 * k < item.list && i0 + 64 * k + lane_id() < item.list) front += parts_of(at(i0, k), item.per);
     }
     const int level0 = own.tiles - tiles_within(own, a.G, a.causal, bound(item.per, 0));
-    return within(__builtin_amdgcn_readlane(wave_scan(front), 63) + partial_number(item.number, level0, cut_tiles_of(own, item.per)),
-                  a.parts);
+    front = __builtin_amdgcn_readlane(wave_scan(front), 63);
+    return within(front + partial_number(item.number, level0, cut_tiles_of(own, item.per)), a.parts);
   }
 
   // item w, and its list
@@ -987,7 +987,8 @@ struct WideLists {
         const int i = i0 + 64 * k + l;
         if (leave) {
           const WideList x = at(i0, k);
-          const int cuts = cut_tiles_of(x, per), cut_upto = wave_scan(cuts), own_parts = parts_of(x, per), part_upto = wave_scan(own_parts);
+          const int cuts = cut_tiles_of(x, per), cut_upto = wave_scan(cuts);
+          const int own_parts = parts_of(x, per), part_upto = wave_scan(own_parts);
           if (i < lists) plan[i] = make_int2(parts + part_upto - own_parts, cut_tiles + cut_upto - cuts);
           parts += __builtin_amdgcn_readlane(part_upto, 63);
           cut_tiles += __builtin_amdgcn_readlane(cut_upto, 63);
@@ -1013,8 +1014,12 @@ struct WideLists {
     else own = wide_at(wide_of(a, list), 0);
     const int piece = piece_of(own.x, per);
     WideItem item = {list, 0, 0, 0, number, per};
-    if (kind > 0) item.tile = tiles_within(own.x, a.G, a.causal, bound(per, kind - 1)) - 1 - number;
-    else if (!piece_at(own.x, a.G, a.causal, piece, bound(per, 0), number, item.tile, item.level)) item.list = -1;
+    if (kind > 0) {
+      item.tile = tiles_within(own.x, a.G, a.causal, bound(per, kind - 1)) - 1 - number;
+      if (item.tile < 0) item.list = -1;  // (counts that decrease, too many to be added up)
+    } else if (!piece_at(own.x, a.G, a.causal, piece, bound(per, 0), number, item.tile, item.level)) {
+      item.list = -1;
+    }
     item.piece = piece;
     return item;
   }

@@ -10,6 +10,13 @@
 
 namespace es {
 
+// The tile that place y of a sequence falls into, whose tiles cost tile_cost each: one of them also for a y that no running counts
+// give. (Counts that decrease name rows twice, and their costs may pass 2^31: no row outside the tensors may follow from that.)
+ES_RULE int place_in(int y, int tile_cost, int tiles) {
+  const int place = y / tile_cost;
+  return place < 0 || tiles < 1 ? 0 : place < tiles ? place : tiles - 1;
+}
+
 struct WideList {
   int rows, tiles, chunks;  // chunks that the last tile reads, the most
   int behind;               // new tokens less all tokens of the sequence: new token i sees i + 1 - behind keys, those that are held
