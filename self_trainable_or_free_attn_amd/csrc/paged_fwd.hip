@@ -467,7 +467,7 @@ __device__ __forceinline__ void paged_job(const FwdArgs& a, Job& j, int q0, int 
 // LDS: two chunks (16 bits, narrow: a run a wave) of keys and values; 4 bits, TOKENS: a run of values a wave
 template <int D, int M>
 constexpr int paged_lds() { return M == TOKENS<4> ? 4 * 32 * D * 2 : 4 * BK * D * 2; }
-// Workgroups that a CU holds. (TOKENS over 4 bits: 163 registers; at 128, for four, the loop reloads spilled ones, and 48 tokens
+// Workgroups that a CU holds. (TOKENS over 4 bits: 157 registers; at 128, for four, the loop reloads spilled ones, and 48 tokens
 // against 8000 keys, 32 heads over 8, take 107 us instead of 88.)
 #define ES_PAGED_RESIDENT(D, M) ((M) == 16 || (D) == 64 ? 3 : 2)
 
@@ -503,8 +503,11 @@ __global__ __launch_bounds__(256, ES_PAGED_RESIDENT(D, M)) void paged_whole_kern
 // tile has some of its own: no workgroup then has two pieces, one after the other (7 tokens against 3 to 9923 keys, 24 heads over
 // 3, 17.9 us instead of 20.4; 18 against 1 to 25716 over 4 bits, 16 heads over 2, 21.2 instead of 23.0). TILE_COST 2 and shares of
 // 4 chunks instead of LEAST = 6 at least: 12 tokens against 6 to 23354 keys, 3 heads, 33.0 us instead of 28.1; 100 against 1 to
-// 40000, 16 heads of 64 over 2, 47.7 instead of 43.3; the large cases above the same. A lane has LISTS sequences one behind the
-// other, so up to 255 are read once.
+// 40000, 16 heads of 64 over 2, 47.7 instead of 43.3; the large cases above the same. SNAP 0: 200 tokens of 1 to 40000 keys over
+// 4 bits 171.5 us instead of 166.9, others up to 1 % slower; 0.25: in 16 bits 564 instead of 544, though 256 against 2000 over 4
+// bits 118 instead of 123. WHOLE 1: 63 tokens against 2000 keys 114 us instead of 101; 2: 48 against 8000 over 4 bits 117 instead
+// of 87, though in 16 bits 269 instead of 293. A lane has LISTS sequences one behind the other, so up to 255 are read once. (Over
+// 16 bits 28 scalar registers are spilled to lanes at D = 64 and 35 at D = 128.)
 struct Share {
   int tile, chunk;  // tile number as in packed.h (first_tile of its sequence and its place there), chunk within it
 };
@@ -791,6 +794,9 @@ __global__ __launch_bounds__(256) void merge_shares_kernel(FwdArgs a) {
 // pieces start anywhere: 4096 tokens of 32 heads over 8 alone 228 us, pieces 155. One count of ranges for all tiles of a sequence,
 // as packed_tiles.h has it, which takes a causal prompt for twice its work: prompts of 3923, 938 and 3440 tokens, 8 heads of 64
 // over one, 114 us, pieces 79; 256 and 512 tokens over 9000 and 512 keys beside two small ones, 24 heads over 8, 65 and 56.)
+// P goes into the products of wide tiles as one 16-bit value: errors are 1.3 to 1.4 times those of its own rounding of the output.
+// With what the rounding leaves as a second product (narrow tiles) they are not, but 256 to 512 tokens over 9000 keys take 68 us
+// instead of 55, 700 over 16384 315 instead of 241, 32760 causal ones 8280 instead of 5980.
 // Every wave derives the cut from the lengths by itself, so they stay on the device: of sizes from the fair share on the one with
 // the shortest schedule, by a model of it. Items over three quarters of the largest come first, then those over a half, over a
 // quarter and the rest, since workgroups are dispatched in order. Lanes have LISTS sequences each, 64 apart; more than 64 * LISTS
@@ -1098,8 +1104,14 @@ struct PagedPlan {
   size_t plan, bytes;  // workspace: partials, then borders (SHARES) or the cut (PIECES)
 };
 
-// `cap`: the keys that a sequence can have. equal: B sequences of Tq / B tokens. Up to 1024 keys a tile is short enough for one
-// workgroup, and a second launch would take as long again.
+// `cap`: the keys that a sequence can have, by the width of its table of pages; equal: B sequences of Tq / B tokens. Both are
+// what the host knows. Up to 1024 keys a tile is short enough for one workgroup, and a second launch would take as long again.
+// Without this form: 4 tokens of 300 keys, 8 heads of 64 over 2, 14.1 us instead of 8.6, of 1000 14.4 instead of 13.2; 48 of 300,
+// 32 heads over 8, 27.8 instead of 18.7; a prompt of 1000 34.7 instead of 23.6, eight 113 instead of 115. With it up to 4096 keys:
+// 48 tokens of 1500 keys 54 us instead of 62 and a prompt of 1500 36 instead of 48, but 4 tokens of 1500 17 instead of 15, of 2500
+// 26 instead of 15. A table that is wider than the histories need pays for the cut: 4 tokens of 1 to 300 keys with one of 32768
+// 13.3 us instead of 8.0, 48 of 300 27 instead of 18, eight prompts of 1000 108 instead of 99. So does one more token than
+// sequences, which makes all tiles wide: 48 tokens of 1 to 16000 keys 302 us, with one more 317; over 4 bits 96 and 129.
 static PagedPlan paged_plan(int B, int Tq, int cap, int H, int Hk, int D, int bits, bool equal) {
   PagedPlan p = {};
   const int G = H / Hk, narrow = bits == 4 ? TOKENS<4> : TOKENS<16>;

@@ -22,8 +22,8 @@ from .rotary import _check_turn
 
 class PagedCache(NamedTuple):
     """Keys and values in pages. 16 bits: k and v [num_pages, Hk, page_size, D] in the tokens' type, with any strides that both
-    have and that leave the channels 1 apart (a cache of [num_pages, page_size, Hk, D] is passed with its middle dimensions
-    transposed), k_scales and v_scales None.
+    have, that leave the channels 1 apart and give each row memory of its own (a cache of [num_pages, page_size, Hk, D] is
+    passed with its middle dimensions transposed), k_scales and v_scales None.
 
     4 bits: k and v are codes, uint8 [num_pages, Hk, page_size, D / 2], channel 2 i in the low half of byte i, and k_scales and
     v_scales uint8 [num_pages, Hk, page_size, D / 32], all contiguous. A code is a sign (bit 3) and the number of one of the

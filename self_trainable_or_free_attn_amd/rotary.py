@@ -111,7 +111,8 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tenso
     of the row's position, channels 2 i and 2 i + 1, with halves i and i + R / 2. positions: int32 [T] ([B, L]) rows of the
     table, clamped to it; None: a row's place in q (in its sequence of the batch).
 
-    Returns the new q and k, contiguous. All arithmetic is float32, rounded once at the end. Gradients are deterministic and those
+    Returns the new q and k, contiguous. All arithmetic is float32, rounded once at the end (so the squares of a row have to stay
+    within float32: bf16 values to about 1e18, with eps = 0 from 1e-19 on). Gradients are deterministic and those
     of the weights are summed in float32; the backward itself is not differentiable, and a table gets no gradient. A capture with
     gradients takes leaves made inside it; those that an eager graph of another stream holds are refused."""
     if q.is_cuda and q.dim() == 3:      # the operator checks everything itself; what it refuses is named by the checks below
