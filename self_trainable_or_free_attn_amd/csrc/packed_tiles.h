@@ -235,7 +235,7 @@ __device__ __forceinline__ void store_row(const FwdArgs& a, size_t at, int col, 
 //   run(a, j, v, u, dst)     narrow tiles: starts those of K (v: V) of the 32-key run u, all of them by this wave
 //   enter / mask             HOLES: keys that a sequence counts may be missing, 16 at a time; their scores become -inf
 //   FINE                     narrow tiles multiply V by what the rounding of P leaves, too (wide ones, which the matrix units
-//                            bound, round P once: its error is that of the output's own rounding, times 1.4 with it)
+//                            bound, round P once: an error about as large as that of the output's own rounding)
 template <int D>
 struct Rowwise {
   static constexpr bool HOLES = false, STAGED = false, FINE = false;
